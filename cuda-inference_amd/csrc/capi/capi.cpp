@@ -20,6 +20,8 @@
 #include "gpu_inference/dispatcher.h"
 #include "gpu_inference/execution_plan.h"
 #include "gpu_inference/hip_graph.h"
+#include "gpu_inference/linear_i8.h"
+#include "gpu_inference/paged_kv.h"
 #include "gpu_inference/perf_model.h"
 #include "gpu_inference/reference.h"
 #include "gpu_inference/testing.h"
@@ -101,6 +103,51 @@ ConstTensorRef to_cref(const gie_tensor* t) {
 TensorRef to_ref(const gie_tensor* t) {
   const ConstTensorRef c = to_cref(t);
   return {const_cast<void*>(c.data), c.dtype, c.shape};
+}
+
+LinearI8Problem to_linear(const gie_linear_i8_problem* p) {
+  GIE_REQUIRE(p != nullptr, StatusCode::kInvalidArgument, "null problem");
+  GIE_REQUIRE(p->precision >= 0 && p->precision <= 3, StatusCode::kInvalidArgument, "bad precision");
+  LinearI8Problem r;
+  r.tokens = p->tokens;
+  r.in_features = p->in_features;
+  r.out_features = p->out_features;
+  r.precision = static_cast<Precision>(p->precision);
+  r.has_bias = p->has_bias != 0;
+  r.activation = p->relu ? Activation::kReLU : Activation::kNone;
+  r.quantized = p->quantized != 0;
+  r.ld_x = p->ld_x;
+  r.ld_w = p->ld_w;
+  r.ld_y = p->ld_y;
+  return r;
+}
+
+PagedKvProblem to_paged(const gie_paged_kv_problem* p) {
+  GIE_REQUIRE(p != nullptr, StatusCode::kInvalidArgument, "null problem");
+  GIE_REQUIRE(p->precision >= 0 && p->precision <= 3, StatusCode::kInvalidArgument, "bad precision");
+  PagedKvProblem r;
+  r.batch = p->batch;
+  r.total_tokens = p->total_tokens;
+  r.q_heads = p->q_heads;
+  r.kv_heads = p->kv_heads;
+  r.head_dim = p->head_dim;
+  r.page_size = p->page_size;
+  r.num_pages = p->num_pages;
+  r.max_pages = p->max_pages;
+  r.precision = static_cast<Precision>(p->precision);
+  r.q_stride = p->q_stride;
+  r.k_stride = p->k_stride;
+  r.v_stride = p->v_stride;
+  r.o_stride = p->o_stride;
+  r.rotary_dim = p->rotary_dim;
+  r.interleaved = p->interleaved != 0;
+  r.max_positions = p->max_positions;
+  r.scale = p->scale;
+  r.softcap = p->softcap;
+  r.window = p->window;
+  r.max_new = p->max_new;
+  r.max_len = p->max_len;
+  return r;
 }
 
 struct PlanHandle {
@@ -897,4 +944,57 @@ extern "C" int gie_testing_add_faulty_kernels(int kind) {
       reg.push_back(std::move(k));
     }
   });
+}
+
+extern "C" int gie_linear_i8_workspace_size(const gie_linear_i8_problem* p, size_t* bytes) {
+  return guarded([&] {
+    GIE_REQUIRE(bytes != nullptr, StatusCode::kInvalidArgument, "null out");
+    *bytes = LinearI8::workspace_size(to_linear(p));
+  });
+}
+
+extern "C" int gie_linear_i8_forward(const gie_linear_i8_problem* p, const void* x, const float* x_scale,
+                                     const int8_t* w, const float* w_scale, const void* bias, void* y,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    LinearI8::forward(x, x_scale, w, w_scale, bias, to_linear(p), y, workspace, workspace_bytes,
+                      static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int gie_quantize_rows(const gie_linear_i8_problem* p, const void* x, int8_t* q, float* scale,
+                                 void* stream) {
+  return guarded([&] { LinearI8::quantize_rows(x, to_linear(p), q, scale, static_cast<hipStream_t>(stream)); });
+}
+
+extern "C" int gie_kv_append(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v,
+                             const float* cos, const float* sin, const int* q_starts, const int* seq_lens,
+                             const int* page_table, void* q_out, void* k_pages, void* v_pages, void* stream) {
+  return guarded([&] {
+    PagedKv::append(q, k, v, cos, sin, q_starts, seq_lens, page_table, to_paged(p), q_out, k_pages, v_pages,
+                    static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int gie_paged_attention_workspace_size(const gie_paged_kv_problem* p, size_t* bytes) {
+  return guarded([&] {
+    GIE_REQUIRE(bytes != nullptr, StatusCode::kInvalidArgument, "null out");
+    *bytes = PagedKv::workspace_size(to_paged(p));
+  });
+}
+
+extern "C" int gie_paged_attention(const gie_paged_kv_problem* p, const void* q, const void* k_pages,
+                                   const void* v_pages, const int* q_starts, const int* seq_lens,
+                                   const int* page_table, void* out, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  return guarded([&] {
+    PagedKv::attention(q, k_pages, v_pages, q_starts, seq_lens, page_table, to_paged(p), out, workspace,
+                       workspace_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int gie_rotary_tables(int max_positions, int rotary_dim, double base, double factor,
+                                 int original_positions, double magnitude, float* cos, float* sin) {
+  return guarded(
+      [&] { rotary_tables(max_positions, rotary_dim, base, factor, original_positions, magnitude, cos, sin); });
 }

@@ -88,6 +88,34 @@ class GieDeviceModel(ctypes.Structure):
                 ("hbm_gbs", ctypes.c_double), ("launch_us", ctypes.c_double), ("lds_per_workgroup", ctypes.c_size_t)]
 
 
+class GieLinearI8Problem(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("tokens", "in_features", "out_features", "precision", "has_bias", "relu",
+                                            "quantized")] + [(n, ctypes.c_int64) for n in ("ld_x", "ld_w", "ld_y")]
+
+
+class GiePagedKvProblem(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("batch", "total_tokens", "q_heads", "kv_heads", "head_dim", "page_size",
+                                            "num_pages", "max_pages", "precision")] + \
+               [(n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + \
+               [(n, ctypes.c_int) for n in ("rotary_dim", "interleaved", "max_positions")] + \
+               [(n, ctypes.c_float) for n in ("scale", "softcap")] + \
+               [(n, ctypes.c_int) for n in ("window", "max_new", "max_len")]
+
+
+class GieLinearGeom(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("tokens", "in_features", "out_features")] + \
+               [(n, ctypes.c_int64) for n in ("ld_x", "ld_w", "ld_y")] + [("relu", ctypes.c_int)]
+
+
+class GiePagedGeom(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("batch", "total_tokens", "q_heads", "kv_heads", "head_dim", "page_size",
+                                            "num_pages", "max_pages")] + \
+               [(n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + \
+               [(n, ctypes.c_int) for n in ("rotary_dim", "interleaved", "max_positions")] + \
+               [(n, ctypes.c_float) for n in ("scale", "softcap")] + \
+               [(n, ctypes.c_int) for n in ("window", "max_new", "max_len")]
+
+
 class GieIgemmConfig(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in (
         "tile_m", "tile_n", "tile_k", "waves_m", "waves_n", "threads", "lds_bytes", "stages", "version")]
@@ -162,6 +190,13 @@ _CAPI = {
                                    ctypes.POINTER(_sz), _ip], _i),
     "gie_graph_launch": ([_vp, _vp], _i),
     "gie_graph_node_count": ([_vp, ctypes.POINTER(_sz)], _i),
+    "gie_linear_i8_workspace_size": ([ctypes.POINTER(GieLinearI8Problem), ctypes.POINTER(_sz)], _i),
+    "gie_linear_i8_forward": ([ctypes.POINTER(GieLinearI8Problem)] + [_vp] * 7 + [_sz, _vp], _i),
+    "gie_quantize_rows": ([ctypes.POINTER(GieLinearI8Problem), _vp, _vp, _vp, _vp], _i),
+    "gie_kv_append": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 12, _i),
+    "gie_paged_attention_workspace_size": ([ctypes.POINTER(GiePagedKvProblem), ctypes.POINTER(_sz)], _i),
+    "gie_paged_attention": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 8 + [_sz, _vp], _i),
+    "gie_rotary_tables": ([_i, _i, ctypes.c_double, ctypes.c_double, _i, ctypes.c_double, _vp, _vp], _i),
     "gie_dev_malloc": ([_sz, ctypes.POINTER(_vp)], _i),
     "gie_dev_free": ([_vp], _i),
     "gie_memcpy_h2d": ([_vp, _vp, _sz], _i),
@@ -241,6 +276,12 @@ _HIP = {
     "gie_hip_f32_config_tile_m": ([_i], _i),
     "gie_hip_f32_check": ([_i, _GP, _vp], _i),
     "gie_hip_conv_f32": ([_i, _i, _GP, _vp, _vp, _vp, _vp, _vp, _i, _vp], _i),
+    "gie_hip_quantize_rows": ([_i, _vp, ctypes.c_int64, _i, _i, _vp, ctypes.c_int64, _vp, _vp], _i),
+    "gie_hip_linear_i8_workspace": ([_i, ctypes.POINTER(GieLinearGeom), _i], _sz),
+    "gie_hip_linear_i8": ([_i, ctypes.POINTER(GieLinearGeom)] + [_vp] * 7 + [_sz, _vp], _i),
+    "gie_hip_kv_append": ([_i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 12, _i),
+    "gie_hip_paged_attention_workspace": ([ctypes.POINTER(GiePagedGeom)], _sz),
+    "gie_hip_paged_attention": ([_i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 8 + [_sz, _vp], _i),
     "gie_hip_reference_conv": ([_i, _GP, _vp, _vp, _vp, _vp, _vp, _vp], _i),
     "gie_hip_ceiling_mfma": ([_i, _i, _vp, _vp], _i),
     "gie_hip_ceiling_copy": ([_vp, _vp, _sz, _vp], _i),
@@ -955,3 +996,116 @@ def igemm_configs() -> list[dict]:
         check_hip(hip().gie_hip_igemm_config_get(i, ctypes.byref(c)), "config")
         out.append({f: getattr(c, f) for f, _ in c._fields_})
     return out
+
+
+# ------------------------------------------------------------------------------------------------- 8-bit linear
+@dataclass(frozen=True)
+class LinearI8:
+    """LinearI8Problem (linear_i8.h): y = act((q @ w.T) * x_scale[:, None] * w_scale + bias), q and w in 8 bits.
+    `quantized`: x is int8 with x_scale; otherwise x is in `precision` and its scales are found on the way."""
+    tokens: int
+    in_features: int
+    out_features: int
+    precision: str = "fp16"
+    has_bias: bool = False
+    relu: bool = False
+    quantized: bool = False
+    ld_x: int = 0
+    ld_w: int = 0
+    ld_y: int = 0
+
+    def __post_init__(self):
+        object.__setattr__(self, "_c", GieLinearI8Problem(
+            self.tokens, self.in_features, self.out_features, PRECISIONS[self.precision], int(self.has_bias),
+            int(self.relu), int(self.quantized), self.ld_x, self.ld_w, self.ld_y))
+        object.__setattr__(self, "_ref", ctypes.byref(self._c))
+
+
+def _stream(stream):
+    """A Stream, a raw hipStream_t address or None."""
+    return stream.h if isinstance(stream, Stream) else stream or None
+
+
+def linear_i8_workspace_size(p: LinearI8) -> int:
+    n = ctypes.c_size_t()
+    check(capi().gie_linear_i8_workspace_size(p._ref, ctypes.byref(n)), "LinearI8::workspace_size")
+    return n.value
+
+
+def linear_i8(p: LinearI8, x: int, w: int, w_scale: int, y: int, x_scale: int | None = None, bias: int | None = None,
+              workspace: int | None = None, ws_bytes: int = 0, stream=None):
+    """LinearI8::forward on raw device addresses."""
+    check(capi().gie_linear_i8_forward(p._ref, x, x_scale, w, w_scale, bias, y, workspace, ws_bytes, _stream(stream)),
+          "LinearI8::forward")
+
+
+def quantize_rows(p: LinearI8, x: int, q: int, scale: int, stream=None):
+    """LinearI8::quantize_rows: x in p's precision -> q int8 [tokens][in_features], scale float [tokens]."""
+    check(capi().gie_quantize_rows(p._ref, x, q, scale, _stream(stream)), "LinearI8::quantize_rows")
+
+
+# ------------------------------------------------------------------------------------------------- paged K/V cache
+@dataclass(frozen=True)
+class PagedKv:
+    """PagedKvProblem (paged_kv.h). Strides are elements between tokens (0: packed), scale 0 is 1 / sqrt(head_dim),
+    softcap 0 and window 0 are off; max_new and max_len only help to choose a launch shape."""
+    batch: int
+    total_tokens: int
+    q_heads: int
+    kv_heads: int
+    head_dim: int
+    page_size: int
+    num_pages: int
+    max_pages: int
+    precision: str = "fp16"
+    q_stride: int = 0
+    k_stride: int = 0
+    v_stride: int = 0
+    o_stride: int = 0
+    rotary_dim: int = 0
+    interleaved: bool = False
+    max_positions: int = 0
+    scale: float = 0.0
+    softcap: float = 0.0
+    window: int = 0
+    max_new: int = 0
+    max_len: int = 0
+
+    def __post_init__(self):
+        object.__setattr__(self, "_c", GiePagedKvProblem(
+            self.batch, self.total_tokens, self.q_heads, self.kv_heads, self.head_dim, self.page_size, self.num_pages,
+            self.max_pages, PRECISIONS[self.precision], self.q_stride, self.k_stride, self.v_stride, self.o_stride,
+            self.rotary_dim, int(self.interleaved), self.max_positions, self.scale, self.softcap, self.window,
+            self.max_new, self.max_len))
+        object.__setattr__(self, "_ref", ctypes.byref(self._c))
+
+
+def kv_append(p: PagedKv, k: int, v: int, q_starts: int, seq_lens: int, page_table: int, k_pages: int, v_pages: int,
+              cos: int | None = None, sin: int | None = None, q: int | None = None, q_out: int | None = None,
+              stream=None):
+    """PagedKv::append on raw device addresses."""
+    check(capi().gie_kv_append(p._ref, q, k, v, cos, sin, q_starts, seq_lens, page_table, q_out, k_pages, v_pages,
+                               _stream(stream)), "PagedKv::append")
+
+
+def paged_attention_workspace_size(p: PagedKv) -> int:
+    n = ctypes.c_size_t()
+    check(capi().gie_paged_attention_workspace_size(p._ref, ctypes.byref(n)), "PagedKv::workspace_size")
+    return n.value
+
+
+def paged_attention(p: PagedKv, q: int, k_pages: int, v_pages: int, q_starts: int, seq_lens: int, page_table: int,
+                    out: int, workspace: int | None = None, ws_bytes: int = 0, stream=None):
+    """PagedKv::attention on raw device addresses."""
+    check(capi().gie_paged_attention(p._ref, q, k_pages, v_pages, q_starts, seq_lens, page_table, out, workspace,
+                                     ws_bytes, _stream(stream)), "PagedKv::attention")
+
+
+def rotary_tables(max_positions: int, rotary_dim: int, base: float = 10000.0, factor: float = 1.0,
+                  original_positions: int = 0, magnitude: float = 1.0):
+    """Host cos and sin tables [max_positions][rotary_dim / 2] (paged_kv.h rotary_tables)."""
+    cos = np.empty((max(max_positions, 0), max(rotary_dim, 0) // 2), np.float32)
+    sin = np.empty_like(cos)
+    check(capi().gie_rotary_tables(max_positions, rotary_dim, base, factor, original_positions, magnitude,
+                                   cos.ctypes.data, sin.ctypes.data), "rotary_tables")
+    return cos, sin

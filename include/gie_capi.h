@@ -190,6 +190,46 @@ int gie_graph_recapture_chain(void* graph, int n, void* const* plans, const void
 int gie_graph_launch(void* graph, void* stream);
 int gie_graph_node_count(void* graph, size_t* nodes);
 
+/* ---- LinearI8 (linear_i8.h): 8-bit matrix product with scales for each token and output channel ---- */
+typedef struct gie_linear_i8_problem {
+  int tokens, in_features, out_features;
+  int precision;              /* of x (unless quantized), bias and y: 0 fp32, 1 fp16, 2 bf16 */
+  int has_bias, relu;
+  int quantized;              /* x is int8 with x_scale; otherwise x_scale is found from x on the way */
+  int64_t ld_x, ld_w, ld_y;   /* elements between rows; 0: packed */
+} gie_linear_i8_problem;
+int gie_linear_i8_workspace_size(const gie_linear_i8_problem* p, size_t* bytes);
+int gie_linear_i8_forward(const gie_linear_i8_problem* p, const void* x, const float* x_scale, const int8_t* w,
+                          const float* w_scale, const void* bias, void* y, void* workspace, size_t workspace_bytes,
+                          void* stream);
+/* the quantization alone: q [tokens][in_features], scale [tokens] from x in the problem's precision */
+int gie_quantize_rows(const gie_linear_i8_problem* p, const void* x, int8_t* q, float* scale, void* stream);
+
+/* ---- PagedKv (paged_kv.h): append to and attention over a paged key/value cache ---- */
+typedef struct gie_paged_kv_problem {
+  int batch, total_tokens, q_heads, kv_heads, head_dim;
+  int page_size, num_pages, max_pages;
+  int precision;                                   /* 1 fp16, 2 bf16 */
+  int64_t q_stride, k_stride, v_stride, o_stride;  /* elements between tokens; 0: packed */
+  int rotary_dim, interleaved, max_positions;
+  float scale, softcap;                            /* scale 0: 1 / sqrt(head_dim) */
+  int window, max_new, max_len;
+} gie_paged_kv_problem;
+int gie_kv_append(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v, const float* cos,
+                  const float* sin, const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
+                  void* k_pages, void* v_pages, void* stream);
+int gie_paged_attention_workspace_size(const gie_paged_kv_problem* p, size_t* bytes);
+int gie_paged_attention(const gie_paged_kv_problem* p, const void* q, const void* k_pages, const void* v_pages,
+                        const int* q_starts, const int* seq_lens, const int* page_table, void* out, void* workspace,
+                        size_t workspace_bytes, void* stream);
+/* host tables of the rotation, [max_positions][rotary_dim / 2] FP32 each, computed in 64 bits:
+   angle(p, j) = p * f_j, f_j = base^(-2j / rotary_dim), long contexts by `factor` >= 1 and `original_positions`:
+   original_positions == 0: every f_j / factor (positions interpolated); otherwise only the frequencies whose
+   wavelength exceeds original_positions are divided, those shorter than a quarter of it stay, between them f_j is
+   blended linearly in original_positions / wavelength. cos and sin are multiplied by `magnitude`. */
+int gie_rotary_tables(int max_positions, int rotary_dim, double base, double factor, int original_positions,
+                      double magnitude, float* cos, float* sin);
+
 /* ---- device memory / streams / events for bindings without their own HIP runtime ---- */
 int gie_dev_malloc(size_t bytes, void** ptr);
 int gie_dev_free(void* ptr);

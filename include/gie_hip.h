@@ -368,6 +368,67 @@ int gie_hip_splitk_reduce_form(int dtype, int64_t total, int split, int vec, int
 int gie_hip_bias_act(int dtype, void* y, const void* bias, int64_t total, int out_channels, int hw_out, int relu,
                      void* stream);
 
+/* ---- 8-bit linear layers (no counterpart in the reference, which has no 8-bit path) ----
+   y[t][n] = round(relu?(float(sum_k q[t][k] * w[n][k]) * (scale[t] * w_scale[n]) + bias[n])), the sum exact in int32
+   (in_features <= 131071 keeps it below 2^31). */
+typedef struct gie_linear_geom {
+  int tokens, in_features, out_features;
+  int64_t ld_x, ld_w, ld_y; /* elements between rows of x [tokens], w [out_features] and y [tokens] */
+  int relu;                 /* 1: ReLU after bias */
+} gie_linear_geom;
+
+/* q[t][k] = rint(x[t][k] * (127 / a)), scale[t] = a / 127 with a = max(max_k |x[t][k]|, 2^-100), in FP32 with
+   nearest-even rounding; a row that holds an infinity or a NaN gets scale NaN and q 0. x in `dtype` (FP32, FP16 or
+   BF16, aligned to its element), q rows ld_q >= features bytes apart (bytes past `features` are not written). */
+int gie_hip_quantize_rows(int dtype, const void* x, int64_t ld_x, int tokens, int features, int8_t* q, int64_t ld_q,
+                          float* scale, void* stream);
+
+/* x_scale == NULL: x is in `dtype` and is quantized on the way (gie_hip_quantize_rows into the workspace, or inside
+   the product's own launch for few tokens); otherwise x is int8 with x_scale[tokens]. bias (may be NULL) and y in
+   `dtype` (FP32, FP16, BF16), aligned to their elements; x, w of any alignment and row distance. The workspace (16-byte aligned, at least
+   gie_hip_linear_i8_workspace bytes) is scratch of this call alone. tokens == 0 does nothing. */
+size_t gie_hip_linear_i8_workspace(int dtype, const gie_linear_geom* g, int quantized);
+int gie_hip_linear_i8(int dtype, const gie_linear_geom* g, const void* x, const float* x_scale, const int8_t* w,
+                      const float* w_scale, const void* bias, void* y, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* ---- paged key/value cache (no counterpart in the reference) ----
+   K and V pages: [num_pages][kv_heads][page_size][head_dim], 16-byte aligned. Sequence b owns the rows
+   q_starts[b] .. q_starts[b + 1] - 1 of q, k, v and out (its new tokens) and holds seq_lens[b] tokens with the new ones
+   counted, so new token i stands at position seq_lens[b] - n_b + i. Position p lies in page
+   page_table[b * max_pages + p / page_size], slot p % page_size. The three arrays live on the device; what they hold
+   is bounded by the kernels (rows to [0, total_tokens), positions to max_pages * page_size): a token without a valid
+   position is not stored and its q and out rows are zero, and a page outside [0, num_pages) is neither written nor
+   read (it reads as zeros). */
+typedef struct gie_paged_geom {
+  int batch, total_tokens;
+  int q_heads, kv_heads, head_dim;
+  int page_size, num_pages, max_pages;
+  int64_t q_stride, k_stride, v_stride, o_stride; /* elements between the tokens' rows; heads are head_dim apart */
+  int rotary_dim;    /* leading part of a head that rotates (even, 0: none) */
+  int interleaved;   /* 1: pairs (2j, 2j + 1); 0: pairs (j, j + rotary_dim / 2) */
+  int max_positions; /* rows of the cos / sin tables, at least max_pages * page_size when rotary_dim > 0 */
+  float scale;       /* of the scores */
+  float softcap;     /* > 0: scores become softcap * tanh(score / softcap) */
+  int window;        /* > 0: a token sees its own position and the window - 1 before it */
+  int max_new;       /* most new tokens and longest length of a sequence, as the host knows them (0: not known): */
+  int max_len;       /* they choose the launch shape, no result depends on them */
+} gie_paged_geom;
+
+/* Rotates q and k by their positions (cos, sin: FP32 [max_positions][rotary_dim / 2]), writes q to q_out (o_stride;
+   may be q itself with the same stride) and k, v to their pages. dtype FP16 or BF16. q and q_out may both be NULL. */
+int gie_hip_kv_append(int dtype, const gie_paged_geom* g, const void* q, const void* k, const void* v, const float* cos,
+                      const float* sin, const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
+                      void* k_pages, void* v_pages, void* stream);
+
+/* out[t][h] = sum_j softmax_j(s_j) v_j over the positions j that token t sees, s_j = scale * q[t][h] . k_j (capped);
+   a token that sees nothing gets zeros. FP32 statistics and sums. dtype FP16 or BF16; head_dim 64, 96, 128 or 256;
+   page_size a multiple of 16. The workspace (16-byte aligned) is scratch of this call alone. */
+size_t gie_hip_paged_attention_workspace(const gie_paged_geom* g);
+int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const void* q, const void* k_pages, const void* v_pages,
+                            const int* q_starts, const int* seq_lens, const int* page_table, void* out,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 /* Double-accumulation direct convolution (validation reference for the autotuner and tests):
    y_ref, scale: float[batch*out_channels*out_h*out_w]. dtype may be GIE_HIP_FP32 here. */
 int gie_hip_reference_conv(int dtype, const gie_conv_geom* g, const void* x, const void* w, const void* bias,
