@@ -1,80 +1,637 @@
 // Attention of new tokens over a paged key/value cache:
 //   out[t][h] = sum_j softmax_j(s_j) v_j,  s_j = scale * q[t][h] . k_j  (or softcap * tanh(that / softcap)),
-// over the positions j <= p (and j > p - window) of the token's sequence. One wave for each row (token, head): the keys
-// one after another with the running maximum and sum of the softmax.
+// over the positions j <= p (and j > p - window) of the token's sequence, in one pass over the keys with the running
+// maximum m and sum l of the softmax.
+//
+// Rows. All (token, head) pairs of a sequence that read one key head are rows of one matrix, r = token * group + head in
+// group, so a tile of rows shares every key it reads and one token of a grouped head fills part of a tile instead of a
+// row of it. A workgroup takes RQ * WR * 32 rows of one key head of one sequence, and the z-th part of their keys.
+//
+// Products. Both are 32x32x16 MFMAs with the rows in the columns: S^T = K Q^T leaves a lane 16 scores (keys) of one row
+// for each 32 keys, so maxima and sums are a lane's own but for one exchange between the wave's halves, and the rescaling
+// of O^T = V^T P^T is a product by a lane's own number. The order of the summed keys in the second product is free: it
+// takes keys {4h..4h+3, 8+4h..8+4h+3} of 16 from half h, which is how S^T left them, so P never leaves its registers;
+// V comes out of LDS in that order with ds_read_b64_tr_b16.
+//
+// Keys and values travel HBM -> LDS by direct loads, 16 positions at a time (a page holds a multiple of 16, so they are
+// contiguous), through a buffer resource that ends at the last position anyone sees: what lies behind it, or in a page
+// outside the cache, arrives as zeros. 16-byte chunks of a row are permuted by the row so that the fragment reads meet
+// no bank twice in a phase. The waves of a workgroup either share a tile of keys (WR > 1: one barrier for each tile) or
+// take tiles of their own (WR == 1, WK waves, no barrier until their results are joined).
 #include "paged_common.h"
+
+#include "lds_pipe.h"
 
 namespace gie_hip {
 namespace {
 
-template <typename E, int D>
-__global__ __launch_bounds__(256) void attention_rows_kernel(gie_paged_geom g, const uint16_t* __restrict__ q,
-                                                             const uint16_t* __restrict__ k_pages,
-                                                             const uint16_t* __restrict__ v_pages,
-                                                             const int* __restrict__ q_starts,
-                                                             const int* __restrict__ seq_lens,
-                                                             const int* __restrict__ page_table,
-                                                             uint16_t* __restrict__ out) {
-  constexpr int kPer = (D + 63) / 64;
-  const int lane = int(threadIdx.x) & 63;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (long long)g.total_tokens * g.q_heads) return;
-  const int t = int(row / g.q_heads), h = int(row % g.q_heads);
-  const int b = find_sequence(g.batch, t, [&](int i) { return q_starts[i]; });
-  const Rows rows = sequence_rows(q_starts, b, g.total_tokens);
-  if (t < rows.first || t >= rows.first + rows.count) return;
-  const long long capacity = (long long)g.max_pages * g.page_size;
-  const long long position = (long long)seq_lens[b] - rows.count + (t - rows.first);
-  const int kvh = h / (g.q_heads / g.kv_heads);
-  float qv[kPer], acc[kPer];
-  for (int i = 0; i < kPer; ++i) {
-    const int d = i * 64 + lane;
-    qv[i] = d < D ? E::to_f32(q[t * g.q_stride + h * D + d]) : 0.f;
-    acc[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  const long long last = position < capacity ? position : -1;  // a token without a valid position sees nothing
-  const long long first = g.window > 0 && position - g.window + 1 > 0 ? position - g.window + 1 : 0;
-  for (long long j = first; j <= last; ++j) {
-    const int page = page_table[(long long)b * g.max_pages + j / g.page_size];
-    const bool ok = page >= 0 && page < g.num_pages;
-    const long long at = ((ok ? (long long)page : 0) * g.kv_heads + kvh) * g.page_size * D + (j % g.page_size) * D;
-    float s = 0.f;
-    for (int i = 0; i < kPer; ++i) {
-      const int d = i * 64 + lane;
-      if (d < D) s += qv[i] * (ok ? E::to_f32(k_pages[at + d]) : 0.f);
+typedef __attribute__((address_space(4))) const int const_int;  // uniform loads through the scalar cache
+typedef __attribute__((address_space(3))) u32x4 lds_v4;
+typedef __attribute__((address_space(3))) u32x2 lds_v2;
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+struct AttnArgs {
+  const uint16_t* q;
+  const uint16_t* k_pages;
+  const uint16_t* v_pages;
+  const int* q_starts;
+  const int* seq_lens;
+  const int* page_table;
+  uint16_t* out;
+  float* part;  // splits > 1: [row = token * q_heads + head][split][head_dim + 2]: O, m (in powers of 2), l
+  long long q_stride, o_stride;
+  int batch, total_tokens, q_heads, kv_heads, group;
+  int page16, num_pages, max_pages;  // page16: a page's size in units of 16 positions
+  unsigned page_magic;               // division by page16
+  int page_shift;
+  int capacity;  // max_pages * page_size
+  int window;
+  float mult;      // a score's power of 2: the product times this, or (capped) the capped score times log2(e)
+  float cap_in, cap;  // softcap > 0: cap * tanh(product * cap_in / 2)
+  int negate;      // a negative scale: q changes its sign, so that the largest product is the largest score
+  int splits, chunk;  // parts of the keys and the fewest tiles of one
+  int q_vec, o_vec;   // q in 16-byte pieces, out in 8-byte pieces
+};
+
+template <int D>
+constexpr int kPitch = D == 96 ? 256 : 2 * D;  // bytes of a row in LDS
+
+// permutation of a row's 16-byte chunks: of keys, read as 16 bytes of 16 rows at a time, and of values, read as 64
+// bytes of 4 rows at a time
+template <int D>
+__device__ __forceinline__ int k_swizzle(int row) {
+  return D == 64 ? (row >> 1) & 7 : row & 15;
+}
+template <int D>
+__device__ __forceinline__ int v_swizzle(int row) {
+  return (D == 64 ? (row >> 1) & 1 : row & 3) << 2;
+}
+
+__device__ __forceinline__ int div_magic(int n, unsigned magic, int shift) {
+  return int((__umulhi(unsigned(n), magic) + unsigned(n)) >> shift);
+}
+
+__device__ __forceinline__ float swap_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float swap_add(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// a 16-lane group reads 4 rows of 16 values; each lane gets the 4 rows' values of its column
+__device__ __forceinline__ u32x2 read_transposed(unsigned at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       reinterpret_cast<__attribute__((address_space(3))) v4s*>(size_t(at))));
+}
+
+// bits 15 and 31: whether the lower and the upper half hold an infinity or a NaN (the exponent's ones carry over)
+template <typename E>
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+  constexpr uint32_t mask = E::kDtype == GIE_HIP_FP16 ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t one = E::kDtype == GIE_HIP_FP16 ? 0x04000400u : 0x00800080u;
+  return ((x & mask) + one) & 0x80008000u;
+}
+
+// the part of a sequence's keys that a tile of rows reads, in tiles of TT positions, and its division
+struct KeyRange {
+  int lo, hi;     // positions [lo, hi), lo a multiple of 16
+  int per_split;  // tiles
+  int splits;     // parts that hold any
+};
+template <int TT>
+__device__ __forceinline__ KeyRange key_range(const AttnArgs& a, int pos_first, int pos_last) {
+  KeyRange r;
+  r.hi = min(pos_last + 1, a.capacity);
+  r.lo = a.window > 0 ? max(0, pos_first - a.window + 1) & ~15 : 0;
+  r.lo = min(r.lo, max(r.hi, 0) & ~15);
+  const int tiles = r.hi > r.lo ? (r.hi - r.lo + TT - 1) / TT : 0;
+  r.per_split = max(a.chunk, (tiles + a.splits - 1) / a.splits);
+  r.splits = (tiles + r.per_split - 1) / r.per_split;
+  return r;
+}
+
+// rows of a tile: sequence, its rows of q, position of its first new token; position(r) = base + r / group
+struct RowTile {
+  int seq, first, count, base, row0, rows;  // rows: valid ones from row0 on, <= 0: none
+};
+template <int R>
+__device__ __forceinline__ RowTile row_tile(const AttnArgs& a, int slot) {
+  // sequence b's tiles start at slot floor(q_starts[b] * group / R) + b: as many slots as it can need lie before the next
+  // one's, whatever it holds
+  const auto start = [&](int b) {
+    return int((long long)min(max(a.q_starts[b], 0), a.total_tokens) * a.group / R) + b;
+  };
+  RowTile t;
+  t.seq = find_sequence(a.batch, slot, start);
+  const Rows rows = sequence_rows(a.q_starts, t.seq, a.total_tokens);
+  t.first = __builtin_amdgcn_readfirstlane(rows.first);
+  t.count = __builtin_amdgcn_readfirstlane(rows.count);
+  const int len = __builtin_amdgcn_readfirstlane(a.seq_lens[t.seq]);
+  t.base = int(max((long long)len - t.count, -(1ll << 30)));
+  t.base = min(t.base, 1 << 30);
+  t.row0 = (slot - int((long long)t.first * a.group / R) - t.seq) * R;
+  t.rows = t.row0 >= 0 ? t.count * a.group - t.row0 : 0;
+  return t;
+}
+
+template <typename E, int D, int RQ, int WR, int WK, int NST>
+__global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) {
+  static_assert(WR == 1 || WK == 1, "waves share a tile of keys or have their own");
+  constexpr int R = RQ * WR * 32;             // rows of the workgroup
+  constexpr int TT = WR > 1 ? 16 * WR : 32;   // positions of a tile
+  constexpr int NS = TT / 32;                 // 32-position parts of a tile
+  constexpr int PN = D == 256 ? 1 : NS;       // parts that go through the softmax together
+  constexpr int GR = TT / 16 / WR;            // 16-position granules that a wave loads
+  constexpr int P = kPitch<D>;
+  constexpr int KS = D / 16, DT = D / 32;     // steps of the first product, 32-wide parts of the second
+  constexpr int kGran = 16 * P;               // LDS bytes of a granule
+  constexpr int IPG = kGran / 1024;           // loads of a granule
+  constexpr int kTileB = TT * P;              // of a tile of K or of V
+  constexpr int kStage = 2 * kTileB;
+  constexpr int LPT = 2 * GR * IPG;           // a wave's loads for a tile
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int tid = int(threadIdx.x), lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = WR > 1 ? wave : 0, wk = WR > 1 ? 0 : wave;
+
+  const int kvh = int(blockIdx.x) % a.kv_heads;
+  const int rest = int(blockIdx.x) / a.kv_heads;
+  const int z = rest % a.splits;
+  const RowTile t = row_tile<R>(a, rest / a.splits);
+  if (t.rows <= 0) return;
+  const int last_row = t.row0 + min(t.rows, R) - 1;
+  const int pos_first = t.base + t.row0 / a.group, pos_last = t.base + last_row / a.group;
+  const KeyRange range = key_range<TT>(a, pos_first, pos_last);
+  const int tile_first = z * range.per_split;
+  const bool none = z > 0 && z >= range.splits;
+  if (none) return;  // the join reads as many parts as hold keys
+  const int key0 = range.lo + tile_first * TT;
+  const int key_end = z + 1 < range.splits ? key0 + range.per_split * TT : max(range.hi, key0);
+  const int tiles = (key_end - key0 + TT - 1) / TT;  // of the workgroup; this wave: wk, wk + WK, ...
+
+  // ---- this lane's rows: row (lane & 31) of each of the wave's RQ tiles; rows past the last repeat it ----
+  int pos[RQ];
+  u32x4 qf[RQ][KS];
+  long long row_q[RQ];
+#pragma unroll
+  for (int r = 0; r < RQ; ++r) {
+    const int row = min(t.row0 + (wr * RQ + r) * 32 + (lane & 31), last_row);
+    const int token = row / a.group, head = kvh * a.group + (row - token * a.group);
+    pos[r] = t.base + token;
+    if (pos[r] >= a.capacity) pos[r] = -1;  // no valid position: sees nothing
+    row_q[r] = (long long)(t.first + token) * a.q_heads + head;
+    const uint16_t* src = a.q + (t.first + token) * a.q_stride + head * D;
+    const uint32_t flip = a.negate ? 0x80008000u : 0u;
+    if (a.q_vec) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[r][ks] = *reinterpret_cast<const u32x4*>(src + (2 * ks + half) * 8);
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint16_t* two = src + (2 * ks + half) * 8 + 2 * e;
+          qf[r][ks][e] = uint32_t(two[0]) | (uint32_t(two[1]) << 16);
+        }
     }
-    for (int x = 32; x > 0; x >>= 1) s += __shfl_xor(s, x);
-    s *= g.scale;
-    if (g.softcap > 0) s = g.softcap * tanhf(s / g.softcap);
-    const float m2 = fmaxf(m, s);
-    const float ref = m2 == -INFINITY ? 0.f : m2;  // scores of -infinity weigh nothing, a NaN stays one
-    const float keep = __expf(m - ref);
-    const float p = __expf(s - ref);
-    m = m2;
-    l = l * keep + p;
-    for (int i = 0; i < kPer; ++i) {
-      const int d = i * 64 + lane;
-      acc[i] = acc[i] * keep + (d < D ? p * (ok ? E::to_f32(v_pages[at + d]) : 0.f) : 0.f);
-    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qf[r][ks][e] ^= flip;
   }
-  for (int i = 0; i < kPer; ++i) {
-    const int d = i * 64 + lane;
-    if (d < D) out[t * g.o_stride + h * D + d] = E::from_f32(l == 0.f ? 0.f : acc[i] / l);
+  const int wave_first = min(t.row0 + wr * RQ * 32, last_row), wave_last = min(t.row0 + (wr + 1) * RQ * 32 - 1, last_row);
+  const int wpos_first = t.base + wave_first / a.group, wpos_last = t.base + wave_last / a.group;
+
+  // ---- loads: granule g of a tile, instruction i covers 1024 / P rows ----
+  int k_off[IPG], v_off[IPG];
+#pragma unroll
+  for (int i = 0; i < IPG; ++i) {
+    const int row = i * (1024 / P) + lane / (P / 16), slot = lane % (P / 16);
+    const int kc = slot ^ k_swizzle<D>(row), vc = slot ^ v_swizzle<D>(row);
+    k_off[i] = kc < D / 8 ? row * 2 * D + kc * 16 : kOut;
+    v_off[i] = vc < D / 8 ? row * 2 * D + vc * 16 : kOut;
+  }
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds) + unsigned(wk * NST * kStage));
+  const const_int* table = (const const_int*)(uintptr_t)(a.page_table + (long long)t.seq * a.max_pages);
+  int page[GR], slot16[GR];  // of the granules that the next issue() loads
+  // uniform by construction; readfirstlane states it for the compiler
+  const auto uniform = [](v4i r) {
+    return v4i{__builtin_amdgcn_readfirstlane(r.x), __builtin_amdgcn_readfirstlane(r.y),
+               __builtin_amdgcn_readfirstlane(r.z), __builtin_amdgcn_readfirstlane(r.w)};
+  };
+  const auto look_up = [&](int tile) {
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      const int gran = min((key0 >> 4) + tile * (TT / 16) + (WR > 1 ? wr : g), (a.capacity >> 4) - 1);
+      const int pg = div_magic(gran, a.page_magic, a.page_shift);
+      page[g] = table[__builtin_amdgcn_readfirstlane(pg)];
+      slot16[g] = gran - pg * a.page16;
+    }
+  };
+  const auto issue = [&](int tile, int stage) {
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      const int gi = WR > 1 ? wr : g;
+      const int at = key0 + tile * TT + gi * 16;
+      const bool there = page[g] >= 0 && page[g] < a.num_pages;
+      const int bytes = there ? min(max(key_end - at, 0), 16) * 2 * D : 0;
+      const long long off =
+          (((long long)(there ? page[g] : 0) * a.kv_heads + kvh) * a.page16 + slot16[g]) * (16ll * 2 * D);
+      v4i rk = uniform(make_vsharp(reinterpret_cast<const char*>(a.k_pages) + off, bytes));
+      v4i rv = uniform(make_vsharp(reinterpret_cast<const char*>(a.v_pages) + off, bytes));
+      // a vector instruction may have written these scalar registers: loads may read them 5 cycles later
+      asm volatile("s_nop 4" : "+s"(rk), "+s"(rv));
+      const unsigned to = lds0 + unsigned(stage * kStage + gi * kGran);
+#pragma unroll
+      for (int i = 0; i < IPG; ++i) dma16(rk, to + i * 1024, k_off[i]);
+#pragma unroll
+      for (int i = 0; i < IPG; ++i) dma16(rv, to + kTileB + i * 1024, v_off[i]);
+    }
+  };
+
+  // ---- fragment addresses ----
+  const int sl = lane & 15, g16 = lane >> 4;
+  const unsigned k_rd = lds0 + unsigned((lane & 31) * P + ((half ^ k_swizzle<D>(lane & 15)) << 4));
+  const unsigned v_row = unsigned(4 * half + (sl >> 2));
+  const unsigned v_chunk = unsigned((2 * (g16 & 1) + ((sl & 3) >> 1)) ^ v_swizzle<D>(sl >> 2));
+  const unsigned v_rd = lds0 + unsigned(kTileB) + v_row * P + (v_chunk << 4) + ((sl & 1) << 3);
+
+  f32x16 o[RQ][DT] = {};
+  float m[RQ], mc[RQ], l[RQ];  // running maximum of the products, its power of 2 (0 while there is none), sum
+#pragma unroll
+  for (int r = 0; r < RQ; ++r) m[r] = -INFINITY, mc[r] = 0.f, l[r] = 0.f;
+
+  const auto compute = [&](int tile, int stage) {
+    const unsigned so = unsigned(stage * kStage);
+    const int at0 = key0 + tile * TT;
+    // A value that is not finite must not reach rows that do not see its position (0 times it is a NaN): where rows of
+    // the workgroup see different keys of this tile, such values are added to the rows that see them and replaced by 0.
+    if ((at0 + TT - 1 > pos_first && pos_first != pos_last) || (a.window > 0 && at0 <= pos_last - a.window)) {
+      uint32_t bad = 0;
+      for (int c = lane; c < kTileB / 16; c += 64) {
+        const u32x4 v = *reinterpret_cast<const lds_v4*>(size_t(lds0 + so + unsigned(kTileB + c * 16)));
+        bad |= not_finite<E>(v.x) | not_finite<E>(v.y) | not_finite<E>(v.z) | not_finite<E>(v.w);
+      }
+      if (__any(bad != 0)) {  // the same answer in all waves that share the tile
+        for (int k = 0; k < TT; ++k) {
+          const int key = at0 + k;
+          const unsigned row = lds0 + so + unsigned(kTileB + k * P);
+          uint32_t sees[RQ];
+#pragma unroll
+          for (int r = 0; r < RQ; ++r) sees[r] = key <= pos[r] && (a.window == 0 || key > pos[r] - a.window) ? ~0u : 0u;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int dim = 32 * d + 8 * i + 4 * half;  // 4 of them
+              const u32x2 v = *reinterpret_cast<const lds_v2*>(
+                  size_t(row + unsigned((((dim >> 3) ^ v_swizzle<D>(k)) << 4) + (dim & 4) * 2)));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t word = e < 2 ? v.x : v.y;
+                const uint32_t odd = 0u - ((not_finite<E>(word) >> (e & 1 ? 31 : 15)) & 1u);
+                const uint32_t value = __float_as_uint(E::to_f32(uint16_t(e & 1 ? word >> 16 : word))) & odd;
+#pragma unroll
+                for (int r = 0; r < RQ; ++r) o[r][d][4 * i + e] += __uint_as_float(value & sees[r]);
+              }
+            }
+        }
+        if (WR > 1) stage_barrier();
+        for (int c = (WR > 1 ? tid : lane); c < kTileB / 16; c += WR * 64) {
+          lds_v4* at16 = reinterpret_cast<lds_v4*>(size_t(lds0 + so + unsigned(kTileB + c * 16)));
+          u32x4 v = *at16;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t f = not_finite<E>(v[e]);
+            v[e] &= ~((f >> 15 & 1 ? 0xffffu : 0u) | (f >> 31 ? 0xffff0000u : 0u));
+          }
+          *at16 = v;
+        }
+        if (WR > 1)
+          stage_barrier();
+        else
+          __builtin_amdgcn_s_waitcnt(0xc07f);
+      }
+    }
+
+#pragma unroll
+    for (int n0 = 0; n0 < NS; n0 += PN) {
+      const int at = at0 + n0 * 32;
+      const unsigned ko = k_rd + so, vo = v_rd + so;
+      // scores: part n holds keys at + 32 n + 8 (i / 4) + 4 half + i % 4 in register i
+      f32x16 s[RQ][PN];
+#pragma unroll
+      for (int n = 0; n < PN; ++n) {
+#pragma unroll
+        for (int r = 0; r < RQ; ++r) s[r][n] = f32x16{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const u32x4 kf = *reinterpret_cast<const lds_v4*>(size_t((ko ^ unsigned(ks * 32)) + unsigned((n0 + n) * 32 * P)));
+#pragma unroll
+          for (int r = 0; r < RQ; ++r) s[r][n] = E::mfma32(kf, qf[r][ks], s[r][n]);
+        }
+      }
+      if (a.cap > 0) {
+#pragma unroll
+        for (int r = 0; r < RQ; ++r)
+#pragma unroll
+          for (int n = 0; n < PN; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float e = __builtin_amdgcn_exp2f(s[r][n][i] * a.cap_in);
+              s[r][n][i] = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(e + 1.f);
+            }
+      }
+      if (at + PN * 32 - 1 > wpos_first || (a.window > 0 && at <= wpos_last - a.window) || wpos_last >= a.capacity) {
+#pragma unroll
+        for (int r = 0; r < RQ; ++r) {
+          const int oldest = a.window > 0 ? pos[r] - a.window : -1;
+#pragma unroll
+          for (int n = 0; n < PN; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int key = at + n * 32 + 8 * (i / 4) + 4 * half + i % 4;
+              s[r][n][i] = key <= pos[r] && key > oldest ? s[r][n][i] : -INFINITY;
+            }
+        }
+      }
+      u32x4 pf[RQ][2 * PN];
+#pragma unroll
+      for (int r = 0; r < RQ; ++r) {
+        float top = s[r][0][0];
+#pragma unroll
+        for (int n = 0; n < PN; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, s[r][n][i]);
+        top = swap_max(top);
+        // the maximum follows only when a weight would pass 2^8: sums and weights keep their relative precision, and
+        // most tiles leave O as it is
+        if (__any((top - m[r]) * a.mult > 8.f)) {
+          const float next = fmaxf(m[r], top);
+          const float nc = next == -INFINITY ? 0.f : next * a.mult;
+          const float keep = m[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc[r] - nc);  // 1: nothing summed yet
+          m[r] = next;
+          mc[r] = nc;
+          l[r] *= keep;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[r][d] *= keep;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < PN; ++n) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            s[r][n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][n][i], a.mult, -mc[r]));
+            sum += s[r][n][i];
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            pf[r][2 * n + i] =
+                u32x4{E::pack2(s[r][n][8 * i], s[r][n][8 * i + 1]), E::pack2(s[r][n][8 * i + 2], s[r][n][8 * i + 3]),
+                      E::pack2(s[r][n][8 * i + 4], s[r][n][8 * i + 5]), E::pack2(s[r][n][8 * i + 6], s[r][n][8 * i + 7])};
+        }
+        l[r] += sum;
+      }
+#pragma unroll
+      for (int n = 0; n < 2 * PN; ++n) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const unsigned p = (vo ^ unsigned(d * 64)) + unsigned((2 * n0 + n) * 16 * P);
+          const u32x2 x = read_transposed(p), y = read_transposed(p + unsigned(8 * P));
+          const u32x4 vf = u32x4{x.x, x.y, y.x, y.y};
+#pragma unroll
+          for (int r = 0; r < RQ; ++r) o[r][d] = E::mfma32(vf, pf[r][n], o[r][d]);
+        }
+      }
+    }
+  };
+
+  // ---- main loop: a wave's j-th tile from stage j % NST while the next NST - 1 load. Loads past the last tile read
+  // nothing and write zeros, so that every wait counts the same ----
+  const int mine = WR > 1 ? tiles : (tiles - wk + WK - 1) / WK;
+  const auto tile_at = [&](int j) { return WR > 1 ? j : wk + j * WK; };
+  look_up(tile_at(0));
+#pragma unroll
+  for (int j = 0; j < NST - 1; ++j) {
+    issue(tile_at(j), j);
+    look_up(tile_at(j + 1));
+  }
+  int stage = 0;
+  for (int j = 0; j < mine; ++j) {
+    wait_vm<(NST - 2) * LPT>();
+    if (WR > 1)
+      stage_barrier();
+    else
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's reads of the stage that is loaded next are done: lgkmcnt(0)
+    issue(tile_at(j + NST - 1), stage == 0 ? NST - 1 : stage - 1);
+    look_up(tile_at(j + NST));
+    compute(tile_at(j), stage);
+    stage = stage + 1 == NST ? 0 : stage + 1;
+  }
+  wait_vm<0>();
+
+#pragma unroll
+  for (int r = 0; r < RQ; ++r) l[r] = swap_add(l[r]);
+
+  // ---- the waves' parts of the keys ----
+  if constexpr (WK > 1) {
+    static_assert(RQ == 1, "one tile of rows for each wave that has keys of its own");
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(lds);  // [wave][32] m, l; then [wave][32 rows][D + 4]
+    if (half == 0) {
+      sums[(wave * 32 + lane) * 2] = m[0] == -INFINITY ? -INFINITY : mc[0];
+      sums[(wave * 32 + lane) * 2 + 1] = l[0];
+    }
+    __syncthreads();
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) top = fmaxf(top, sums[(w * 32 + (lane & 31)) * 2]);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      const float other = sums[(w * 32 + (lane & 31)) * 2];
+      // a wave without a maximum may hold a NaN all the same
+      total += sums[(w * 32 + (lane & 31)) * 2 + 1] * __builtin_amdgcn_exp2f(other == -INFINITY ? 0.f : other - ref);
+    }
+    const float keep = __builtin_amdgcn_exp2f(m[0] == -INFINITY ? 0.f : mc[0] - ref);
+    constexpr int kRow = D + 4;
+    float* mine_o = reinterpret_cast<float*>(lds + WK * 256) + (wave * 32 + (lane & 31)) * kRow;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(mine_o + 32 * d + 8 * i + 4 * half) =
+            f32x4{o[0][d][4 * i], o[0][d][4 * i + 1], o[0][d][4 * i + 2], o[0][d][4 * i + 3]} * keep;
+    // row (tid & 31) of the sums: every wave joins a part of the values
+    m[0] = top;
+    mc[0] = ref;
+    l[0] = total;
+    __syncthreads();
+    const float* all = reinterpret_cast<const float*>(lds + WK * 256);
+    const int row = lane & 31;
+    if (row < t.rows) {
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      for (int d = (wave * 2 + half) * 4; d < D; d += WK * 8) {
+        f32x4 v = {};
+#pragma unroll
+        for (int w = 0; w < WK; ++w) v += *reinterpret_cast<const f32x4*>(all + (w * 32 + row) * kRow + d);
+        if (range.splits > 1) {
+          float* dst = a.part + (row_q[0] * a.splits + z) * (D + 4);
+          *reinterpret_cast<f32x4*>(dst + d) = v;
+          if (d == 0) dst[D] = top, dst[D + 1] = total;
+        } else {
+          const int head = int(row_q[0] % a.q_heads);
+          uint16_t* dst = a.out + (row_q[0] / a.q_heads) * a.o_stride + head * D + d;
+          if (total == 0.f) v = f32x4{};
+          v *= inv;
+          if (a.o_vec) {
+            *reinterpret_cast<u32x2*>(dst) = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dst[e] = E::from_f32(v[e]);
+          }
+        }
+      }
+    }
+    return;
+  }
+
+  // ---- rows to out, or to the parts that are joined ----
+#pragma unroll
+  for (int r = 0; r < RQ; ++r) {
+    const int row = (wr * RQ + r) * 32 + (lane & 31);
+    if (row >= t.rows) continue;
+    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+    const int head = int(row_q[r] % a.q_heads);
+    float* part = a.part + (row_q[r] * a.splits + z) * (D + 4);
+    uint16_t* dst = a.out + (row_q[r] / a.q_heads) * a.o_stride + head * D;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int dim = 32 * d + 8 * i + 4 * half;
+        f32x4 v = {o[r][d][4 * i], o[r][d][4 * i + 1], o[r][d][4 * i + 2], o[r][d][4 * i + 3]};
+        if (range.splits > 1) {
+          *reinterpret_cast<f32x4*>(part + dim) = v;
+          if (dim == 0) part[D] = m[r] == -INFINITY ? -INFINITY : mc[r], part[D + 1] = l[r];
+        } else {
+          if (l[r] == 0.f) v = f32x4{};
+          v *= inv;
+          if (a.o_vec) {
+            *reinterpret_cast<u32x2*>(dst + dim) = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dst[dim + e] = E::from_f32(v[e]);
+          }
+        }
+      }
   }
 }
 
-template <typename E>
-int launch(const gie_paged_geom& g, const void* q, const void* k, const void* v, const int* q_starts,
-           const int* seq_lens, const int* page_table, void* out, hipStream_t s) {
-  const auto kernel = g.head_dim == 64    ? attention_rows_kernel<E, 64>
-                      : g.head_dim == 96  ? attention_rows_kernel<E, 96>
-                      : g.head_dim == 128 ? attention_rows_kernel<E, 128>
-                                          : attention_rows_kernel<E, 256>;
-  const long long rows = (long long)g.total_tokens * g.q_heads;
-  hipLaunchKernelGGL(kernel, dim3(unsigned((rows + 3) / 4)), dim3(256), 0, s, g, static_cast<const uint16_t*>(q),
-                     static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), q_starts, seq_lens, page_table,
-                     static_cast<uint16_t*>(out));
+// Joins the parts of the keys: one wave for each row (token, head), lanes over the head's values.
+template <typename E, int D, int R, int TT>
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+  constexpr int kPer = (D + 63) / 64;
+  const int lane = int(threadIdx.x) & 63;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (long long)a.total_tokens * a.q_heads) return;
+  const int token = int(row / a.q_heads), head = int(row % a.q_heads);
+  const int seq = find_sequence(a.batch, token, [&](int b) { return a.q_starts[b]; });
+  const Rows rows = sequence_rows(a.q_starts, seq, a.total_tokens);
+  if (token < rows.first || token >= rows.first + rows.count) return;
+  const int slot = int((long long)rows.first * a.group / R) + seq +
+                   ((token - rows.first) * a.group + head % a.group) / R;
+  const RowTile t = row_tile<R>(a, slot);
+  const int last_row = t.row0 + min(t.rows, R) - 1;
+  const KeyRange range = key_range<TT>(a, t.base + t.row0 / a.group, t.base + last_row / a.group);
+  if (range.splits <= 1) return;  // written already
+  const float* part = a.part + row * a.splits * (D + 4);
+  float top = -INFINITY;
+  for (int z = 0; z < range.splits; ++z) top = fmaxf(top, part[z * (D + 4) + D]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float total = 0.f, v[kPer] = {};
+  for (int z = 0; z < range.splits; ++z) {
+    const float* p = part + z * (D + 4);
+    const float keep = __builtin_amdgcn_exp2f(p[D] == -INFINITY ? 0.f : p[D] - ref);
+    total += p[D + 1] * keep;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i * 64 + lane < D) v[i] += p[i * 64 + lane] * keep;
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (i * 64 + lane < D)
+      a.out[token * a.o_stride + head * D + i * 64 + lane] = E::from_f32(total == 0.f ? 0.f : v[i] * inv);
+}
+
+// ---- launch shape: the same on both sides of the workspace query ----
+struct Shape {
+  bool wide;  // rows of a workgroup: 256 that share tiles of 64 keys, or 32 with keys of their own for each wave
+  int slots, splits, chunk;
+};
+
+constexpr int kNarrowRows = 32;
+// 64 rows for each wave halve the LDS reads of a product; at head_dim 256 their sums would not fit the registers
+template <int D>
+constexpr int kWideTiles = D == 256 ? 1 : 2;
+constexpr int wide_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
+
+Shape shape_of(const gie_paged_geom& g) {
+  Shape s;
+  const int group = g.q_heads / g.kv_heads;
+  const long long rows = (long long)g.total_tokens * group;
+  const int most_new = g.max_new > 0 ? g.max_new : (g.total_tokens + g.batch - 1) / g.batch;
+  s.wide = (long long)most_new * group > kNarrowRows;
+  const int R = s.wide ? wide_rows(g.head_dim) : kNarrowRows, tt = s.wide ? 64 : 32;
+  s.slots = int(rows / R) + g.batch;
+  // tiles of rows that hold any, about
+  const long long busy = (rows + R - 1) / R > g.batch ? (rows + R - 1) / R : g.batch;
+  long long len = (long long)g.max_pages * g.page_size;
+  if (g.max_len > 0 && g.max_len < len) len = g.max_len;
+  if (g.window > 0 && (long long)g.window + most_new < len) len = g.window + most_new;
+  const long long tiles = (len + tt - 1) / tt;
+  const long long blocks = busy * g.kv_heads;
+  const int fewest = s.wide ? 4 : 8;  // tiles of a part: below that the join costs more than it gives
+  const long long want = 2 * 256 / blocks;
+  long long splits = want < tiles / fewest ? want : tiles / fewest;
+  if (splits < 1) splits = 1;
+  s.chunk = int((tiles + splits - 1) / splits);
+  s.splits = int((tiles + s.chunk - 1) / s.chunk);
+  return s;
+}
+
+template <typename K>
+int start(K kernel, int grid, int threads, int lds_bytes, hipStream_t stream, const AttnArgs& a) {
+  const int rc = set_lds_limit(reinterpret_cast<const void*>(kernel), lds_bytes);
+  if (rc != GIE_HIP_OK) return rc;
+  hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(unsigned(threads)), unsigned(lds_bytes), stream, a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? GIE_HIP_OK : int(e);
+}
+
+template <typename E, int D>
+int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
+  const long long grid = (long long)s.slots * s.splits * a.kv_heads;
+  if (grid > 0x7fffffff) return GIE_HIP_EINVAL;
+  constexpr int P = kPitch<D>;
+  int rc;
+  if (s.wide) {
+    constexpr int NST = 2;
+    rc = start(attention_kernel<E, D, kWideTiles<D>, 4, 1, NST>, int(grid), 256, NST * 2 * 64 * P, stream, a);
+  } else {
+    constexpr int WK = D == 256 ? 2 : 4, NST = D == 64 ? 4 : 2;
+    constexpr int bytes = WK * NST * 2 * 32 * P, join = WK * 256 + WK * 32 * (D + 4) * 4;
+    rc = start(attention_kernel<E, D, 1, 1, WK, NST>, int(grid), 64 * WK, bytes > join ? bytes : join, stream, a);
+  }
+  if (rc != GIE_HIP_OK || s.splits == 1) return rc;
+  const long long rows = (long long)a.total_tokens * a.q_heads;
+  if (s.wide)
+    hipLaunchKernelGGL((join_kernel<E, D, wide_rows(D), 64>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((join_kernel<E, D, kNarrowRows, 32>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, stream, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? GIE_HIP_OK : int(e);
 }
@@ -84,7 +641,12 @@ int launch(const gie_paged_geom& g, const void* q, const void* k, const void* v,
 
 using namespace gie_hip;
 
-extern "C" size_t gie_hip_paged_attention_workspace(const gie_paged_geom* g) { return 0; }
+extern "C" size_t gie_hip_paged_attention_workspace(const gie_paged_geom* g) {
+  if (!valid_paged(g) || g->total_tokens == 0) return 0;
+  const Shape s = shape_of(*g);
+  if (s.splits == 1) return 0;
+  return size_t(g->total_tokens) * g->q_heads * s.splits * (g->head_dim + 4) * sizeof(float);
+}
 
 extern "C" int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const void* q, const void* k_pages,
                                        const void* v_pages, const int* q_starts, const int* seq_lens,
@@ -97,7 +659,56 @@ extern "C" int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const
   if (!q || !k_pages || !v_pages || !q_starts || !seq_lens || !page_table || !out || q == out) return GIE_HIP_EINVAL;
   if (!aligned_to(q, 2) || !aligned_to(out, 2) || !aligned_to(k_pages, 16) || !aligned_to(v_pages, 16))
     return GIE_HIP_EINVAL;
+  const size_t need = gie_hip_paged_attention_workspace(g);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))) return GIE_HIP_EINVAL;
+  const Shape shape = shape_of(*g);
+  AttnArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k_pages = static_cast<const uint16_t*>(k_pages);
+  a.v_pages = static_cast<const uint16_t*>(v_pages);
+  a.q_starts = q_starts;
+  a.seq_lens = seq_lens;
+  a.page_table = page_table;
+  a.out = static_cast<uint16_t*>(out);
+  a.part = static_cast<float*>(workspace);
+  a.q_stride = g->q_stride;
+  a.o_stride = g->o_stride;
+  a.batch = g->batch;
+  a.total_tokens = g->total_tokens;
+  a.q_heads = g->q_heads;
+  a.kv_heads = g->kv_heads;
+  a.group = g->q_heads / g->kv_heads;
+  a.page16 = g->page_size / 16;
+  a.num_pages = g->num_pages;
+  a.max_pages = g->max_pages;
+  // n / page16 = (umulhi(n, magic) + n) >> shift for n < 2^31: shift = ceil(log2(page16)), magic = 2^32 (2^shift /
+  // page16 - 1), rounded up
+  int shift = 0;
+  while ((1ll << shift) < a.page16) ++shift;
+  a.page_shift = shift;
+  a.page_magic = unsigned(((((1ull << shift) - unsigned(a.page16)) << 32) / unsigned(a.page16)) + 1);
+  a.capacity = g->max_pages * g->page_size;
+  a.window = g->window;
+  constexpr float kLog2E = 1.44269504088896341f;
+  const float scale = g->scale < 0 ? -g->scale : g->scale;
+  a.negate = g->scale < 0;
+  if (g->softcap > 0) {
+    a.mult = kLog2E;
+    a.cap = g->softcap;
+    a.cap_in = 2.f * kLog2E * (scale / g->softcap);  // tanh(x) = 1 - 2 / (2^(2 log2(e) x) + 1)
+  } else {
+    a.mult = scale * kLog2E;
+  }
+  a.splits = shape.splits;
+  a.chunk = shape.chunk;
+  a.q_vec = g->q_stride % 8 == 0 && aligned_to(q, 16);
+  a.o_vec = g->o_stride % 4 == 0 && aligned_to(out, 8);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == GIE_HIP_FP16 ? launch<Fp16>(*g, q, k_pages, v_pages, q_starts, seq_lens, page_table, out, s)
-                               : launch<Bf16>(*g, q, k_pages, v_pages, q_starts, seq_lens, page_table, out, s);
+  const bool h = dtype == GIE_HIP_FP16;
+  switch (g->head_dim) {
+    case 64: return h ? launch<Fp16, 64>(a, shape, s) : launch<Bf16, 64>(a, shape, s);
+    case 96: return h ? launch<Fp16, 96>(a, shape, s) : launch<Bf16, 96>(a, shape, s);
+    case 128: return h ? launch<Fp16, 128>(a, shape, s) : launch<Bf16, 128>(a, shape, s);
+    default: return h ? launch<Fp16, 256>(a, shape, s) : launch<Bf16, 256>(a, shape, s);
+  }
 }
