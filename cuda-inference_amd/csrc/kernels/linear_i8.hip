@@ -1,39 +1,509 @@
 // Matrix product in 8-bit integers with scales for each token and output channel:
 //   y[t][n] = round(relu?(float(sum_k q[t][k] w[n][k]) * (x_scale[t] * w_scale[n]) + bias[n]))
+// The sum runs on the i8 matrix cores into int32 (exact in any order); scales, bias and the one rounding in FP32.
+//
+// Three forms, by the number of tokens:
+//   * few tokens (<= 16): the weights' one pass through memory is all there is. A workgroup owns 16 output channels and
+//     its 8 waves take every 8th step of 64 input values of them, straight from memory into the operands of
+//     16x16x64 MFMAs; their sums meet in LDS. Where x is not in 8 bits yet and short enough, every workgroup quantizes it for
+//     itself, which costs less than a launch before this one.
+//   * tiles: BM tokens x BN channels, 128 input values of each in LDS at a time, two stages (loads of the next slice run
+//     under the products of this one), 4 waves of 32x32x32 MFMAs. Channels are the rows of a product and tokens its
+//     columns, so a lane holds 4 neighbouring channels of one token; the finished tile goes through LDS and out in
+//     whole rows. Rows of 128 bytes with their 16-byte chunks permuted by the row meet no LDS bank twice.
+//   * tiles over parts of the input values, where there are too few of them to fill the device: int32 partial sums
+//     in the workspace and a second launch that joins them (integers: the order does not matter).
 #include "quantize_common.h"
+
+#include "lds_pipe.h"
 
 namespace gie_hip {
 namespace {
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) u32x4 lds_v4;
+typedef __attribute__((address_space(3))) f32x4 lds_f4;
+typedef __attribute__((address_space(3))) float lds_f;
+
+struct LinArgs {
+  const int8_t* x;
+  const float* x_scale;
+  const int8_t* w;
+  const float* w_scale;
+  const void* bias;
+  void* y;
+  int* part;        // splits > 1: [split][tokens][out_features]
+  const void* x16;  // few tokens: x before its quantization, or null
+  long long ld_x, ld_w, ld_y;
+  int M, N, K;
+  int relu;
+  int splits, per_split;  // parts of the input values, and their steps of 128
+  int tiles_m, tiles_n;
+  int y_vec;  // rows of y in 16-byte pieces
+};
+
 template <typename E>
-__global__ __launch_bounds__(256) void linear_i8_kernel(const int8_t* __restrict__ x, const float* __restrict__ x_scale,
-                                                        const int8_t* __restrict__ w, const float* __restrict__ w_scale,
-                                                        const void* __restrict__ bias, void* __restrict__ y,
-                                                        gie_linear_geom g) {
-  const int n = int(blockIdx.x) * 64 + int(threadIdx.x & 63);
-  const long long t = (long long)blockIdx.y * 4 + (threadIdx.x >> 6);
-  if (n >= g.out_features || t >= g.tokens) return;
-  int acc = 0;
-  for (int k = 0; k < g.in_features; ++k) acc += int(x[t * g.ld_x + k]) * int(w[n * g.ld_w + k]);
-  float v = float(acc) * (x_scale[t] * w_scale[n]);  // the scales first: acc times a large one could pass FP32
-  if (bias != nullptr) v += load_value<E>(bias, n);
-  if (g.relu) v = v < 0.f ? 0.f : v;  // a NaN stays
-  store_value<E>(y, t * g.ld_y + n, v);
+constexpr int kBytesOf = 2;
+template <>
+constexpr int kBytesOf<F32> = 4;
+
+__device__ __forceinline__ u32x4 load16(const int8_t* p) {  // any alignment
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+// values k .. k + 15 of a row, zeros from K on; nothing behind the row's end is read
+__device__ __forceinline__ u32x4 load16_upto(const int8_t* row, int k, int K) {
+  if (k + 16 <= K) return load16(row + k);
+  u32x4 v = {};
+  for (int i = 0; i < 16; ++i)
+    if (k + i < K) v[i / 4] |= uint32_t(uint8_t(row[k + i])) << (8 * (i % 4));
+  return v;
 }
 
+__device__ __forceinline__ float finish(int acc, float scale, float w_scale, float bias, int relu) {
+  float v = float(acc) * (scale * w_scale);  // the scales first: acc times a large one could pass FP32
+  v += bias;
+  return relu && v < 0.f ? 0.f : v;  // a NaN stays
+}
+
+template <typename E>
+__device__ __forceinline__ float bias_at(const void* bias, int n) {
+  return bias != nullptr ? load_value<E>(bias, n) : 0.f;
+}
+
+// ---------------------------------------------------------------------------------------------- tiles
+template <typename E, int BM, int BN, int WM, int WN, bool ALIGNED>
+__global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(LinArgs a) {
+  constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32x32 products of a wave
+  constexpr int kRows = BM + BN, kStage = kRows * 128;
+  constexpr int IPW = kRows / 8 / kWaves;  // loads of 8 rows for each wave
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int tid = int(threadIdx.x), lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+
+  // tile: workgroup L runs on XCD L % 8, which takes a run of neighbouring tiles: 4 of tokens for each of channels, so
+  // that those which run together share rows of x and w in its L2
+  int tm, tn;
+  {
+    const int total = a.tiles_m * a.tiles_n;
+    const int L = int(blockIdx.x), xcd = L & 7;
+    const int lo = total / 8, more = total % 8;
+    const int id = xcd * lo + min(xcd, more) + (L >> 3);
+    const int group = 4 * a.tiles_n, first = id / group * 4, high = min(4, a.tiles_m - first);
+    tm = first + id % group % high;
+    tn = id % group / high;
+  }
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int k_first = int(blockIdx.y) * a.per_split * 128;
+  const int k_last = min(a.K, k_first + a.per_split * 128);
+  const int steps = (k_last - k_first + 127) / 128;
+
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds));
+  i32x16 acc[TN][TM] = {};
+
+  // ---- loads: instruction i of the wave covers rows 8 (wave IPW + i) .. + 7 of the stage, x first ----
+  const int r0 = lane >> 3;
+  const int chunk_even = (lane & 7) ^ (r0 >> 1), chunk_odd = chunk_even ^ 4;
+  const auto uniform = [](v4i r) {
+    return v4i{__builtin_amdgcn_readfirstlane(r.x), __builtin_amdgcn_readfirstlane(r.y),
+               __builtin_amdgcn_readfirstlane(r.z), __builtin_amdgcn_readfirstlane(r.w)};
+  };
+  const auto issue = [&](int step, int stage) {
+    const int k0 = k_first + step * 128, left = k_last - k0;
+    // bytes to the end of the last row, its last 16-byte piece whole (it holds a byte of the row, and a piece of 16 lies
+    // in one page): the hardware would drop a word that passes the end
+    const long long rx = (long long)(min(BM, a.M - m0) - 1) * a.ld_x + ((left + 15) & ~15);
+    const long long rw = (long long)(min(BN, a.N - n0) - 1) * a.ld_w + ((left + 15) & ~15);
+    v4i sx = uniform(make_vsharp(a.x + m0 * a.ld_x + k0, int(rx)));
+    v4i sw = uniform(make_vsharp(a.w + n0 * a.ld_w + k0, int(rw)));
+    // a vector instruction may have written these scalar registers: loads may read them 5 cycles later
+    asm volatile("s_nop 4" : "+s"(sx), "+s"(sw));
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) {
+      const int at = wave * IPW + i;  // uniform
+      const bool is_x = at < BM / 8;
+      const int row = (is_x ? at : at - BM / 8) * 8 + r0;
+      const int chunk = at & 1 ? chunk_odd : chunk_even;
+      const int off = chunk * 16 < left ? row * int(is_x ? a.ld_x : a.ld_w) + chunk * 16 : kOut;
+      if (is_x)
+        dma16(sx, lds0 + unsigned(stage * kStage + at * 1024), off);
+      else
+        dma16(sw, lds0 + unsigned(stage * kStage + at * 1024), off);
+    }
+  };
+  // rows of any alignment: 16 bytes for each thread and round through registers
+  constexpr int kRounds = kRows * 8 / kThreads;
+  u32x4 held[ALIGNED ? 1 : kRounds];
+  const auto fetch = [&](int step) {
+    const int k0 = k_first + step * 128;
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int c = i * kThreads + tid, row = c >> 3, k = k0 + (c & 7) * 16;
+      const bool is_x = row < BM;
+      const int r = is_x ? m0 + row : n0 + row - BM;
+      u32x4 v = {};
+      if (r < (is_x ? a.M : a.N) && k < k_last)
+        v = load16_upto(is_x ? a.x + r * a.ld_x : a.w + r * a.ld_w, k, k_last);
+      held[i] = v;
+    }
+  };
+  const auto put = [&](int stage) {
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int c = i * kThreads + tid, row = c >> 3, slot = (c & 7) ^ ((row >> 1) & 7);
+      *reinterpret_cast<lds_v4*>(size_t(lds0 + unsigned(stage * kStage + row * 128 + slot * 16))) = held[i];
+    }
+  };
+
+  // ---- fragments: lane row (lane & 31), 16 bytes at 32 ks + 16 half ----
+  const unsigned swz = unsigned((half ^ ((lane >> 1) & 7)) << 4);
+  const unsigned x_rd = lds0 + unsigned((wm * TM * 32 + (lane & 31)) * 128) + swz;
+  const unsigned w_rd = lds0 + unsigned((BM + wn * TN * 32 + (lane & 31)) * 128) + swz;
+  const auto compute = [&](int stage) {
+    const unsigned so = unsigned(stage * kStage);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      u32x4 xf[TM], wf[TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+        xf[i] = *reinterpret_cast<const lds_v4*>(size_t(((x_rd + so) ^ unsigned(ks * 32)) + unsigned(i * 32 * 128)));
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+        wf[i] = *reinterpret_cast<const lds_v4*>(size_t(((w_rd + so) ^ unsigned(ks * 32)) + unsigned(i * 32 * 128)));
+#pragma unroll
+      for (int n = 0; n < TN; ++n)
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+          acc[n][m] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, wf[n]),
+                                                            __builtin_bit_cast(i32x4, xf[m]), acc[n][m], 0, 0, 0);
+    }
+  };
+  // a 16-byte chunk that the row ends in holds bytes of what lies behind it: they are cleared in x, so what w holds there
+  // does not matter
+  const auto clear_tail = [&](int stage) {
+    const int left = (k_last - k_first) % 128, bytes = left % 16;
+    if (bytes == 0) return;
+    for (int row = tid; row < BM; row += kThreads) {
+      const int slot = (left >> 4) ^ ((row >> 1) & 7);
+      lds_v4* at = reinterpret_cast<lds_v4*>(size_t(lds0 + unsigned(stage * kStage + row * 128 + slot * 16)));
+      u32x4 v = *at;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int keep = min(max(bytes - 4 * e, 0), 4);
+        v[e] &= keep == 4 ? ~0u : (1u << (8 * keep)) - 1u;
+      }
+      *at = v;
+    }
+    stage_barrier();
+  };
+
+  if constexpr (ALIGNED) {
+    issue(0, 0);
+    for (int s = 0; s < steps; ++s) {
+      wait_vm<0>();
+      stage_barrier();
+      if (s + 1 < steps)
+        issue(s + 1, (s + 1) & 1);
+      else
+        clear_tail(s & 1);
+      compute(s & 1);
+    }
+  } else {
+    fetch(0);
+    for (int s = 0; s < steps; ++s) {
+      put(s & 1);
+      __syncthreads();
+      if (s + 1 < steps) fetch(s + 1);
+      compute(s & 1);
+    }
+  }
+  __syncthreads();
+
+  // ---- 32 tokens at a time through the wave's own part of LDS, then out in rows ----
+  if (a.splits > 1) {
+    int* part = a.part + (long long)blockIdx.y * a.M * a.N;
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+      const int t = m0 + (wm * TM + m) * 32 + (lane & 31);
+      if (t >= a.M) continue;
+#pragma unroll
+      for (int n = 0; n < TN; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int c = n0 + (wn * TN + n) * 32 + 8 * g + 4 * half;
+          int* dst = part + (long long)t * a.N + c;
+          if (a.N % 4 == 0 && c < a.N) {
+            *reinterpret_cast<i32x4*>(dst) =
+                i32x4{acc[n][m][4 * g], acc[n][m][4 * g + 1], acc[n][m][4 * g + 2], acc[n][m][4 * g + 3]};
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c + e < a.N) dst[e] = acc[n][m][4 * g + e];
+          }
+        }
+    }
+    return;
+  }
+  constexpr int kE = kBytesOf<E>, kRowB = TN * 32 * kE, kPad = kRowB + 16;
+  const unsigned tile = lds0 + unsigned(wave * 32 * kPad);
+  const unsigned scales = lds0 + unsigned(kWaves * 32 * kPad);  // of the tile's channels, and their biases behind them
+  for (int c = tid; c < BN; c += kThreads) {
+    const int n = min(n0 + c, a.N - 1);
+    *reinterpret_cast<lds_f*>(size_t(scales + c * 4)) = a.w_scale[n];
+    *reinterpret_cast<lds_f*>(size_t(scales + (BN + c) * 4)) = bias_at<E>(a.bias, n);
+  }
+  __syncthreads();
+  const int c0 = n0 + wn * TN * 32;  // the wave's first channel
+  const unsigned mine = scales + unsigned((wn * TN * 32 + 4 * half) * 4);
+#pragma unroll
+  for (int m = 0; m < TM; ++m) {
+    const int t0 = m0 + (wm * TM + m) * 32;
+    if (t0 >= a.M) break;
+    const float xs = a.x_scale[min(t0 + (lane & 31), a.M - 1)];
+#pragma unroll
+    for (int n = 0; n < TN; ++n) {
+      asm volatile("" ::: "memory");  // a part's sums at a time: all of them at once would not fit the registers
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int col = n * 32 + 8 * g;
+        const f32x4 ws = *reinterpret_cast<const lds_f4*>(size_t(mine + col * 4));
+        const f32x4 bs = *reinterpret_cast<const lds_f4*>(size_t(mine + (BN + col) * 4));
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = finish(acc[n][m][4 * g + e], xs, ws[e], bs[e], a.relu);
+        const unsigned at = tile + unsigned((lane & 31) * kPad + (col + 4 * half) * kE);
+        if constexpr (kE == 4)
+          *reinterpret_cast<lds_v4*>(size_t(at)) =
+              u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+        else
+          *reinterpret_cast<__attribute__((address_space(3))) u32x2*>(size_t(at)) =
+              u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // the wave's own writes
+    constexpr int kLanesRow = kRowB / 16, kRowsIt = 64 / kLanesRow > 0 ? 64 / kLanesRow : 1;
+    static_assert(kLanesRow <= 64, "a row fits one instruction");
+#pragma unroll 4
+    for (int r = 0; r < 32; r += kRowsIt) {
+      const int row = r + lane / kLanesRow, piece = lane % kLanesRow;
+      const int t = t0 + row, c = c0 + piece * (16 / kE);
+      const u32x4 v = *reinterpret_cast<const lds_v4*>(size_t(tile + unsigned(row * kPad + piece * 16)));
+      if (t >= a.M) continue;
+      char* dst = static_cast<char*>(a.y) + (t * a.ld_y + c) * kE;
+      if (a.y_vec && c + 16 / kE <= a.N) {
+        *reinterpret_cast<u32x4*>(dst) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16 / kE; ++e) {
+          if (c + e >= a.N) break;
+          if constexpr (kE == 4)
+            reinterpret_cast<uint32_t*>(dst)[e] = v[e];
+          else
+            reinterpret_cast<uint16_t*>(dst)[e] = uint16_t(v[e / 2] >> (16 * (e & 1)));
+        }
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- join
+template <typename E>
+__global__ __launch_bounds__(256) void join_kernel(LinArgs a) {
+  const long long total = (long long)a.M * a.N, pieces = (total + 3) / 4;
+  for (long long p = (long long)blockIdx.x * 256 + threadIdx.x; p < pieces; p += (long long)gridDim.x * 256) {
+    const long long i = p * 4;
+    const bool whole = a.N % 4 == 0;
+    int acc[4] = {};
+    for (int z = 0; z < a.splits; ++z) {
+      const int* src = a.part + z * total + i;
+      if (whole) {
+        const i32x4 v = *reinterpret_cast<const i32x4*>(src);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + e < total) acc[e] += src[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (i + e >= total) break;
+      const long long t = (i + e) / a.N;
+      const int n = int((i + e) - t * a.N);
+      store_value<E>(a.y, t * a.ld_y + n,
+                     finish(acc[e], a.x_scale[t], a.w_scale[n], bias_at<E>(a.bias, n), a.relu));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- few tokens
+constexpr int kFew = 16, kFewWaves = 8, kFewThreads = 64 * kFewWaves;
+
+// FUSED: x16 is quantized here, into LDS; otherwise x is read as the weights are
+template <typename E, bool FUSED>
+__global__ __launch_bounds__(kFewThreads) void few_kernel(LinArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  __shared__ i32x4 sums[kFewWaves][64];
+  __shared__ float scales[kFew];
+  const int tid = int(threadIdx.x), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = int(blockIdx.x) * 16;
+  const int row = lane & 15, part = (lane >> 4) * 16;
+  const int K16 = (a.K + 15) & ~15;
+  const int8_t* w = a.w + min(n0 + row, a.N - 1) * a.ld_w;
+  const int token = min(row, a.M - 1);
+  const int8_t* x = FUSED ? reinterpret_cast<const int8_t*>(lds) + token * K16 : a.x + token * a.ld_x;
+  const int steps = (a.K + 63) / 64;
+  constexpr int U = 8;  // steps in flight
+  u32x4 wf[U];
+  const auto load_w = [&](int s) {
+    const int k = s * 64 + part;
+    return s < steps && k < a.K ? load16_upto(w, k, a.K) : u32x4{};
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) wf[u] = load_w(wave + u * kFewWaves);
+  if constexpr (FUSED) {
+    for (int t = 0; t < a.M; ++t) {
+      float most = 0.f;
+      for (int k = tid; k < a.K; k += kFewThreads) most = magnitude_max(most, load_value<E>(a.x16, t * a.ld_x + k));
+      most = block_magnitude_max<kFewThreads>(most);
+      const RowScale s = row_scale(most);
+      if (tid == 0) scales[t] = s.scale;
+      for (int k = tid; k < K16; k += kFewThreads)
+        lds[t * K16 + k] = k < a.K ? uint8_t(quantize_value(load_value<E>(a.x16, t * a.ld_x + k), s.inverse)) : 0;
+      __syncthreads();
+    }
+  }
+  i32x4 acc = {};
+  for (int s0 = wave; s0 < steps; s0 += U * kFewWaves) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * kFewWaves;
+      if (s >= steps) break;
+      const int k = s * 64 + part;
+      u32x4 xf = {};
+      if (k < a.K) {
+        if constexpr (FUSED)
+          xf = *reinterpret_cast<const u32x4*>(x + k);
+        else
+          xf = load16_upto(x, k, a.K);
+      }
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wf[u]), __builtin_bit_cast(i32x4, xf), acc, 0,
+                                                  0, 0);
+      wf[u] = load_w(s + U * kFewWaves);
+    }
+  }
+  sums[wave][lane] = acc;
+  __syncthreads();
+  if (tid < 64) {
+#pragma unroll
+    for (int v = 1; v < kFewWaves; ++v) acc += sums[v][lane];
+    if (row < a.M) {
+      const float xs = FUSED ? scales[row] : a.x_scale[row];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = n0 + (lane >> 4) * 4 + e;
+        if (n < a.N)
+          store_value<E>(a.y, row * a.ld_y + n, finish(acc[e], xs, a.w_scale[n], bias_at<E>(a.bias, n), a.relu));
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
-
-template <typename E>
-void launch(const gie_linear_geom& g, const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale,
-            const void* bias, void* y, hipStream_t s) {
-  hipLaunchKernelGGL(linear_i8_kernel<E>, dim3((g.out_features + 63) / 64, (g.tokens + 3) / 4), dim3(256), 0, s, x,
-                     x_scale, w, w_scale, bias, y, g);
-}
 
 bool valid(int dtype, const gie_linear_geom* g) {
   return g && (dtype == GIE_HIP_FP32 || dtype == GIE_HIP_FP16 || dtype == GIE_HIP_BF16) && g->tokens >= 0 &&
          g->in_features > 0 && g->in_features <= 131071 && g->out_features > 0 && g->ld_x >= g->in_features &&
          g->ld_w >= g->in_features && g->ld_y >= g->out_features;
+}
+
+enum Form { kFewForm, kTile32, kTile64, kTile128, kTile256 };
+struct Plan {
+  Form form;
+  int bm, bn, tiles_m, tiles_n, splits, per_split;
+};
+
+Plan plan_of(const gie_linear_geom& g) {
+  Plan p{};
+  const int M = g.tokens, N = g.out_features, steps = (g.in_features + 127) / 128;
+  const auto tiles = [&](int b, int n) { return (n + b - 1) / b; };
+  p.splits = 1;
+  if (M <= kFew) {
+    p.form = kFewForm;
+  } else if (M <= 32) {
+    p.form = kTile32, p.bm = 32, p.bn = 128;
+  } else if (M <= 64) {
+    p.form = kTile64, p.bm = 64, p.bn = 128;
+  } else if ((long long)tiles(256, M) * tiles(256, N) >= 192) {
+    p.form = kTile256, p.bm = 256, p.bn = 256;
+  } else {
+    p.form = kTile128, p.bm = 128, p.bn = 128;
+  }
+  p.per_split = steps;
+  if (p.form == kFewForm) return p;
+  p.tiles_m = tiles(p.bm, M);
+  p.tiles_n = tiles(p.bn, N);
+  const long long count = (long long)p.tiles_m * p.tiles_n;
+  // at least 4 steps for a part, and no more parts than fill the device once
+  const long long want = count >= 256 ? 1 : 256 / count, most = steps / 4 > 0 ? steps / 4 : 1;
+  const int splits = int(want < most ? want : most);
+  p.per_split = (steps + splits - 1) / splits;
+  p.splits = (steps + p.per_split - 1) / p.per_split;
+  return p;
+}
+
+bool fuses(const gie_linear_geom& g) { return g.tokens <= 4 && (long long)g.tokens * g.in_features <= 32 * 1024; }
+
+template <typename E, int BM, int BN, int WM, int WN>
+int run_tiles(const LinArgs& a, bool aligned, hipStream_t s) {
+  constexpr int kStages = 2 * (BM + BN) * 128;
+  constexpr int kOutB = WM * WN * 32 * (BN / WN * kBytesOf<E> + 16) + BN * 8;
+  constexpr int bytes = kStages > kOutB ? kStages : kOutB;
+  auto kernel = tile_kernel<E, BM, BN, WM, WN, true>;
+  if constexpr (BM < 256)
+    if (!aligned) kernel = tile_kernel<E, BM, BN, WM, WN, false>;
+  const int rc = set_lds_limit(reinterpret_cast<const void*>(kernel), bytes);
+  if (rc != GIE_HIP_OK) return rc;
+  hipLaunchKernelGGL(kernel, dim3(unsigned(a.tiles_m * a.tiles_n), unsigned(a.splits)), dim3(64 * WM * WN), bytes, s, a);
+  return GIE_HIP_OK;
+}
+
+template <typename E>
+int run(const Plan& p, const LinArgs& a, bool aligned, hipStream_t s) {
+  int rc = GIE_HIP_OK;
+  switch (p.form) {
+    case kFewForm: {
+      const int bytes = a.x16 ? a.M * int(round16(a.K)) : 0;
+      const dim3 grid((a.N + 15) / 16);
+      if (a.x16)
+        hipLaunchKernelGGL((few_kernel<E, true>), grid, dim3(kFewThreads), bytes, s, a);
+      else
+        hipLaunchKernelGGL((few_kernel<E, false>), grid, dim3(kFewThreads), 0, s, a);
+      break;
+    }
+    case kTile32: rc = run_tiles<E, 32, 128, 1, 4>(a, aligned, s); break;
+    case kTile64: rc = run_tiles<E, 64, 128, 1, 4>(a, aligned, s); break;
+    case kTile128: rc = run_tiles<E, 128, 128, 2, 2>(a, aligned, s); break;
+    case kTile256:
+      rc = aligned ? run_tiles<E, 256, 256, 2, 4>(a, true, s) : run_tiles<E, 128, 128, 2, 2>(a, false, s);
+      break;
+  }
+  if (rc != GIE_HIP_OK) return rc;
+  if (a.splits > 1) {
+    const long long pieces = ((long long)a.M * a.N + 3) / 4;
+    const long long blocks = (pieces + 255) / 256;
+    hipLaunchKernelGGL(join_kernel<E>, dim3(unsigned(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, a);
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? GIE_HIP_OK : int(e);
 }
 
 }  // namespace
@@ -42,8 +512,12 @@ bool valid(int dtype, const gie_linear_geom* g) {
 using namespace gie_hip;
 
 extern "C" size_t gie_hip_linear_i8_workspace(int dtype, const gie_linear_geom* g, int quantized) {
-  if (!valid(dtype, g) || quantized) return 0;
-  return round16(size_t(g->tokens) * round16(g->in_features)) + round16(size_t(g->tokens) * 4);
+  if (!valid(dtype, g) || g->tokens == 0) return 0;
+  const Plan p = plan_of(*g);
+  size_t n = p.splits > 1 ? round16(size_t(p.splits) * g->tokens * g->out_features * 4) : 0;
+  if (!quantized && !(p.form == kFewForm && fuses(*g)))
+    n += round16(size_t(g->tokens) * round16(g->in_features)) + round16(size_t(g->tokens) * 4);
+  return n;
 }
 
 extern "C" int gie_hip_linear_i8(int dtype, const gie_linear_geom* g, const void* x, const float* x_scale,
@@ -53,31 +527,61 @@ extern "C" int gie_hip_linear_i8(int dtype, const gie_linear_geom* g, const void
   if (g->tokens == 0) return GIE_HIP_OK;
   if (!x || !w || !w_scale || !y || x == y) return GIE_HIP_EINVAL;
   const size_t esz = dtype == GIE_HIP_FP32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(y) % esz != 0 || reinterpret_cast<uintptr_t>(bias) % esz != 0 ||
-      reinterpret_cast<uintptr_t>(w_scale) % 4 != 0 || reinterpret_cast<uintptr_t>(x_scale) % 4 != 0)
+  const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  if (at(y) % esz != 0 || at(bias) % esz != 0 || at(w_scale) % 4 != 0 || at(x_scale) % 4 != 0 ||
+      (x_scale == nullptr && at(x) % esz != 0))
     return GIE_HIP_EINVAL;
   const size_t need = gie_hip_linear_i8_workspace(dtype, g, x_scale != nullptr);
-  if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
-    return GIE_HIP_EINVAL;
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  gie_linear_geom gg = *g;
-  const int8_t* xq = static_cast<const int8_t*>(x);
-  if (x_scale == nullptr) {
-    int8_t* q = static_cast<int8_t*>(workspace);
-    const size_t ld = round16(g->in_features);
-    float* scale = reinterpret_cast<float*>(q + round16(g->tokens * ld));
-    const int rc = gie_hip_quantize_rows(dtype, x, g->ld_x, g->tokens, g->in_features, q, ld, scale, stream);
-    if (rc != GIE_HIP_OK) return rc;
-    xq = q;
-    x_scale = scale;
-    gg.ld_x = int64_t(ld);
+  if (need > 0 && (!workspace || workspace_bytes < need || at(workspace) % 16 != 0)) return GIE_HIP_EINVAL;
+  const Plan p = plan_of(*g);
+  LinArgs a{};
+  a.x = static_cast<const int8_t*>(x);
+  a.x_scale = x_scale;
+  a.w = w;
+  a.w_scale = w_scale;
+  a.bias = bias;
+  a.y = y;
+  a.ld_x = g->ld_x;
+  a.ld_w = g->ld_w;
+  a.ld_y = g->ld_y;
+  a.M = g->tokens;
+  a.N = g->out_features;
+  a.K = g->in_features;
+  a.relu = g->relu ? 1 : 0;
+  a.splits = p.splits;
+  a.per_split = p.per_split;
+  char* ws = static_cast<char*>(workspace);
+  if (p.splits > 1) {
+    a.part = reinterpret_cast<int*>(ws);
+    ws += round16(size_t(p.splits) * g->tokens * g->out_features * 4);
   }
-  if (dtype == GIE_HIP_FP32)
-    launch<F32>(gg, xq, x_scale, w, w_scale, bias, y, s);
-  else if (dtype == GIE_HIP_FP16)
-    launch<Fp16>(gg, xq, x_scale, w, w_scale, bias, y, s);
-  else
-    launch<Bf16>(gg, xq, x_scale, w, w_scale, bias, y, s);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? GIE_HIP_OK : int(e);
+  if (x_scale == nullptr) {
+    if (p.form == kFewForm && fuses(*g)) {
+      a.x16 = x;
+    } else {
+      const size_t ld = round16(g->in_features);
+      int8_t* q = reinterpret_cast<int8_t*>(ws);
+      float* scale = reinterpret_cast<float*>(ws + round16(size_t(g->tokens) * ld));
+      const int rc = gie_hip_quantize_rows(dtype, x, g->ld_x, g->tokens, g->in_features, q, int64_t(ld), scale, stream);
+      if (rc != GIE_HIP_OK) return rc;
+      a.x = q;
+      a.x_scale = scale;
+      a.ld_x = int64_t(ld);
+    }
+  }
+  // direct loads into LDS take 16-byte pieces, and reach a tile's last row with a 32-bit offset
+  const bool aligned = a.ld_x % 16 == 0 && a.ld_w % 16 == 0 && at(a.x) % 16 == 0 && at(w) % 16 == 0 &&
+                       a.ld_x < (1 << 22) && a.ld_w < (1 << 22);
+  const int bm = p.form == kTile256 && !aligned ? 128 : p.bm, bn = p.form == kTile256 && !aligned ? 128 : p.bn;
+  if (p.form != kFewForm) {
+    const long long tm = (g->tokens + bm - 1) / bm, tn = (g->out_features + bn - 1) / bn;
+    if (tm * tn > 0x7fffffff) return GIE_HIP_EINVAL;
+    a.tiles_m = int(tm);
+    a.tiles_n = int(tn);
+  }
+  a.y_vec = g->ld_y * esz % 16 == 0 && at(y) % 16 == 0;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == GIE_HIP_FP32) return run<F32>(p, a, aligned, s);
+  if (dtype == GIE_HIP_FP16) return run<Fp16>(p, a, aligned, s);
+  return run<Bf16>(p, a, aligned, s);
 }

@@ -6,7 +6,9 @@
 
 namespace gie_hip {
 
-struct F32 {};  // 4-byte storage, no conversion
+struct F32 {  // 4-byte storage, no conversion
+  static constexpr int kDtype = GIE_HIP_FP32;
+};
 
 template <typename E>
 __device__ __forceinline__ float load_value(const void* p, long long i) {

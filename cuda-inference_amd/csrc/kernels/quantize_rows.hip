@@ -1,33 +1,91 @@
 // Quantization of activations to 8 bits with one scale for each token (row):
 //   a = max(max_k |x_k|, 2^-100), scale = a / 127, q_k = rint(x_k * (127 / a))
 // in FP32 with nearest-even rounding; a row that holds an infinity or a NaN gets scale NaN and q 0, so that what is
-// computed from it is NaN as well. HBM-bound: the row is read once from HBM and a second time from the cache.
+// computed from it is NaN as well. HBM-bound: a row is read once, in 16-byte pieces that its threads keep in
+// registers between the maximum and the rounding; what passes the registers is read a second time from the cache.
+// A wave takes a row of up to 2048 bytes (four rows for each workgroup), a workgroup a longer one.
 #include "quantize_common.h"
 
 namespace gie_hip {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kKeep = 4;
 
 template <typename E>
-__global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* __restrict__ x, long long ld_x,
+__device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = E::to_f32(uint16_t(v[e / 2] >> (16 * (e & 1))));
+}
+template <>
+__device__ __forceinline__ void unpack<F32>(u32x4 v, float (&f)[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[e]);
+}
+
+// T threads for each row. kVec: rows of x in 16-byte pieces, rows of q in the pieces that these become
+template <typename E, int T, bool kVec>
+__global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* __restrict__ x, long long ld_x, int tokens,
                                                                  int features, int8_t* __restrict__ q, long long ld_q,
                                                                  float* __restrict__ scale) {
-  const long long row = blockIdx.x;
-  const long long x0 = row * ld_x;
+  constexpr int kE = E::kDtype == GIE_HIP_FP32 ? 4 : 2, kPer = 16 / kE;
+  const long long row = (long long)blockIdx.x * (kThreads / T) + threadIdx.x / T;
+  const bool there = row < tokens;  // a wave without a row still meets the others' barriers
+  const int me = int(threadIdx.x) % T;
+  const long long x0 = there ? row * ld_x : 0;
+  const int pieces = kVec && there ? features / kPer : 0;  // whole ones; the rest value by value
+  const int rest = there ? pieces * kPer : features;
+  const u32x4* xv = reinterpret_cast<const u32x4*>(static_cast<const char*>(x) + x0 * kE);
   float a = 0;
-  for (int k = threadIdx.x; k < features; k += kThreads) a = magnitude_max(a, load_value<E>(x, x0 + k));
-  a = block_magnitude_max<kThreads>(a);
+  u32x4 keep[kKeep];
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) keep[i] = i * T + me < pieces ? xv[i * T + me] : u32x4{};
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    float f[8];
+    unpack<E>(keep[i], f);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) a = magnitude_max(a, f[e]);
+  }
+  for (int p = kKeep * T + me; p < pieces; p += T) {
+    float f[8];
+    unpack<E>(xv[p], f);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) a = magnitude_max(a, f[e]);
+  }
+  for (int k = rest + me; k < features; k += T) a = magnitude_max(a, load_value<E>(x, x0 + k));
+  a = T == 64 ? wave_magnitude_max(a) : block_magnitude_max<kThreads>(a);
   const RowScale s = row_scale(a);
-  if (threadIdx.x == 0) scale[row] = s.scale;
-  for (int k = threadIdx.x; k < features; k += kThreads)
-    q[row * ld_q + k] = quantize_value(load_value<E>(x, x0 + k), s.inverse);
+  if (me == 0 && there) scale[row] = s.scale;
+  int8_t* out = q + (there ? row * ld_q : 0);
+  const auto put = [&](int p, u32x4 v) {
+    float f[8];
+    unpack<E>(v, f);
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) w[e / 4] |= uint32_t(uint8_t(quantize_value(f[e], s.inverse))) << (8 * (e & 3));
+    if constexpr (kPer == 8)
+      reinterpret_cast<u32x2*>(out)[p] = u32x2{w[0], w[1]};
+    else
+      reinterpret_cast<uint32_t*>(out)[p] = w[0];
+  };
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i)
+    if (i * T + me < pieces) put(i * T + me, keep[i]);
+  for (int p = kKeep * T + me; p < pieces; p += T) put(p, xv[p]);
+  for (int k = rest + me; k < features; k += T) out[k] = quantize_value(load_value<E>(x, x0 + k), s.inverse);
 }
 
 template <typename E>
-void launch(const void* x, long long ld_x, int tokens, int features, int8_t* q, long long ld_q, float* scale,
+void launch(const void* x, long long ld_x, int tokens, int features, int8_t* q, long long ld_q, float* scale, bool vec,
             hipStream_t s) {
-  hipLaunchKernelGGL(quantize_rows_kernel<E>, dim3(tokens), dim3(kThreads), 0, s, x, ld_x, features, q, ld_q, scale);
+  constexpr int kE = E::kDtype == GIE_HIP_FP32 ? 4 : 2;
+  if (features * kE <= 64 * 16 * 2) {
+    const auto kernel = vec ? quantize_rows_kernel<E, 64, true> : quantize_rows_kernel<E, 64, false>;
+    hipLaunchKernelGGL(kernel, dim3((tokens + 3) / 4), dim3(kThreads), 0, s, x, ld_x, tokens, features, q, ld_q, scale);
+  } else {
+    const auto kernel = vec ? quantize_rows_kernel<E, kThreads, true> : quantize_rows_kernel<E, kThreads, false>;
+    hipLaunchKernelGGL(kernel, dim3(tokens), dim3(kThreads), 0, s, x, ld_x, tokens, features, q, ld_q, scale);
+  }
 }
 
 }  // namespace
@@ -42,13 +100,15 @@ extern "C" int gie_hip_quantize_rows(int dtype, const void* x, int64_t ld_x, int
   if (!x || !q || !scale) return GIE_HIP_EINVAL;
   const size_t esz = dtype == GIE_HIP_FP32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(x) % esz != 0 || reinterpret_cast<uintptr_t>(scale) % 4 != 0) return GIE_HIP_EINVAL;
+  const bool vec = ld_x * esz % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_q % (16 / esz) == 0 &&
+                   reinterpret_cast<uintptr_t>(q) % (16 / esz) == 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == GIE_HIP_FP32)
-    launch<F32>(x, ld_x, tokens, features, q, ld_q, scale, s);
+    launch<F32>(x, ld_x, tokens, features, q, ld_q, scale, vec, s);
   else if (dtype == GIE_HIP_FP16)
-    launch<Fp16>(x, ld_x, tokens, features, q, ld_q, scale, s);
+    launch<Fp16>(x, ld_x, tokens, features, q, ld_q, scale, vec, s);
   else if (dtype == GIE_HIP_BF16)
-    launch<Bf16>(x, ld_x, tokens, features, q, ld_q, scale, s);
+    launch<Bf16>(x, ld_x, tokens, features, q, ld_q, scale, vec, s);
   else
     return GIE_HIP_EUNSUPPORTED;
   const hipError_t e = hipGetLastError();
