@@ -112,27 +112,22 @@ __device__ __forceinline__ KeyRange key_range(const AttnArgs& a, int pos_first, 
   return r;
 }
 
-// rows of a tile: sequence, its rows of q, position of its first new token; position(r) = base + r / group
+// rows of a tile: its sequence, the first of its rows; position(r) = seq.base + r / group
 struct RowTile {
-  int seq, first, count, base, row0, rows;  // rows: valid ones from row0 on, <= 0: none
+  Sequence seq;
+  int row0, rows;  // rows: valid ones from row0 on, <= 0: none
 };
 template <int R>
 __device__ __forceinline__ RowTile row_tile(const AttnArgs& a, int slot) {
   // sequence b's tiles start at slot floor(q_starts[b] * group / R) + b: as many slots as it can need lie before the next
   // one's, whatever it holds
-  const auto start = [&](int b) {
-    return int((long long)min(max(a.q_starts[b], 0), a.total_tokens) * a.group / R) + b;
+  const auto start = [&](int first, int b) {
+    return int((long long)min(max(first, 0), a.total_tokens) * a.group / R) + b;
   };
   RowTile t;
-  t.seq = find_sequence(a.batch, slot, start);
-  const Rows rows = sequence_rows(a.q_starts, t.seq, a.total_tokens);
-  t.first = __builtin_amdgcn_readfirstlane(rows.first);
-  t.count = __builtin_amdgcn_readfirstlane(rows.count);
-  const int len = __builtin_amdgcn_readfirstlane(a.seq_lens[t.seq]);
-  t.base = int(max((long long)len - t.count, -(1ll << 30)));
-  t.base = min(t.base, 1 << 30);
-  t.row0 = (slot - int((long long)t.first * a.group / R) - t.seq) * R;
-  t.rows = t.row0 >= 0 ? t.count * a.group - t.row0 : 0;
+  t.seq = locate(a.q_starts, a.seq_lens, a.batch, a.total_tokens, slot, start);
+  t.row0 = (slot - start(t.seq.first, t.seq.index)) * R;
+  t.rows = t.row0 >= 0 ? t.seq.count * a.group - t.row0 : 0;
   return t;
 }
 
@@ -142,7 +137,7 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
   constexpr int R = RQ * WR * 32;             // rows of the workgroup
   constexpr int TT = WR > 1 ? 16 * WR : 32;   // positions of a tile
   constexpr int NS = TT / 32;                 // 32-position parts of a tile
-  constexpr int PN = D == 256 ? 1 : NS;       // parts that go through the softmax together
+  constexpr int PN = D == 256 || NS < 2 || WR == 8 ? 1 : 2;  // parts that go through the softmax together
   constexpr int GR = TT / 16 / WR;            // 16-position granules that a wave loads
   constexpr int P = kPitch<D>;
   constexpr int KS = D / 16, DT = D / 32;     // steps of the first product, 32-wide parts of the second
@@ -156,13 +151,16 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = WR > 1 ? wave : 0, wk = WR > 1 ? 0 : wave;
 
-  const int kvh = int(blockIdx.x) % a.kv_heads;
-  const int rest = int(blockIdx.x) / a.kv_heads;
+  // neighbouring workgroups take different key heads, so that one head's keys stay in one XCD's L2; the last rows of a
+  // sequence, which see the most keys, go first
+  const int id = int(gridDim.x) - 1 - int(blockIdx.x);
+  const int kvh = id % a.kv_heads;
+  const int rest = id / a.kv_heads;
   const int z = rest % a.splits;
   const RowTile t = row_tile<R>(a, rest / a.splits);
   if (t.rows <= 0) return;
   const int last_row = t.row0 + min(t.rows, R) - 1;
-  const int pos_first = t.base + t.row0 / a.group, pos_last = t.base + last_row / a.group;
+  const int pos_first = t.seq.base + t.row0 / a.group, pos_last = t.seq.base + last_row / a.group;
   const KeyRange range = key_range<TT>(a, pos_first, pos_last);
   const int tile_first = z * range.per_split;
   const bool none = z > 0 && z >= range.splits;
@@ -179,10 +177,10 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
   for (int r = 0; r < RQ; ++r) {
     const int row = min(t.row0 + (wr * RQ + r) * 32 + (lane & 31), last_row);
     const int token = row / a.group, head = kvh * a.group + (row - token * a.group);
-    pos[r] = t.base + token;
+    pos[r] = t.seq.base + token;
     if (pos[r] >= a.capacity) pos[r] = -1;  // no valid position: sees nothing
-    row_q[r] = (long long)(t.first + token) * a.q_heads + head;
-    const uint16_t* src = a.q + (t.first + token) * a.q_stride + head * D;
+    row_q[r] = (long long)(t.seq.first + token) * a.q_heads + head;
+    const uint16_t* src = a.q + (t.seq.first + token) * a.q_stride + head * D;
     const uint32_t flip = a.negate ? 0x80008000u : 0u;
     if (a.q_vec) {
 #pragma unroll
@@ -202,19 +200,20 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
       for (int e = 0; e < 4; ++e) qf[r][ks][e] ^= flip;
   }
   const int wave_first = min(t.row0 + wr * RQ * 32, last_row), wave_last = min(t.row0 + (wr + 1) * RQ * 32 - 1, last_row);
-  const int wpos_first = t.base + wave_first / a.group, wpos_last = t.base + wave_last / a.group;
+  const int wpos_first = t.seq.base + wave_first / a.group, wpos_last = t.seq.base + wave_last / a.group;
 
   // ---- loads: granule g of a tile, instruction i covers 1024 / P rows ----
-  int k_off[IPG], v_off[IPG];
+  constexpr int RI = 1024 / P, VP = RI < 4 ? 4 / RI : 1;  // rows of a load; loads after which V's permutation repeats
+  int k_off[IPG], v_off[VP];
 #pragma unroll
   for (int i = 0; i < IPG; ++i) {
-    const int row = i * (1024 / P) + lane / (P / 16), slot = lane % (P / 16);
+    const int row = i * RI + lane / (P / 16), slot = lane % (P / 16);
     const int kc = slot ^ k_swizzle<D>(row), vc = slot ^ v_swizzle<D>(row);
     k_off[i] = kc < D / 8 ? row * 2 * D + kc * 16 : kOut;
-    v_off[i] = vc < D / 8 ? row * 2 * D + vc * 16 : kOut;
+    if (i < VP) v_off[i] = vc < D / 8 ? row * 2 * D + vc * 16 : kOut;
   }
   const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds) + unsigned(wk * NST * kStage));
-  const const_int* table = (const const_int*)(uintptr_t)(a.page_table + (long long)t.seq * a.max_pages);
+  const const_int* table = (const const_int*)(uintptr_t)(a.page_table + (long long)t.seq.index * a.max_pages);
   int page[GR], slot16[GR];  // of the granules that the next issue() loads
   // uniform by construction; readfirstlane states it for the compiler
   const auto uniform = [](v4i r) {
@@ -247,7 +246,7 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
 #pragma unroll
       for (int i = 0; i < IPG; ++i) dma16(rk, to + i * 1024, k_off[i]);
 #pragma unroll
-      for (int i = 0; i < IPG; ++i) dma16(rv, to + kTileB + i * 1024, v_off[i]);
+      for (int i = 0; i < IPG; ++i) dma16(rv, to + kTileB + i * 1024, v_off[i % VP] + i / VP * VP * RI * 2 * D);
     }
   };
 
@@ -530,41 +529,56 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
   }
 }
 
-// Joins the parts of the keys: one wave for each row (token, head), lanes over the head's values.
+// Joins the parts of the keys: a workgroup for each row (token, head), lanes over the head's values 4 at a time, the
+// parts dealt out to what the values leave of it.
 template <typename E, int D, int R, int TT>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
-  constexpr int kPer = (D + 63) / 64;
-  const int lane = int(threadIdx.x) & 63;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (long long)a.total_tokens * a.q_heads) return;
+  constexpr int kLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, kGroups = 256 / kLanes;
+  __shared__ f32x4 sums[kGroups][kLanes];
+  const int tid = int(threadIdx.x), lane = tid & 63;
+  const long long row = blockIdx.x;
   const int token = int(row / a.q_heads), head = int(row % a.q_heads);
-  const int seq = find_sequence(a.batch, token, [&](int b) { return a.q_starts[b]; });
-  const Rows rows = sequence_rows(a.q_starts, seq, a.total_tokens);
-  if (token < rows.first || token >= rows.first + rows.count) return;
-  const int slot = int((long long)rows.first * a.group / R) + seq +
-                   ((token - rows.first) * a.group + head % a.group) / R;
-  const RowTile t = row_tile<R>(a, slot);
-  const int last_row = t.row0 + min(t.rows, R) - 1;
-  const KeyRange range = key_range<TT>(a, t.base + t.row0 / a.group, t.base + last_row / a.group);
-  if (range.splits <= 1) return;  // written already
   const float* part = a.part + row * a.splits * (D + 4);
+  const Sequence seq =
+      locate(a.q_starts, a.seq_lens, a.batch, a.total_tokens, token, [](int first, int) { return first; });
+  if (token < seq.first || token >= seq.first + seq.count) return;
+  const int row0 = ((token - seq.first) * a.group + head % a.group) / R * R;
+  const int last_row = min(row0 + R, seq.count * a.group) - 1;
+  const int splits = key_range<TT>(a, seq.base + row0 / a.group, seq.base + last_row / a.group).splits;
+  if (splits <= 1) return;  // written already
   float top = -INFINITY;
-  for (int z = 0; z < range.splits; ++z) top = fmaxf(top, part[z * (D + 4) + D]);
+  for (int z = lane; z < splits; z += 64) top = fmaxf(top, part[z * (D + 4) + D]);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   const float ref = top == -INFINITY ? 0.f : top;
-  float total = 0.f, v[kPer] = {};
-  for (int z = 0; z < range.splits; ++z) {
-    const float* p = part + z * (D + 4);
-    const float keep = __builtin_amdgcn_exp2f(p[D] == -INFINITY ? 0.f : p[D] - ref);
-    total += p[D + 1] * keep;
+  // a part without a maximum weighs 1: it holds zeros, or a NaN that has to stay
+  const auto weight = [&](float m) { return m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - ref); };
+  float total = 0.f;
+  for (int z = lane; z < splits; z += 64) total += part[z * (D + 4) + D + 1] * weight(part[z * (D + 4) + D]);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (i * 64 + lane < D) v[i] += p[i * 64 + lane] * keep;
+  for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d);
+  const int at = tid % kLanes, group = tid / kLanes;
+  f32x4 v = {};
+  if (at * 4 < D) {
+#pragma unroll 4
+    for (int z = group; z < splits; z += kGroups)
+      v += *reinterpret_cast<const f32x4*>(part + z * (D + 4) + at * 4) * weight(part[z * (D + 4) + D]);
   }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
+  sums[group][at] = v;
+  __syncthreads();
+  if (group != 0 || at * 4 >= D) return;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (i * 64 + lane < D)
-      a.out[token * a.o_stride + head * D + i * 64 + lane] = E::from_f32(total == 0.f ? 0.f : v[i] * inv);
+  for (int g = 1; g < kGroups; ++g) v += sums[g][at];
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  uint16_t* dst = a.out + token * a.o_stride + head * D + at * 4;
+  if (total == 0.f) v = f32x4{};
+  v *= inv;
+  if (a.o_vec) {
+    *reinterpret_cast<u32x2*>(dst) = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dst[e] = E::from_f32(v[e]);
+  }
 }
 
 // ---- launch shape: the same on both sides of the workspace query ----
@@ -577,7 +591,8 @@ constexpr int kNarrowRows = 32;
 // 64 rows for each wave halve the LDS reads of a product; at head_dim 256 their sums would not fit the registers
 template <int D>
 constexpr int kWideTiles = D == 256 ? 1 : 2;
-constexpr int wide_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
+constexpr int wide_waves(int head_dim) { return head_dim == 256 ? 4 : 8; }
+constexpr int wide_rows(int head_dim) { return 32 * wide_waves(head_dim); }
 
 Shape shape_of(const gie_paged_geom& g) {
   Shape s;
@@ -585,7 +600,7 @@ Shape shape_of(const gie_paged_geom& g) {
   const long long rows = (long long)g.total_tokens * group;
   const int most_new = g.max_new > 0 ? g.max_new : (g.total_tokens + g.batch - 1) / g.batch;
   s.wide = (long long)most_new * group > kNarrowRows;
-  const int R = s.wide ? wide_rows(g.head_dim) : kNarrowRows, tt = s.wide ? 64 : 32;
+  const int R = s.wide ? wide_rows(g.head_dim) : kNarrowRows, tt = s.wide ? 16 * wide_waves(g.head_dim) : 32;
   s.slots = int(rows / R) + g.batch;
   // tiles of rows that hold any, about
   const long long busy = (rows + R - 1) / R > g.batch ? (rows + R - 1) / R : g.batch;
@@ -595,7 +610,7 @@ Shape shape_of(const gie_paged_geom& g) {
   const long long tiles = (len + tt - 1) / tt;
   const long long blocks = busy * g.kv_heads;
   const int fewest = s.wide ? 4 : 8;  // tiles of a part: below that the join costs more than it gives
-  const long long want = 2 * 256 / blocks;
+  const long long want = 256 / blocks;
   long long splits = want < tiles / fewest ? want : tiles / fewest;
   if (splits < 1) splits = 1;
   s.chunk = int((tiles + splits - 1) / splits);
@@ -620,7 +635,7 @@ int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   int rc;
   if (s.wide) {
     constexpr int NST = 2;
-    rc = start(attention_kernel<E, D, kWideTiles<D>, 4, 1, NST>, int(grid), 256, NST * 2 * 64 * P, stream, a);
+    rc = start(attention_kernel<E, D, 1, wide_waves(D), 1, NST>, int(grid), 64 * wide_waves(D), NST * 2 * 16 * wide_waves(D) * P, stream, a);
   } else {
     constexpr int WK = D == 256 ? 2 : 4, NST = D == 64 ? 4 : 2;
     constexpr int bytes = WK * NST * 2 * 32 * P, join = WK * 256 + WK * 32 * (D + 4) * 4;
@@ -629,9 +644,9 @@ int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   if (rc != GIE_HIP_OK || s.splits == 1) return rc;
   const long long rows = (long long)a.total_tokens * a.q_heads;
   if (s.wide)
-    hipLaunchKernelGGL((join_kernel<E, D, wide_rows(D), 64>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((join_kernel<E, D, wide_rows(D), 16 * wide_waves(D)>), dim3(unsigned(rows)), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((join_kernel<E, D, kNarrowRows, 32>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((join_kernel<E, D, kNarrowRows, 32>), dim3(unsigned(rows)), dim3(256), 0, stream, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? GIE_HIP_OK : int(e);
 }

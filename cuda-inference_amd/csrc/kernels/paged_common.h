@@ -25,14 +25,42 @@ __device__ __forceinline__ int find_sequence(int batch, int x, Key key) {
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
-// rows of sequence b, whatever q_starts holds: 0 <= first <= last <= total
-struct Rows {
-  int first, count;
+// A sequence as a row finds it: its rows of q (0 <= first, first + count <= total whatever q_starts holds) and the
+// position of its first new token (whatever seq_lens holds).
+struct Sequence {
+  int index, first, count, base;
 };
-__device__ __forceinline__ Rows sequence_rows(const int* __restrict__ q_starts, int b, int total) {
-  const int s = min(max(q_starts[b], 0), total);
-  const int e = min(max(q_starts[b + 1], s), total);
-  return {s, e - s};
+
+// The sequence of largest index b with key(q_starts[b], b) <= x, for a key that does not fall with b. The whole wave takes
+// part and gets the same answer. A batch of up to 64 takes one round of loads; a larger one a search that looks at 64
+// places at a time, and then the loads.
+template <typename Key>
+__device__ __forceinline__ Sequence locate(const int* __restrict__ q_starts, const int* __restrict__ seq_lens, int batch,
+                                           int total, int x, Key key) {
+  const int lane = int(threadIdx.x) & 63;
+  Sequence s;
+  int start, end, len;
+  if (batch <= 64) {
+    const bool there = lane < batch;
+    const int at = there ? lane : 0;
+    start = q_starts[at];
+    end = q_starts[at + 1];
+    len = seq_lens[at];
+    const unsigned long long below = __ballot(there && key(start, at) <= x);
+    s.index = below == 0 ? 0 : __builtin_amdgcn_readfirstlane(__popcll(below) - 1);
+    start = __builtin_amdgcn_readlane(start, s.index);
+    end = __builtin_amdgcn_readlane(end, s.index);
+    len = __builtin_amdgcn_readlane(len, s.index);
+  } else {
+    s.index = find_sequence(batch, x, [&](int b) { return key(q_starts[b], b); });
+    start = __builtin_amdgcn_readfirstlane(q_starts[s.index]);
+    end = __builtin_amdgcn_readfirstlane(q_starts[s.index + 1]);
+    len = __builtin_amdgcn_readfirstlane(seq_lens[s.index]);
+  }
+  s.first = min(max(start, 0), total);
+  s.count = min(max(end, s.first), total) - s.first;
+  s.base = int(min(max((long long)len - s.count, -(1ll << 30)), 1ll << 30));
+  return s;
 }
 
 // what the kernels' grids and offsets assume
