@@ -40,7 +40,7 @@ struct LinArgs {
   int relu;
   int splits, per_split;  // parts of the input values, and their steps of 128
   int tiles_m, tiles_n;
-  int y_vec;  // rows of y in 16-byte pieces
+  int x_vec, y_vec;  // rows of x before its quantization, and of y, in 16-byte pieces
 };
 
 template <typename E>
@@ -74,16 +74,17 @@ __device__ __forceinline__ float bias_at(const void* bias, int n) {
 }
 
 // ---------------------------------------------------------------------------------------------- tiles
-template <typename E, int BM, int BN, int WM, int WN, bool ALIGNED>
-__global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(LinArgs a) {
-  constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+// WK waves share a part of the tile and take every WK-th 32 of a stage's input values; NST stages
+template <typename E, int BM, int BN, int WM, int WN, int WK, int NST, bool ALIGNED>
+__global__ __launch_bounds__(64 * WM * WN * WK, 1) void tile_kernel(LinArgs a) {
+  constexpr int kWaves = WM * WN * WK, kThreads = 64 * kWaves;
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32x32 products of a wave
   constexpr int kRows = BM + BN, kStage = kRows * 128;
   constexpr int IPW = kRows / 8 / kWaves;  // loads of 8 rows for each wave
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = int(threadIdx.x), lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave % WM, wn = wave / WM;
+  const int wm = wave % WM, wn = wave / WM % WN, wk = wave / (WM * WN);
 
   // tile: workgroup L runs on XCD L % 8, which takes a run of neighbouring tiles: 4 of tokens for each of channels, so
   // that those which run together share rows of x and w in its L2
@@ -118,8 +119,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(LinArgs a) {
     // in one page): the hardware would drop a word that passes the end
     const long long rx = (long long)(min(BM, a.M - m0) - 1) * a.ld_x + ((left + 15) & ~15);
     const long long rw = (long long)(min(BN, a.N - n0) - 1) * a.ld_w + ((left + 15) & ~15);
-    v4i sx = uniform(make_vsharp(a.x + m0 * a.ld_x + k0, int(rx)));
-    v4i sw = uniform(make_vsharp(a.w + n0 * a.ld_w + k0, int(rw)));
+    v4i sx = uniform(make_vsharp(a.x + m0 * a.ld_x + k0, left > 0 ? int(rx) : 0));
+    v4i sw = uniform(make_vsharp(a.w + n0 * a.ld_w + k0, left > 0 ? int(rw) : 0));
     // a vector instruction may have written these scalar registers: loads may read them 5 cycles later
     asm volatile("s_nop 4" : "+s"(sx), "+s"(sw));
 #pragma unroll
@@ -137,8 +138,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(LinArgs a) {
   };
   // rows of any alignment: 16 bytes for each thread and round through registers
   constexpr int kRounds = kRows * 8 / kThreads;
-  u32x4 held[ALIGNED ? 1 : kRounds];
-  const auto fetch = [&](int step) {
+  constexpr int kAhead = kRounds <= 4 ? 4 : 1;  // slices held
+  u32x4 held[ALIGNED ? 1 : kAhead][ALIGNED ? 1 : kRounds];
+  const auto fetch = [&](int step, u32x4* to) {
     const int k0 = k_first + step * 128;
 #pragma unroll
     for (int i = 0; i < kRounds; ++i) {
@@ -148,14 +150,14 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(LinArgs a) {
       u32x4 v = {};
       if (r < (is_x ? a.M : a.N) && k < k_last)
         v = load16_upto(is_x ? a.x + r * a.ld_x : a.w + r * a.ld_w, k, k_last);
-      held[i] = v;
+      to[i] = v;
     }
   };
-  const auto put = [&](int stage) {
+  const auto put = [&](int stage, const u32x4* from) {
 #pragma unroll
     for (int i = 0; i < kRounds; ++i) {
       const int c = i * kThreads + tid, row = c >> 3, slot = (c & 7) ^ ((row >> 1) & 7);
-      *reinterpret_cast<lds_v4*>(size_t(lds0 + unsigned(stage * kStage + row * 128 + slot * 16))) = held[i];
+      *reinterpret_cast<lds_v4*>(size_t(lds0 + unsigned(stage * kStage + row * 128 + slot * 16))) = from[i];
     }
   };
 
@@ -166,7 +168,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(LinArgs a) {
   const auto compute = [&](int stage) {
     const unsigned so = unsigned(stage * kStage);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
+    for (int kk = 0; kk < 4 / WK; ++kk) {
+      const int ks = kk * WK + wk;
       u32x4 xf[TM], wf[TN];
 #pragma unroll
       for (int i = 0; i < TM; ++i)
@@ -202,29 +205,69 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(LinArgs a) {
   };
 
   if constexpr (ALIGNED) {
-    issue(0, 0);
+    // loads past the last slice read nothing, so that every wait counts the same
+#pragma unroll
+    for (int s = 0; s < NST - 1; ++s) issue(s, s);
+    int stage = 0;
     for (int s = 0; s < steps; ++s) {
-      wait_vm<0>();
+      wait_vm<(NST - 2) * IPW>();
       stage_barrier();
-      if (s + 1 < steps)
-        issue(s + 1, (s + 1) & 1);
-      else
-        clear_tail(s & 1);
-      compute(s & 1);
+      issue(s + NST - 1, stage == 0 ? NST - 1 : stage - 1);
+      if (s + 1 == steps) clear_tail(stage);
+      compute(stage);
+      stage = stage + 1 == NST ? 0 : stage + 1;
     }
+    wait_vm<0>();
   } else {
-    fetch(0);
-    for (int s = 0; s < steps; ++s) {
-      put(s & 1);
-      __syncthreads();
-      if (s + 1 < steps) fetch(s + 1);
-      compute(s & 1);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) fetch(u, held[u]);
+    for (int s = 0; s < steps; s += kAhead) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (s + u >= steps) break;
+        put((s + u) & 1, held[u]);
+        fetch(s + u + kAhead, held[u]);
+        __syncthreads();
+        compute((s + u) & 1);
+      }
     }
   }
   __syncthreads();
 
+  if constexpr (WK > 1) {  // the waves' sums meet in the first's
+    static_assert(WM == 1 && WN == 1, "one part of the tile");
+    lds_v4* sums = reinterpret_cast<lds_v4*>(size_t(lds0));
+#pragma unroll
+    for (int n = 0; n < TN; ++n)
+#pragma unroll
+      for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (wk > 0)
+            sums[(((wk - 1) * TN + n) * TM + m) * 256 + g * 64 + lane] =
+                u32x4{uint32_t(acc[n][m][4 * g]), uint32_t(acc[n][m][4 * g + 1]), uint32_t(acc[n][m][4 * g + 2]),
+                      uint32_t(acc[n][m][4 * g + 3])};
+    __syncthreads();
+    if (wk == 0) {
+#pragma unroll
+      for (int n = 0; n < TN; ++n)
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+#pragma unroll
+          for (int w = 0; w < WK - 1; ++w)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const u32x4 v = sums[((w * TN + n) * TM + m) * 256 + g * 64 + lane];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[n][m][4 * g + e] += int(v[e]);
+            }
+    }
+    __syncthreads();
+  }
+
   // ---- 32 tokens at a time through the wave's own part of LDS, then out in rows ----
   if (a.splits > 1) {
+    if (WK > 1 && wk > 0) return;
     int* part = a.part + (long long)blockIdx.y * a.M * a.N;
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
@@ -257,6 +300,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(LinArgs a) {
     *reinterpret_cast<lds_f*>(size_t(scales + (BN + c) * 4)) = bias_at<E>(a.bias, n);
   }
   __syncthreads();
+  if (WK > 1 && wk > 0) return;
   const int c0 = n0 + wn * TN * 32;  // the wave's first channel
   const unsigned mine = scales + unsigned((wn * TN * 32 + 4 * half) * 4);
 #pragma unroll
@@ -366,19 +410,47 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(LinArgs a) {
     const int k = s * 64 + part;
     return s < steps && k < a.K ? load16_upto(w, k, a.K) : u32x4{};
   };
-#pragma unroll
-  for (int u = 0; u < U; ++u) wf[u] = load_w(wave + u * kFewWaves);
   if constexpr (FUSED) {
+    // x first: its way to 8 bits is the longer one, and the weights arrive under it
+    constexpr int kPer = 16 / kBytesOf<E>, kKeep = 4;
     for (int t = 0; t < a.M; ++t) {
+      const char* row = static_cast<const char*>(a.x16) + t * a.ld_x * kBytesOf<E>;
+      const int pieces = a.x_vec ? a.K / kPer : 0;
+      u32x4 keep[kKeep];
+#pragma unroll
+      for (int i = 0; i < kKeep; ++i) {
+        const int p = i * kFewThreads + tid;
+        keep[i] = p < pieces ? reinterpret_cast<const u32x4*>(row)[p] : u32x4{};
+      }
+      if (t == 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) wf[u] = load_w(wave + u * kFewWaves);
+      }
       float most = 0.f;
-      for (int k = tid; k < a.K; k += kFewThreads) most = magnitude_max(most, load_value<E>(a.x16, t * a.ld_x + k));
+#pragma unroll
+      for (int i = 0; i < kKeep; ++i) {
+        float f[8];
+        unpack<E>(keep[i], f);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) most = magnitude_max(most, f[e]);
+      }
+      const int rest = min(pieces, kKeep * kFewThreads) * kPer;  // value by value from here
+      for (int k = rest + tid; k < a.K; k += kFewThreads) most = magnitude_max(most, load_value<E>(a.x16, t * a.ld_x + k));
       most = block_magnitude_max<kFewThreads>(most);
       const RowScale s = row_scale(most);
       if (tid == 0) scales[t] = s.scale;
-      for (int k = tid; k < K16; k += kFewThreads)
+#pragma unroll
+      for (int i = 0; i < kKeep; ++i) {
+        const int p = i * kFewThreads + tid;
+        if (p < pieces) quantize_piece<E>(keep[i], s.inverse, lds + t * K16 + p * kPer);
+      }
+      for (int k = rest + tid; k < K16; k += kFewThreads)
         lds[t * K16 + k] = k < a.K ? uint8_t(quantize_value(load_value<E>(a.x16, t * a.ld_x + k), s.inverse)) : 0;
       __syncthreads();
     }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) wf[u] = load_w(wave + u * kFewWaves);
   }
   i32x4 acc = {};
   for (int s0 = wave; s0 < steps; s0 += U * kFewWaves) {
@@ -428,51 +500,70 @@ bool valid(int dtype, const gie_linear_geom* g) {
 enum Form { kFewForm, kTile32, kTile64, kTile128, kTile256 };
 struct Plan {
   Form form;
-  int bm, bn, tiles_m, tiles_n, splits, per_split;
+  int tile, tiles_m, tiles_n, splits, per_split;  // tile: tokens and channels of one
 };
 
+// Square tiles of 256, 128, 64 and 32, the largest that still make 192 workgroups (of 256 compute units): a tile moves
+// (1 / tokens + 1 / channels) bytes from the L2 for each product. Measured at 4096 input values, us by tile: 4096x4096 70
+// (256), 84 (128), 144 (64); 1024x4096 29.6 (128), 42 (64), 55 (256); 512x4096 19.6 (64), 27 (128).
+// With less of them, tiles of 64 and 32 and parts of the input values are weighed by what they move: L2 to LDS 14 TB/s
+// (64) and 11.6 TB/s (32), weights 4.2 TB/s, less where the device is not full; 2.5 us and 4 TB/s for parts that are
+// joined. Measured / so estimated, us: 64x4096x4096 10.9 (32, whole) 12.2 (64, 4 parts) / 10.8, 13.5; 64x8192x8192
+// 22.0 (64, 2 parts) 25.3 (32) / 25, 28; 256x1024x16384 19.8 (64, 4 parts) 25.7 (32) / 19, 28.
 Plan plan_of(const gie_linear_geom& g) {
   Plan p{};
   const int M = g.tokens, N = g.out_features, steps = (g.in_features + 127) / 128;
-  const auto tiles = [&](int b, int n) { return (n + b - 1) / b; };
   p.splits = 1;
+  p.per_split = steps;
   if (M <= kFew) {
     p.form = kFewForm;
-  } else if (M <= 32) {
-    p.form = kTile32, p.bm = 32, p.bn = 128;
-  } else if (M <= 64) {
-    p.form = kTile64, p.bm = 64, p.bn = 128;
-  } else if ((long long)tiles(256, M) * tiles(256, N) >= 192) {
-    p.form = kTile256, p.bm = 256, p.bn = 256;
-  } else {
-    p.form = kTile128, p.bm = 128, p.bn = 128;
+    return p;
   }
-  p.per_split = steps;
-  if (p.form == kFewForm) return p;
-  p.tiles_m = tiles(p.bm, M);
-  p.tiles_n = tiles(p.bn, N);
-  const long long count = (long long)p.tiles_m * p.tiles_n;
-  // at least 4 steps for a part, and no more parts than fill the device once
-  const long long want = count >= 256 ? 1 : 256 / count, most = steps / 4 > 0 ? steps / 4 : 1;
-  const int splits = int(want < most ? want : most);
-  p.per_split = (steps + splits - 1) / splits;
-  p.splits = (steps + p.per_split - 1) / p.per_split;
+  const auto count = [&](int tile) { return (long long)((M + tile - 1) / tile) * ((N + tile - 1) / tile); };
+  if (count(256) >= 192) {
+    p.form = kTile256, p.tile = 256;
+  } else if (count(128) >= 192) {
+    p.form = kTile128, p.tile = 128;
+  } else if (count(64) >= 192) {
+    p.form = kTile64, p.tile = 64;
+  } else {
+    double best = 0;
+    for (int tile = 64; tile >= 32; tile /= 2) {
+      for (int n = 1; n <= 16 && (n == 1 || steps / n >= 2); n *= 2) {
+        const double full = count(tile) * n < 256 ? 256.0 / (count(tile) * n) : 1.0;
+        const double l2 = count(tile) * 2.0 * tile * g.in_features / (tile == 64 ? 14e6 : 11.6e6);
+        const double hbm = double(N) * g.in_features / 4.2e6;
+        const double join = n == 1 ? 0 : 2.5 + 8.0 * M * N * n / 4e6;
+        const double us = (l2 > hbm ? l2 : hbm) * full + join;
+        if (p.tile == 0 || us < best) {
+          best = us;
+          p.form = tile == 64 ? kTile64 : kTile32, p.tile = tile;
+          p.per_split = (steps + n - 1) / n;
+        }
+      }
+    }
+    p.splits = (steps + p.per_split - 1) / p.per_split;
+  }
+  p.tiles_m = (M + p.tile - 1) / p.tile;
+  p.tiles_n = (N + p.tile - 1) / p.tile;
   return p;
 }
 
 bool fuses(const gie_linear_geom& g) { return g.tokens <= 4 && (long long)g.tokens * g.in_features <= 32 * 1024; }
 
-template <typename E, int BM, int BN, int WM, int WN>
+template <typename E, int BM, int BN, int WM, int WN, int WK, int NST>
 int run_tiles(const LinArgs& a, bool aligned, hipStream_t s) {
-  constexpr int kStages = 2 * (BM + BN) * 128;
-  constexpr int kOutB = WM * WN * 32 * (BN / WN * kBytesOf<E> + 16) + BN * 8;
-  constexpr int bytes = kStages > kOutB ? kStages : kOutB;
-  auto kernel = tile_kernel<E, BM, BN, WM, WN, true>;
+  constexpr int kStages = NST * (BM + BN) * 128;
+  constexpr int kOutB = WM * WN * WK * 32 * (BN / WN * kBytesOf<E> + 16) + BN * 8;
+  constexpr int kSums = (WK - 1) * BM * BN * 4;
+  constexpr int most = kStages > kOutB ? kStages : kOutB, bytes = most > kSums ? most : kSums;
+  auto kernel = tile_kernel<E, BM, BN, WM, WN, WK, NST, true>;
   if constexpr (BM < 256)
-    if (!aligned) kernel = tile_kernel<E, BM, BN, WM, WN, false>;
+    if (!aligned) kernel = tile_kernel<E, BM, BN, WM, WN, WK, NST, false>;
   const int rc = set_lds_limit(reinterpret_cast<const void*>(kernel), bytes);
   if (rc != GIE_HIP_OK) return rc;
-  hipLaunchKernelGGL(kernel, dim3(unsigned(a.tiles_m * a.tiles_n), unsigned(a.splits)), dim3(64 * WM * WN), bytes, s, a);
+  hipLaunchKernelGGL(kernel, dim3(unsigned(a.tiles_m * a.tiles_n), unsigned(a.splits)), dim3(64 * WM * WN * WK), bytes,
+                     s, a);
   return GIE_HIP_OK;
 }
 
@@ -489,11 +580,11 @@ int run(const Plan& p, const LinArgs& a, bool aligned, hipStream_t s) {
         hipLaunchKernelGGL((few_kernel<E, false>), grid, dim3(kFewThreads), 0, s, a);
       break;
     }
-    case kTile32: rc = run_tiles<E, 32, 128, 1, 4>(a, aligned, s); break;
-    case kTile64: rc = run_tiles<E, 64, 128, 1, 4>(a, aligned, s); break;
-    case kTile128: rc = run_tiles<E, 128, 128, 2, 2>(a, aligned, s); break;
+    case kTile32: rc = run_tiles<E, 32, 32, 1, 1, 4, 8>(a, aligned, s); break;
+    case kTile64: rc = run_tiles<E, 64, 64, 2, 2, 1, 4>(a, aligned, s); break;
+    case kTile128: rc = run_tiles<E, 128, 128, 2, 2, 1, 2>(a, aligned, s); break;
     case kTile256:
-      rc = aligned ? run_tiles<E, 256, 256, 2, 4>(a, true, s) : run_tiles<E, 128, 128, 2, 2>(a, false, s);
+      rc = aligned ? run_tiles<E, 256, 256, 2, 4, 1, 2>(a, true, s) : run_tiles<E, 128, 128, 2, 2, 1, 2>(a, false, s);
       break;
   }
   if (rc != GIE_HIP_OK) return rc;
@@ -558,6 +649,7 @@ extern "C" int gie_hip_linear_i8(int dtype, const gie_linear_geom* g, const void
   if (x_scale == nullptr) {
     if (p.form == kFewForm && fuses(*g)) {
       a.x16 = x;
+      a.x_vec = g->ld_x * esz % 16 == 0 && at(x) % 16 == 0;
     } else {
       const size_t ld = round16(g->in_features);
       int8_t* q = reinterpret_cast<int8_t*>(ws);
@@ -572,10 +664,10 @@ extern "C" int gie_hip_linear_i8(int dtype, const gie_linear_geom* g, const void
   // direct loads into LDS take 16-byte pieces, and reach a tile's last row with a 32-bit offset
   const bool aligned = a.ld_x % 16 == 0 && a.ld_w % 16 == 0 && at(a.x) % 16 == 0 && at(w) % 16 == 0 &&
                        a.ld_x < (1 << 22) && a.ld_w < (1 << 22);
-  const int bm = p.form == kTile256 && !aligned ? 128 : p.bm, bn = p.form == kTile256 && !aligned ? 128 : p.bn;
+  const int tile = p.form == kTile256 && !aligned ? 128 : p.tile;
   if (p.form != kFewForm) {
-    const long long tm = (g->tokens + bm - 1) / bm, tn = (g->out_features + bn - 1) / bn;
-    if (tm * tn > 0x7fffffff) return GIE_HIP_EINVAL;
+    const long long tm = (g->tokens + tile - 1) / tile, tn = (g->out_features + tile - 1) / tile;
+    if (tm * tn > (1 << 23)) return GIE_HIP_EINVAL;
     a.tiles_m = int(tm);
     a.tiles_n = int(tn);
   }

@@ -28,6 +28,7 @@ namespace {
 typedef __attribute__((address_space(4))) const int const_int;  // uniform loads through the scalar cache
 typedef __attribute__((address_space(3))) u32x4 lds_v4;
 typedef __attribute__((address_space(3))) u32x2 lds_v2;
+typedef __attribute__((address_space(3))) int lds_i;
 typedef short v4s __attribute__((ext_vector_type(4)));
 
 struct AttnArgs {
@@ -132,12 +133,11 @@ __device__ __forceinline__ RowTile row_tile(const AttnArgs& a, int slot) {
 }
 
 template <typename E, int D, int RQ, int WR, int WK, int NST>
-__global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * WR * WK, D == 256 ? 1 : 2) void attention_kernel(AttnArgs a) {
   static_assert(WR == 1 || WK == 1, "waves share a tile of keys or have their own");
   constexpr int R = RQ * WR * 32;             // rows of the workgroup
   constexpr int TT = WR > 1 ? 16 * WR : 32;   // positions of a tile
   constexpr int NS = TT / 32;                 // 32-position parts of a tile
-  constexpr int PN = D == 256 || NS < 2 || WR == 8 ? 1 : 2;  // parts that go through the softmax together
   constexpr int GR = TT / 16 / WR;            // 16-position granules that a wave loads
   constexpr int P = kPitch<D>;
   constexpr int KS = D / 16, DT = D / 32;     // steps of the first product, 32-wide parts of the second
@@ -172,14 +172,12 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
   // ---- this lane's rows: row (lane & 31) of each of the wave's RQ tiles; rows past the last repeat it ----
   int pos[RQ];
   u32x4 qf[RQ][KS];
-  long long row_q[RQ];
 #pragma unroll
   for (int r = 0; r < RQ; ++r) {
     const int row = min(t.row0 + (wr * RQ + r) * 32 + (lane & 31), last_row);
     const int token = row / a.group, head = kvh * a.group + (row - token * a.group);
     pos[r] = t.seq.base + token;
     if (pos[r] >= a.capacity) pos[r] = -1;  // no valid position: sees nothing
-    row_q[r] = (long long)(t.seq.first + token) * a.q_heads + head;
     const uint16_t* src = a.q + (t.seq.first + token) * a.q_stride + head * D;
     const uint32_t flip = a.negate ? 0x80008000u : 0u;
     if (a.q_vec) {
@@ -269,11 +267,22 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
     // the workgroup see different keys of this tile, such values are added to the rows that see them and replaced by 0.
     if ((at0 + TT - 1 > pos_first && pos_first != pos_last) || (a.window > 0 && at0 <= pos_last - a.window)) {
       uint32_t bad = 0;
-      for (int c = lane; c < kTileB / 16; c += 64) {
-        const u32x4 v = *reinterpret_cast<const lds_v4*>(size_t(lds0 + so + unsigned(kTileB + c * 16)));
+#pragma unroll
+      for (int i = 0; i < kTileB / 1024 / WR; ++i) {
+        const u32x4 v =
+            *reinterpret_cast<const lds_v4*>(size_t(lds0 + so + unsigned(kTileB + (i * WR + wr) * 1024 + lane * 16)));
         bad |= not_finite<E>(v.x) | not_finite<E>(v.y) | not_finite<E>(v.z) | not_finite<E>(v.w);
       }
-      if (__any(bad != 0)) {  // the same answer in all waves that share the tile
+      bool any = __any(bad != 0);
+      if constexpr (WR > 1) {  // waves that share the tile looked at a part of it each
+        lds_i* found = reinterpret_cast<lds_i*>(size_t(lds0 + unsigned(NST * kStage)));
+        if (lane == 0) found[wr] = any;
+        stage_barrier();
+        any = false;
+#pragma unroll
+        for (int w = 0; w < WR; ++w) any |= __builtin_amdgcn_readfirstlane(found[w]) != 0;
+      }
+      if (any) {
         for (int k = 0; k < TT; ++k) {
           const int key = at0 + k;
           const unsigned row = lds0 + so + unsigned(kTileB + k * P);
@@ -315,55 +324,73 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
       }
     }
 
+
+    // Part by part of 32 keys. What a product reads from LDS is requested ahead of it: half of V under the softmax, the
+    // other half and the next part's K under the second product.
+    constexpr bool kAhead = D < 256;  // where the registers hold it
+    u32x4 kf[KS];
+    const auto read_k = [&](int n) {
+      unsigned ko = k_rd + so;
+      asm volatile("" : "+v"(ko));  // the permuted addresses are worked out for every part: kept, they cost registers
 #pragma unroll
-    for (int n0 = 0; n0 < NS; n0 += PN) {
-      const int at = at0 + n0 * 32;
-      const unsigned ko = k_rd + so, vo = v_rd + so;
-      // scores: part n holds keys at + 32 n + 8 (i / 4) + 4 half + i % 4 in register i
-      f32x16 s[RQ][PN];
+      for (int ks = 0; ks < KS; ++ks)
+        kf[ks] = *reinterpret_cast<const lds_v4*>(size_t((ko ^ unsigned(ks * 32)) + unsigned(n * 32 * P)));
+    };
+    if (kAhead) read_k(0);
 #pragma unroll
-      for (int n = 0; n < PN; ++n) {
+    for (int n = 0; n < NS; ++n) {
+      const int at = at0 + n * 32;
+      // scores: register i holds key at + 8 (i / 4) + 4 half + i % 4
+      f32x16 s[RQ];
 #pragma unroll
-        for (int r = 0; r < RQ; ++r) s[r][n] = f32x16{};
+      for (int r = 0; r < RQ; ++r) s[r] = f32x16{};
+      if (!kAhead) read_k(n);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const u32x4 kf = *reinterpret_cast<const lds_v4*>(size_t((ko ^ unsigned(ks * 32)) + unsigned((n0 + n) * 32 * P)));
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int r = 0; r < RQ; ++r) s[r][n] = E::mfma32(kf, qf[r][ks], s[r][n]);
+        for (int r = 0; r < RQ; ++r) s[r] = E::mfma32(kf[ks], qf[r][ks], s[r]);
+      // both halves of a part's V (16 keys each) where the registers hold them
+      constexpr int VH = D < 256 ? 2 : 1;
+      u32x4 vf[VH][DT];
+      const auto read_v = [&](int h) {
+        unsigned vo = v_rd + so;
+        asm volatile("" : "+v"(vo));
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const unsigned p = (vo ^ unsigned(d * 64)) + unsigned((2 * n + h) * 16 * P);
+          const u32x2 x = read_transposed(p), y = read_transposed(p + unsigned(8 * P));
+          vf[h % VH][d] = u32x4{x.x, x.y, y.x, y.y};
         }
-      }
+      };
+      if (VH == 2) read_v(0);
       if (a.cap > 0) {
 #pragma unroll
         for (int r = 0; r < RQ; ++r)
 #pragma unroll
-          for (int n = 0; n < PN; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float e = __builtin_amdgcn_exp2f(s[r][n][i] * a.cap_in);
-              s[r][n][i] = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(e + 1.f);
-            }
+          for (int i = 0; i < 16; ++i) {
+            const float e = __builtin_amdgcn_exp2f(s[r][i] * a.cap_in);
+            s[r][i] = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(e + 1.f);
+          }
       }
-      if (at + PN * 32 - 1 > wpos_first || (a.window > 0 && at <= wpos_last - a.window) || wpos_last >= a.capacity) {
+      const bool masked =
+          at + 31 > wpos_first || (a.window > 0 && at <= wpos_last - a.window) || wpos_last >= a.capacity;
+      if (masked) {
 #pragma unroll
         for (int r = 0; r < RQ; ++r) {
           const int oldest = a.window > 0 ? pos[r] - a.window : -1;
 #pragma unroll
-          for (int n = 0; n < PN; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int key = at + n * 32 + 8 * (i / 4) + 4 * half + i % 4;
-              s[r][n][i] = key <= pos[r] && key > oldest ? s[r][n][i] : -INFINITY;
-            }
+          for (int i = 0; i < 16; ++i) {
+            const int key = at + 8 * (i / 4) + 4 * half + i % 4;
+            s[r][i] = key <= pos[r] && key > oldest ? s[r][i] : -INFINITY;
+          }
         }
       }
-      u32x4 pf[RQ][2 * PN];
+      u32x4 pf[RQ][2];
 #pragma unroll
       for (int r = 0; r < RQ; ++r) {
-        float top = s[r][0][0];
+        float top = s[r][0];
 #pragma unroll
-        for (int n = 0; n < PN; ++n)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, s[r][n][i]);
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[r][i]);
         top = swap_max(top);
         // the maximum follows only when a weight would pass 2^8: sums and weights keep their relative precision, and
         // most tiles leave O as it is
@@ -377,32 +404,29 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
 #pragma unroll
           for (int d = 0; d < DT; ++d) o[r][d] *= keep;
         }
-        float sum = 0.f;
+        float sum[4] = {};
 #pragma unroll
-        for (int n = 0; n < PN; ++n) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            s[r][n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][n][i], a.mult, -mc[r]));
-            sum += s[r][n][i];
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            pf[r][2 * n + i] =
-                u32x4{E::pack2(s[r][n][8 * i], s[r][n][8 * i + 1]), E::pack2(s[r][n][8 * i + 2], s[r][n][8 * i + 3]),
-                      E::pack2(s[r][n][8 * i + 4], s[r][n][8 * i + 5]), E::pack2(s[r][n][8 * i + 6], s[r][n][8 * i + 7])};
+        for (int i = 0; i < 16; ++i) {
+          s[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i], a.mult, -mc[r]));
+          sum[i % 4] += s[r][i];
         }
-        l[r] += sum;
+        l[r] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          pf[r][h] = u32x4{E::pack2(s[r][8 * h], s[r][8 * h + 1]), E::pack2(s[r][8 * h + 2], s[r][8 * h + 3]),
+                           E::pack2(s[r][8 * h + 4], s[r][8 * h + 5]), E::pack2(s[r][8 * h + 6], s[r][8 * h + 7])};
+      }
+      if (VH == 2) {
+        read_v(1);
+        if (kAhead && n + 1 < NS) read_k(n + 1);
       }
 #pragma unroll
-      for (int n = 0; n < 2 * PN; ++n) {
+      for (int h = 0; h < 2; ++h) {
+        if (VH == 1) read_v(h);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const unsigned p = (vo ^ unsigned(d * 64)) + unsigned((2 * n0 + n) * 16 * P);
-          const u32x2 x = read_transposed(p), y = read_transposed(p + unsigned(8 * P));
-          const u32x4 vf = u32x4{x.x, x.y, y.x, y.y};
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int r = 0; r < RQ; ++r) o[r][d] = E::mfma32(vf, pf[r][n], o[r][d]);
-        }
+          for (int r = 0; r < RQ; ++r) o[r][d] = E::mfma32(vf[h % VH][d], pf[r][h], o[r][d]);
       }
     }
   };
@@ -433,6 +457,15 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
 
 #pragma unroll
   for (int r = 0; r < RQ; ++r) l[r] = swap_add(l[r]);
+
+  // where the lane's rows go, worked out again here: kept from above it would cost registers in the loop
+  int row_first = t.row0;
+  asm volatile("" : "+s"(row_first));
+  const auto place = [&](int r, int& token, int& head) {
+    const int row = min(row_first + (wr * RQ + r) * 32 + (lane & 31), last_row), i = row / a.group;
+    token = t.seq.first + i;
+    head = kvh * a.group + (row - i * a.group);
+  };
 
   // ---- the waves' parts of the keys ----
   if constexpr (WK > 1) {
@@ -471,18 +504,19 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
     const float* all = reinterpret_cast<const float*>(lds + WK * 256);
     const int row = lane & 31;
     if (row < t.rows) {
+      int token, head;
+      place(0, token, head);
       const float inv = total == 0.f ? 0.f : 1.f / total;
       for (int d = (wave * 2 + half) * 4; d < D; d += WK * 8) {
         f32x4 v = {};
 #pragma unroll
         for (int w = 0; w < WK; ++w) v += *reinterpret_cast<const f32x4*>(all + (w * 32 + row) * kRow + d);
         if (range.splits > 1) {
-          float* dst = a.part + (row_q[0] * a.splits + z) * (D + 4);
+          float* dst = a.part + (((long long)token * a.q_heads + head) * a.splits + z) * (D + 4);
           *reinterpret_cast<f32x4*>(dst + d) = v;
           if (d == 0) dst[D] = top, dst[D + 1] = total;
         } else {
-          const int head = int(row_q[0] % a.q_heads);
-          uint16_t* dst = a.out + (row_q[0] / a.q_heads) * a.o_stride + head * D + d;
+          uint16_t* dst = a.out + token * a.o_stride + head * D + d;
           if (total == 0.f) v = f32x4{};
           v *= inv;
           if (a.o_vec) {
@@ -503,9 +537,10 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
     const int row = (wr * RQ + r) * 32 + (lane & 31);
     if (row >= t.rows) continue;
     const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-    const int head = int(row_q[r] % a.q_heads);
-    float* part = a.part + (row_q[r] * a.splits + z) * (D + 4);
-    uint16_t* dst = a.out + (row_q[r] / a.q_heads) * a.o_stride + head * D;
+    int token, head;
+    place(r, token, head);
+    float* part = a.part + (((long long)token * a.q_heads + head) * a.splits + z) * (D + 4);
+    uint16_t* dst = a.out + token * a.o_stride + head * D;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -529,14 +564,16 @@ __global__ __launch_bounds__(64 * WR * WK, 1) void attention_kernel(AttnArgs a) 
   }
 }
 
-// Joins the parts of the keys: a workgroup for each row (token, head), lanes over the head's values 4 at a time, the
-// parts dealt out to what the values leave of it.
-template <typename E, int D, int R, int TT>
+// Joins the parts of the keys: WAVES waves for each row (token, head), lanes over the head's values 4 at a time, the parts
+// dealt out to the groups of lanes that this leaves. One wave (4 rows to a workgroup) where there are few parts and many
+// rows, four where one row has dozens of parts.
+template <typename E, int D, int R, int TT, int WAVES>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
-  constexpr int kLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, kGroups = 256 / kLanes;
-  __shared__ f32x4 sums[kGroups][kLanes];
-  const int tid = int(threadIdx.x), lane = tid & 63;
-  const long long row = blockIdx.x;
+  constexpr int kLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, kInWave = 64 / kLanes, kGroups = WAVES * kInWave;
+  __shared__ f32x4 sums[WAVES][kLanes];
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = WAVES > 1 ? tid >> 6 : 0;
+  const long long row = WAVES > 1 ? blockIdx.x : blockIdx.x * 4ll + (tid >> 6);
+  if (row >= (long long)a.total_tokens * a.q_heads) return;
   const int token = int(row / a.q_heads), head = int(row % a.q_heads);
   const float* part = a.part + row * a.splits * (D + 4);
   const Sequence seq =
@@ -557,18 +594,25 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   for (int z = lane; z < splits; z += 64) total += part[z * (D + 4) + D + 1] * weight(part[z * (D + 4) + D]);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d);
-  const int at = tid % kLanes, group = tid / kLanes;
+  const int at = lane % kLanes, group = wave * kInWave + lane / kLanes;
   f32x4 v = {};
   if (at * 4 < D) {
 #pragma unroll 4
     for (int z = group; z < splits; z += kGroups)
       v += *reinterpret_cast<const f32x4*>(part + z * (D + 4) + at * 4) * weight(part[z * (D + 4) + D]);
   }
-  sums[group][at] = v;
-  __syncthreads();
-  if (group != 0 || at * 4 >= D) return;
 #pragma unroll
-  for (int g = 1; g < kGroups; ++g) v += sums[g][at];
+  for (int d = kLanes; d < 64; d <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], d);
+  if (WAVES > 1) {
+    if (lane < kLanes) sums[wave][at] = v;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) v += sums[w][at];
+  }
+  if (lane >= kLanes || at * 4 >= D) return;
   const float inv = total == 0.f ? 0.f : 1.f / total;
   uint16_t* dst = a.out + token * a.o_stride + head * D + at * 4;
   if (total == 0.f) v = f32x4{};
@@ -591,7 +635,7 @@ constexpr int kNarrowRows = 32;
 // 64 rows for each wave halve the LDS reads of a product; at head_dim 256 their sums would not fit the registers
 template <int D>
 constexpr int kWideTiles = D == 256 ? 1 : 2;
-constexpr int wide_waves(int head_dim) { return head_dim == 256 ? 4 : 8; }
+constexpr int wide_waves(int) { return 4; }
 constexpr int wide_rows(int head_dim) { return 32 * wide_waves(head_dim); }
 
 Shape shape_of(const gie_paged_geom& g) {
@@ -609,9 +653,27 @@ Shape shape_of(const gie_paged_geom& g) {
   if (g.window > 0 && (long long)g.window + most_new < len) len = g.window + most_new;
   const long long tiles = (len + tt - 1) / tt;
   const long long blocks = busy * g.kv_heads;
-  const int fewest = s.wide ? 4 : 8;  // tiles of a part: below that the join costs more than it gives
-  const long long want = 256 / blocks;
-  long long splits = want < tiles / fewest ? want : tiles / fewest;
+  const int fewest = s.wide ? 2 : 8;  // tiles of a part
+  const long long most = tiles / fewest > 1 ? tiles / fewest : 1;
+  long long splits = 1;
+  if (!s.wide) {
+    // bytes bound: one workgroup for each compute unit, whose LDS holds 64 KiB and more on their way
+    splits = 256 / blocks;
+  } else {
+    // Products: a tile takes 1.4 us on a compute unit by itself and 1.08 us of one that two workgroups share (64 keys,
+    // head_dim 128: measured 990 TFLOP/s over long keys). Parts: a launch, and their sums written and read once.
+    const double unit = g.head_dim / 128.0, mean = tiles - (most_new < len ? most_new : len) / (2.0 * tt);
+    double best = 0;
+    for (long long n = 1; n <= most && n <= 64; ++n) {
+      const long long each = (blocks * n + 255) / 256;  // workgroups of a compute unit
+      const double path = (each == 1 ? 1.4 : 2.16) * unit * double((tiles + n - 1) / n);
+      const double share = 1.08 * unit * blocks * mean / 256;
+      const double join = n == 1 ? 0 : 4 + 2.0 * rows * g.kv_heads * n * (g.head_dim + 4) * 4 / 3.5e6;
+      const double us = (path > share ? path : share) + join;
+      if (n == 1 || us < 0.95 * best) best = us, splits = n;
+    }
+  }
+  if (splits > most) splits = most;
   if (splits < 1) splits = 1;
   s.chunk = int((tiles + splits - 1) / splits);
   s.splits = int((tiles + s.chunk - 1) / s.chunk);
@@ -635,7 +697,7 @@ int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   int rc;
   if (s.wide) {
     constexpr int NST = 2;
-    rc = start(attention_kernel<E, D, 1, wide_waves(D), 1, NST>, int(grid), 64 * wide_waves(D), NST * 2 * 16 * wide_waves(D) * P, stream, a);
+    rc = start(attention_kernel<E, D, 1, wide_waves(D), 1, NST>, int(grid), 64 * wide_waves(D), NST * 2 * 16 * wide_waves(D) * P + 64, stream, a);
   } else {
     constexpr int WK = D == 256 ? 2 : 4, NST = D == 64 ? 4 : 2;
     constexpr int bytes = WK * NST * 2 * 32 * P, join = WK * 256 + WK * 32 * (D + 4) * 4;
@@ -643,10 +705,11 @@ int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   }
   if (rc != GIE_HIP_OK || s.splits == 1) return rc;
   const long long rows = (long long)a.total_tokens * a.q_heads;
-  if (s.wide)
-    hipLaunchKernelGGL((join_kernel<E, D, wide_rows(D), 16 * wide_waves(D)>), dim3(unsigned(rows)), dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((join_kernel<E, D, kNarrowRows, 32>), dim3(unsigned(rows)), dim3(256), 0, stream, a);
+  const bool many = s.splits > 8;
+  constexpr int RW = wide_rows(D), TW = 16 * wide_waves(D), RN = kNarrowRows;
+  const auto join = s.wide ? (many ? join_kernel<E, D, RW, TW, 4> : join_kernel<E, D, RW, TW, 1>)
+                           : (many ? join_kernel<E, D, RN, 32, 4> : join_kernel<E, D, RN, 32, 1>);
+  hipLaunchKernelGGL(join, dim3(unsigned(many ? rows : (rows + 3) / 4)), dim3(256), 0, stream, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? GIE_HIP_OK : int(e);
 }

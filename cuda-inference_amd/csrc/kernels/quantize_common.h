@@ -66,4 +66,30 @@ __device__ __forceinline__ int8_t quantize_value(float v, float inverse) {
   return inverse == 0.f ? int8_t(0) : int8_t(int(rintf(v * inverse)));
 }
 
+// a 16-byte piece of a row: 8 values of 16 bits or 4 of 32
+template <typename E>
+__device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = E::to_f32(uint16_t(v[e / 2] >> (16 * (e & 1))));
+}
+template <>
+__device__ __forceinline__ void unpack<F32>(u32x4 v, float (&f)[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[e]);
+}
+// ... and what it becomes, 8 or 4 bytes at `to`
+template <typename E>
+__device__ __forceinline__ void quantize_piece(u32x4 v, float inverse, void* to) {
+  constexpr int kPer = E::kDtype == GIE_HIP_FP32 ? 4 : 8;
+  float f[8];
+  unpack<E>(v, f);
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) w[e / 4] |= uint32_t(uint8_t(quantize_value(f[e], inverse))) << (8 * (e & 3));
+  if constexpr (kPer == 8)
+    *static_cast<u32x2*>(to) = u32x2{w[0], w[1]};
+  else
+    *static_cast<uint32_t*>(to) = w[0];
+}
+
 }  // namespace gie_hip

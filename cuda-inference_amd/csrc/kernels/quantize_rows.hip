@@ -11,17 +11,6 @@ namespace {
 
 constexpr int kThreads = 256, kKeep = 4;
 
-template <typename E>
-__device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = E::to_f32(uint16_t(v[e / 2] >> (16 * (e & 1))));
-}
-template <>
-__device__ __forceinline__ void unpack<F32>(u32x4 v, float (&f)[8]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[e]);
-}
-
 // T threads for each row. kVec: rows of x in 16-byte pieces, rows of q in the pieces that these become
 template <typename E, int T, bool kVec>
 __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* __restrict__ x, long long ld_x, int tokens,
@@ -57,17 +46,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* __r
   const RowScale s = row_scale(a);
   if (me == 0 && there) scale[row] = s.scale;
   int8_t* out = q + (there ? row * ld_q : 0);
-  const auto put = [&](int p, u32x4 v) {
-    float f[8];
-    unpack<E>(v, f);
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) w[e / 4] |= uint32_t(uint8_t(quantize_value(f[e], s.inverse))) << (8 * (e & 3));
-    if constexpr (kPer == 8)
-      reinterpret_cast<u32x2*>(out)[p] = u32x2{w[0], w[1]};
-    else
-      reinterpret_cast<uint32_t*>(out)[p] = w[0];
-  };
+  const auto put = [&](int p, u32x4 v) { quantize_piece<E>(v, s.inverse, out + p * kPer); };
 #pragma unroll
   for (int i = 0; i < kKeep; ++i)
     if (i * T + me < pieces) put(i * T + me, keep[i]);
