@@ -205,6 +205,7 @@ extern "C" int gie_hip_kv_append(int dtype, const gie_paged_geom* g, const void*
   if (dtype != GIE_HIP_FP16 && dtype != GIE_HIP_BF16) return GIE_HIP_EUNSUPPORTED;
   if (g->head_dim != 64 && g->head_dim != 96 && g->head_dim != 128 && g->head_dim != 256) return GIE_HIP_EUNSUPPORTED;
   if (g->total_tokens == 0) return GIE_HIP_OK;
+  if (g->total_tokens > (1 << 23) - 1) return GIE_HIP_EUNSUPPORTED;  // 512 threads for each: a launch's limit
   if (!k || !v || !q_starts || !seq_lens || !page_table || !k_pages || !v_pages || k_pages == v_pages ||
       (q == nullptr) != (q_out == nullptr))
     return GIE_HIP_EINVAL;

@@ -512,7 +512,8 @@ struct Plan {
 // 22.0 (64, 2 parts) 25.3 (32) / 25, 28; 256x1024x16384 19.8 (64, 4 parts) 25.7 (32) / 19, 28.
 Plan plan_of(const gie_linear_geom& g) {
   Plan p{};
-  const int M = g.tokens, N = g.out_features, steps = (g.in_features + 127) / 128;
+  const long long M = g.tokens, N = g.out_features;
+  const int steps = (g.in_features + 127) / 128;
   p.splits = 1;
   p.per_split = steps;
   if (M <= kFew) {
@@ -544,8 +545,8 @@ Plan plan_of(const gie_linear_geom& g) {
     }
     p.splits = (steps + p.per_split - 1) / p.per_split;
   }
-  p.tiles_m = (M + p.tile - 1) / p.tile;
-  p.tiles_n = (N + p.tile - 1) / p.tile;
+  p.tiles_m = int((M + p.tile - 1) / p.tile);
+  p.tiles_n = int((N + p.tile - 1) / p.tile);
   return p;
 }
 
@@ -625,6 +626,7 @@ extern "C" int gie_hip_linear_i8(int dtype, const gie_linear_geom* g, const void
   const size_t need = gie_hip_linear_i8_workspace(dtype, g, x_scale != nullptr);
   if (need > 0 && (!workspace || workspace_bytes < need || at(workspace) % 16 != 0)) return GIE_HIP_EINVAL;
   const Plan p = plan_of(*g);
+  if (p.form == kFewForm && g->out_features > (1 << 26)) return GIE_HIP_EUNSUPPORTED;
   LinArgs a{};
   a.x = static_cast<const int8_t*>(x);
   a.x_scale = x_scale;
@@ -667,7 +669,7 @@ extern "C" int gie_hip_linear_i8(int dtype, const gie_linear_geom* g, const void
   const int tile = p.form == kTile256 && !aligned ? 128 : p.tile;
   if (p.form != kFewForm) {
     const long long tm = (g->tokens + tile - 1) / tile, tn = (g->out_features + tile - 1) / tile;
-    if (tm * tn > (1 << 23)) return GIE_HIP_EINVAL;
+    if (tm * tn >= (1 << 23)) return GIE_HIP_EUNSUPPORTED;  // 512 threads for each: a launch's limit
     a.tiles_m = int(tm);
     a.tiles_n = int(tn);
   }

@@ -132,24 +132,27 @@ __device__ __forceinline__ RowTile row_tile(const AttnArgs& a, int slot) {
   return t;
 }
 
-template <typename E, int D, int RQ, int WR, int WK, int NST>
-__global__ __launch_bounds__(64 * WR * WK, D == 256 ? 1 : 2) void attention_kernel(AttnArgs a) {
+// WD waves take the same rows and a part of the head's values each: they work out the same scores (the first product is
+// theirs in full) and sum their part of V.
+template <typename E, int D, int RQ, int WR, int WK, int WD, int NST>
+__global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_kernel(AttnArgs a) {
   static_assert(WR == 1 || WK == 1, "waves share a tile of keys or have their own");
+  static_assert(WD == 1 || (WD == 2 && WR > 1), "one of two loads K, the other V");
   constexpr int R = RQ * WR * 32;             // rows of the workgroup
   constexpr int TT = WR > 1 ? 16 * WR : 32;   // positions of a tile
   constexpr int NS = TT / 32;                 // 32-position parts of a tile
   constexpr int GR = TT / 16 / WR;            // 16-position granules that a wave loads
   constexpr int P = kPitch<D>;
-  constexpr int KS = D / 16, DT = D / 32;     // steps of the first product, 32-wide parts of the second
+  constexpr int KS = D / 16, DT = D / 32 / WD;  // steps of the first product, a wave's 32-wide parts of the second
   constexpr int kGran = 16 * P;               // LDS bytes of a granule
   constexpr int IPG = kGran / 1024;           // loads of a granule
   constexpr int kTileB = TT * P;              // of a tile of K or of V
   constexpr int kStage = 2 * kTileB;
-  constexpr int LPT = 2 * GR * IPG;           // a wave's loads for a tile
+  constexpr int LPT = 2 / WD * GR * IPG;      // a wave's loads for a tile
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = int(threadIdx.x), lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wr = WR > 1 ? wave : 0, wk = WR > 1 ? 0 : wave;
+  const int wr = WR > 1 ? wave % WR : 0, wk = WR > 1 ? 0 : wave, wd = WD > 1 ? wave / WR : 0;
 
   // neighbouring workgroups take different key heads, so that one head's keys stay in one XCD's L2; the last rows of a
   // sequence, which see the most keys, go first
@@ -241,10 +244,12 @@ __global__ __launch_bounds__(64 * WR * WK, D == 256 ? 1 : 2) void attention_kern
       // a vector instruction may have written these scalar registers: loads may read them 5 cycles later
       asm volatile("s_nop 4" : "+s"(rk), "+s"(rv));
       const unsigned to = lds0 + unsigned(stage * kStage + gi * kGran);
+      if (WD == 1 || wd == 0)
 #pragma unroll
-      for (int i = 0; i < IPG; ++i) dma16(rk, to + i * 1024, k_off[i]);
+        for (int i = 0; i < IPG; ++i) dma16(rk, to + i * 1024, k_off[i]);
+      if (WD == 1 || wd == 1)
 #pragma unroll
-      for (int i = 0; i < IPG; ++i) dma16(rv, to + kTileB + i * 1024, v_off[i % VP] + i / VP * VP * RI * 2 * D);
+        for (int i = 0; i < IPG; ++i) dma16(rv, to + kTileB + i * 1024, v_off[i % VP] + i / VP * VP * RI * 2 * D);
     }
   };
 
@@ -253,7 +258,7 @@ __global__ __launch_bounds__(64 * WR * WK, D == 256 ? 1 : 2) void attention_kern
   const unsigned k_rd = lds0 + unsigned((lane & 31) * P + ((half ^ k_swizzle<D>(lane & 15)) << 4));
   const unsigned v_row = unsigned(4 * half + (sl >> 2));
   const unsigned v_chunk = unsigned((2 * (g16 & 1) + ((sl & 3) >> 1)) ^ v_swizzle<D>(sl >> 2));
-  const unsigned v_rd = lds0 + unsigned(kTileB) + v_row * P + (v_chunk << 4) + ((sl & 1) << 3);
+  const unsigned v_rd = (lds0 + unsigned(kTileB) + v_row * P + (v_chunk << 4) + ((sl & 1) << 3)) ^ unsigned(wd * DT * 64);
 
   f32x16 o[RQ][DT] = {};
   float m[RQ], mc[RQ], l[RQ];  // running maximum of the products, its power of 2 (0 while there is none), sum
@@ -268,19 +273,19 @@ __global__ __launch_bounds__(64 * WR * WK, D == 256 ? 1 : 2) void attention_kern
     if ((at0 + TT - 1 > pos_first && pos_first != pos_last) || (a.window > 0 && at0 <= pos_last - a.window)) {
       uint32_t bad = 0;
 #pragma unroll
-      for (int i = 0; i < kTileB / 1024 / WR; ++i) {
+      for (int i = 0; i < kTileB / 1024 / (WR * WD); ++i) {
         const u32x4 v =
-            *reinterpret_cast<const lds_v4*>(size_t(lds0 + so + unsigned(kTileB + (i * WR + wr) * 1024 + lane * 16)));
+            *reinterpret_cast<const lds_v4*>(size_t(lds0 + so + unsigned(kTileB + (i * WR * WD + (WR > 1 ? wave : 0)) * 1024 + lane * 16)));
         bad |= not_finite<E>(v.x) | not_finite<E>(v.y) | not_finite<E>(v.z) | not_finite<E>(v.w);
       }
       bool any = __any(bad != 0);
       if constexpr (WR > 1) {  // waves that share the tile looked at a part of it each
         lds_i* found = reinterpret_cast<lds_i*>(size_t(lds0 + unsigned(NST * kStage)));
-        if (lane == 0) found[wr] = any;
+        if (lane == 0) found[wave] = any;
         stage_barrier();
         any = false;
 #pragma unroll
-        for (int w = 0; w < WR; ++w) any |= __builtin_amdgcn_readfirstlane(found[w]) != 0;
+        for (int w = 0; w < WR * WD; ++w) any |= __builtin_amdgcn_readfirstlane(found[w]) != 0;
       }
       if (any) {
         for (int k = 0; k < TT; ++k) {
@@ -293,7 +298,7 @@ __global__ __launch_bounds__(64 * WR * WK, D == 256 ? 1 : 2) void attention_kern
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int dim = 32 * d + 8 * i + 4 * half;  // 4 of them
+              const int dim = 32 * (wd * DT + d) + 8 * i + 4 * half;  // 4 of them
               const u32x2 v = *reinterpret_cast<const lds_v2*>(
                   size_t(row + unsigned((((dim >> 3) ^ v_swizzle<D>(k)) << 4) + (dim & 4) * 2)));
 #pragma unroll
@@ -307,7 +312,7 @@ __global__ __launch_bounds__(64 * WR * WK, D == 256 ? 1 : 2) void attention_kern
             }
         }
         if (WR > 1) stage_barrier();
-        for (int c = (WR > 1 ? tid : lane); c < kTileB / 16; c += WR * 64) {
+        for (int c = (WR > 1 ? tid : lane); c < kTileB / 16; c += WR * WD * 64) {
           lds_v4* at16 = reinterpret_cast<lds_v4*>(size_t(lds0 + so + unsigned(kTileB + c * 16)));
           u32x4 v = *at16;
 #pragma unroll
@@ -350,7 +355,7 @@ __global__ __launch_bounds__(64 * WR * WK, D == 256 ? 1 : 2) void attention_kern
 #pragma unroll
         for (int r = 0; r < RQ; ++r) s[r] = E::mfma32(kf[ks], qf[r][ks], s[r]);
       // both halves of a part's V (16 keys each) where the registers hold them
-      constexpr int VH = D < 256 ? 2 : 1;
+      constexpr int VH = DT < 8 ? 2 : 1;
       u32x4 vf[VH][DT];
       const auto read_v = [&](int h) {
         unsigned vo = v_rd + so;
@@ -545,7 +550,7 @@ __global__ __launch_bounds__(64 * WR * WK, D == 256 ? 1 : 2) void attention_kern
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int dim = 32 * d + 8 * i + 4 * half;
+        const int dim = 32 * (wd * DT + d) + 8 * i + 4 * half;
         f32x4 v = {o[r][d][4 * i], o[r][d][4 * i + 1], o[r][d][4 * i + 2], o[r][d][4 * i + 3]};
         if (range.splits > 1) {
           *reinterpret_cast<f32x4*>(part + dim) = v;
@@ -627,16 +632,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 
 // ---- launch shape: the same on both sides of the workspace query ----
 struct Shape {
-  bool wide;  // rows of a workgroup: 256 that share tiles of 64 keys, or 32 with keys of their own for each wave
+  bool wide;  // rows of a workgroup: 128 that share tiles of 64 keys, or 32 with tiles of 32 for each wave
   int slots, splits, chunk;
 };
 
-constexpr int kNarrowRows = 32;
-// 64 rows for each wave halve the LDS reads of a product; at head_dim 256 their sums would not fit the registers
-template <int D>
-constexpr int kWideTiles = D == 256 ? 1 : 2;
-constexpr int wide_waves(int) { return 4; }
-constexpr int wide_rows(int head_dim) { return 32 * wide_waves(head_dim); }
+constexpr int kNarrowRows = 32, kWideRows = 128, kNarrowKeys = 32, kWideKeys = 64;  // a tile's
 
 Shape shape_of(const gie_paged_geom& g) {
   Shape s;
@@ -644,7 +644,7 @@ Shape shape_of(const gie_paged_geom& g) {
   const long long rows = (long long)g.total_tokens * group;
   const int most_new = g.max_new > 0 ? g.max_new : (g.total_tokens + g.batch - 1) / g.batch;
   s.wide = (long long)most_new * group > kNarrowRows;
-  const int R = s.wide ? wide_rows(g.head_dim) : kNarrowRows, tt = s.wide ? 16 * wide_waves(g.head_dim) : 32;
+  const int R = s.wide ? kWideRows : kNarrowRows, tt = s.wide ? kWideKeys : kNarrowKeys;
   s.slots = int(rows / R) + g.batch;
   // tiles of rows that hold any, about
   const long long busy = (rows + R - 1) / R > g.batch ? (rows + R - 1) / R : g.batch;
@@ -692,23 +692,24 @@ int start(K kernel, int grid, int threads, int lds_bytes, hipStream_t stream, co
 template <typename E, int D>
 int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   const long long grid = (long long)s.slots * s.splits * a.kv_heads;
-  if (grid > 0x7fffffff) return GIE_HIP_EINVAL;
+  const long long rows = (long long)a.total_tokens * a.q_heads;
+  if (grid * 512 > 0xffffffffll || rows * 64 > 0xffffffffll) return GIE_HIP_EUNSUPPORTED;  // a launch's threads
   constexpr int P = kPitch<D>;
   int rc;
   if (s.wide) {
     constexpr int NST = 2;
-    rc = start(attention_kernel<E, D, 1, wide_waves(D), 1, NST>, int(grid), 64 * wide_waves(D), NST * 2 * 16 * wide_waves(D) * P + 64, stream, a);
+    constexpr int WR = kWideRows / 32, WD = D == 256 ? 2 : 1;
+    rc = start(attention_kernel<E, D, 1, WR, 1, WD, NST>, int(grid), 64 * WR * WD, NST * 2 * 16 * WR * P + 64, stream, a);
   } else {
     constexpr int WK = D == 256 ? 2 : 4, NST = D == 64 ? 4 : 2;
     constexpr int bytes = WK * NST * 2 * 32 * P, join = WK * 256 + WK * 32 * (D + 4) * 4;
-    rc = start(attention_kernel<E, D, 1, 1, WK, NST>, int(grid), 64 * WK, bytes > join ? bytes : join, stream, a);
+    rc = start(attention_kernel<E, D, 1, 1, WK, 1, NST>, int(grid), 64 * WK, bytes > join ? bytes : join, stream, a);
   }
   if (rc != GIE_HIP_OK || s.splits == 1) return rc;
-  const long long rows = (long long)a.total_tokens * a.q_heads;
   const bool many = s.splits > 8;
-  constexpr int RW = wide_rows(D), TW = 16 * wide_waves(D), RN = kNarrowRows;
-  const auto join = s.wide ? (many ? join_kernel<E, D, RW, TW, 4> : join_kernel<E, D, RW, TW, 1>)
-                           : (many ? join_kernel<E, D, RN, 32, 4> : join_kernel<E, D, RN, 32, 1>);
+  const auto join =
+      s.wide ? (many ? join_kernel<E, D, kWideRows, kWideKeys, 4> : join_kernel<E, D, kWideRows, kWideKeys, 1>)
+             : (many ? join_kernel<E, D, kNarrowRows, kNarrowKeys, 4> : join_kernel<E, D, kNarrowRows, kNarrowKeys, 1>);
   hipLaunchKernelGGL(join, dim3(unsigned(many ? rows : (rows + 3) / 4)), dim3(256), 0, stream, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? GIE_HIP_OK : int(e);
@@ -766,16 +767,17 @@ extern "C" int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const
   a.page_shift = shift;
   a.page_magic = unsigned(((((1ull << shift) - unsigned(a.page16)) << 32) / unsigned(a.page16)) + 1);
   a.capacity = g->max_pages * g->page_size;
-  a.window = g->window;
+  a.window = g->window < a.capacity ? g->window : 0;  // no position lies further back
   constexpr float kLog2E = 1.44269504088896341f;
   const float scale = g->scale < 0 ? -g->scale : g->scale;
   a.negate = g->scale < 0;
   if (g->softcap > 0) {
     a.mult = kLog2E;
     a.cap = g->softcap;
-    a.cap_in = 2.f * kLog2E * (scale / g->softcap);  // tanh(x) = 1 - 2 / (2^(2 log2(e) x) + 1)
+    // tanh(x) = 1 - 2 / (2^(2 log2(e) x) + 1); factors stay finite, or a product of 0 would become a NaN
+    a.cap_in = fminf(2.f * kLog2E * (scale / g->softcap), 3e38f);
   } else {
-    a.mult = scale * kLog2E;
+    a.mult = fminf(scale * kLog2E, 3e38f);
   }
   a.splits = shape.splits;
   a.chunk = shape.chunk;

@@ -17,7 +17,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* __r
                                                                  int features, int8_t* __restrict__ q, long long ld_q,
                                                                  float* __restrict__ scale) {
   constexpr int kE = E::kDtype == GIE_HIP_FP32 ? 4 : 2, kPer = 16 / kE;
-  const long long row = (long long)blockIdx.x * (kThreads / T) + threadIdx.x / T;
+  const long long row = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * (kThreads / T) + threadIdx.x / T;
   const bool there = row < tokens;  // a wave without a row still meets the others' barriers
   const int me = int(threadIdx.x) % T;
   const long long x0 = there ? row * ld_x : 0;
@@ -58,13 +58,12 @@ template <typename E>
 void launch(const void* x, long long ld_x, int tokens, int features, int8_t* q, long long ld_q, float* scale, bool vec,
             hipStream_t s) {
   constexpr int kE = E::kDtype == GIE_HIP_FP32 ? 4 : 2;
-  if (features * kE <= 64 * 16 * 2) {
-    const auto kernel = vec ? quantize_rows_kernel<E, 64, true> : quantize_rows_kernel<E, 64, false>;
-    hipLaunchKernelGGL(kernel, dim3((tokens + 3) / 4), dim3(kThreads), 0, s, x, ld_x, tokens, features, q, ld_q, scale);
-  } else {
-    const auto kernel = vec ? quantize_rows_kernel<E, kThreads, true> : quantize_rows_kernel<E, kThreads, false>;
-    hipLaunchKernelGGL(kernel, dim3(tokens), dim3(kThreads), 0, s, x, ld_x, tokens, features, q, ld_q, scale);
-  }
+  const bool small = features * kE <= 64 * 16 * 2;
+  const int blocks = small ? tokens / 4 + (tokens % 4 != 0) : tokens, across = blocks < (1 << 20) ? blocks : 1 << 20;
+  const auto kernel = small ? (vec ? quantize_rows_kernel<E, 64, true> : quantize_rows_kernel<E, 64, false>)
+                            : (vec ? quantize_rows_kernel<E, kThreads, true> : quantize_rows_kernel<E, kThreads, false>);
+  hipLaunchKernelGGL(kernel, dim3(across, blocks / across + (blocks % across != 0)), dim3(kThreads), 0, s, x, ld_x, tokens, features,
+                     q, ld_q, scale);
 }
 
 }  // namespace
