@@ -182,7 +182,6 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
     pos[r] = t.seq.base + token;
     if (pos[r] >= a.capacity) pos[r] = -1;  // no valid position: sees nothing
     const uint16_t* src = a.q + (t.seq.first + token) * a.q_stride + head * D;
-    const uint32_t flip = a.negate ? 0x80008000u : 0u;
     if (a.q_vec) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) qf[r][ks] = *reinterpret_cast<const u32x4*>(src + (2 * ks + half) * 8);
@@ -195,10 +194,6 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
           qf[r][ks][e] = uint32_t(two[0]) | (uint32_t(two[1]) << 16);
         }
     }
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) qf[r][ks][e] ^= flip;
   }
   const int wave_first = min(t.row0 + wr * RQ * 32, last_row), wave_last = min(t.row0 + (wr + 1) * RQ * 32 - 1, last_row);
   const int wpos_first = t.seq.base + wave_first / a.group, wpos_last = t.seq.base + wave_last / a.group;
@@ -446,6 +441,14 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
     issue(tile_at(j), j);
     look_up(tile_at(j + 1));
   }
+  if (a.negate) {  // first use of q: it arrives under the loads above
+#pragma unroll
+    for (int r = 0; r < RQ; ++r)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qf[r][ks][e] ^= 0x80008000u;
+  }
   int stage = 0;
   for (int j = 0; j < mine; ++j) {
     wait_vm<(NST - 2) * LPT>();
@@ -660,15 +663,20 @@ Shape shape_of(const gie_paged_geom& g) {
     // bytes bound: one workgroup for each compute unit, whose LDS holds 64 KiB and more on their way
     splits = 256 / blocks;
   } else {
-    // Products: a tile takes 1.4 us on a compute unit by itself and 1.08 us of one that two workgroups share (64 keys,
-    // head_dim 128: measured 990 TFLOP/s over long keys). Parts: a launch, and their sums written and read once.
-    const double unit = g.head_dim / 128.0, mean = tiles - (most_new < len ? most_new : len) / (2.0 * tt);
+    // Products: a tile (64 keys, head_dim 128) takes 1.4 us on a compute unit by itself and 1.08 us of one that two
+    // workgroups share; at head_dim 256, where one fits, 3.5 us. The device's share of all tiles, and as much of a
+    // part's path as the parts differ in length (a prompt's rows see from nothing to all of it). Parts: a launch, and
+    // their sums written and read once. Measured / so estimated, us: 512 tokens over 7680 in 4 parts 93 / 93, in 2 113 /
+    // 104; one prompt of 4096, 16 heads, whole 145 / 138, in 2 parts 178 / 147.
+    const bool single = g.head_dim == 256;
+    const double alone = single ? 3.5 : 1.4 * g.head_dim / 128, shared = single ? 3.5 : 1.08 * g.head_dim / 128;
+    const double mean = tiles - (most_new < len ? most_new : len) / (2.0 * tt), uneven = 1 - mean / tiles;
     double best = 0;
     for (long long n = 1; n <= most && n <= 64; ++n) {
       const long long each = (blocks * n + 255) / 256;  // workgroups of a compute unit
-      const double path = (each == 1 ? 1.4 : 2.16) * unit * double((tiles + n - 1) / n);
-      const double share = 1.08 * unit * blocks * mean / 256;
-      const double join = n == 1 ? 0 : 4 + 2.0 * rows * g.kv_heads * n * (g.head_dim + 4) * 4 / 3.5e6;
+      const double path = (each == 1 || single ? alone : 2 * shared) * double((tiles + n - 1) / n);
+      const double share = shared * blocks * mean / 256 + uneven * path;
+      const double join = n == 1 ? 0 : 4 + 2.0 * rows * g.kv_heads * n * (g.head_dim + 4) * 4 / 5e6;
       const double us = (path > share ? path : share) + join;
       if (n == 1 || us < 0.95 * best) best = us, splits = n;
     }
