@@ -76,6 +76,16 @@ __device__ __forceinline__ uint16_t epilogue(float acc, const uint16_t* __restri
   return E::from_f32(acc);
 }
 
+// Global memory of any alignment in whole pieces: the target reads and writes such with one instruction (its unaligned
+// access mode, which the HSA ABI has on).
+__device__ __forceinline__ u32x4 load_16_bytes(const void* p) {
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+__device__ __forceinline__ void store_16_bytes(void* p, u32x4 v) { __builtin_memcpy(p, &v, 16); }
+__device__ __forceinline__ void store_8_bytes(void* p, u32x2 v) { __builtin_memcpy(p, &v, 8); }
+
 inline int ceil_div_i(long long a, long long b) { return int((a + b - 1) / b); }
 
 // Sets a kernel's dynamic-LDS limit to `bytes` once per (function, device). Each host thread remembers the pairs it

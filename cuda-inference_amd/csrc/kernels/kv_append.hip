@@ -6,8 +6,7 @@
 // Bytes-bound: every value is read once and written once, the tables' rows are shared by all heads of a token and come
 // from the caches. A thread takes 16 values of a head, 8 pairs where they rotate, in 16-byte pieces. A workgroup takes
 // one or more whole tokens: a wave for each finds its sequence, position and page, then the threads go over all of the
-// tokens' values. Rows that are not 16-byte aligned, or whose rotating part is no multiple of 16, take a form that goes
-// value by value.
+// tokens' values. Heads whose rotating part is no multiple of 16 take a form that goes value by value.
 #include "paged_common.h"
 
 namespace gie_hip {
@@ -74,8 +73,8 @@ __device__ __forceinline__ Head head_of(const AppendArgs& a, int t, int head, co
 
 template <typename E, bool INTERLEAVED>
 __device__ __forceinline__ void rotate8(u32x4& a, u32x4& b, const float* cos, const float* sin) {
-  const f32x4 c0 = *reinterpret_cast<const f32x4*>(cos), c1 = *reinterpret_cast<const f32x4*>(cos + 4);
-  const f32x4 s0 = *reinterpret_cast<const f32x4*>(sin), s1 = *reinterpret_cast<const f32x4*>(sin + 4);
+  const f32x4 c0 = __builtin_bit_cast(f32x4, load_16_bytes(cos)), c1 = __builtin_bit_cast(f32x4, load_16_bytes(cos + 4));
+  const f32x4 s0 = __builtin_bit_cast(f32x4, load_16_bytes(sin)), s1 = __builtin_bit_cast(f32x4, load_16_bytes(sin + 4));
   u32x4 x, y;
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
@@ -125,13 +124,13 @@ __global__ __launch_bounds__(1024) void append_kernel(AppendArgs a) {
     const bool pairs = unit < turning;
     const int at = pairs && !INTERLEAVED ? unit * 8 : unit * 16;
     const int next = pairs && !INTERLEAVED ? at + half : at + 8;
-    u32x4 x = *reinterpret_cast<const u32x4*>(h.src + at), y = *reinterpret_cast<const u32x4*>(h.src + next);
+    u32x4 x = load_16_bytes(h.src + at), y = load_16_bytes(h.src + next);
     if (pairs && h.turns && p.position >= 0)
       rotate8<E, INTERLEAVED>(x, y, a.cos + (long long)p.position * half + unit * 8,
                               a.sin + (long long)p.position * half + unit * 8);
     if (p.position < 0) x = u32x4{}, y = u32x4{};
-    *reinterpret_cast<u32x4*>(h.dst + at) = x;
-    *reinterpret_cast<u32x4*>(h.dst + next) = y;
+    store_16_bytes(h.dst + at, x);
+    store_16_bytes(h.dst + next, y);
   }
 }
 
@@ -215,9 +214,7 @@ extern "C" int gie_hip_kv_append(int dtype, const gie_paged_geom* g, const void*
   if (!aligned_to(q, 2) || !aligned_to(k, 2) || !aligned_to(v, 2) || !aligned_to(q_out, 2) ||
       !aligned_to(k_pages, 16) || !aligned_to(v_pages, 16) || !aligned_to(cos, 4) || !aligned_to(sin, 4))
     return GIE_HIP_EINVAL;
-  const bool vec = g->rotary_dim % 16 == 0 && g->k_stride % 8 == 0 && g->v_stride % 8 == 0 && aligned_to(k, 16) &&
-                   aligned_to(v, 16) && aligned_to(cos, 16) && aligned_to(sin, 16) &&
-                   (!q || (g->q_stride % 8 == 0 && g->o_stride % 8 == 0 && aligned_to(q, 16) && aligned_to(q_out, 16)));
+  const bool vec = g->rotary_dim % 16 == 0;
   AppendArgs a{*g, static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                cos, sin, q_starts, seq_lens, page_table, static_cast<uint16_t*>(q_out),
                static_cast<uint16_t*>(k_pages), static_cast<uint16_t*>(v_pages), 1};

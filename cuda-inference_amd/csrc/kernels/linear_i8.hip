@@ -40,7 +40,7 @@ struct LinArgs {
   int relu;
   int splits, per_split;  // parts of the input values, and their steps of 128
   int tiles_m, tiles_n;
-  int x_vec, y_vec;  // rows of x before its quantization, and of y, in 16-byte pieces
+  int y_vec;  // rows of y in 16-byte pieces
 };
 
 template <typename E>
@@ -48,14 +48,9 @@ constexpr int kBytesOf = 2;
 template <>
 constexpr int kBytesOf<F32> = 4;
 
-__device__ __forceinline__ u32x4 load16(const int8_t* p) {  // any alignment
-  u32x4 v;
-  __builtin_memcpy(&v, p, 16);
-  return v;
-}
 // values k .. k + 15 of a row, zeros from K on; nothing behind the row's end is read
 __device__ __forceinline__ u32x4 load16_upto(const int8_t* row, int k, int K) {
-  if (k + 16 <= K) return load16(row + k);
+  if (k + 16 <= K) return load_16_bytes(row + k);
   u32x4 v = {};
   for (int i = 0; i < 16; ++i)
     if (k + i < K) v[i / 4] |= uint32_t(uint8_t(row[k + i])) << (8 * (i % 4));
@@ -140,17 +135,22 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 1) void tile_kernel(LinArgs a) {
   constexpr int kRounds = kRows * 8 / kThreads;
   constexpr int kAhead = kRounds <= 4 ? 4 : 1;  // slices held
   u32x4 held[ALIGNED ? 1 : kAhead][ALIGNED ? 1 : kRounds];
-  const auto fetch = [&](int step, u32x4* to) {
-    const int k0 = k_first + step * 128;
+  const int8_t* rows[ALIGNED ? 1 : kRounds];  // of this thread's pieces; those past the last repeat it and are not stored
+  if constexpr (!ALIGNED) {
 #pragma unroll
     for (int i = 0; i < kRounds; ++i) {
-      const int c = i * kThreads + tid, row = c >> 3, k = k0 + (c & 7) * 16;
-      const bool is_x = row < BM;
-      const int r = is_x ? m0 + row : n0 + row - BM;
-      u32x4 v = {};
-      if (r < (is_x ? a.M : a.N) && k < k_last)
-        v = load16_upto(is_x ? a.x + r * a.ld_x : a.w + r * a.ld_w, k, k_last);
-      to[i] = v;
+      const int row = (i * kThreads + tid) >> 3;
+      rows[i] = row < BM ? a.x + min(m0 + row, a.M - 1) * a.ld_x : a.w + min(n0 + row - BM, a.N - 1) * a.ld_w;
+    }
+  }
+  const auto fetch = [&](int step, u32x4* to) {
+    const int k0 = k_first + step * 128, k = k0 + (tid & 7) * 16;
+    if (k0 + 128 <= k_last) {
+#pragma unroll
+      for (int i = 0; i < kRounds; ++i) to[i] = load_16_bytes(rows[i] + k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRounds; ++i) to[i] = k < k_last ? load16_upto(rows[i], k, k_last) : u32x4{};
     }
   };
   const auto put = [&](int stage, const u32x4* from) {
@@ -415,12 +415,12 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(LinArgs a) {
     constexpr int kPer = 16 / kBytesOf<E>, kKeep = 4;
     for (int t = 0; t < a.M; ++t) {
       const char* row = static_cast<const char*>(a.x16) + t * a.ld_x * kBytesOf<E>;
-      const int pieces = a.x_vec ? a.K / kPer : 0;
+      const int pieces = a.K / kPer;
       u32x4 keep[kKeep];
 #pragma unroll
       for (int i = 0; i < kKeep; ++i) {
         const int p = i * kFewThreads + tid;
-        keep[i] = p < pieces ? reinterpret_cast<const u32x4*>(row)[p] : u32x4{};
+        keep[i] = p < pieces ? load_16_bytes(row + p * 16ll) : u32x4{};
       }
       if (t == 0) {
 #pragma unroll
@@ -503,13 +503,16 @@ struct Plan {
   int tile, tiles_m, tiles_n, splits, per_split;  // tile: tokens and channels of one
 };
 
-// Square tiles of 256, 128, 64 and 32, the largest that still make 192 workgroups (of 256 compute units): a tile moves
-// (1 / tokens + 1 / channels) bytes from the L2 for each product. Measured at 4096 input values, us by tile: 4096x4096 70
-// (256), 84 (128), 144 (64); 1024x4096 29.6 (128), 42 (64), 55 (256); 512x4096 19.6 (64), 27 (128).
-// With less of them, tiles of 64 and 32 and parts of the input values are weighed by what they move: L2 to LDS 14 TB/s
-// (64) and 11.6 TB/s (32), weights 4.2 TB/s, less where the device is not full; 2.5 us and 4 TB/s for parts that are
-// joined. Measured / so estimated, us: 64x4096x4096 10.9 (32, whole) 12.2 (64, 4 parts) / 10.8, 13.5; 64x8192x8192
-// 22.0 (64, 2 parts) 25.3 (32) / 25, 28; 256x1024x16384 19.8 (64, 4 parts) 25.7 (32) / 19, 28.
+// Square tiles of 256, 128, 64 and 32 tokens and channels. A larger one moves less from the L2 for each product, a smaller
+// one leaves less of the device without work; times of a step (128 input values) as measured with 4096 of them: 2.1 us
+// for a round of 256 tiles of 256; 0.85 us for up to 256 tiles of 128, 1.26 us for 512 of them (two to a compute unit);
+// 0.33 us for up to 256 tiles of 64 and 0.27 us for each 256 more. Measured / so estimated, us: 4096x4096 70 / 67 (256),
+// 84 / 81 (128), 144 / 138 (64); 1024x4096 55 / 67, 29.6 / 27, 42 / 35; 512x4096 - , 27 / 27, 19.6 / 17.
+// With less than 192 tiles of 64, these and tiles of 32, whole or over parts of the input values, are weighed by what
+// they move: L2 to LDS 14 TB/s (64) and 11.6 TB/s (32), weights 4.2 TB/s, less where the device is not full; 2.5 us and
+// 4 TB/s for parts that are joined. Measured / so estimated, us: 64x4096x4096 10.9 (32, whole) 12.2 (64, 4 parts) / 5.8,
+// 8.5; 64x8192x8192 22.0 (64, 2 parts) 25.3 (32) / 20, 23; 256x1024x16384 19.8 (64, 4 parts) 25.7 (32) / 14, 23, each
+// without the 5 us that a call costs in any form.
 Plan plan_of(const gie_linear_geom& g) {
   Plan p{};
   const long long M = g.tokens, N = g.out_features;
@@ -521,12 +524,17 @@ Plan plan_of(const gie_linear_geom& g) {
     return p;
   }
   const auto count = [&](int tile) { return (long long)((M + tile - 1) / tile) * ((N + tile - 1) / tile); };
-  if (count(256) >= 192) {
-    p.form = kTile256, p.tile = 256;
-  } else if (count(128) >= 192) {
-    p.form = kTile128, p.tile = 128;
-  } else if (count(64) >= 192) {
-    p.form = kTile64, p.tile = 64;
+  const auto rounds = [](long long n, int of) { return double((n + of - 1) / of); };
+  if (count(64) >= 192) {
+    const double us256 = 2.1 * rounds(count(256), 256);
+    const double us128 = count(128) <= 256 ? 0.85 : 1.26 * rounds(count(128), 512);
+    const double us64 = count(64) <= 256 ? 0.33 : 0.27 * rounds(count(64), 256);
+    if (us256 <= us128 && us256 <= us64)
+      p.form = kTile256, p.tile = 256;
+    else if (us128 <= us64)
+      p.form = kTile128, p.tile = 128;
+    else
+      p.form = kTile64, p.tile = 64;
   } else {
     double best = 0;
     for (int tile = 64; tile >= 32; tile /= 2) {
@@ -651,7 +659,6 @@ extern "C" int gie_hip_linear_i8(int dtype, const gie_linear_geom* g, const void
   if (x_scale == nullptr) {
     if (p.form == kFewForm && fuses(*g)) {
       a.x16 = x;
-      a.x_vec = g->ld_x * esz % 16 == 0 && at(x) % 16 == 0;
     } else {
       const size_t ld = round16(g->in_features);
       int8_t* q = reinterpret_cast<int8_t*>(ws);

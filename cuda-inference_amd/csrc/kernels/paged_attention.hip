@@ -51,7 +51,6 @@ struct AttnArgs {
   float cap_in, cap;  // softcap > 0: cap * tanh(product * cap_in / 2)
   int negate;      // a negative scale: q changes its sign, so that the largest product is the largest score
   int splits, chunk;  // parts of the keys and the fewest tiles of one
-  int q_vec, o_vec;   // q in 16-byte pieces, out in 8-byte pieces
 };
 
 template <int D>
@@ -182,18 +181,8 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
     pos[r] = t.seq.base + token;
     if (pos[r] >= a.capacity) pos[r] = -1;  // no valid position: sees nothing
     const uint16_t* src = a.q + (t.seq.first + token) * a.q_stride + head * D;
-    if (a.q_vec) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qf[r][ks] = *reinterpret_cast<const u32x4*>(src + (2 * ks + half) * 8);
-    } else {
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint16_t* two = src + (2 * ks + half) * 8 + 2 * e;
-          qf[r][ks][e] = uint32_t(two[0]) | (uint32_t(two[1]) << 16);
-        }
-    }
+    for (int ks = 0; ks < KS; ++ks) qf[r][ks] = load_16_bytes(src + (2 * ks + half) * 8);
   }
   const int wave_first = min(t.row0 + wr * RQ * 32, last_row), wave_last = min(t.row0 + (wr + 1) * RQ * 32 - 1, last_row);
   const int wpos_first = t.seq.base + wave_first / a.group, wpos_last = t.seq.base + wave_last / a.group;
@@ -527,12 +516,7 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
           uint16_t* dst = a.out + token * a.o_stride + head * D + d;
           if (total == 0.f) v = f32x4{};
           v *= inv;
-          if (a.o_vec) {
-            *reinterpret_cast<u32x2*>(dst) = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dst[e] = E::from_f32(v[e]);
-          }
+          store_8_bytes(dst, u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])});
         }
       }
     }
@@ -561,12 +545,7 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
         } else {
           if (l[r] == 0.f) v = f32x4{};
           v *= inv;
-          if (a.o_vec) {
-            *reinterpret_cast<u32x2*>(dst + dim) = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dst[dim + e] = E::from_f32(v[e]);
-          }
+          store_8_bytes(dst + dim, u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])});
         }
       }
   }
@@ -625,12 +604,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   uint16_t* dst = a.out + token * a.o_stride + head * D + at * 4;
   if (total == 0.f) v = f32x4{};
   v *= inv;
-  if (a.o_vec) {
-    *reinterpret_cast<u32x2*>(dst) = u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) dst[e] = E::from_f32(v[e]);
-  }
+  store_8_bytes(dst, u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])});
 }
 
 // ---- launch shape: the same on both sides of the workspace query ----
@@ -789,8 +763,6 @@ extern "C" int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const
   }
   a.splits = shape.splits;
   a.chunk = shape.chunk;
-  a.q_vec = g->q_stride % 8 == 0 && aligned_to(q, 16);
-  a.o_vec = g->o_stride % 4 == 0 && aligned_to(out, 8);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool h = dtype == GIE_HIP_FP16;
   switch (g->head_dim) {

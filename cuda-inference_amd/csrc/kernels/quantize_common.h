@@ -77,7 +77,7 @@ __device__ __forceinline__ void unpack<F32>(u32x4 v, float (&f)[8]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[e]);
 }
-// ... and what it becomes, 8 or 4 bytes at `to`
+// ... and what it becomes, 8 or 4 bytes at `to` (any alignment)
 template <typename E>
 __device__ __forceinline__ void quantize_piece(u32x4 v, float inverse, void* to) {
   constexpr int kPer = E::kDtype == GIE_HIP_FP32 ? 4 : 8;
@@ -86,10 +86,7 @@ __device__ __forceinline__ void quantize_piece(u32x4 v, float inverse, void* to)
   uint32_t w[2] = {0, 0};
 #pragma unroll
   for (int e = 0; e < kPer; ++e) w[e / 4] |= uint32_t(uint8_t(quantize_value(f[e], inverse))) << (8 * (e & 3));
-  if constexpr (kPer == 8)
-    *static_cast<u32x2*>(to) = u32x2{w[0], w[1]};
-  else
-    *static_cast<uint32_t*>(to) = w[0];
+  __builtin_memcpy(to, w, kPer);
 }
 
 }  // namespace gie_hip

@@ -11,8 +11,8 @@ namespace {
 
 constexpr int kThreads = 256, kKeep = 4;
 
-// T threads for each row. kVec: rows of x in 16-byte pieces, rows of q in the pieces that these become
-template <typename E, int T, bool kVec>
+// T threads for each row; rows of x and q of any alignment
+template <typename E, int T>
 __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* __restrict__ x, long long ld_x, int tokens,
                                                                  int features, int8_t* __restrict__ q, long long ld_q,
                                                                  float* __restrict__ scale) {
@@ -21,13 +21,13 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* __r
   const bool there = row < tokens;  // a wave without a row still meets the others' barriers
   const int me = int(threadIdx.x) % T;
   const long long x0 = there ? row * ld_x : 0;
-  const int pieces = kVec && there ? features / kPer : 0;  // whole ones; the rest value by value
+  const int pieces = there ? features / kPer : 0;  // whole ones; the rest value by value
   const int rest = there ? pieces * kPer : features;
-  const u32x4* xv = reinterpret_cast<const u32x4*>(static_cast<const char*>(x) + x0 * kE);
+  const char* xv = static_cast<const char*>(x) + x0 * kE;
   float a = 0;
   u32x4 keep[kKeep];
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i) keep[i] = i * T + me < pieces ? xv[i * T + me] : u32x4{};
+  for (int i = 0; i < kKeep; ++i) keep[i] = i * T + me < pieces ? load_16_bytes(xv + (i * T + me) * 16ll) : u32x4{};
 #pragma unroll
   for (int i = 0; i < kKeep; ++i) {
     float f[8];
@@ -37,7 +37,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* __r
   }
   for (int p = kKeep * T + me; p < pieces; p += T) {
     float f[8];
-    unpack<E>(xv[p], f);
+    unpack<E>(load_16_bytes(xv + p * 16ll), f);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) a = magnitude_max(a, f[e]);
   }
@@ -50,18 +50,16 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* __r
 #pragma unroll
   for (int i = 0; i < kKeep; ++i)
     if (i * T + me < pieces) put(i * T + me, keep[i]);
-  for (int p = kKeep * T + me; p < pieces; p += T) put(p, xv[p]);
+  for (int p = kKeep * T + me; p < pieces; p += T) put(p, load_16_bytes(xv + p * 16ll));
   for (int k = rest + me; k < features; k += T) out[k] = quantize_value(load_value<E>(x, x0 + k), s.inverse);
 }
 
 template <typename E>
-void launch(const void* x, long long ld_x, int tokens, int features, int8_t* q, long long ld_q, float* scale, bool vec,
-            hipStream_t s) {
+void launch(const void* x, long long ld_x, int tokens, int features, int8_t* q, long long ld_q, float* scale, hipStream_t s) {
   constexpr int kE = E::kDtype == GIE_HIP_FP32 ? 4 : 2;
   const bool small = features * kE <= 64 * 16 * 2;
   const int blocks = small ? tokens / 4 + (tokens % 4 != 0) : tokens, across = blocks < (1 << 20) ? blocks : 1 << 20;
-  const auto kernel = small ? (vec ? quantize_rows_kernel<E, 64, true> : quantize_rows_kernel<E, 64, false>)
-                            : (vec ? quantize_rows_kernel<E, kThreads, true> : quantize_rows_kernel<E, kThreads, false>);
+  const auto kernel = small ? quantize_rows_kernel<E, 64> : quantize_rows_kernel<E, kThreads>;
   hipLaunchKernelGGL(kernel, dim3(across, blocks / across + (blocks % across != 0)), dim3(kThreads), 0, s, x, ld_x, tokens, features,
                      q, ld_q, scale);
 }
@@ -78,15 +76,13 @@ extern "C" int gie_hip_quantize_rows(int dtype, const void* x, int64_t ld_x, int
   if (!x || !q || !scale) return GIE_HIP_EINVAL;
   const size_t esz = dtype == GIE_HIP_FP32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(x) % esz != 0 || reinterpret_cast<uintptr_t>(scale) % 4 != 0) return GIE_HIP_EINVAL;
-  const bool vec = ld_x * esz % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld_q % (16 / esz) == 0 &&
-                   reinterpret_cast<uintptr_t>(q) % (16 / esz) == 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == GIE_HIP_FP32)
-    launch<F32>(x, ld_x, tokens, features, q, ld_q, scale, vec, s);
+    launch<F32>(x, ld_x, tokens, features, q, ld_q, scale, s);
   else if (dtype == GIE_HIP_FP16)
-    launch<Fp16>(x, ld_x, tokens, features, q, ld_q, scale, vec, s);
+    launch<Fp16>(x, ld_x, tokens, features, q, ld_q, scale, s);
   else if (dtype == GIE_HIP_BF16)
-    launch<Bf16>(x, ld_x, tokens, features, q, ld_q, scale, vec, s);
+    launch<Bf16>(x, ld_x, tokens, features, q, ld_q, scale, s);
   else
     return GIE_HIP_EUNSUPPORTED;
   const hipError_t e = hipGetLastError();
