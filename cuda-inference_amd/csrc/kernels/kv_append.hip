@@ -7,6 +7,10 @@
 // from the caches. A thread takes 16 values of a head, 8 pairs where they rotate, in 16-byte pieces. A workgroup takes
 // one or more whole tokens: a wave for each finds its sequence, position and page, then the threads go over all of the
 // tokens' values. Heads whose rotating part is no multiple of 16 take a form that goes value by value.
+//
+// 8192 tokens of 32 + 2 x 8 heads of 128: 32 us, 6.4 TB/s (a large copy reaches 4.7: part of what is written stays in the
+// caches); 64 tokens of one sequence each 3.6 us, which is a launch and the chain lengths -> page -> tables -> store. One
+// value for each thread, and a search that loads one place after another, took 63 and 7.0 us.
 #include "paged_common.h"
 
 namespace gie_hip {

@@ -18,6 +18,14 @@
 // outside the cache, arrives as zeros. 16-byte chunks of a row are permuted by the row so that the fragment reads meet
 // no bank twice in a phase. The waves of a workgroup either share a tile of keys (WR > 1: one barrier for each tile) or
 // take tiles of their own (WR == 1, WK waves, no barrier until their results are joined).
+//
+// Few rows (one token of a grouped head: up to 32) are bound by the cache's bytes: one token over 32768 positions of 8 key
+// heads of 128 in 32 parts 24 us + 4 for the join, 4.6 TB/s in all; a step of 64 sequences 219 us, 5.0 TB/s (a large copy
+// reaches 4.7). Many rows are bound by the products: two prompts of 4096 tokens, 32 heads of 128, 303-312 us, 0.9 PFLOP/s
+// (a large library product 1.23); 2048 tokens over 30000 1.0. Matrix cores are busy 0.4 of the time, the vector unit
+// (softmax) 0.35 and LDS 0.22, on two workgroups of 4 waves for each compute unit: measured without exponentials -5 %,
+// without any softmax -13 %, without loads -16 %. 64 rows for each wave (half the LDS reads, one wave for each SIMD)
+// took 408 us for what now takes 310, eight waves sharing a tile 318 and more for ragged batches.
 #include "paged_common.h"
 
 #include "lds_pipe.h"
@@ -637,13 +645,15 @@ Shape shape_of(const gie_paged_geom& g) {
     // bytes bound: one workgroup for each compute unit, whose LDS holds 64 KiB and more on their way
     splits = 256 / blocks;
   } else {
-    // Products: a tile (64 keys, head_dim 128) takes 1.4 us on a compute unit by itself and 1.08 us of one that two
-    // workgroups share; at head_dim 256, where one fits, 3.5 us. The device's share of all tiles, and as much of a
-    // part's path as the parts differ in length (a prompt's rows see from nothing to all of it). Parts: a launch, and
-    // their sums written and read once. Measured / so estimated, us: 512 tokens over 7680 in 4 parts 93 / 93, in 2 113 /
-    // 104; one prompt of 4096, 16 heads, whole 145 / 138, in 2 parts 178 / 147.
+    // Products: what a tile of 64 keys takes on a compute unit by itself, and the share of one that two workgroups have,
+    // us as measured (head_dim 64, 96, 128: 1.5, 1.8, 2.0 by itself over caches of their own, 1.4 at 128 over a shared
+    // one, 1.08 shared; capped scores 0.75 more; head_dim 256, where one fits: 3.5). The device's share of all tiles, and
+    // as much of a part's path as the parts differ in length (a prompt's rows see from nothing to all of it). Parts: a
+    // launch, and their sums written and read once. Measured / so estimated, us: 512 tokens over 7680 in 4 parts 93 / 88,
+    // in 2 113 / 112; one prompt of 4096, 16 heads, whole 118 / 138, in 2 parts 178 / 131 (so only 10 % less counts).
     const bool single = g.head_dim == 256;
-    const double alone = single ? 3.5 : 1.4 * g.head_dim / 128, shared = single ? 3.5 : 1.08 * g.head_dim / 128;
+    const double size = g.head_dim / 128.0, cap = g.softcap > 0 ? 0.7 : 0;
+    const double alone = single ? 3.5 : 0.9 + 0.6 * size + cap, shared = single ? 3.5 : 0.5 + 0.58 * size + cap;
     const double mean = tiles - (most_new < len ? most_new : len) / (2.0 * tt), uneven = 1 - mean / tiles;
     double best = 0;
     for (long long n = 1; n <= most && n <= 64; ++n) {
@@ -652,7 +662,7 @@ Shape shape_of(const gie_paged_geom& g) {
       const double share = shared * blocks * mean / 256 + uneven * path;
       const double join = n == 1 ? 0 : 4 + 2.0 * rows * g.kv_heads * n * (g.head_dim + 4) * 4 / 5e6;
       const double us = (path > share ? path : share) + join;
-      if (n == 1 || us < 0.95 * best) best = us, splits = n;
+      if (n == 1 || us < 0.9 * best) best = us, splits = n;
     }
   }
   if (splits > most) splits = most;
