@@ -37,6 +37,8 @@ typedef __attribute__((address_space(4))) const int const_int;  // uniform loads
 typedef __attribute__((address_space(3))) u32x4 lds_v4;
 typedef __attribute__((address_space(3))) u32x2 lds_v2;
 typedef __attribute__((address_space(3))) int lds_i;
+typedef __attribute__((address_space(3))) long long lds_ll;
+typedef __attribute__((address_space(3))) f32x4 lds_f4;
 typedef short v4s __attribute__((ext_vector_type(4)));
 
 struct AttnArgs {
@@ -324,7 +326,7 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
 
     // Part by part of 32 keys. What a product reads from LDS is requested ahead of it: half of V under the softmax, the
     // other half and the next part's K under the second product.
-    constexpr bool kAhead = D < 256;  // where the registers hold it
+    constexpr bool kAhead = WD == 1;  // where the registers hold it, or little else waits (narrow, bytes bound)
     u32x4 kf[KS];
     const auto read_k = [&](int n) {
       unsigned ko = k_rd + so;
@@ -341,11 +343,32 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
       f32x16 s[RQ];
 #pragma unroll
       for (int r = 0; r < RQ; ++r) s[r] = f32x16{};
-      if (!kAhead) read_k(n);
+      if constexpr (kAhead) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int r = 0; r < RQ; ++r) s[r] = E::mfma32(kf[ks], qf[r][ks], s[r]);
+          for (int r = 0; r < RQ; ++r) s[r] = E::mfma32(kf[ks], qf[r][ks], s[r]);
+      } else {  // four steps ahead; left to itself the compiler waits for every read (head_dim 256: x us a tile for y)
+        unsigned ko = k_rd + so;
+        asm volatile("" : "+v"(ko));
+        const auto read_4 = [&](int g) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            kf[g % 2 * 4 + i] =
+                *reinterpret_cast<const lds_v4*>(size_t((ko ^ unsigned((g * 4 + i) * 32)) + unsigned(n * 32 * P)));
+        };
+        read_4(0);
+#pragma unroll
+        for (int g = 0; g < KS / 4; ++g) {
+          if (g + 1 < KS / 4) read_4(g + 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < RQ; ++r) s[r] = E::mfma32(kf[g % 2 * 4 + i], qf[r][g * 4 + i], s[r]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
       // both halves of a part's V (16 keys each) where the registers hold them
       constexpr int VH = DT < 8 ? 2 : 1;
       u32x4 vf[VH][DT];
@@ -531,31 +554,68 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
     return;
   }
 
-  // ---- rows to out, or to the parts that are joined ----
+  // ---- rows to out, or to the parts that are joined: through LDS, so that a store covers whole lines of a row (from
+  // where the products leave them, 8 bytes of 32 rows at a time, they took 3.3 us longer at head_dim 256, 1.3 at 128) ----
+  __syncthreads();  // the stages are free
+  constexpr int kRowB = DT * 64, kPad = kRowB + 16, kPadF = 128 + 16;  // a wave's part of a row; 32 FP32 values of one
+  const unsigned mine_rows = lds0 + unsigned(wave * 32 * kPad);
 #pragma unroll
   for (int r = 0; r < RQ; ++r) {
-    const int row = (wr * RQ + r) * 32 + (lane & 31);
-    if (row >= t.rows) continue;
-    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+    const int rl = lane & 31;
+    const bool there = (wr * RQ + r) * 32 + rl < t.rows;
     int token, head;
     place(r, token, head);
-    float* part = a.part + (((long long)token * a.q_heads + head) * a.splits + z) * (D + 4);
-    uint16_t* dst = a.out + token * a.o_stride + head * D;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int dim = 32 * (wd * DT + d) + 8 * i + 4 * half;
-        f32x4 v = {o[r][d][4 * i], o[r][d][4 * i + 1], o[r][d][4 * i + 2], o[r][d][4 * i + 3]};
-        if (range.splits > 1) {
-          *reinterpret_cast<f32x4*>(part + dim) = v;
-          if (dim == 0) part[D] = m[r] == -INFINITY ? -INFINITY : mc[r], part[D + 1] = l[r];
-        } else {
-          if (l[r] == 0.f) v = f32x4{};
-          v *= inv;
-          store_8_bytes(dst + dim, u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])});
-        }
+    const bool parts = range.splits > 1;
+    const long long to = !there  ? -1
+                         : parts ? (((long long)token * a.q_heads + head) * a.splits + z) * (D + 4) + wd * DT * 32
+                                 : token * a.o_stride + head * D + wd * DT * 32;
+    const unsigned row = mine_rows + unsigned(rl * (parts ? kPadF : kPad));
+    if (half == 0) *reinterpret_cast<lds_ll*>(size_t(row + unsigned(parts ? 128 : kRowB))) = to;
+    if (parts) {
+      if (there && half == 0 && wd == 0) {
+        a.part[to + D] = m[r] == -INFINITY ? -INFINITY : mc[r];
+        a.part[to + D + 1] = l[r];
       }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<lds_f4*>(size_t(row + unsigned((8 * i + 4 * half) * 4))) =
+              f32x4{o[r][d][4 * i], o[r][d][4 * i + 1], o[r][d][4 * i + 2], o[r][d][4 * i + 3]};
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned from = mine_rows + unsigned((j * 8 + lane / 8) * kPadF);
+          const long long at = *reinterpret_cast<const lds_ll*>(size_t(from + 128u));
+          const f32x4 v = *reinterpret_cast<const lds_f4*>(size_t(from + unsigned(lane % 8 * 16)));
+          if (at >= 0) *reinterpret_cast<f32x4*>(a.part + at + d * 32 + lane % 8 * 4) = v;
+        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+      }
+    } else {
+      const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f32x4 v = {o[r][d][4 * i], o[r][d][4 * i + 1], o[r][d][4 * i + 2], o[r][d][4 * i + 3]};
+          if (l[r] == 0.f) v = f32x4{};  // nothing seen (and what was summed for it may be a NaN)
+          v *= inv;
+          *reinterpret_cast<lds_v2*>(size_t(row + unsigned((32 * d + 8 * i + 4 * half) * 2))) =
+              u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
+        }
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      constexpr int kPieces = kRowB / 16;
+#pragma unroll
+      for (int j = 0; j < kPieces / 2; ++j) {
+        const int piece = j * 64 + lane, from_row = piece / kPieces, c = piece % kPieces;
+        const unsigned from = mine_rows + unsigned(from_row * kPad);
+        const long long at = *reinterpret_cast<const lds_ll*>(size_t(from + unsigned(kRowB)));
+        const u32x4 v = *reinterpret_cast<const lds_v4*>(size_t(from + unsigned(c * 16)));
+        if (at >= 0) store_16_bytes(a.out + at + c * 8, v);
+      }
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+    }
   }
 }
 
