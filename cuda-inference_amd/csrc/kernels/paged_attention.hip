@@ -190,9 +190,18 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
     const int token = row / a.group, head = kvh * a.group + (row - token * a.group);
     pos[r] = t.seq.base + token;
     if (pos[r] >= a.capacity) pos[r] = -1;  // no valid position: sees nothing
-    const uint16_t* src = a.q + (t.seq.first + token) * a.q_stride + head * D;
+    const long long src = (t.seq.first + token) * a.q_stride + head * D;
+    if constexpr (WR == 1) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[r][ks] = load_16_bytes(src + (2 * ks + half) * 8);
+      for (int ks = 0; ks < KS; ++ks) qf[r][ks] = load_16_bytes(a.q + src + (2 * ks + half) * 8);
+    } else {  // whole rows, 16 bytes for each lane; they go through LDS below (WD waves: a part of the rows each)
+#pragma unroll
+      for (int j = 0; j < KS / WD; ++j) {
+        const int piece = (j + wd * (KS / WD)) * 64 + lane, row_of = piece / (D / 8);
+        const unsigned lo = unsigned(__shfl(int(src), row_of)), hi = unsigned(__shfl(int(src >> 32), row_of));
+        qf[r][j] = load_16_bytes(a.q + (long long)((unsigned long long)hi << 32 | lo) + piece % (D / 8) * 8);
+      }
+    }
   }
   const int wave_first = min(t.row0 + wr * RQ * 32, last_row), wave_last = min(t.row0 + (wr + 1) * RQ * 32 - 1, last_row);
   const int wpos_first = t.seq.base + wave_first / a.group, wpos_last = t.seq.base + wave_last / a.group;
@@ -460,6 +469,22 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
   for (int j = 0; j < NST - 1; ++j) {
     issue(tile_at(j), j);
     look_up(tile_at(j + 1));
+  }
+  if constexpr (WR > 1) {  // rows of q to the lanes that multiply them, by way of the stage that is loaded last
+    static_assert(RQ == 1 && WR * 32 * P <= kStage, "one tile of rows for each wave fits a stage");
+    const unsigned rows = lds0 + unsigned((NST - 1) * kStage + wr * 32 * P);
+#pragma unroll
+    for (int j = 0; j < KS / WD; ++j) {
+      const int piece = (j + wd * (KS / WD)) * 64 + lane, row = piece / (D / 8), c = piece % (D / 8);
+      *reinterpret_cast<lds_v4*>(size_t(rows + unsigned(row * P + ((c ^ k_swizzle<D>(row & 15)) << 4)))) = qf[0][j];
+    }
+    if (WD > 1)
+      stage_barrier();
+    else
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+    const unsigned mine = rows + unsigned((lane & 31) * P + ((half ^ k_swizzle<D>(lane & 15)) << 4));
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[0][ks] = *reinterpret_cast<const lds_v4*>(size_t(mine ^ unsigned(ks * 32)));
   }
   if (a.negate) {  // first use of q: it arrives under the loads above
 #pragma unroll
