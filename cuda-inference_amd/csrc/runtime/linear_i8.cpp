@@ -68,7 +68,7 @@ void LinearI8::forward(const void* x, const float* x_scale, const int8_t* w, con
   GIE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), StatusCode::kWorkspaceTooSmall,
               "LinearI8: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) +
                   " needed");
-  require(need == 0 || aligned(workspace, 16), "workspace must be 16-byte aligned");
+  require(aligned(workspace, 16), "workspace must be 16-byte aligned");
   RoctxRange range("gie::LinearI8::forward");
   check_kernel_status(
       gie_hip_linear_i8(dtype, &g, x, x_scale, w, w_scale, bias, y, workspace, workspace_bytes, stream),

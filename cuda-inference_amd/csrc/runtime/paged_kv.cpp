@@ -129,7 +129,7 @@ void PagedKv::attention(const void* q, const void* k_pages, const void* v_pages,
   GIE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), StatusCode::kWorkspaceTooSmall,
               "PagedKv: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) +
                   " needed");
-  require(need == 0 || aligned(workspace, 16), "workspace must be 16-byte aligned");
+  require(aligned(workspace, 16), "workspace must be 16-byte aligned");
   RoctxRange range("gie::PagedKv::attention");
   check_kernel_status(gie_hip_paged_attention(dtype_of(p.precision), &g, q, k_pages, v_pages, q_starts, seq_lens,
                                               page_table, out, workspace, workspace_bytes, stream),
