@@ -201,3 +201,12 @@ def test_no_tokens_is_no_work():
     gie.linear_i8(p, 0, 0, 0, 0)
     gie.quantize_rows(p, 0, 0, 0)
     gie.synchronize()
+
+
+@pytest.mark.parametrize("shape", [(4090, 200, 4085), (4096, 128, 4096), (2040, 200, 2030), (1000, 333, 1000)])
+@pytest.mark.parametrize("layout", [dict(), dict(ld_x=352, ld_w=336, ld_y=4104), dict(ld_x=353, ld_w=341, ld_y=4099)])
+def test_large_tiles(shape, layout):
+    """Enough tokens and channels for tiles of 256, 128 and 64, whole and with ragged edges, rows that 16-byte pieces fit
+    and rows that they do not."""
+    check(*shape, precision="bf16", bias=True, **layout)
+    check(*shape, precision="fp32", quantized=True, relu=True, **layout)

@@ -78,6 +78,16 @@ def test_long_contexts_and_hints(length, new, hints):
     check(c, window=600, **hints)
 
 
+@pytest.mark.parametrize("dim", [96, 128, 256])
+@pytest.mark.parametrize("new", [1, 40, 130])
+def test_long_contexts_are_joined(dim, new):
+    """Few workgroups over a long context: its keys are split, one part and many for the rows of one call."""
+    for heads, kv_heads in ((2, 1), (12, 2)):
+        c = Cache([new, 3], [3000, 50], dim=dim, heads=heads, kv_heads=kv_heads, page=48, precision="bf16", seed=new)
+        check(c, max_new=new, max_len=3000)
+    check(c, window=1500, softcap=5.0)
+
+
 def test_rows_that_see_nothing():
     """More new tokens than the sequence holds, and sequences longer than their row of the page table."""
     got = check(Cache([20, 3, 1], [7, 3, 0], dim=64, seed=1))
@@ -118,6 +128,27 @@ def test_not_finite_values_reach_only_rows_that_see_them(bad, new, lens, window)
                     assert (np.abs(got - want) <= bound)[sees][:, 2:, rest].all()
                 elif np.isnan(bad):
                     assert np.isnan(got[sees][:, 2:]).all()
+
+
+@pytest.mark.parametrize("dim", [96, 256])
+@pytest.mark.parametrize("precision", ["fp16", "bf16"])
+@pytest.mark.parametrize("new,window", [(150, 0), (9, 0), (150, 20)])
+def test_not_finite_values_in_wide_heads(dim, precision, new, window):
+    """As above at the other head sizes, an infinity and a NaN in different values of different positions."""
+    c = Cache([new], [200], heads=4, kv_heads=2, dim=dim, precision=precision, seed=dim + new)
+    want, bound = c.plain(window=window)
+    spots = [(195, 0, np.inf), (190, dim - 1, -np.inf), (150, dim // 2 + 3, np.nan)]
+    for at, d, bad in spots:
+        c.v_pages[c.table[0, at // c.page], 1, at % c.page, d] = bad
+    got = c.attend(window=window)
+    position = np.arange(200 - new, 200)
+    touched = np.zeros((new, 4, dim), bool)
+    for at, d, bad in spots:
+        sees = (position >= at) & ((position < at + window) if window else True)
+        touched[sees, 2:, d] = True
+        hit = got[sees][:, 2:, d]
+        assert (np.isnan(hit) if np.isnan(bad) else hit == bad).all()
+    assert (np.abs(got - want) <= bound)[~touched].all()
 
 
 def test_not_finite_queries_stay_in_their_row():
