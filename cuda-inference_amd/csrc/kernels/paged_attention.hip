@@ -5,7 +5,7 @@
 //
 // Rows. All (token, head) pairs of a sequence that read one key head are rows of one matrix, r = token * group + head in
 // group, so a tile of rows shares every key it reads and one token of a grouped head fills part of a tile instead of a
-// row of it. A workgroup takes RQ * WR * 32 rows of one key head of one sequence, and the z-th part of their keys.
+// row of it. A workgroup takes WR * 32 rows of one key head of one sequence, and the z-th part of their keys.
 //
 // Products. Both are 32x32x16 MFMAs with the rows in the columns: S^T = K Q^T leaves a lane 16 scores (keys) of one row
 // for each 32 keys, so maxima and sums are a lane's own but for one exchange between the wave's halves, and the rescaling
@@ -143,11 +143,11 @@ __device__ __forceinline__ RowTile row_tile(const AttnArgs& a, int slot) {
 
 // WD waves take the same rows and a part of the head's values each: they work out the same scores (the first product is
 // theirs in full) and sum their part of V.
-template <typename E, int D, int RQ, int WR, int WK, int WD, int NST>
+template <typename E, int D, int WR, int WK, int WD, int NST>
 __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_kernel(AttnArgs a) {
   static_assert(WR == 1 || WK == 1, "waves share a tile of keys or have their own");
   static_assert(WD == 1 || (WD == 2 && WR > 1), "one of two loads K, the other V");
-  constexpr int R = RQ * WR * 32;             // rows of the workgroup
+  constexpr int R = WR * 32;                  // rows of the workgroup
   constexpr int TT = WR > 1 ? 16 * WR : 32;   // positions of a tile
   constexpr int NS = TT / 32;                 // 32-position parts of a tile
   constexpr int GR = TT / 16 / WR;            // 16-position granules that a wave loads
@@ -181,29 +181,28 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
   const int key_end = z + 1 < range.splits ? key0 + range.per_split * TT : max(range.hi, key0);
   const int tiles = (key_end - key0 + TT - 1) / TT;  // of the workgroup; this wave: wk, wk + WK, ...
 
-  // ---- this lane's rows: row (lane & 31) of each of the wave's RQ tiles; rows past the last repeat it ----
-  int pos[RQ];
-  u32x4 qf[RQ][KS];
-#pragma unroll
-  for (int r = 0; r < RQ; ++r) {
-    const int row = min(t.row0 + (wr * RQ + r) * 32 + (lane & 31), last_row);
+  // ---- this lane's row: row (lane & 31) of the wave's 32; rows past the last repeat it ----
+  int pos;
+  u32x4 qf[KS];
+  {
+    const int row = min(t.row0 + wr * 32 + (lane & 31), last_row);
     const int token = row / a.group, head = kvh * a.group + (row - token * a.group);
-    pos[r] = t.seq.base + token;
-    if (pos[r] >= a.capacity) pos[r] = -1;  // no valid position: sees nothing
+    pos = t.seq.base + token;
+    if (pos >= a.capacity) pos = -1;  // no valid position: sees nothing
     const long long src = (t.seq.first + token) * a.q_stride + head * D;
     if constexpr (WR == 1) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qf[r][ks] = load_16_bytes(a.q + src + (2 * ks + half) * 8);
+      for (int ks = 0; ks < KS; ++ks) qf[ks] = load_16_bytes(a.q + src + (2 * ks + half) * 8);
     } else {  // whole rows, 16 bytes for each lane; they go through LDS below (WD waves: a part of the rows each)
 #pragma unroll
       for (int j = 0; j < KS / WD; ++j) {
         const int piece = (j + wd * (KS / WD)) * 64 + lane, row_of = piece / (D / 8);
         const unsigned lo = unsigned(__shfl(int(src), row_of)), hi = unsigned(__shfl(int(src >> 32), row_of));
-        qf[r][j] = load_16_bytes(a.q + (long long)((unsigned long long)hi << 32 | lo) + piece % (D / 8) * 8);
+        qf[j] = load_16_bytes(a.q + (long long)((unsigned long long)hi << 32 | lo) + piece % (D / 8) * 8);
       }
     }
   }
-  const int wave_first = min(t.row0 + wr * RQ * 32, last_row), wave_last = min(t.row0 + (wr + 1) * RQ * 32 - 1, last_row);
+  const int wave_first = min(t.row0 + wr * 32, last_row), wave_last = min(t.row0 + (wr + 1) * 32 - 1, last_row);
   const int wpos_first = t.seq.base + wave_first / a.group, wpos_last = t.seq.base + wave_last / a.group;
 
   // ---- loads: granule g of a tile, instruction i covers 1024 / P rows ----
@@ -263,10 +262,9 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
   const unsigned v_chunk = unsigned((2 * (g16 & 1) + ((sl & 3) >> 1)) ^ v_swizzle<D>(sl >> 2));
   const unsigned v_rd = (lds0 + unsigned(kTileB) + v_row * P + (v_chunk << 4) + ((sl & 1) << 3)) ^ unsigned(wd * DT * 64);
 
-  f32x16 o[RQ][DT] = {};
-  float m[RQ], mc[RQ], l[RQ];  // running maximum of the products, its power of 2 (0 while there is none), sum
-#pragma unroll
-  for (int r = 0; r < RQ; ++r) m[r] = -INFINITY, mc[r] = 0.f, l[r] = 0.f;
+  f32x16 o[DT] = {};
+  float m, mc, l;  // running maximum of the products, its power of 2 (0 while there is none), sum
+  m = -INFINITY, mc = 0.f, l = 0.f;
 
   const auto compute = [&](int tile, int stage) {
     const unsigned so = unsigned(stage * kStage);
@@ -294,9 +292,7 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
         for (int k = 0; k < TT; ++k) {
           const int key = at0 + k;
           const unsigned row = lds0 + so + unsigned(kTileB + k * P);
-          uint32_t sees[RQ];
-#pragma unroll
-          for (int r = 0; r < RQ; ++r) sees[r] = key <= pos[r] && (a.window == 0 || key > pos[r] - a.window) ? ~0u : 0u;
+          const uint32_t sees = key <= pos && (a.window == 0 || key > pos - a.window) ? ~0u : 0u;
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -309,8 +305,7 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
                 const uint32_t word = e < 2 ? v.x : v.y;
                 const uint32_t odd = 0u - ((not_finite<E>(word) >> (e & 1 ? 31 : 15)) & 1u);
                 const uint32_t value = __float_as_uint(E::to_f32(uint16_t(e & 1 ? word >> 16 : word))) & odd;
-#pragma unroll
-                for (int r = 0; r < RQ; ++r) o[r][d][4 * i + e] += __uint_as_float(value & sees[r]);
+                o[d][4 * i + e] += __uint_as_float(value & sees);
               }
             }
         }
@@ -332,7 +327,6 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
       }
     }
 
-
     // Part by part of 32 keys. What a product reads from LDS is requested ahead of it: half of V under the softmax, the
     // other half and the next part's K under the second product.
     constexpr bool kAhead = WD == 1;  // where the registers hold it, or little else waits (narrow, bytes bound)
@@ -349,15 +343,13 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
     for (int n = 0; n < NS; ++n) {
       const int at = at0 + n * 32;
       // scores: register i holds key at + 8 (i / 4) + 4 half + i % 4
-      f32x16 s[RQ];
-#pragma unroll
-      for (int r = 0; r < RQ; ++r) s[r] = f32x16{};
+      f32x16 s;
+      s = f32x16{};
       if constexpr (kAhead) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int r = 0; r < RQ; ++r) s[r] = E::mfma32(kf[ks], qf[r][ks], s[r]);
-      } else {  // four steps ahead; left to itself the compiler waits for every read (head_dim 256: x us a tile for y)
+        for (int ks = 0; ks < KS; ++ks) s = E::mfma32(kf[ks], qf[ks], s);
+      } else {  // four steps ahead; left to itself the compiler waits for every read (one prompt
+                // of 4096 at head_dim 256: 225 us, and 206 so)
         unsigned ko = k_rd + so;
         asm volatile("" : "+v"(ko));
         const auto read_4 = [&](int g) {
@@ -372,9 +364,7 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
           if (g + 1 < KS / 4) read_4(g + 1);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int r = 0; r < RQ; ++r) s[r] = E::mfma32(kf[g % 2 * 4 + i], qf[r][g * 4 + i], s[r]);
+          for (int i = 0; i < 4; ++i) s = E::mfma32(kf[g % 2 * 4 + i], qf[g * 4 + i], s);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -394,57 +384,49 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
       if (VH == 2) read_v(0);
       if (a.cap > 0) {
 #pragma unroll
-        for (int r = 0; r < RQ; ++r)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e = __builtin_amdgcn_exp2f(s[r][i] * a.cap_in);
-            s[r][i] = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(e + 1.f);
-          }
+        for (int i = 0; i < 16; ++i) {
+          const float e = __builtin_amdgcn_exp2f(s[i] * a.cap_in);
+          s[i] = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(e + 1.f);
+        }
       }
       const bool masked =
           at + 31 > wpos_first || (a.window > 0 && at <= wpos_last - a.window) || wpos_last >= a.capacity;
       if (masked) {
-#pragma unroll
-        for (int r = 0; r < RQ; ++r) {
-          const int oldest = a.window > 0 ? pos[r] - a.window : -1;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = at + 8 * (i / 4) + 4 * half + i % 4;
-            s[r][i] = key <= pos[r] && key > oldest ? s[r][i] : -INFINITY;
-          }
-        }
-      }
-      u32x4 pf[RQ][2];
-#pragma unroll
-      for (int r = 0; r < RQ; ++r) {
-        float top = s[r][0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[r][i]);
-        top = swap_max(top);
-        // the maximum follows only when a weight would pass 2^8: sums and weights keep their relative precision, and
-        // most tiles leave O as it is
-        if (__any((top - m[r]) * a.mult > 8.f)) {
-          const float next = fmaxf(m[r], top);
-          const float nc = next == -INFINITY ? 0.f : next * a.mult;
-          const float keep = m[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc[r] - nc);  // 1: nothing summed yet
-          m[r] = next;
-          mc[r] = nc;
-          l[r] *= keep;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[r][d] *= keep;
-        }
-        float sum[4] = {};
+        const int oldest = a.window > 0 ? pos - a.window : -1;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i], a.mult, -mc[r]));
-          sum[i % 4] += s[r][i];
+          const int key = at + 8 * (i / 4) + 4 * half + i % 4;
+          s[i] = key <= pos && key > oldest ? s[i] : -INFINITY;
         }
-        l[r] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          pf[r][h] = u32x4{E::pack2(s[r][8 * h], s[r][8 * h + 1]), E::pack2(s[r][8 * h + 2], s[r][8 * h + 3]),
-                           E::pack2(s[r][8 * h + 4], s[r][8 * h + 5]), E::pack2(s[r][8 * h + 6], s[r][8 * h + 7])};
       }
+      u32x4 pf[2];
+      float top = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+      top = swap_max(top);
+      // the maximum follows only when a weight would pass 2^8: sums and weights keep their relative precision, and
+      // most tiles leave O as it is
+      if (__any((top - m) * a.mult > 8.f)) {
+        const float next = fmaxf(m, top);
+        const float nc = next == -INFINITY ? 0.f : next * a.mult;
+        const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - nc);  // 1: nothing summed yet
+        m = next;
+        mc = nc;
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= keep;
+      }
+      float sum[4] = {};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.mult, -mc));
+        sum[i % 4] += s[i];
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        pf[h] = u32x4{E::pack2(s[8 * h], s[8 * h + 1]), E::pack2(s[8 * h + 2], s[8 * h + 3]),
+                      E::pack2(s[8 * h + 4], s[8 * h + 5]), E::pack2(s[8 * h + 6], s[8 * h + 7])};
       if (VH == 2) {
         read_v(1);
         if (kAhead && n + 1 < NS) read_k(n + 1);
@@ -453,9 +435,7 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
       for (int h = 0; h < 2; ++h) {
         if (VH == 1) read_v(h);
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int r = 0; r < RQ; ++r) o[r][d] = E::mfma32(vf[h % VH][d], pf[r][h], o[r][d]);
+        for (int d = 0; d < DT; ++d) o[d] = E::mfma32(vf[h % VH][d], pf[h], o[d]);
       }
     }
   };
@@ -471,12 +451,12 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
     look_up(tile_at(j + 1));
   }
   if constexpr (WR > 1) {  // rows of q to the lanes that multiply them, by way of the stage that is loaded last
-    static_assert(RQ == 1 && WR * 32 * P <= kStage, "one tile of rows for each wave fits a stage");
+    static_assert(WR * 32 * P <= kStage, "the rows fit a stage");
     const unsigned rows = lds0 + unsigned((NST - 1) * kStage + wr * 32 * P);
 #pragma unroll
     for (int j = 0; j < KS / WD; ++j) {
       const int piece = (j + wd * (KS / WD)) * 64 + lane, row = piece / (D / 8), c = piece % (D / 8);
-      *reinterpret_cast<lds_v4*>(size_t(rows + unsigned(row * P + ((c ^ k_swizzle<D>(row & 15)) << 4)))) = qf[0][j];
+      *reinterpret_cast<lds_v4*>(size_t(rows + unsigned(row * P + ((c ^ k_swizzle<D>(row & 15)) << 4)))) = qf[j];
     }
     if (WD > 1)
       stage_barrier();
@@ -484,15 +464,13 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
       __builtin_amdgcn_s_waitcnt(0xc07f);
     const unsigned mine = rows + unsigned((lane & 31) * P + ((half ^ k_swizzle<D>(lane & 15)) << 4));
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[0][ks] = *reinterpret_cast<const lds_v4*>(size_t(mine ^ unsigned(ks * 32)));
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const lds_v4*>(size_t(mine ^ unsigned(ks * 32)));
   }
   if (a.negate) {  // first use of q: it arrives under the loads above
 #pragma unroll
-    for (int r = 0; r < RQ; ++r)
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) qf[r][ks][e] ^= 0x80008000u;
+      for (int e = 0; e < 4; ++e) qf[ks][e] ^= 0x80008000u;
   }
   int stage = 0;
   for (int j = 0; j < mine; ++j) {
@@ -508,26 +486,24 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
   }
   wait_vm<0>();
 
-#pragma unroll
-  for (int r = 0; r < RQ; ++r) l[r] = swap_add(l[r]);
+  l = swap_add(l);
 
   // where the lane's rows go, worked out again here: kept from above it would cost registers in the loop
   int row_first = t.row0;
   asm volatile("" : "+s"(row_first));
-  const auto place = [&](int r, int& token, int& head) {
-    const int row = min(row_first + (wr * RQ + r) * 32 + (lane & 31), last_row), i = row / a.group;
+  const auto place = [&](int& token, int& head) {
+    const int row = min(row_first + wr * 32 + (lane & 31), last_row), i = row / a.group;
     token = t.seq.first + i;
     head = kvh * a.group + (row - i * a.group);
   };
 
   // ---- the waves' parts of the keys ----
   if constexpr (WK > 1) {
-    static_assert(RQ == 1, "one tile of rows for each wave that has keys of its own");
     __syncthreads();
     float* sums = reinterpret_cast<float*>(lds);  // [wave][32] m, l; then [wave][32 rows][D + 4]
     if (half == 0) {
-      sums[(wave * 32 + lane) * 2] = m[0] == -INFINITY ? -INFINITY : mc[0];
-      sums[(wave * 32 + lane) * 2 + 1] = l[0];
+      sums[(wave * 32 + lane) * 2] = m == -INFINITY ? -INFINITY : mc;
+      sums[(wave * 32 + lane) * 2 + 1] = l;
     }
     __syncthreads();
     float top = -INFINITY, total = 0.f;
@@ -540,7 +516,7 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
       // a wave without a maximum may hold a NaN all the same
       total += sums[(w * 32 + (lane & 31)) * 2 + 1] * __builtin_amdgcn_exp2f(other == -INFINITY ? 0.f : other - ref);
     }
-    const float keep = __builtin_amdgcn_exp2f(m[0] == -INFINITY ? 0.f : mc[0] - ref);
+    const float keep = __builtin_amdgcn_exp2f(m == -INFINITY ? 0.f : mc - ref);
     constexpr int kRow = D + 4;
     float* mine_o = reinterpret_cast<float*>(lds + WK * 256) + (wave * 32 + (lane & 31)) * kRow;
 #pragma unroll
@@ -548,17 +524,17 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<f32x4*>(mine_o + 32 * d + 8 * i + 4 * half) =
-            f32x4{o[0][d][4 * i], o[0][d][4 * i + 1], o[0][d][4 * i + 2], o[0][d][4 * i + 3]} * keep;
+            f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * keep;
     // row (tid & 31) of the sums: every wave joins a part of the values
-    m[0] = top;
-    mc[0] = ref;
-    l[0] = total;
+    m = top;
+    mc = ref;
+    l = total;
     __syncthreads();
     const float* all = reinterpret_cast<const float*>(lds + WK * 256);
     const int row = lane & 31;
     if (row < t.rows) {
       int token, head;
-      place(0, token, head);
+      place(token, head);
       const float inv = total == 0.f ? 0.f : 1.f / total;
       for (int d = (wave * 2 + half) * 4; d < D; d += WK * 8) {
         f32x4 v = {};
@@ -584,63 +560,60 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
   __syncthreads();  // the stages are free
   constexpr int kRowB = DT * 64, kPad = kRowB + 16, kPadF = 128 + 16;  // a wave's part of a row; 32 FP32 values of one
   const unsigned mine_rows = lds0 + unsigned(wave * 32 * kPad);
+  const int rl = lane & 31;
+  const bool there = wr * 32 + rl < t.rows;
+  int token, head;
+  place(token, head);
+  const bool parts = range.splits > 1;
+  const long long to = !there  ? -1
+                       : parts ? (((long long)token * a.q_heads + head) * a.splits + z) * (D + 4) + wd * DT * 32
+                               : token * a.o_stride + head * D + wd * DT * 32;
+  const unsigned row = mine_rows + unsigned(rl * (parts ? kPadF : kPad));
+  if (half == 0) *reinterpret_cast<lds_ll*>(size_t(row + unsigned(parts ? 128 : kRowB))) = to;
+  if (parts) {
+    if (there && half == 0 && wd == 0) {
+      a.part[to + D] = m == -INFINITY ? -INFINITY : mc;
+      a.part[to + D + 1] = l;
+    }
 #pragma unroll
-  for (int r = 0; r < RQ; ++r) {
-    const int rl = lane & 31;
-    const bool there = (wr * RQ + r) * 32 + rl < t.rows;
-    int token, head;
-    place(r, token, head);
-    const bool parts = range.splits > 1;
-    const long long to = !there  ? -1
-                         : parts ? (((long long)token * a.q_heads + head) * a.splits + z) * (D + 4) + wd * DT * 32
-                                 : token * a.o_stride + head * D + wd * DT * 32;
-    const unsigned row = mine_rows + unsigned(rl * (parts ? kPadF : kPad));
-    if (half == 0) *reinterpret_cast<lds_ll*>(size_t(row + unsigned(parts ? 128 : kRowB))) = to;
-    if (parts) {
-      if (there && half == 0 && wd == 0) {
-        a.part[to + D] = m[r] == -INFINITY ? -INFINITY : mc[r];
-        a.part[to + D + 1] = l[r];
-      }
+    for (int d = 0; d < DT; ++d) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<lds_f4*>(size_t(row + unsigned((8 * i + 4 * half) * 4))) =
-              f32x4{o[r][d][4 * i], o[r][d][4 * i + 1], o[r][d][4 * i + 2], o[r][d][4 * i + 3]};
-        __builtin_amdgcn_s_waitcnt(0xc07f);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const unsigned from = mine_rows + unsigned((j * 8 + lane / 8) * kPadF);
-          const long long at = *reinterpret_cast<const lds_ll*>(size_t(from + 128u));
-          const f32x4 v = *reinterpret_cast<const lds_f4*>(size_t(from + unsigned(lane % 8 * 16)));
-          if (at >= 0) *reinterpret_cast<f32x4*>(a.part + at + d * 32 + lane % 8 * 4) = v;
-        }
-        __builtin_amdgcn_s_waitcnt(0xc07f);
-      }
-    } else {
-      const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f32x4 v = {o[r][d][4 * i], o[r][d][4 * i + 1], o[r][d][4 * i + 2], o[r][d][4 * i + 3]};
-          if (l[r] == 0.f) v = f32x4{};  // nothing seen (and what was summed for it may be a NaN)
-          v *= inv;
-          *reinterpret_cast<lds_v2*>(size_t(row + unsigned((32 * d + 8 * i + 4 * half) * 2))) =
-              u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
-        }
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<lds_f4*>(size_t(row + unsigned((8 * i + 4 * half) * 4))) =
+            f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
       __builtin_amdgcn_s_waitcnt(0xc07f);
-      constexpr int kPieces = kRowB / 16;
 #pragma unroll
-      for (int j = 0; j < kPieces / 2; ++j) {
-        const int piece = j * 64 + lane, from_row = piece / kPieces, c = piece % kPieces;
-        const unsigned from = mine_rows + unsigned(from_row * kPad);
-        const long long at = *reinterpret_cast<const lds_ll*>(size_t(from + unsigned(kRowB)));
-        const u32x4 v = *reinterpret_cast<const lds_v4*>(size_t(from + unsigned(c * 16)));
-        if (at >= 0) store_16_bytes(a.out + at + c * 8, v);
+      for (int j = 0; j < 4; ++j) {
+        const unsigned from = mine_rows + unsigned((j * 8 + lane / 8) * kPadF);
+        const long long at = *reinterpret_cast<const lds_ll*>(size_t(from + 128u));
+        const f32x4 v = *reinterpret_cast<const lds_f4*>(size_t(from + unsigned(lane % 8 * 16)));
+        if (at >= 0) *reinterpret_cast<f32x4*>(a.part + at + d * 32 + lane % 8 * 4) = v;
       }
       __builtin_amdgcn_s_waitcnt(0xc07f);
     }
+  } else {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4 v = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        if (l == 0.f) v = f32x4{};  // nothing seen (and what was summed for it may be a NaN)
+        v *= inv;
+        *reinterpret_cast<lds_v2*>(size_t(row + unsigned((32 * d + 8 * i + 4 * half) * 2))) =
+            u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
+      }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    constexpr int kPieces = kRowB / 16;
+#pragma unroll
+    for (int j = 0; j < kPieces / 2; ++j) {
+      const int piece = j * 64 + lane, from_row = piece / kPieces, c = piece % kPieces;
+      const unsigned from = mine_rows + unsigned(from_row * kPad);
+      const long long at = *reinterpret_cast<const lds_ll*>(size_t(from + unsigned(kRowB)));
+      const u32x4 v = *reinterpret_cast<const lds_v4*>(size_t(from + unsigned(c * 16)));
+      if (at >= 0) store_16_bytes(a.out + at + c * 8, v);
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
   }
 }
 
@@ -776,11 +749,11 @@ int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   if (s.wide) {
     constexpr int NST = 2;
     constexpr int WR = kWideRows / 32, WD = D == 256 ? 2 : 1;
-    rc = start(attention_kernel<E, D, 1, WR, 1, WD, NST>, int(grid), 64 * WR * WD, NST * 2 * 16 * WR * P + 64, stream, a);
+    rc = start(attention_kernel<E, D, WR, 1, WD, NST>, int(grid), 64 * WR * WD, NST * 2 * 16 * WR * P + 64, stream, a);
   } else {
     constexpr int WK = D == 256 ? 2 : 4, NST = D == 64 ? 4 : 2;
     constexpr int bytes = WK * NST * 2 * 32 * P, join = WK * 256 + WK * 32 * (D + 4) * 4;
-    rc = start(attention_kernel<E, D, 1, 1, WK, 1, NST>, int(grid), 64 * WK, bytes > join ? bytes : join, stream, a);
+    rc = start(attention_kernel<E, D, 1, WK, 1, NST>, int(grid), 64 * WK, bytes > join ? bytes : join, stream, a);
   }
   if (rc != GIE_HIP_OK || s.splits == 1) return rc;
   const bool many = s.splits > 8;
