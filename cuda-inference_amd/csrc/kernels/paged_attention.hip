@@ -19,13 +19,14 @@
 // no bank twice in a phase. The waves of a workgroup either share a tile of keys (WR > 1: one barrier for each tile) or
 // take tiles of their own (WR == 1, WK waves, no barrier until their results are joined).
 //
-// Few rows (one token of a grouped head: up to 32) are bound by the cache's bytes: one token over 32768 positions of 8 key
-// heads of 128 in 32 parts 24 us + 4 for the join, 4.6 TB/s in all; a step of 64 sequences 219 us, 5.0 TB/s (a large copy
-// reaches 4.7). Many rows are bound by the products: two prompts of 4096 tokens, 32 heads of 128, 303-312 us, 0.9 PFLOP/s
-// (a large library product 1.23); 2048 tokens over 30000 1.0. Matrix cores are busy 0.4 of the time, the vector unit
-// (softmax) 0.35 and LDS 0.22, on two workgroups of 4 waves for each compute unit: measured without exponentials -5 %,
-// without any softmax -13 %, without loads -16 %. 64 rows for each wave (half the LDS reads, one wave for each SIMD)
-// took 408 us for what now takes 310, eight waves sharing a tile 318 and more for ragged batches.
+// Few rows (one token of a grouped head: up to 32) are bound by the cache's bytes: one token over 32768 positions of 8
+// key heads of 128 in 32 parts 24 us + 4 for the join, 4.6 TB/s in all; a step of 64 sequences 219 us, 5.0 TB/s (a large
+// copy reaches 4.7). Many rows are bound by the products: two prompts of 4096 tokens, 32 heads of 128, 293-301 us, 0.93
+// PFLOP/s (a large library product 1.23); 2048 tokens over 30000 1.0. Matrix cores are busy 0.4 of the time, the vector
+// unit (softmax) 0.35 and LDS 0.22, on two workgroups of 4 waves for each compute unit: measured (at 310 us for a call,
+// before q and out went through LDS) without exponentials -5 %, without any softmax -13 %, without loads -16 %. At that
+// time 64 rows for each wave (half the LDS reads, one wave for each SIMD) took 408 us, eight waves sharing a tile 318 and
+// more for ragged batches.
 #include "paged_common.h"
 
 #include "lds_pipe.h"
@@ -275,8 +276,8 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
       uint32_t bad = 0;
 #pragma unroll
       for (int i = 0; i < kTileB / 1024 / (WR * WD); ++i) {
-        const u32x4 v =
-            *reinterpret_cast<const lds_v4*>(size_t(lds0 + so + unsigned(kTileB + (i * WR * WD + (WR > 1 ? wave : 0)) * 1024 + lane * 16)));
+        const int piece = i * WR * WD + (WR > 1 ? wave : 0);
+        const u32x4 v = *reinterpret_cast<const lds_v4*>(size_t(lds0 + so + unsigned(kTileB + piece * 1024 + lane * 16)));
         bad |= not_finite<E>(v.x) | not_finite<E>(v.y) | not_finite<E>(v.z) | not_finite<E>(v.w);
       }
       bool any = __any(bad != 0);
@@ -556,7 +557,7 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
   }
 
   // ---- rows to out, or to the parts that are joined: through LDS, so that a store covers whole lines of a row (from
-  // where the products leave them, 8 bytes of 32 rows at a time, they took 3.3 us longer at head_dim 256, 1.3 at 128) ----
+  // where the products leave them, 8 bytes of 32 rows at a time: 3.3 us longer at head_dim 256, 1.3 at 128) ----
   __syncthreads();  // the stages are free
   constexpr int kRowB = DT * 64, kPad = kRowB + 16, kPadF = 128 + 16;  // a wave's part of a row; 32 FP32 values of one
   const unsigned mine_rows = lds0 + unsigned(wave * 32 * kPad);
