@@ -70,7 +70,7 @@ inline bool valid_paged(const gie_paged_geom* g) {
   if (g->head_dim <= 0 || g->page_size <= 0 || g->page_size % 16 != 0 || g->num_pages <= 0 || g->max_pages <= 0)
     return false;
   if (g->head_dim % 32 != 0 || g->head_dim > 256 || (long long)g->max_pages * g->page_size > (1 << 30)) return false;
-  if ((long long)g->total_tokens * (g->q_heads / g->kv_heads) > (1 << 30)) return false;
+  if ((long long)g->total_tokens * (g->q_heads / g->kv_heads) > (1 << 30) || g->batch > (1 << 30)) return false;
   if ((long long)g->page_size * g->head_dim > (1 << 26)) return false;
   const long long q = (long long)g->q_heads * g->head_dim, kv = (long long)g->kv_heads * g->head_dim;
   if (g->q_stride < q || g->o_stride < q || g->k_stride < kv || g->v_stride < kv) return false;

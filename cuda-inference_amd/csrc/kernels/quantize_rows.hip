@@ -58,7 +58,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* __r
 template <typename E>
 void launch(const void* x, long long ld_x, int tokens, int features, int8_t* q, long long ld_q, float* scale, hipStream_t s) {
   constexpr int kE = E::kDtype == GIE_HIP_FP32 ? 4 : 2;
-  const bool small = features * kE <= 64 * 16 * 2;
+  const bool small = features <= 64 * 16 * 2 / kE;
   const int blocks = small ? tokens / 4 + (tokens % 4 != 0) : tokens, across = blocks < (1 << 20) ? blocks : 1 << 20;
   const auto kernel = small ? quantize_rows_kernel<E, 64> : quantize_rows_kernel<E, kThreads>;
   hipLaunchKernelGGL(kernel, dim3(across, blocks / across + (blocks % across != 0)), dim3(kThreads), 0, s, x, ld_x, tokens, features,

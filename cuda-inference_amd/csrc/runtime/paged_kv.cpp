@@ -83,6 +83,7 @@ void validate_problem(const PagedKvProblem& p) {
           "max_pages * page_size passes 2^30 positions");
   support(int64_t(p.total_tokens) * (p.q_heads / p.kv_heads) <= std::numeric_limits<int32_t>::max() / 2,
           "total_tokens * (q_heads / kv_heads) passes 2^30 rows");
+  support(p.batch <= std::numeric_limits<int32_t>::max() / 2, "batch passes 2^30 sequences");
   support(int64_t(p.page_size) * p.head_dim <= (1 << 26), "a page of one head is over 128 MiB");
 }
 

@@ -116,6 +116,15 @@ def test_attention_refuses_bad_pointers(bad):
     assert status(attend, paged(), **bad) == "InvalidArgument"
 
 
+def test_paged_refuses_a_batch_past_its_indexes():
+    # the host's tile counts and the device's search add tokens and sequences in 32 bits
+    for batch in (1 << 30, (1 << 31) - 1):
+        bad = paged(batch=batch)
+        assert status(gie.paged_attention_workspace_size, bad) == "Unsupported"
+        assert status(append, bad) == "Unsupported"
+        assert status(attend, bad) == "Unsupported"
+
+
 def test_attention_workspace_is_checked():
     p = paged(total_tokens=1, batch=1, max_pages=4096, max_new=1, max_len=65536)
     n = gie.paged_attention_workspace_size(p)
