@@ -58,8 +58,8 @@ struct AttnArgs {
   int page_shift;
   int capacity;  // max_pages * page_size
   int window;
-  float mult;      // a score's power of 2: the product times this, or (capped) the capped score times log2(e)
-  float cap_in, cap;  // softcap > 0: cap * tanh(product * cap_in / 2)
+  float mult;      // a score's power of 2: the product times this, or (cap > 0) what the cap leaves of it times this
+  float cap_in, cap;  // cap > 0: cap * tanh(product * cap_in / (2 log2(e)))
   int negate;      // a negative scale: q changes its sign, so that the largest product is the largest score
   int splits, chunk;  // parts of the keys and the fewest tiles of one
 };
@@ -105,6 +105,46 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t x) {
   return ((x & mask) + one) & 0x80008000u;
 }
 
+// Scores under a cap. 1 - 2 / (2^z + 1) is off by about 2^-23 however small z is, and the score by the cap times that:
+// less than what the sum of a product is off by, up to caps of kExpCap.
+constexpr float kTwoLog2E = 2.f * 1.44269504088896341f, kExpCap = 64.f;
+__device__ __forceinline__ void cap_scores(const AttnArgs& a, f32x16& s) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float e = __builtin_amdgcn_exp2f(s[i] * a.cap_in);
+    s[i] = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(e + 1.f);
+  }
+}
+// Under a cap past kExpCap, in units of the product x = s[i]: where |x / cap| < 0.2 the odd polynomial of tanh, times x
+// itself (its next term is 2^-30 of it), so that scores keep FP32's relative precision under any cap; the exponential
+// only where a wave has a larger one. In a kernel of its own: beside the other form it took 1 % from calls that need
+// neither (registers, a longer loop). Two prompts of 4096 tokens, 32 heads of 128, scores around 1: 362 us under a cap of
+// 65, 352 under one of 50.
+__device__ __forceinline__ void cap_products(const AttnArgs& a, f32x16& s) {
+  constexpr float kBound = 0.2f * kTwoLog2E, k2 = 1.f / (kTwoLog2E * kTwoLog2E);
+  const auto polynomial = [](float x, float z) {
+    const float z2 = z * z;
+    float p = __builtin_fmaf(z2, 62.f / 2835.f * k2 * k2 * k2 * k2, -17.f / 315.f * k2 * k2 * k2);
+    p = __builtin_fmaf(z2, p, 2.f / 15.f * k2 * k2);
+    p = __builtin_fmaf(z2, p, -1.f / 3.f * k2);
+    return x * __builtin_fmaf(z2, p, 1.f);
+  };
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(s[i]));
+  if (!__any(most * a.cap_in >= kBound)) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = polynomial(s[i], s[i] * a.cap_in);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float z = fabsf(s[i] * a.cap_in), r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(z) + 1.f);
+      const float t = __builtin_copysignf(a.cap * __builtin_fmaf(-2.f, r, 1.f), s[i]);
+      s[i] = z < kBound ? polynomial(s[i], z) : t;  // a NaN stays one
+    }
+  }
+}
+
 // the part of a sequence's keys that a tile of rows reads, in tiles of TT positions, and its division
 struct KeyRange {
   int lo, hi;     // positions [lo, hi), lo a multiple of 16
@@ -143,8 +183,8 @@ __device__ __forceinline__ RowTile row_tile(const AttnArgs& a, int slot) {
 }
 
 // WD waves take the same rows and a part of the head's values each: they work out the same scores (the first product is
-// theirs in full) and sum their part of V.
-template <typename E, int D, int WR, int WK, int WD, int NST>
+// theirs in full) and sum their part of V. LARGE_CAP: scores under a cap past kExpCap.
+template <typename E, int D, int WR, int WK, int WD, int NST, bool LARGE_CAP>
 __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_kernel(AttnArgs a) {
   static_assert(WR == 1 || WK == 1, "waves share a tile of keys or have their own");
   static_assert(WD == 1 || (WD == 2 && WR > 1), "one of two loads K, the other V");
@@ -383,13 +423,10 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
         }
       };
       if (VH == 2) read_v(0);
-      if (a.cap > 0) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(s[i] * a.cap_in);
-          s[i] = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(e + 1.f);
-        }
-      }
+      if constexpr (LARGE_CAP)
+        cap_products(a, s);
+      else if (a.cap > 0)
+        cap_scores(a, s);
       const bool masked =
           at + 31 > wpos_first || (a.window > 0 && at <= wpos_last - a.window) || wpos_last >= a.capacity;
       if (masked) {
@@ -740,7 +777,7 @@ int start(K kernel, int grid, int threads, int lds_bytes, hipStream_t stream, co
   return e == hipSuccess ? GIE_HIP_OK : int(e);
 }
 
-template <typename E, int D>
+template <typename E, int D, bool LARGE_CAP>
 int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   const long long grid = (long long)s.slots * s.splits * a.kv_heads;
   const long long rows = (long long)a.total_tokens * a.q_heads;
@@ -750,11 +787,11 @@ int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   if (s.wide) {
     constexpr int NST = 2;
     constexpr int WR = kWideRows / 32, WD = D == 256 ? 2 : 1;
-    rc = start(attention_kernel<E, D, WR, 1, WD, NST>, int(grid), 64 * WR * WD, NST * 2 * 16 * WR * P + 64, stream, a);
+    rc = start(attention_kernel<E, D, WR, 1, WD, NST, LARGE_CAP>, int(grid), 64 * WR * WD, NST * 2 * 16 * WR * P + 64, stream, a);
   } else {
     constexpr int WK = D == 256 ? 2 : 4, NST = D == 64 ? 4 : 2;
     constexpr int bytes = WK * NST * 2 * 32 * P, join = WK * 256 + WK * 32 * (D + 4) * 4;
-    rc = start(attention_kernel<E, D, 1, WK, 1, NST>, int(grid), 64 * WK, bytes > join ? bytes : join, stream, a);
+    rc = start(attention_kernel<E, D, 1, WK, 1, NST, LARGE_CAP>, int(grid), 64 * WK, bytes > join ? bytes : join, stream, a);
   }
   if (rc != GIE_HIP_OK || s.splits == 1) return rc;
   const bool many = s.splits > 8;
@@ -764,6 +801,16 @@ int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   hipLaunchKernelGGL(join, dim3(unsigned(many ? rows : (rows + 3) / 4)), dim3(256), 0, stream, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? GIE_HIP_OK : int(e);
+}
+
+template <typename E, bool LARGE_CAP>
+int launch(const AttnArgs& a, const Shape& s, int head_dim, hipStream_t stream) {
+  switch (head_dim) {
+    case 64: return launch<E, 64, LARGE_CAP>(a, s, stream);
+    case 96: return launch<E, 96, LARGE_CAP>(a, s, stream);
+    case 128: return launch<E, 128, LARGE_CAP>(a, s, stream);
+    default: return launch<E, 256, LARGE_CAP>(a, s, stream);
+  }
 }
 
 }  // namespace
@@ -822,22 +869,23 @@ extern "C" int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const
   constexpr float kLog2E = 1.44269504088896341f;
   const float scale = g->scale < 0 ? -g->scale : g->scale;
   a.negate = g->scale < 0;
+  // factors stay finite, or a product of 0 would become a NaN
+  a.mult = fminf(scale * kLog2E, 3e38f);
+  bool large_cap = false;
   if (g->softcap > 0) {
-    a.mult = kLog2E;
-    a.cap = g->softcap;
-    // tanh(x) = 1 - 2 / (2^(2 log2(e) x) + 1); factors stay finite, or a product of 0 would become a NaN
-    a.cap_in = fminf(2.f * kLog2E * (scale / g->softcap), 3e38f);
-  } else {
-    a.mult = fminf(scale * kLog2E, 3e38f);
+    a.cap_in = fminf(kTwoLog2E * (scale / g->softcap), 3e38f);
+    large_cap = g->softcap > kExpCap;
+    if (!large_cap) {
+      a.mult = kLog2E;
+      a.cap = g->softcap;
+    } else {
+      a.cap = fminf(g->softcap / scale, 3e38f);
+    }
   }
   a.splits = shape.splits;
   a.chunk = shape.chunk;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool h = dtype == GIE_HIP_FP16;
-  switch (g->head_dim) {
-    case 64: return h ? launch<Fp16, 64>(a, shape, s) : launch<Bf16, 64>(a, shape, s);
-    case 96: return h ? launch<Fp16, 96>(a, shape, s) : launch<Bf16, 96>(a, shape, s);
-    case 128: return h ? launch<Fp16, 128>(a, shape, s) : launch<Bf16, 128>(a, shape, s);
-    default: return h ? launch<Fp16, 256>(a, shape, s) : launch<Bf16, 256>(a, shape, s);
-  }
+  const int D = g->head_dim;
+  if (dtype == GIE_HIP_FP16) return large_cap ? launch<Fp16, true>(a, shape, D, s) : launch<Fp16, false>(a, shape, D, s);
+  return large_cap ? launch<Bf16, true>(a, shape, D, s) : launch<Bf16, false>(a, shape, D, s);
 }
