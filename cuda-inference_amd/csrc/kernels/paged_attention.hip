@@ -303,8 +303,12 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
   const unsigned v_chunk = unsigned((2 * (g16 & 1) + ((sl & 3) >> 1)) ^ v_swizzle<D>(sl >> 2));
   const unsigned v_rd = (lds0 + unsigned(kTileB) + v_row * P + (v_chunk << 4) + ((sl & 1) << 3)) ^ unsigned(wd * DT * 64);
 
+  // Weights are 2^(score - mc), rounded to the storage type. FP16 has no step under 2^-24, which the small weights of a
+  // long cache reach: they are lifted, so that the largest lies in 2^7 .. 2^15 and one of 2^-25 of it keeps 6 bits.
+  // Without the lift 131072 keys of 2^-25.2 each beside one of 1 lose their share of 0.3 % (at the same time for a call).
+  constexpr float kLift = E::kDtype == GIE_HIP_FP16 ? 7.f : 0.f;
   f32x16 o[DT] = {};
-  float m, mc, l;  // running maximum of the products, its power of 2 (0 while there is none), sum
+  float m, mc, l;  // running maximum of the products, its power of 2 less kLift (0 while there is none), sum
   m = -INFINITY, mc = 0.f, l = 0.f;
 
   const auto compute = [&](int tile, int stage) {
@@ -446,7 +450,9 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
       // most tiles leave O as it is
       if (__any((top - m) * a.mult > 8.f)) {
         const float next = fmaxf(m, top);
-        const float nc = next == -INFINITY ? 0.f : next * a.mult;
+        float nc = next == -INFINITY ? 0.f : next * a.mult;
+        // what rounding takes from nc would come on top of the lift: 2^-23 of it and more are added
+        if constexpr (kLift > 0) nc += __builtin_fmaf(fabsf(nc), 0x1p-23f, -kLift);
         const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - nc);  // 1: nothing summed yet
         m = next;
         mc = nc;

@@ -1,7 +1,9 @@
-"""PagedKv::attention where its scores are hardest to hold: caps far above every score and far below them."""
+"""PagedKv::attention where its scores and weights are hardest to hold: caps far above every score and far below them,
+a key that outweighs a long rest of the cache by more than the storage type's steps reach, scores of millions."""
 import numpy as np
 import pytest
 
+import gie
 from paged_plain import TINY, UNIT, Cache
 
 pytestmark = pytest.mark.gpu
@@ -87,3 +89,73 @@ def test_a_key_that_is_infinite_scores_the_cap(cap):
     c.k_pages[c.table[0, 2], :, 5, 3] = np.inf  # position 37 of the first sequence
     c.k_pages[c.table[1, 0], :, 7, 9] = -np.inf  # position 7 of the second
     check(c, cap)
+
+
+@pytest.mark.parametrize("gap", [20.0, 23.4, 25.2, 27.0])
+@pytest.mark.parametrize("new", [1, 33])
+@pytest.mark.parametrize("precision", ["fp16", "bf16"])
+def test_small_weights_of_a_long_cache_are_not_lost(gap, new, precision):
+    """One key at the front and a rest of 2^17 - 1 whose weights are 2^-gap of its own, in one part or in few (the batch fills
+    the device). All values are 1, so the result is too, if what the sum of the weights counts also enters the product.
+
+    Bound: a weight is rounded once (u), or to within 2^-32 of the first key's in FP16's last steps (its weights are
+    at least 2^7 at the maximum); n / 16 and n / 32 additions in FP32 follow one another in the product and in the
+    sum; the argument of 2^x is off by the score's rounding in FP32 (2^-24 of up to 32), and its result by 2^-22."""
+    import torch
+    dim, kv, page, batch, n = 64, 64, 256, 4, 1 << 17
+    pages = n // page
+    dtype = torch.float16 if precision == "fp16" else torch.bfloat16
+    k, v = (torch.zeros((pages, kv, page, dim), dtype=dtype, device="cuda") for _ in range(2))
+    v += 1
+    # scores in powers of 2: q k log2(e) scale, all of it exact in the storage type but the scale
+    k[:, :, :, 0] = -1
+    k[0, :, 0, 0] = 0
+    q = torch.zeros((batch * new, kv, dim), dtype=dtype, device="cuda")
+    q[:, :, 0] = 1
+    scale = float(np.float32(gap * np.log(2.0)))
+    out = torch.full_like(q, 7)
+    starts = torch.arange(0, batch * new + 1, new, dtype=torch.int32).cuda()
+    lens = torch.full((batch,), n, dtype=torch.int32).cuda()
+    table = torch.arange(pages, dtype=torch.int32).repeat(batch, 1).contiguous().cuda()
+    p = gie.PagedKv(batch, batch * new, kv, kv, dim, page, pages, pages, precision=precision, scale=scale, max_new=new,
+                    max_len=n)
+    size = gie.paged_attention_workspace_size(p)
+    ws = gie.DeviceBuffer(max(16, size))
+    torch.cuda.synchronize()
+    print("attend", p, flush=True)
+    gie.paged_attention(p, q.data_ptr(), k.data_ptr(), v.data_ptr(), starts.data_ptr(), lens.data_ptr(), table.data_ptr(),
+                        out.data_ptr(), workspace=ws.addr, ws_bytes=size)
+    torch.cuda.synchronize()
+    u, rest = UNIT[precision], n * 2.0 ** -gap
+    share = rest / (1 + rest)
+    small = 2.0 ** -32 * n / (1 + rest) if precision == "fp16" else 0
+    bound = u * share + small + (n / 16 + n / 32 + 40) * 2.0 ** -24 * share + 2.0 ** -17 * share
+    bound += u * (1 + bound)
+    worst = float((out.float() - 1).abs().max())
+    assert worst <= bound, (worst, bound)
+
+
+@pytest.mark.parametrize("k0,step", [(512, 1), (10240, 2), (24576, 4)])  # scores of 1e6, 2.1e7 and 5e7
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("precision", ["fp16", "bf16"])
+def test_scores_of_millions(k0, step, new, precision):
+    """Every 32 keys a score that is larger by one step of FP32 (or 1): all of them exact, so that the weights are
+    exp(step * i) whatever the scores' size is. Bound: weights and result rounded once, 2^x within 2^-20 of itself."""
+    c = Cache([new], [320], dim=64, heads=2, kv_heads=1, precision=precision, seed=3)
+    block = np.arange(320) // 32
+    c.q[:] = 0
+    c.q[..., 0], c.q[..., 1] = 2048, 1
+    c.k_pages[:] = 0
+    for j in range(320):
+        c.k_pages[c.table[0, j // c.page], :, j % c.page, :2] = k0, step * block[j]
+    got = c.attend(scale=1.0).astype(np.float64)
+    v = c.v_pages[c.table[0, np.arange(320) // c.page], 0, np.arange(320) % c.page].astype(np.float64)
+    u = UNIT[precision]
+    for i in range(new):
+        seen = 320 - new + i + 1
+        w = np.exp(step * (block[:seen] - block[seen - 1]).astype(np.float64))
+        w /= w.sum()
+        want, size = w @ v[:seen], w @ np.abs(v[:seen])
+        bound = (u + 2.0 ** -20 + seen * 2.0 ** -24 + 2.0 ** -16) * size
+        bound += u * (np.abs(want) + bound) + TINY[precision]
+        assert (np.abs(got[i] - want) <= bound).all(), (k0, i, float((np.abs(got[i] - want) - bound).max()))
