@@ -27,6 +27,8 @@
 // before q and out went through LDS) without exponentials -5 %, without any softmax -13 %, without loads -16 %. At that
 // time 64 rows for each wave (half the LDS reads, one wave for each SIMD) took 408 us, eight waves sharing a tile 318 and
 // more for ragged batches.
+#include <cmath>
+
 #include "paged_common.h"
 
 #include "lds_pipe.h"
@@ -838,6 +840,8 @@ extern "C" int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const
   if (!valid_paged(g)) return GIE_HIP_EINVAL;
   if (dtype != GIE_HIP_FP16 && dtype != GIE_HIP_BF16) return GIE_HIP_EUNSUPPORTED;
   if (g->head_dim != 64 && g->head_dim != 96 && g->head_dim != 128 && g->head_dim != 256) return GIE_HIP_EUNSUPPORTED;
+  // (a scale of 0 times a masked score is a NaN)
+  if (!std::isfinite(g->scale) || g->scale == 0 || !std::isfinite(g->softcap)) return GIE_HIP_EINVAL;
   if (g->total_tokens == 0) return GIE_HIP_OK;
   if (!q || !k_pages || !v_pages || !q_starts || !seq_lens || !page_table || !out || q == out) return GIE_HIP_EINVAL;
   if (!aligned_to(q, 2) || !aligned_to(out, 2) || !aligned_to(k_pages, 16) || !aligned_to(v_pages, 16))

@@ -408,7 +408,7 @@ typedef struct gie_paged_geom {
   int rotary_dim;    /* leading part of a head that rotates (even, 0: none) */
   int interleaved;   /* 1: pairs (2j, 2j + 1); 0: pairs (j, j + rotary_dim / 2) */
   int max_positions; /* rows of the cos / sin tables, at least max_pages * page_size when rotary_dim > 0 */
-  float scale;       /* of the scores */
+  float scale;       /* of the scores; attention refuses 0 (GIE_HIP_EINVAL) and, as in softcap, what is not finite */
   float softcap;     /* > 0: scores become softcap * tanh(score / softcap) */
   int window;        /* > 0: a token sees its own position and the window - 1 before it */
   int max_new;       /* most new tokens and longest length of a sequence, as the host knows them (0: not known): */

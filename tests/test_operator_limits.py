@@ -1,0 +1,28 @@
+"""Refusals of the kernels' own C-ABI (gie_hip_*) and limits on sizes. Needs no GPU: each call returns from the host's
+checks before anything is enqueued."""
+import ctypes
+import math
+
+import pytest
+
+import gie
+
+A, B, C, W, S, T = 0x10000, 0x20000, 0x30000, 0x40000, 0x50000, 0x60000  # addresses that are never read
+EINVAL, EUNSUPPORTED = -1, -2
+
+
+def geom(**k):
+    d = dict(batch=2, total_tokens=3, q_heads=8, kv_heads=2, head_dim=64, page_size=16, num_pages=8, max_pages=4,
+             q_stride=512, k_stride=128, v_stride=128, o_stride=512, scale=0.125)
+    return gie.GiePagedGeom(**{**d, **k})
+
+
+def attend(**k):
+    return gie.hip().gie_hip_paged_attention(gie.FP16, ctypes.byref(geom(**k)), A, C, W, S, S, T, B, W, 1 << 40, None)
+
+
+@pytest.mark.parametrize("bad", [dict(scale=0.0), dict(scale=-0.0), dict(scale=math.inf), dict(scale=-math.inf),
+                                 dict(scale=math.nan), dict(softcap=math.inf), dict(softcap=math.nan)])
+def test_attention_refuses_scales_without_an_answer(bad):
+    # a scale of 0 times a masked score is a NaN; 0 stands for the default in PagedKvProblem only
+    assert attend(**bad) == EINVAL
