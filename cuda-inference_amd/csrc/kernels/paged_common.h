@@ -73,6 +73,7 @@ inline bool valid_paged(const gie_paged_geom* g) {
   if ((long long)g->total_tokens * (g->q_heads / g->kv_heads) > (1 << 30) || g->batch > (1 << 30)) return false;
   if ((long long)g->page_size * g->head_dim > (1 << 26)) return false;
   const long long q = (long long)g->q_heads * g->head_dim, kv = (long long)g->kv_heads * g->head_dim;
+  if (q + 2 * kv > (1 << 30)) return false;  // a head's offset within its token, and a token's pieces, in 32 bits
   if (g->q_stride < q || g->o_stride < q || g->k_stride < kv || g->v_stride < kv) return false;
   return g->rotary_dim >= 0 && g->rotary_dim % 2 == 0 && g->rotary_dim <= g->head_dim && g->window >= 0 &&
          g->softcap >= 0 && g->max_new >= 0 && g->max_len >= 0;

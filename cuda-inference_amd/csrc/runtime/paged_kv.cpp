@@ -84,6 +84,7 @@ void validate_problem(const PagedKvProblem& p) {
   support(int64_t(p.total_tokens) * (p.q_heads / p.kv_heads) <= std::numeric_limits<int32_t>::max() / 2,
           "total_tokens * (q_heads / kv_heads) passes 2^30 rows");
   support(p.batch <= std::numeric_limits<int32_t>::max() / 2, "batch passes 2^30 sequences");
+  support(q + 2 * kv <= (1 << 30), "a token's heads of q, k and v pass 2^30 values");
   support(int64_t(p.page_size) * p.head_dim <= (1 << 26), "a page of one head is over 128 MiB");
 }
 

@@ -26,3 +26,26 @@ def attend(**k):
 def test_attention_refuses_scales_without_an_answer(bad):
     # a scale of 0 times a masked score is a NaN; 0 stands for the default in PagedKvProblem only
     assert attend(**bad) == EINVAL
+
+
+def paged(**k):
+    d = dict(batch=1, total_tokens=1, q_heads=8, kv_heads=2, head_dim=256, page_size=16, num_pages=8, max_pages=4)
+    return gie.PagedKv(**{**d, **k})
+
+
+@pytest.mark.parametrize("heads", [dict(q_heads=1 << 25, kv_heads=1), dict(q_heads=1 << 23, kv_heads=1 << 23),
+                                   dict(q_heads=1 << 22, kv_heads=1 << 21)])
+def test_heads_past_their_offsets_are_refused(heads):
+    """The kernels place a head within its token by a 32-bit offset, and count a token's pieces in 32 bits."""
+    p = paged(**heads)
+    for call in (lambda: gie.paged_attention_workspace_size(p),
+                 lambda: gie.kv_append(p, A, B, S, S, T, C, W),
+                 lambda: gie.paged_attention(p, A, C, W, S, S, T, B, workspace=W, ws_bytes=1 << 40)):
+        with pytest.raises(gie.GieError) as e:
+            call()
+        assert e.value.status == "Unsupported"
+    wide = dict(batch=1, total_tokens=1, head_dim=256, q_stride=1 << 34, o_stride=1 << 34, k_stride=1 << 33,
+                v_stride=1 << 33, **heads)
+    assert attend(**wide) == EINVAL
+    g = geom(**wide)
+    assert gie.hip().gie_hip_kv_append(gie.FP16, ctypes.byref(g), None, A, B, None, None, S, S, T, None, C, W, None) == EINVAL
