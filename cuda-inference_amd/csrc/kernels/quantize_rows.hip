@@ -73,6 +73,7 @@ using namespace gie_hip;
 extern "C" int gie_hip_quantize_rows(int dtype, const void* x, int64_t ld_x, int tokens, int features, int8_t* q,
                                      int64_t ld_q, float* scale, void* stream) {
   if (tokens < 0 || features <= 0 || ld_x < features || ld_q < features) return GIE_HIP_EINVAL;
+  if (features > (1 << 30)) return GIE_HIP_EUNSUPPORTED;  // a step past the row's end still has to fit 32 bits
   if (tokens == 0) return GIE_HIP_OK;
   if (!x || !q || !scale) return GIE_HIP_EINVAL;
   const size_t esz = dtype == GIE_HIP_FP32 ? 4 : 2;

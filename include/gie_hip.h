@@ -379,7 +379,8 @@ typedef struct gie_linear_geom {
 
 /* q[t][k] = rint(x[t][k] * (127 / a)), scale[t] = a / 127 with a = max(max_k |x[t][k]|, 2^-100), in FP32 with
    nearest-even rounding; a row that holds an infinity or a NaN gets scale NaN and q 0. x in `dtype` (FP32, FP16 or
-   BF16, aligned to its element), q rows ld_q >= features bytes apart (bytes past `features` are not written). */
+   BF16, aligned to its element), q rows ld_q >= features bytes apart (bytes past `features` are not written);
+   features <= 2^30, GIE_HIP_EUNSUPPORTED otherwise. */
 int gie_hip_quantize_rows(int dtype, const void* x, int64_t ld_x, int tokens, int features, int8_t* q, int64_t ld_q,
                           float* scale, void* stream);
 

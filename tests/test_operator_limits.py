@@ -49,3 +49,11 @@ def test_heads_past_their_offsets_are_refused(heads):
     assert attend(**wide) == EINVAL
     g = geom(**wide)
     assert gie.hip().gie_hip_kv_append(gie.FP16, ctypes.byref(g), None, A, B, None, None, S, S, T, None, C, W, None) == EINVAL
+
+
+@pytest.mark.parametrize("dtype", [gie.FP32, gie.FP16, gie.BF16])
+def test_quantize_rows_refuses_rows_past_its_counters(dtype):
+    """A row's last step would wrap the 32-bit counter of its values."""
+    for features in ((1 << 30) + 1, (1 << 31) - 1):
+        n = 1 << 31
+        assert gie.hip().gie_hip_quantize_rows(dtype, A, n, 1, features, B, n, S, None) == EUNSUPPORTED
