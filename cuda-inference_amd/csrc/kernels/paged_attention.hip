@@ -789,7 +789,9 @@ template <typename E, int D, bool LARGE_CAP>
 int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   const long long grid = (long long)s.slots * s.splits * a.kv_heads;
   const long long rows = (long long)a.total_tokens * a.q_heads;
-  if (grid * 512 > 0xffffffffll || rows * 64 > 0xffffffffll) return GIE_HIP_EUNSUPPORTED;  // a launch's threads
+  const bool many = s.splits > 8;
+  const long long joining = s.splits == 1 ? 0 : many ? rows * 256 : rows * 64;
+  if (grid * 512 > 0xffffffffll || joining > 0xffffff00ll) return GIE_HIP_EUNSUPPORTED;  // a launch's threads
   constexpr int P = kPitch<D>;
   int rc;
   if (s.wide) {
@@ -802,7 +804,6 @@ int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
     rc = start(attention_kernel<E, D, 1, WK, 1, NST, LARGE_CAP>, int(grid), 64 * WK, bytes > join ? bytes : join, stream, a);
   }
   if (rc != GIE_HIP_OK || s.splits == 1) return rc;
-  const bool many = s.splits > 8;
   const auto join =
       s.wide ? (many ? join_kernel<E, D, kWideRows, kWideKeys, 4> : join_kernel<E, D, kWideRows, kWideKeys, 1>)
              : (many ? join_kernel<E, D, kNarrowRows, kNarrowKeys, 4> : join_kernel<E, D, kNarrowRows, kNarrowKeys, 1>);
