@@ -643,15 +643,28 @@ extern "C" int gie_hip_linear_i8(int dtype, const gie_linear_geom* g, const void
   const size_t need = gie_hip_linear_i8_workspace(dtype, g, x_scale != nullptr);
   if (need > 0 && (!workspace || workspace_bytes < need || at(workspace) % 16 != 0)) return GIE_HIP_EINVAL;
   const Plan p = plan_of(*g);
-  if (p.form == kFewForm && g->out_features > (1 << 26)) return GIE_HIP_EUNSUPPORTED;
+  const bool own_x = x_scale == nullptr && !(p.form == kFewForm && fuses(*g));  // quantized into the workspace
+  const long long ld_x = own_x ? (long long)round16(g->in_features) : g->ld_x;
+  // direct loads into LDS take 16-byte pieces, and reach a tile's last row with a 32-bit offset
+  const bool aligned = ld_x % 16 == 0 && g->ld_w % 16 == 0 && (own_x || at(x) % 16 == 0) && at(w) % 16 == 0 &&
+                       ld_x < (1 << 22) && g->ld_w < (1 << 22);
   LinArgs a{};
+  if (p.form == kFewForm) {
+    if (g->out_features > (1 << 26)) return GIE_HIP_EUNSUPPORTED;
+  } else {
+    const int tile = p.form == kTile256 && !aligned ? 128 : p.tile;
+    const long long tm = (g->tokens + tile - 1) / tile, tn = (g->out_features + tile - 1) / tile;
+    if (tm * tn >= (1 << 23)) return GIE_HIP_EUNSUPPORTED;  // 512 threads for each: a launch's limit
+    a.tiles_m = int(tm);
+    a.tiles_n = int(tn);
+  }
   a.x = static_cast<const int8_t*>(x);
   a.x_scale = x_scale;
   a.w = w;
   a.w_scale = w_scale;
   a.bias = bias;
   a.y = y;
-  a.ld_x = g->ld_x;
+  a.ld_x = ld_x;
   a.ld_w = g->ld_w;
   a.ld_y = g->ld_y;
   a.M = g->tokens;
@@ -665,29 +678,15 @@ extern "C" int gie_hip_linear_i8(int dtype, const gie_linear_geom* g, const void
     a.part = reinterpret_cast<int*>(ws);
     ws += round16(size_t(p.splits) * g->tokens * g->out_features * 4);
   }
-  if (x_scale == nullptr) {
-    if (p.form == kFewForm && fuses(*g)) {
-      a.x16 = x;
-    } else {
-      const size_t ld = round16(g->in_features);
-      int8_t* q = reinterpret_cast<int8_t*>(ws);
-      float* scale = reinterpret_cast<float*>(ws + round16(size_t(g->tokens) * ld));
-      const int rc = gie_hip_quantize_rows(dtype, x, g->ld_x, g->tokens, g->in_features, q, int64_t(ld), scale, stream);
-      if (rc != GIE_HIP_OK) return rc;
-      a.x = q;
-      a.x_scale = scale;
-      a.ld_x = int64_t(ld);
-    }
-  }
-  // direct loads into LDS take 16-byte pieces, and reach a tile's last row with a 32-bit offset
-  const bool aligned = a.ld_x % 16 == 0 && a.ld_w % 16 == 0 && at(a.x) % 16 == 0 && at(w) % 16 == 0 &&
-                       a.ld_x < (1 << 22) && a.ld_w < (1 << 22);
-  const int tile = p.form == kTile256 && !aligned ? 128 : p.tile;
-  if (p.form != kFewForm) {
-    const long long tm = (g->tokens + tile - 1) / tile, tn = (g->out_features + tile - 1) / tile;
-    if (tm * tn >= (1 << 23)) return GIE_HIP_EUNSUPPORTED;  // 512 threads for each: a launch's limit
-    a.tiles_m = int(tm);
-    a.tiles_n = int(tn);
+  if (own_x) {
+    int8_t* q = reinterpret_cast<int8_t*>(ws);
+    float* scale = reinterpret_cast<float*>(ws + round16(size_t(g->tokens) * ld_x));
+    const int rc = gie_hip_quantize_rows(dtype, x, g->ld_x, g->tokens, g->in_features, q, ld_x, scale, stream);
+    if (rc != GIE_HIP_OK) return rc;
+    a.x = q;
+    a.x_scale = scale;
+  } else if (x_scale == nullptr) {
+    a.x16 = x;
   }
   a.y_vec = g->ld_y * esz % 16 == 0 && at(y) % 16 == 0;
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -57,3 +57,8 @@ def test_quantize_rows_refuses_rows_past_its_counters(dtype):
     for features in ((1 << 30) + 1, (1 << 31) - 1):
         n = 1 << 31
         assert gie.hip().gie_hip_quantize_rows(dtype, A, n, 1, features, B, n, S, None) == EUNSUPPORTED
+
+
+def test_linear_refuses_too_many_tiles_before_it_quantizes():
+    g = gie.GieLinearGeom(1 << 20, 64, 1 << 20, 64, 64, 1 << 20, 0)
+    assert gie.hip().gie_hip_linear_i8(gie.FP16, ctypes.byref(g), A, None, B, S, None, C, W, 1 << 60, None) == EUNSUPPORTED
