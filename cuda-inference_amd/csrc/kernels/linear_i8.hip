@@ -653,7 +653,7 @@ extern "C" int gie_hip_linear_i8(int dtype, const gie_linear_geom* g, const void
     if (g->out_features > (1 << 26)) return GIE_HIP_EUNSUPPORTED;
   } else {
     const int tile = p.form == kTile256 && !aligned ? 128 : p.tile;
-    const long long tm = (g->tokens + tile - 1) / tile, tn = (g->out_features + tile - 1) / tile;
+    const long long tm = (g->tokens + (long long)tile - 1) / tile, tn = (g->out_features + (long long)tile - 1) / tile;
     if (tm * tn >= (1 << 23)) return GIE_HIP_EUNSUPPORTED;  // 512 threads for each: a launch's limit
     a.tiles_m = int(tm);
     a.tiles_n = int(tn);

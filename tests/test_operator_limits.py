@@ -62,3 +62,9 @@ def test_quantize_rows_refuses_rows_past_its_counters(dtype):
 def test_linear_refuses_too_many_tiles_before_it_quantizes():
     g = gie.GieLinearGeom(1 << 20, 64, 1 << 20, 64, 64, 1 << 20, 0)
     assert gie.hip().gie_hip_linear_i8(gie.FP16, ctypes.byref(g), A, None, B, S, None, C, W, 1 << 60, None) == EUNSUPPORTED
+
+
+@pytest.mark.parametrize("tokens,out", [((1 << 31) - 1, 1), (17, (1 << 31) - 1), ((1 << 31) - 60, 200)])
+def test_linear_counts_tiles_in_64_bits(tokens, out):
+    g = gie.GieLinearGeom(tokens, 16, out, 16, 16, out, 0)
+    assert gie.hip().gie_hip_linear_i8(gie.FP16, ctypes.byref(g), A, S, B, S, None, C, W, 1 << 60, None) == EUNSUPPORTED
