@@ -31,3 +31,33 @@ def test_more_rows_than_a_join_could_take():
     want, bound = c.plain()
     assert (np.abs(out[:new].float().cpu().numpy() - want) <= bound).all()
     assert bool((out.view(batch, -1) == out[:new].reshape(1, -1)).all())
+
+
+def check(c, **hints):
+    got = c.attend(**hints).astype(np.float64)
+    want, bound = c.plain()
+    assert np.isfinite(got).all() and (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("batch", [64, 65, 70])
+@pytest.mark.parametrize("chunk", [1, 40])
+def test_parts_are_joined_in_large_batches(batch, chunk):
+    """The join finds a token's sequence by lanes up to 64 sequences and by a search past them; sequences without new
+    tokens and one with a chunk among them, one context long enough to be split, the others in one part."""
+    new = [b % 3 > 0 for b in range(batch)]
+    new = [int(n) for n in new]
+    new[batch - 4] = chunk
+    lens = [n + 11 * b % 60 for b, n in enumerate(new)]
+    lens[batch - 4] = 3000
+    c = Cache(new, lens, heads=2, kv_heads=1, dim=64, page=32, seed=batch)
+    hints = dict(max_new=max(new), max_len=3000)
+    assert gie.paged_attention_workspace_size(c.p(**hints)) > 0
+    check(c, **hints)
+
+
+def test_more_sequences_than_two_searches_cover():
+    """Past 4096 sequences the search for a row's sequence takes three steps."""
+    rng = np.random.default_rng(5)
+    new = rng.integers(0, 3, 4200).tolist()
+    lens = [n + int(rng.integers(0, 20)) for n in new]
+    check(Cache(new, lens, heads=2, kv_heads=1, dim=64, seed=6))

@@ -68,3 +68,29 @@ def test_linear_refuses_too_many_tiles_before_it_quantizes():
 def test_linear_counts_tiles_in_64_bits(tokens, out):
     g = gie.GieLinearGeom(tokens, 16, out, 16, 16, out, 0)
     assert gie.hip().gie_hip_linear_i8(gie.FP16, ctypes.byref(g), A, S, B, S, None, C, W, 1 << 60, None) == EUNSUPPORTED
+
+
+def test_linear_workspace_that_is_needed_is_checked():
+    p = gie.LinearI8(64, 512, 128)  # tokens quantized into it
+    n = gie.linear_i8_workspace_size(p)
+    assert n >= 64 * 512 + 64 * 4
+    for workspace, ws_bytes, want in ((W, n - 1, "WorkspaceTooSmall"), (None, 0, "WorkspaceTooSmall"),
+                                      (None, n, "WorkspaceTooSmall"), (W + 8, n, "InvalidArgument")):
+        with pytest.raises(gie.GieError) as e:
+            gie.linear_i8(p, A, B, S, C, workspace=workspace, ws_bytes=ws_bytes)
+        assert e.value.status == want
+
+
+def test_attention_workspace_that_is_needed_is_checked():
+    p = gie.PagedKv(1, 1, 8, 2, 64, 16, 8, 4096, max_new=1, max_len=65536)
+    n = gie.paged_attention_workspace_size(p)
+    assert n > 0
+    for workspace, ws_bytes, want in ((W, n - 1, "WorkspaceTooSmall"), (None, 0, "WorkspaceTooSmall"),
+                                      (W + 4, n, "InvalidArgument")):
+        with pytest.raises(gie.GieError) as e:
+            gie.paged_attention(p, A, C, B, S, S, T, W, workspace=workspace, ws_bytes=ws_bytes)
+        assert e.value.status == want
+
+
+def test_no_tokens_need_no_workspace():
+    assert gie.paged_attention_workspace_size(gie.PagedKv(2, 0, 8, 2, 64, 16, 8, 4096, max_len=65536)) == 0
