@@ -8,18 +8,19 @@
 //     16x16x64 MFMAs, 8 steps in flight (64 KiB for a compute unit); their sums meet in LDS. Where x is not in 8 bits yet
 //     and short (up to 4 tokens, 32 Ki values), every workgroup quantizes it for itself under the weights' loads: a
 //     launch before this one costs 3.3 us. 1x4096x4096: 8.6 us, of which the 16.8 MB of weights are 3.6 at the copy's
-//     rate and the rest a launch and one chain x -> scale -> 8 bits -> product; 2x8192x8192 18 us, 3.7 TB/s.
+//     rate; the rest is a launch, one chain x -> scale -> 8 bits -> product, and the moves of 211 scalars that do not fit
+//     their registers (the form that reads x in 8 bits has none); 2x8192x8192 18 us, 3.7 TB/s.
 //   * tiles of 32 to 256 tokens and channels: 128 input values of each in LDS at a time, NST stages of direct loads,
 //     32x32x32 MFMAs. Channels are the rows of a product and tokens its columns, so a lane holds 4 neighbouring channels of
 //     one token; the finished tile goes through LDS and out in whole rows. Rows of 128 bytes with their 16-byte chunks
 //     permuted by the row meet no LDS bank twice. Tiles of 32 are shared by 4 waves along the input values. Where there
 //     are too few tiles to fill the device they are split over parts of the input values: int32 partial sums in the
 //     workspace and a second launch that joins them (integers: the order does not matter).
-//     4096x4096x16384: 264-280 us, 2.0-2.1 POP/s; 8192x8192x8192: 486 us, 2.26 POP/s (the library product of the same
-//     size 2.13). The matrix cores are busy half of the time; without loads the same products take 218 us, loads alone
-//     217: L2 -> LDS runs at 10-13 TB/s, whatever the number of stages (2, 3, 4 measured), the order of a row's chunks
-//     (measured without the permutation) and the order of the tiles (1 to 16 of tokens in a run: 265-283 us).
-//     64x8192x8192: 17.3 us for 67 MB of weights, 3.9 TB/s, and 4 us for the join.
+//     4096x4096x16384: 265-288 us with its quantization (11 us), 1.9-2.1 POP/s; 8192x8192x8192 in 8 bits already: 473-486
+//     us, 2.3 POP/s (the library product of the same size 2.13). The matrix cores are busy half of the time; without
+//     loads the same products take 218 us, loads alone 217: L2 -> LDS runs at 10-13 TB/s, whatever the number of stages
+//     (2, 3, 4 measured), the order of a row's chunks (measured without the permutation) and the order of the tiles (1 to
+//     16 of tokens in a run: 265-283 us). 64x8192x8192: 17 us for 67 MB of weights, 4.0 TB/s, and 4 us for the join.
 // Rows that no 16-byte piece fits (ld or address) go through registers instead of direct loads, in pieces of any
 // alignment, up to 4 slices ahead: 429x9468x1888 40 us against 36 at 9472.
 #include "quantize_common.h"
@@ -567,6 +568,10 @@ Plan plan_of(const gie_linear_geom& g) {
   return p;
 }
 
+// Quantized inside the product: one launch less, but every workgroup does it. us in one launch / in two, 16 bits: 1x4096x4096
+// 7.8 / 9.4, 1x16384x4096 19.2 / 27.8, 1x28672x4096 31.4 / 48.2, 1x32768x8192 67.7 / 69.6, 4x8192x4096 14.7 / 14.9,
+// 4x8192x8192 21.9 / 19.8; 32 bits: 1x14336x4096 18.8 / 27.8, 2x14336x8192 31.5 / 32.6. (Rows past what the threads keep
+// are read a second time, value by value; that, too, is less than the second launch.)
 bool fuses(const gie_linear_geom& g) { return g.tokens <= 4 && (long long)g.tokens * g.in_features <= 32 * 1024; }
 
 template <typename E, int BM, int BN, int WM, int WN, int WK, int NST>

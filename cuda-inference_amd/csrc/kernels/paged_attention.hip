@@ -21,12 +21,15 @@
 //
 // Few rows (one token of a grouped head: up to 32) are bound by the cache's bytes: one token over 32768 positions of 8
 // key heads of 128 in 32 parts 24 us + 4 for the join, 4.6 TB/s in all; a step of 64 sequences 219 us, 5.0 TB/s (a large
-// copy reaches 4.7). Many rows are bound by the products: two prompts of 4096 tokens, 32 heads of 128, 293-301 us, 0.93
-// PFLOP/s (a large library product 1.23); 2048 tokens over 30000 1.0. Matrix cores are busy 0.4 of the time, the vector
-// unit (softmax) 0.35 and LDS 0.22, on two workgroups of 4 waves for each compute unit: measured (at 310 us for a call,
-// before q and out went through LDS) without exponentials -5 %, without any softmax -13 %, without loads -16 %. At that
-// time 64 rows for each wave (half the LDS reads, one wave for each SIMD) took 408 us, eight waves sharing a tile 318 and
-// more for ragged batches.
+// copy reaches 4.7). Many rows are bound by the products: two prompts of 4096 tokens, 32 heads of 128, 288-311 us, 0.88 to
+// 0.95 PFLOP/s (a large library product 1.23); 2048 tokens over 30000 1.0. Matrix cores are busy 0.42 of the time, the
+// vector unit (softmax) 0.47 and LDS 0.35, on two workgroups of 4 waves for each compute unit (BF16): measured (at 310 us
+// for a call, before q and out went through LDS) without exponentials -5 %, without any softmax -13 %, without loads
+// -16 %. At that time 64 rows for each wave (half the LDS reads, one wave for each SIMD) took 408 us, eight waves sharing
+// a tile 318 and more for ragged batches.
+// The weights enter the second product in the storage type, since the matrix cores take FP32 at a sixteenth of the rate:
+// outputs are off by 2.1e-3 to 2.3e-3 of their size in BF16 and 2.8e-4 in FP16, where the same in FP32 with one rounding
+// at the end has 1.7e-3 and 2.1e-4.
 #include <cmath>
 
 #include "paged_common.h"
