@@ -456,7 +456,7 @@ __global__ __launch_bounds__(64 * WR * WK * WD, WK == 2 ? 1 : 2) void attention_
       if (__any((top - m) * a.mult > 8.f)) {
         const float next = fmaxf(m, top);
         float nc = next == -INFINITY ? 0.f : next * a.mult;
-        // what rounding takes from nc would come on top of the lift: 2^-23 of it and more are added
+        // what rounding takes from nc would come on top of the lift, so 2^-23 of it is added, which is no less
         if constexpr (kLift > 0) nc += __builtin_fmaf(fabsf(nc), 0x1p-23f, -kLift);
         const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - nc);  // 1: nothing summed yet
         m = next;
@@ -800,7 +800,8 @@ int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   if (s.wide) {
     constexpr int NST = 2;
     constexpr int WR = kWideRows / 32, WD = D == 256 ? 2 : 1;
-    rc = start(attention_kernel<E, D, WR, 1, WD, NST, LARGE_CAP>, int(grid), 64 * WR * WD, NST * 2 * 16 * WR * P + 64, stream, a);
+    constexpr int bytes = NST * 2 * 16 * WR * P + 64;
+    rc = start(attention_kernel<E, D, WR, 1, WD, NST, LARGE_CAP>, int(grid), 64 * WR * WD, bytes, stream, a);
   } else {
     constexpr int WK = D == 256 ? 2 : 4, NST = D == 64 ? 4 : 2;
     constexpr int bytes = WK * NST * 2 * 32 * P, join = WK * 256 + WK * 32 * (D + 4) * 4;
