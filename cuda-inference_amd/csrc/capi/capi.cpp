@@ -147,6 +147,10 @@ PagedKvProblem to_paged(const gie_paged_kv_problem* p) {
   r.window = p->window;
   r.max_new = p->max_new;
   r.max_len = p->max_len;
+  r.sinks = p->sinks;
+  r.norm_eps = p->norm_eps;
+  GIE_REQUIRE(p->code >= 0 && p->code <= 2, StatusCode::kInvalidArgument, "bad code");
+  r.code = static_cast<KvCode>(p->code);
   return r;
 }
 
@@ -990,6 +994,58 @@ extern "C" int gie_paged_attention(const gie_paged_kv_problem* p, const void* q,
   return guarded([&] {
     PagedKv::attention(q, k_pages, v_pages, q_starts, seq_lens, page_table, to_paged(p), out, workspace,
                        workspace_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int gie_kv_append_normed(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v,
+                                    const float* q_norm, const float* k_norm, const float* cos, const float* sin,
+                                    const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
+                                    void* k_pages, void* v_pages, void* stream) {
+  return guarded([&] {
+    PagedKv::append_normed(q, k, v, q_norm, k_norm, cos, sin, q_starts, seq_lens, page_table, to_paged(p), q_out,
+                           k_pages, v_pages, static_cast<hipStream_t>(stream));
+  });
+}
+
+namespace {
+Kv8Pages kv8_pages(const void* k, const void* v, const float* k_scales, const float* v_scales) {
+  return {const_cast<void*>(k), const_cast<void*>(v), const_cast<float*>(k_scales), const_cast<float*>(v_scales)};
+}
+}  // namespace
+
+extern "C" int gie_kv8_append(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v,
+                              const float* q_norm, const float* k_norm, const float* cos, const float* sin,
+                              const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
+                              void* k_pages, void* v_pages, float* k_scales, float* v_scales, void* stream) {
+  return guarded([&] {
+    PagedKv8::append(q, k, v, q_norm, k_norm, cos, sin, q_starts, seq_lens, page_table, to_paged(p), q_out,
+                     kv8_pages(k_pages, v_pages, k_scales, v_scales), static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int gie_kv8_read(const gie_paged_kv_problem* p, const void* k_pages, const void* v_pages,
+                            const float* k_scales, const float* v_scales, const int* q_starts, const int* seq_lens,
+                            const int* page_table, void* k, void* v, void* stream) {
+  return guarded([&] {
+    PagedKv8::read(kv8_pages(k_pages, v_pages, k_scales, v_scales), q_starts, seq_lens, page_table, to_paged(p), k, v,
+                   static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int gie_kv8_attention_workspace_size(const gie_paged_kv_problem* p, size_t* bytes) {
+  return guarded([&] {
+    GIE_REQUIRE(bytes != nullptr, StatusCode::kInvalidArgument, "null out");
+    *bytes = PagedKv8::workspace_size(to_paged(p));
+  });
+}
+
+extern "C" int gie_kv8_attention(const gie_paged_kv_problem* p, const void* q, const void* k_pages,
+                                 const void* v_pages, const float* k_scales, const float* v_scales,
+                                 const int* q_starts, const int* seq_lens, const int* page_table, void* out,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    PagedKv8::attention(q, kv8_pages(k_pages, v_pages, k_scales, v_scales), q_starts, seq_lens, page_table,
+                        to_paged(p), out, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
   });
 }
 

@@ -1,0 +1,77 @@
+// Device vocabulary of the paged cache in 8 bits (kv_append_normed, kv8_read, kv8_attention): codes, their blocks and
+// scales. Private to csrc/kernels.
+#pragma once
+
+#include "paged_common.h"
+
+namespace gie_hip {
+
+constexpr int kKvBlock = 16;  // positions of a head that share a scale
+// No block counts as smaller than this: a scale of 0 would have no reciprocal, and the attention divides sums by a
+// block's scale, which stays far inside FP32's range so.
+constexpr float kKvLeast = 0x1p-64f;
+
+// Codes: encode4 rounds four values (already divided by the scale, so within the largest code but for FP32's rounding)
+// to nearest even, byte by byte; decode2 gives bytes 0 and 1, or 2 and 3, as FP16 times 1 / kUnit, exactly.
+struct Int8Code {
+  static constexpr float kUnit = 1.f;
+  static __device__ __forceinline__ float scale(float most) { return fmaxf(most, kKvLeast) / 127.f; }
+  static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    const auto one = [](float x) { return uint32_t(int(rintf(fminf(fmaxf(x, -127.f), 127.f)))) & 255u; };
+    return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+  }
+  static __device__ __forceinline__ uint32_t encode1(float a) { return encode4(a, 0.f, 0.f, 0.f); }
+  static __device__ __forceinline__ float decode1(uint32_t code) { return float(int8_t(code)); }
+};
+
+// e4m3 with a power of 2 as scale: a larger scale moves exponents alone, so codes that are rounded again keep their bits
+// unless they fall among the subnormals.
+struct E4m3Code {
+  static constexpr float kUnit = 256.f;  // bits moved into FP16's fields stand for 2^(7 - 15) of the value
+  static __device__ __forceinline__ float scale(float most) {
+    const uint32_t bits = __float_as_uint(fmaxf(most, kKvLeast));  // 448 = 1.75 2^8
+    return __uint_as_float(((bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u)) << 23);
+  }
+  static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    const auto in = [](float x) { return fminf(fmaxf(x, -448.f), 448.f); };
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(in(a), in(b), 0, false);
+    return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(in(c), in(d), r, true));
+  }
+  static __device__ __forceinline__ uint32_t encode1(float a) { return encode4(a, 0.f, 0.f, 0.f) & 255u; }
+  static __device__ __forceinline__ float decode1(uint32_t code) {  // the NaN codes (0x7f, 0xff) become 480
+    return float(__builtin_bit_cast(_Float16, uint16_t((code & 0x80u) << 8 | (code & 0x7fu) << 7))) * kUnit;
+  }
+};
+
+// The block of a slot of a sequence's new tokens: positions [first, end) are new, the block's own start at `start`;
+// none: first >= end. page -1: not stored.
+struct Block {
+  int start, first, end, page, slot;
+  int row0;  // row of q, k, v of position `first`
+};
+__device__ __forceinline__ Block block_of(const gie_paged_geom& g, const int* __restrict__ q_starts,
+                                          const int* __restrict__ seq_lens, const int* __restrict__ page_table, int slot) {
+  // n tokens from any position on touch at most n / 16 + 2 blocks, so sequence b's slots start at floor(first / 16) + 2 b
+  const auto from = [&](int first, int b) { return min(max(first, 0), g.total_tokens) / kKvBlock + 2 * b; };
+  const Sequence s = locate(q_starts, seq_lens, g.batch, g.total_tokens, slot, from);
+  const int p0 = max(s.base, 0), p1 = int(min((long long)s.base + s.count, (long long)g.max_pages * g.page_size)), at = slot - from(s.first, s.index);
+  Block r;
+  r.start = (p0 / kKvBlock + at) * kKvBlock;
+  r.first = max(r.start, p0);
+  r.end = at >= 0 ? min(r.start + kKvBlock, p1) : r.first;
+  r.row0 = s.first + (r.first - s.base);
+  r.page = -1;
+  r.slot = 0;
+  if (r.first < r.end) {
+    const int row = r.start / g.page_size;
+    const int page = page_table[(long long)s.index * g.max_pages + row];
+    if (page >= 0 && page < g.num_pages) r.page = page;
+    r.slot = r.start - row * g.page_size;
+  }
+  return r;
+}
+inline long long block_slots(const gie_paged_geom& g) { return (long long)g.total_tokens / kKvBlock + 2ll * g.batch; }
+
+inline bool valid_code(int code) { return code == GIE_HIP_KV_INT8 || code == GIE_HIP_KV_E4M3; }
+
+}  // namespace gie_hip

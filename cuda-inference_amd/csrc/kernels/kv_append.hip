@@ -34,29 +34,6 @@ struct AppendArgs {
   int tokens;  // of a workgroup
 };
 
-// where a token goes: position -1 without a valid one, page -1 if it is not stored, tokens of no sequence: absent
-struct Place {
-  int position, page, slot, present;
-};
-
-__device__ __forceinline__ Place place_of(const AppendArgs& a, int t) {
-  const gie_paged_geom& g = a.g;
-  const Sequence s = locate(a.q_starts, a.seq_lens, g.batch, g.total_tokens, t, [](int first, int) { return first; });
-  Place p;
-  p.present = t >= s.first && t < s.first + s.count;
-  p.position = s.base + (t - s.first);
-  if (!p.present || p.position < 0 || p.position >= g.max_pages * g.page_size) p.position = -1;
-  p.page = -1;
-  p.slot = 0;
-  if (p.position >= 0) {
-    const int row = p.position / g.page_size;
-    const int page = a.page_table[(long long)s.index * g.max_pages + row];
-    if (page >= 0 && page < g.num_pages) p.page = page;
-    p.slot = p.position - row * g.page_size;
-  }
-  return p;
-}
-
 // a head's place in its source and its destination, for head `head` of a token's q, k and v heads one after another
 struct Head {
   const uint16_t* src;
@@ -111,7 +88,7 @@ __global__ __launch_bounds__(1024) void append_kernel(AppendArgs a) {
   const int tid = int(threadIdx.x), threads = int(blockDim.x);
   const int t0 = int(blockIdx.x) * a.tokens, count = min(a.tokens, a.g.total_tokens - t0);
   for (int i = tid >> 6; i < count; i += threads >> 6) {
-    const Place p = place_of(a, t0 + i);
+    const Place p = place_of(a.g, a.q_starts, a.seq_lens, a.page_table, t0 + i);
     if ((tid & 63) == 0) places[i] = p;
   }
   __syncthreads();
@@ -141,7 +118,7 @@ __global__ __launch_bounds__(1024) void append_kernel(AppendArgs a) {
 template <typename E>
 __global__ __launch_bounds__(256) void append_values_kernel(AppendArgs a) {
   const int t = int(blockIdx.x);
-  const Place p = place_of(a, t);
+  const Place p = place_of(a.g, a.q_starts, a.seq_lens, a.page_table, t);
   if (!p.present) return;
   const int half = a.g.rotary_dim / 2, units = a.g.head_dim - half;  // of a head: pairs, then single values
   const int heads = (a.q ? a.g.q_heads : 0) + 2 * a.g.kv_heads;

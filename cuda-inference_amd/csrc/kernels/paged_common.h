@@ -63,6 +63,29 @@ __device__ __forceinline__ Sequence locate(const int* __restrict__ q_starts, con
   return s;
 }
 
+// where a token goes: position -1 without a valid one, page -1 if it is not stored, tokens of no sequence: absent
+struct Place {
+  int position, page, slot, present;
+};
+
+__device__ __forceinline__ Place place_of(const gie_paged_geom& g, const int* __restrict__ q_starts,
+                                          const int* __restrict__ seq_lens, const int* __restrict__ page_table, int t) {
+  const Sequence s = locate(q_starts, seq_lens, g.batch, g.total_tokens, t, [](int first, int) { return first; });
+  Place p;
+  p.present = t >= s.first && t < s.first + s.count;
+  p.position = s.base + (t - s.first);
+  if (!p.present || p.position < 0 || p.position >= g.max_pages * g.page_size) p.position = -1;
+  p.page = -1;
+  p.slot = 0;
+  if (p.position >= 0) {
+    const int row = p.position / g.page_size;
+    const int page = page_table[(long long)s.index * g.max_pages + row];
+    if (page >= 0 && page < g.num_pages) p.page = page;
+    p.slot = p.position - row * g.page_size;
+  }
+  return p;
+}
+
 // what the kernels' grids and offsets assume
 inline bool valid_paged(const gie_paged_geom* g) {
   if (!g || g->batch < 0 || g->total_tokens < 0 || (g->batch == 0 && g->total_tokens > 0)) return false;
@@ -76,7 +99,7 @@ inline bool valid_paged(const gie_paged_geom* g) {
   if (q + 2 * kv > (1 << 30)) return false;  // a head's offset within its token, and a token's pieces, in 32 bits
   if (g->q_stride < q || g->o_stride < q || g->k_stride < kv || g->v_stride < kv) return false;
   return g->rotary_dim >= 0 && g->rotary_dim % 2 == 0 && g->rotary_dim <= g->head_dim && g->window >= 0 &&
-         g->softcap >= 0 && g->max_new >= 0 && g->max_len >= 0;
+         g->softcap >= 0 && g->max_new >= 0 && g->max_len >= 0 && g->sinks >= 0;
 }
 
 inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

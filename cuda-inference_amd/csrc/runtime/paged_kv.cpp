@@ -40,10 +40,14 @@ gie_paged_geom geom_of(const PagedKvProblem& p) {
   g.window = p.window;
   g.max_new = p.max_new;
   g.max_len = p.max_len;
+  g.sinks = p.sinks;
+  g.norm_eps = p.norm_eps;
   return g;
 }
 
 int dtype_of(Precision p) { return p == Precision::kFp16 ? GIE_HIP_FP16 : GIE_HIP_BF16; }
+
+int code_of(KvCode c) { return c == KvCode::kInt8 ? GIE_HIP_KV_INT8 : GIE_HIP_KV_E4M3; }
 
 void require_cache(const void* k_pages, const void* v_pages, const int* q_starts, const int* seq_lens,
                    const int* page_table) {
@@ -53,6 +57,46 @@ void require_cache(const void* k_pages, const void* v_pages, const int* q_starts
   require(k_pages != v_pages, "K and V need pages of their own");
   require(aligned(q_starts, 4) && aligned(seq_lens, 4) && aligned(page_table, 4),
           "q_starts, seq_lens and page_table must be 4-byte aligned");
+}
+
+void require_held(const PagedKvProblem& p, bool in_8_bits) {
+  if (in_8_bits)
+    require(p.code == KvCode::kInt8 || p.code == KvCode::kE4m3, "code must be kInt8 or kE4m3 for a cache in 8 bits");
+  else
+    require(p.code == KvCode::kNone, "code must be kNone for a cache in the problem's precision");
+}
+
+void require_pages(const Kv8Pages& c, const int* q_starts, const int* seq_lens, const int* page_table) {
+  require_cache(c.k, c.v, q_starts, seq_lens, page_table);
+  require(c.k_scales && c.v_scales && c.k_scales != c.v_scales, "k_scales and v_scales must be there and differ");
+  require(aligned(c.k_scales, 4) && aligned(c.v_scales, 4), "scales must be 4-byte aligned");
+}
+
+void require_rows(const void* q, const void* k, const void* v, const float* q_norm, const float* k_norm,
+                  const float* cos, const float* sin, const PagedKvProblem& p, const gie_paged_geom& g,
+                  const void* q_out) {
+  require(k && v, "k and v must not be null");
+  require((q == nullptr) == (q_out == nullptr), "q and q_out go together");
+  require(aligned(q, 2) && aligned(k, 2) && aligned(v, 2) && aligned(q_out, 2),
+          "q, k, v and q_out must be aligned to their elements");
+  require(q != q_out || q == nullptr || g.q_stride == g.o_stride, "q in place needs q_stride == o_stride");
+  require(q_norm == nullptr || q != nullptr, "q_norm without q");
+  require(aligned(q_norm, 4) && aligned(k_norm, 4), "q_norm and k_norm must be 4-byte aligned");
+  if (p.rotary_dim > 0) {
+    require(cos && sin && aligned(cos, 4) && aligned(sin, 4), "cos and sin must be there and 4-byte aligned");
+    require(int64_t(p.max_positions) >= int64_t(p.max_pages) * p.page_size,
+            "max_positions must cover max_pages * page_size positions");
+  }
+}
+
+void require_attention(const void* q, const void* out, const void* workspace, size_t workspace_bytes, size_t need) {
+  require(q && out, "q and out must not be null");
+  require(q != out, "out must not be q");
+  require(aligned(q, 2) && aligned(out, 2), "q and out must be aligned to their elements");
+  GIE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), StatusCode::kWorkspaceTooSmall,
+              "PagedKv: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) +
+                  " needed");
+  require(aligned(workspace, 16), "workspace must be 16-byte aligned");
 }
 
 }  // namespace
@@ -66,8 +110,9 @@ void validate_problem(const PagedKvProblem& p) {
           "page_size, num_pages, max_pages and head_dim must be positive");
   require(p.rotary_dim >= 0 && p.rotary_dim % 2 == 0 && p.rotary_dim <= p.head_dim,
           "rotary_dim must be even and within head_dim");
-  require(p.window >= 0 && p.max_new >= 0 && p.max_len >= 0 && p.max_positions >= 0,
-          "window, max_new, max_len and max_positions must not be negative");
+  require(p.window >= 0 && p.max_new >= 0 && p.max_len >= 0 && p.max_positions >= 0 && p.sinks >= 0,
+          "window, sinks, max_new, max_len and max_positions must not be negative");
+  require(std::isfinite(p.norm_eps) && p.norm_eps >= 0, "norm_eps must be finite and not negative");
   require(std::isfinite(p.scale) && std::isfinite(p.softcap) && p.softcap >= 0,
           "scale must be finite, softcap finite and not negative");
   const int64_t q = int64_t(p.q_heads) * p.head_dim, kv = int64_t(p.kv_heads) * p.head_dim;
@@ -93,26 +138,90 @@ void PagedKv::append(const void* q, const void* k, const void* v, const float* c
                      void* q_out, void* k_pages, void* v_pages, hipStream_t stream) {
   validate_problem(p);
   if (p.total_tokens == 0) return;
+  require_held(p, false);
   require_cache(k_pages, v_pages, q_starts, seq_lens, page_table);
-  require(k && v, "k and v must not be null");
-  require((q == nullptr) == (q_out == nullptr), "q and q_out go together");
-  require(aligned(q, 2) && aligned(k, 2) && aligned(v, 2) && aligned(q_out, 2),
-          "q, k, v and q_out must be aligned to their elements");
   const gie_paged_geom g = geom_of(p);
-  require(q != q_out || q == nullptr || g.q_stride == g.o_stride, "q in place needs q_stride == o_stride");
-  if (p.rotary_dim > 0) {
-    require(cos && sin && aligned(cos, 4) && aligned(sin, 4), "cos and sin must be there and 4-byte aligned");
-    require(int64_t(p.max_positions) >= int64_t(p.max_pages) * p.page_size,
-            "max_positions must cover max_pages * page_size positions");
-  }
+  require_rows(q, k, v, nullptr, nullptr, cos, sin, p, g, q_out);
   RoctxRange range("gie::PagedKv::append");
   check_kernel_status(gie_hip_kv_append(dtype_of(p.precision), &g, q, k, v, cos, sin, q_starts, seq_lens, page_table,
                                         q_out, k_pages, v_pages, stream),
                       "PagedKv::append");
 }
 
+void PagedKv::append_normed(const void* q, const void* k, const void* v, const float* q_norm, const float* k_norm,
+                            const float* cos, const float* sin, const int* q_starts, const int* seq_lens,
+                            const int* page_table, const PagedKvProblem& p, void* q_out, void* k_pages, void* v_pages,
+                            hipStream_t stream) {
+  validate_problem(p);
+  if (p.total_tokens == 0) return;
+  require_held(p, false);
+  require_cache(k_pages, v_pages, q_starts, seq_lens, page_table);
+  const gie_paged_geom g = geom_of(p);
+  require_rows(q, k, v, q_norm, k_norm, cos, sin, p, g, q_out);
+  RoctxRange range("gie::PagedKv::append_normed");
+  check_kernel_status(gie_hip_kv_append_normed(dtype_of(p.precision), &g, q, k, v, q_norm, k_norm, cos, sin, q_starts,
+                                               seq_lens, page_table, q_out, k_pages, v_pages, stream),
+                      "PagedKv::append_normed");
+}
+
+void PagedKv8::append(const void* q, const void* k, const void* v, const float* q_norm, const float* k_norm,
+                      const float* cos, const float* sin, const int* q_starts, const int* seq_lens,
+                      const int* page_table, const PagedKvProblem& p, void* q_out, const Kv8Pages& pages,
+                      hipStream_t stream) {
+  validate_problem(p);
+  require_held(p, true);
+  if (p.total_tokens == 0) return;
+  require_pages(pages, q_starts, seq_lens, page_table);
+  const gie_paged_geom g = geom_of(p);
+  require_rows(q, k, v, q_norm, k_norm, cos, sin, p, g, q_out);
+  RoctxRange range("gie::PagedKv8::append");
+  check_kernel_status(gie_hip_kv8_append(dtype_of(p.precision), code_of(p.code), &g, q, k, v, q_norm, k_norm, cos, sin,
+                                         q_starts, seq_lens, page_table, q_out, pages.k, pages.v, pages.k_scales,
+                                         pages.v_scales, stream),
+                      "PagedKv8::append");
+}
+
+void PagedKv8::read(const Kv8Pages& pages, const int* q_starts, const int* seq_lens, const int* page_table,
+                    const PagedKvProblem& p, void* k, void* v, hipStream_t stream) {
+  validate_problem(p);
+  require_held(p, true);
+  if (p.total_tokens == 0 || (!k && !v)) return;
+  require_pages(pages, q_starts, seq_lens, page_table);
+  require(aligned(k, 2) && aligned(v, 2), "k and v must be aligned to their elements");
+  require(k != v, "k and v need rows of their own");
+  const gie_paged_geom g = geom_of(p);
+  RoctxRange range("gie::PagedKv8::read");
+  check_kernel_status(gie_hip_kv8_read(dtype_of(p.precision), code_of(p.code), &g, pages.k, pages.v, pages.k_scales,
+                                       pages.v_scales, q_starts, seq_lens, page_table, k, v, stream),
+                      "PagedKv8::read");
+}
+
+size_t PagedKv8::workspace_size(const PagedKvProblem& p) {
+  validate_problem(p);
+  require_held(p, true);
+  const gie_paged_geom g = geom_of(p);
+  return gie_hip_kv8_attention_workspace(&g);
+}
+
+void PagedKv8::attention(const void* q, const Kv8Pages& pages, const int* q_starts, const int* seq_lens,
+                         const int* page_table, const PagedKvProblem& p, void* out, void* workspace,
+                         size_t workspace_bytes, hipStream_t stream) {
+  validate_problem(p);
+  require_held(p, true);
+  if (p.total_tokens == 0) return;
+  require_pages(pages, q_starts, seq_lens, page_table);
+  const gie_paged_geom g = geom_of(p);
+  require_attention(q, out, workspace, workspace_bytes, gie_hip_kv8_attention_workspace(&g));
+  RoctxRange range("gie::PagedKv8::attention");
+  check_kernel_status(gie_hip_kv8_attention(dtype_of(p.precision), code_of(p.code), &g, q, pages.k, pages.v,
+                                            pages.k_scales, pages.v_scales, q_starts, seq_lens, page_table, out,
+                                            workspace, workspace_bytes, stream),
+                      "PagedKv8::attention");
+}
+
 size_t PagedKv::workspace_size(const PagedKvProblem& p) {
   validate_problem(p);
+  require_held(p, false);
   const gie_paged_geom g = geom_of(p);
   return gie_hip_paged_attention_workspace(&g);
 }
@@ -122,16 +231,10 @@ void PagedKv::attention(const void* q, const void* k_pages, const void* v_pages,
                         void* workspace, size_t workspace_bytes, hipStream_t stream) {
   validate_problem(p);
   if (p.total_tokens == 0) return;
+  require_held(p, false);
   require_cache(k_pages, v_pages, q_starts, seq_lens, page_table);
-  require(q && out, "q and out must not be null");
-  require(q != out, "out must not be q");
-  require(aligned(q, 2) && aligned(out, 2), "q and out must be aligned to their elements");
   const gie_paged_geom g = geom_of(p);
-  const size_t need = gie_hip_paged_attention_workspace(&g);
-  GIE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), StatusCode::kWorkspaceTooSmall,
-              "PagedKv: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) +
-                  " needed");
-  require(aligned(workspace, 16), "workspace must be 16-byte aligned");
+  require_attention(q, out, workspace, workspace_bytes, gie_hip_paged_attention_workspace(&g));
   RoctxRange range("gie::PagedKv::attention");
   check_kernel_status(gie_hip_paged_attention(dtype_of(p.precision), &g, q, k_pages, v_pages, q_starts, seq_lens,
                                               page_table, out, workspace, workspace_bytes, stream),

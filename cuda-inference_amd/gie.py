@@ -99,7 +99,8 @@ class GiePagedKvProblem(ctypes.Structure):
                [(n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + \
                [(n, ctypes.c_int) for n in ("rotary_dim", "interleaved", "max_positions")] + \
                [(n, ctypes.c_float) for n in ("scale", "softcap")] + \
-               [(n, ctypes.c_int) for n in ("window", "max_new", "max_len")]
+               [(n, ctypes.c_int) for n in ("window", "max_new", "max_len", "sinks")] + \
+               [("norm_eps", ctypes.c_float), ("code", ctypes.c_int)]
 
 
 class GieLinearGeom(ctypes.Structure):
@@ -113,7 +114,7 @@ class GiePagedGeom(ctypes.Structure):
                [(n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + \
                [(n, ctypes.c_int) for n in ("rotary_dim", "interleaved", "max_positions")] + \
                [(n, ctypes.c_float) for n in ("scale", "softcap")] + \
-               [(n, ctypes.c_int) for n in ("window", "max_new", "max_len")]
+               [(n, ctypes.c_int) for n in ("window", "max_new", "max_len", "sinks")] + [("norm_eps", ctypes.c_float)]
 
 
 class GieIgemmConfig(ctypes.Structure):
@@ -195,6 +196,11 @@ _CAPI = {
     "gie_quantize_rows": ([ctypes.POINTER(GieLinearI8Problem), _vp, _vp, _vp, _vp], _i),
     "gie_kv_append": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 12, _i),
     "gie_paged_attention_workspace_size": ([ctypes.POINTER(GiePagedKvProblem), ctypes.POINTER(_sz)], _i),
+    "gie_kv_append_normed": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 14, _i),
+    "gie_kv8_append": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 16, _i),
+    "gie_kv8_read": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 10, _i),
+    "gie_kv8_attention_workspace_size": ([ctypes.POINTER(GiePagedKvProblem), ctypes.POINTER(_sz)], _i),
+    "gie_kv8_attention": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 10 + [_sz, _vp], _i),
     "gie_paged_attention": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 8 + [_sz, _vp], _i),
     "gie_rotary_tables": ([_i, _i, ctypes.c_double, ctypes.c_double, _i, ctypes.c_double, _vp, _vp], _i),
     "gie_dev_malloc": ([_sz, ctypes.POINTER(_vp)], _i),
@@ -280,6 +286,11 @@ _HIP = {
     "gie_hip_linear_i8_workspace": ([_i, ctypes.POINTER(GieLinearGeom), _i], _sz),
     "gie_hip_linear_i8": ([_i, ctypes.POINTER(GieLinearGeom)] + [_vp] * 7 + [_sz, _vp], _i),
     "gie_hip_kv_append": ([_i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 12, _i),
+    "gie_hip_kv_append_normed": ([_i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 14, _i),
+    "gie_hip_kv8_append": ([_i, _i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 16, _i),
+    "gie_hip_kv8_read": ([_i, _i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 10, _i),
+    "gie_hip_kv8_attention_workspace": ([ctypes.POINTER(GiePagedGeom)], _sz),
+    "gie_hip_kv8_attention": ([_i, _i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 10 + [_sz, _vp], _i),
     "gie_hip_paged_attention_workspace": ([ctypes.POINTER(GiePagedGeom)], _sz),
     "gie_hip_paged_attention": ([_i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 8 + [_sz, _vp], _i),
     "gie_hip_reference_conv": ([_i, _GP, _vp, _vp, _vp, _vp, _vp, _vp], _i),
@@ -1045,10 +1056,14 @@ def quantize_rows(p: LinearI8, x: int, q: int, scale: int, stream=None):
 
 
 # ------------------------------------------------------------------------------------------------- paged K/V cache
+KV_CODES = {"": 0, "int8": 1, "fp8": 2}
+
+
 @dataclass(frozen=True)
 class PagedKv:
     """PagedKvProblem (paged_kv.h). Strides are elements between tokens (0: packed), scale 0 is 1 / sqrt(head_dim),
-    softcap 0 and window 0 are off; max_new and max_len only help to choose a launch shape."""
+    softcap 0 and window 0 are off; max_new and max_len only help to choose a launch shape. `cache`: "int8" or "fp8"
+    (e4m3) for the calls of the cache in 8 bits (kv8_*), "" for the others."""
     batch: int
     total_tokens: int
     q_heads: int
@@ -1070,13 +1085,16 @@ class PagedKv:
     window: int = 0
     max_new: int = 0
     max_len: int = 0
+    sinks: int = 0
+    norm_eps: float = 0.0
+    cache: str = ""
 
     def __post_init__(self):
         object.__setattr__(self, "_c", GiePagedKvProblem(
             self.batch, self.total_tokens, self.q_heads, self.kv_heads, self.head_dim, self.page_size, self.num_pages,
             self.max_pages, PRECISIONS[self.precision], self.q_stride, self.k_stride, self.v_stride, self.o_stride,
             self.rotary_dim, int(self.interleaved), self.max_positions, self.scale, self.softcap, self.window,
-            self.max_new, self.max_len))
+            self.max_new, self.max_len, self.sinks, self.norm_eps, KV_CODES[self.cache]))
         object.__setattr__(self, "_ref", ctypes.byref(self._c))
 
 
@@ -1099,6 +1117,43 @@ def paged_attention(p: PagedKv, q: int, k_pages: int, v_pages: int, q_starts: in
     """PagedKv::attention on raw device addresses."""
     check(capi().gie_paged_attention(p._ref, q, k_pages, v_pages, q_starts, seq_lens, page_table, out, workspace,
                                      ws_bytes, _stream(stream)), "PagedKv::attention")
+
+
+def kv_append_normed(p: PagedKv, k: int, v: int, q_starts: int, seq_lens: int, page_table: int, k_pages: int,
+                     v_pages: int, q_norm: int | None = None, k_norm: int | None = None, cos: int | None = None,
+                     sin: int | None = None, q: int | None = None, q_out: int | None = None, stream=None):
+    """PagedKv::append_normed on raw device addresses."""
+    check(capi().gie_kv_append_normed(p._ref, q, k, v, q_norm, k_norm, cos, sin, q_starts, seq_lens, page_table, q_out,
+                                      k_pages, v_pages, _stream(stream)), "PagedKv::append_normed")
+
+
+def kv8_append(p: PagedKv, k: int, v: int, q_starts: int, seq_lens: int, page_table: int, k_pages: int, v_pages: int,
+               k_scales: int, v_scales: int, q_norm: int | None = None, k_norm: int | None = None,
+               cos: int | None = None, sin: int | None = None, q: int | None = None, q_out: int | None = None,
+               stream=None):
+    """PagedKv8::append on raw device addresses."""
+    check(capi().gie_kv8_append(p._ref, q, k, v, q_norm, k_norm, cos, sin, q_starts, seq_lens, page_table, q_out,
+                                k_pages, v_pages, k_scales, v_scales, _stream(stream)), "PagedKv8::append")
+
+
+def kv8_read(p: PagedKv, k_pages: int, v_pages: int, k_scales: int, v_scales: int, q_starts: int, seq_lens: int,
+             page_table: int, k: int | None, v: int | None, stream=None):
+    """PagedKv8::read on raw device addresses."""
+    check(capi().gie_kv8_read(p._ref, k_pages, v_pages, k_scales, v_scales, q_starts, seq_lens, page_table, k, v,
+                              _stream(stream)), "PagedKv8::read")
+
+
+def kv8_attention_workspace_size(p: PagedKv) -> int:
+    n = ctypes.c_size_t()
+    check(capi().gie_kv8_attention_workspace_size(p._ref, ctypes.byref(n)), "PagedKv8::workspace_size")
+    return n.value
+
+
+def kv8_attention(p: PagedKv, q: int, k_pages: int, v_pages: int, k_scales: int, v_scales: int, q_starts: int,
+                  seq_lens: int, page_table: int, out: int, workspace: int | None = None, ws_bytes: int = 0, stream=None):
+    """PagedKv8::attention on raw device addresses."""
+    check(capi().gie_kv8_attention(p._ref, q, k_pages, v_pages, k_scales, v_scales, q_starts, seq_lens, page_table, out,
+                                   workspace, ws_bytes, _stream(stream)), "PagedKv8::attention")
 
 
 def rotary_tables(max_positions: int, rotary_dim: int, base: float = 10000.0, factor: float = 1.0,

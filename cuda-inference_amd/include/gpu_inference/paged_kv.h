@@ -11,9 +11,23 @@
 // append: pairs (u, v) of the leading rotary_dim values of each head of q and k become (u cos - v sin, u sin + v cos)
 //   with the tables' row of the token's position, in FP32 with one rounding. Tables from rotary_tables() or the
 //   caller's own (any scaling for long contexts is in them).
-// attention: out = sum_j softmax_j(s_j) v_j over the positions j <= p (and j > p - window), with
+// append_normed: each head of q and k is normed first, x_d / sqrt(mean_d x_d^2 + norm_eps) * weight_d, with weights
+//   [head_dim] in FP32 shared by the heads (either may be null: not normed), and rotated without a rounding between.
+// attention: out = sum_j softmax_j(s_j) v_j over the positions j <= p (and j > p - window or j < sinks), with
 //   s_j = scale * q . k_j, or softcap * tanh(that / softcap). Query head h reads key head h / (q_heads / kv_heads).
 //   Scores, statistics and sums are FP32. A token that sees nothing gets zeros.
+//
+// PagedKv8 is the same cache held in 8 bits: pages of codes, int8 or e4m3, and FP32 scales [num_pages][kv_heads]
+// [page_size / 16], one for each head's block of 16 positions; a code c stands for c * scale.
+// append: a block's scale follows the largest |x| in it, a = max(that, 2^-64): a / 127 for int8, the power of 2 that is
+//   at least a / 448 for e4m3. A block that gets its first position starts anew; one that holds earlier positions keeps
+//   its scale unless the new tokens need a larger one, and then the codes that it holds are rounded again to that. Codes
+//   are rounded to nearest even. A block that gets an infinity or a NaN has scale NaN: all of it reads as NaN until its
+//   first position is written again. No two sequences of a call may append to the same block.
+// read: the rows' keys and values back in the problem's precision, one rounding: the tokens that append would write,
+//   so n_b = seq_lens[b] reads a whole sequence. A row without a valid position, or of a page outside the cache, is zero.
+// attention: as above over code * scale. A code of e4m3 that stands for a NaN (append writes none) counts as 480 with its
+//   sign. Scales are taken to lie within 2^-73 and 2^120; one that is not counts as the nearer of these.
 // Calls only enqueue work on `stream`; no allocation, no synchronization, so both can be captured into a graph.
 #pragma once
 
@@ -25,6 +39,8 @@
 #include "gpu_inference/conv2d.h"
 
 namespace gie {
+
+enum class KvCode : int { kNone = 0, kInt8 = 1, kE4m3 = 2 };
 
 struct PagedKvProblem {
   int batch = 1, total_tokens = 1;
@@ -40,6 +56,9 @@ struct PagedKvProblem {
   int window = 0;            // 0: unlimited
   int max_new = 0, max_len = 0;  // most new tokens and longest sequence if the host knows them (0: not known): they
                                  // choose the launch shape, no result depends on them
+  int sinks = 0;         // attention: positions from 0 on that stay visible to rows whose window has passed them
+  float norm_eps = 0;    // of append_normed and PagedKv8::append
+  KvCode code = KvCode::kNone;  // PagedKv8: what its pages hold; PagedKv: kNone
 };
 
 void validate_problem(const PagedKvProblem& prob);
@@ -50,9 +69,35 @@ class PagedKv {
   static void append(const void* q, const void* k, const void* v, const float* cos, const float* sin,
                      const int* q_starts, const int* seq_lens, const int* page_table, const PagedKvProblem& prob,
                      void* q_out, void* k_pages, void* v_pages, hipStream_t stream);
+  // q_norm, k_norm: FP32 weights [head_dim], either may be null (q_norm has to be where q is)
+  static void append_normed(const void* q, const void* k, const void* v, const float* q_norm, const float* k_norm,
+                            const float* cos, const float* sin, const int* q_starts, const int* seq_lens,
+                            const int* page_table, const PagedKvProblem& prob, void* q_out, void* k_pages,
+                            void* v_pages, hipStream_t stream);
   static void attention(const void* q, const void* k_pages, const void* v_pages, const int* q_starts,
                         const int* seq_lens, const int* page_table, const PagedKvProblem& prob, void* out,
                         void* workspace, size_t workspace_bytes, hipStream_t stream);
+  static size_t workspace_size(const PagedKvProblem& prob);  // of attention
+};
+
+// pages of codes and their scales
+struct Kv8Pages {
+  void *k = nullptr, *v = nullptr;
+  float *k_scales = nullptr, *v_scales = nullptr;
+};
+
+class PagedKv8 {
+ public:
+  static void append(const void* q, const void* k, const void* v, const float* q_norm, const float* k_norm,
+                     const float* cos, const float* sin, const int* q_starts, const int* seq_lens,
+                     const int* page_table, const PagedKvProblem& prob, void* q_out, const Kv8Pages& pages,
+                     hipStream_t stream);
+  // rows of k and v are k_stride and v_stride apart; either may be null
+  static void read(const Kv8Pages& pages, const int* q_starts, const int* seq_lens, const int* page_table,
+                   const PagedKvProblem& prob, void* k, void* v, hipStream_t stream);
+  static void attention(const void* q, const Kv8Pages& pages, const int* q_starts, const int* seq_lens,
+                        const int* page_table, const PagedKvProblem& prob, void* out, void* workspace,
+                        size_t workspace_bytes, hipStream_t stream);
   static size_t workspace_size(const PagedKvProblem& prob);  // of attention
 };
 

@@ -214,14 +214,34 @@ typedef struct gie_paged_kv_problem {
   int rotary_dim, interleaved, max_positions;
   float scale, softcap;                            /* scale 0: 1 / sqrt(head_dim) */
   int window, max_new, max_len;
+  int sinks;                                       /* with a window: first positions that stay visible beside it */
+  float norm_eps;
+  int code;                                        /* of gie_kv8_*: 1 int8, 2 e4m3; 0 for the others */
 } gie_paged_kv_problem;
 int gie_kv_append(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v, const float* cos,
                   const float* sin, const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
                   void* k_pages, void* v_pages, void* stream);
+/* each head of q and k normed on the way (q_norm, k_norm: FP32 [head_dim] or null) */
+int gie_kv_append_normed(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v,
+                         const float* q_norm, const float* k_norm, const float* cos, const float* sin,
+                         const int* q_starts, const int* seq_lens, const int* page_table, void* q_out, void* k_pages,
+                         void* v_pages, void* stream);
 int gie_paged_attention_workspace_size(const gie_paged_kv_problem* p, size_t* bytes);
 int gie_paged_attention(const gie_paged_kv_problem* p, const void* q, const void* k_pages, const void* v_pages,
                         const int* q_starts, const int* seq_lens, const int* page_table, void* out, void* workspace,
                         size_t workspace_bytes, void* stream);
+/* PagedKv8: the cache in 8 bits, FP32 scales [num_pages][kv_heads][page_size / 16] */
+int gie_kv8_append(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v, const float* q_norm,
+                   const float* k_norm, const float* cos, const float* sin, const int* q_starts, const int* seq_lens,
+                   const int* page_table, void* q_out, void* k_pages, void* v_pages, float* k_scales, float* v_scales,
+                   void* stream);
+int gie_kv8_read(const gie_paged_kv_problem* p, const void* k_pages, const void* v_pages, const float* k_scales,
+                 const float* v_scales, const int* q_starts, const int* seq_lens, const int* page_table, void* k,
+                 void* v, void* stream);
+int gie_kv8_attention_workspace_size(const gie_paged_kv_problem* p, size_t* bytes);
+int gie_kv8_attention(const gie_paged_kv_problem* p, const void* q, const void* k_pages, const void* v_pages,
+                      const float* k_scales, const float* v_scales, const int* q_starts, const int* seq_lens,
+                      const int* page_table, void* out, void* workspace, size_t workspace_bytes, void* stream);
 /* host tables of the rotation, [max_positions][rotary_dim / 2] FP32 each, computed in 64 bits:
    angle(p, j) = p * f_j, f_j = base^(-2j / rotary_dim), long contexts by `factor` >= 1 and `original_positions`:
    original_positions == 0: every f_j / factor (positions interpolated); otherwise only the frequencies whose
