@@ -1,92 +1,720 @@
 // Attention of new tokens over a paged key/value cache held in 8 bits:
 //   out[t][h] = sum_j p_j vs_j c^v_j / sum_j p_j,  p_j = exp(s_j - m),  s_j = scale * ks_j * q[t][h] . c^k_j
-// (or softcap * tanh(that / softcap)) with codes c and the scales ks, vs of position j's block of 16.
+// (or softcap * tanh(s_j / softcap)) with codes c and the scales ks, vs of position j's block of 16, over the positions
+// j <= p (and j > p - window or j < sinks), in one pass over the keys.
 //
-// One workgroup for each row (token, head), tiles of 64 keys: four lanes take a key's product, then every lane sums its
-// value over the tile.
+// Rows, tiles, parts and both products are those of paged_attention: 32x32x16 MFMAs with the rows in the columns. Here
+// everything is FP16 in them, whatever the tokens' type: codes are exact in it, and a row of q is under a power of 2 of its
+// own that puts its largest value into 2^14 .. 2^15, so that what it rounds away is under 2^-39 of that one.
+//
+// Scales. A block of 16 positions is half of the 32 scores that a lane has, so its scales are two constants of 8
+// registers: ks is a factor of the exponent, vs a term of it, x_j = s_j log2(e) + log2(vs_j). The weight 2^(x_j - m) that
+// the second product takes has vs in it, and m is the maximum of x: weights keep their bits however much the blocks'
+// sizes differ. The sum of p_j takes 1 / vs once for each block.
 #include "attention_common.h"
 #include "kv8_common.h"
 
 namespace gie_hip {
 namespace {
 
+typedef __attribute__((address_space(4))) const float const_float;
+
 struct Kv8Args : AttnArgs {
   const uint8_t* k_pages;
   const uint8_t* v_pages;
   const float* k_scales;
   const float* v_scales;
+  int bf16;  // type of q and out
 };
 
-// a scale inside the range that the products assume; a NaN stays one
-__device__ __forceinline__ float clamp_scale(float s) {
-  return s == s ? fminf(fmaxf(s, 0x1p-73f), 0x1p120f) : s;
+constexpr float kLift = 7.f;  // weights lie in 2^7 .. 2^15 at their largest: FP16 has no step under 2^-24
+
+// A block's scales as the scores take them: f times the product of codes is the product of keys (a NaN if either scale
+// is one: every score of the block becomes a NaN), lv = log2(vs), inv = 1 / vs.
+struct BlockScales {
+  float f, lv, inv;
+};
+template <typename C>
+__device__ __forceinline__ BlockScales block_scales(float ks, float vs) {
+  const float k = fminf(fmaxf(ks, 0x1p-73f), 0x1p120f), v = fminf(fmaxf(vs, 0x1p-73f), 0x1p120f);
+  const bool bad = !(ks == ks) || !(vs == vs);
+  // the exponent and the quotient from the same logarithm, so that a weight and what the sum takes of it agree
+  const float lv = __builtin_amdgcn_logf(v);
+  return {bad ? __builtin_nanf("") : k * C::kUnit, lv, __builtin_amdgcn_exp2f(-lv)};
 }
 
-template <typename E, typename C>
-__global__ __launch_bounds__(256) void rows_kernel(Kv8Args a, int D, float scale) {
-  constexpr int TT = 64;
-  __shared__ float q[256], weight[TT], top[4];
-  const int tid = int(threadIdx.x);
-  const int t = int(blockIdx.x) / a.q_heads, head = int(blockIdx.x) % a.q_heads, kvh = head / a.group;
-  const Sequence seq = locate(a.q_starts, a.seq_lens, a.batch, a.total_tokens, t, [](int first, int) { return first; });
-  if (t < seq.first || t >= seq.first + seq.count) return;
-  int pos = seq.base + t - seq.first;
-  if (pos >= a.capacity) pos = -1;
-  const int oldest = a.window > 0 ? pos - a.window : -1;
-  const KeyRange range = key_range<TT>(a, pos, pos);
-  if (tid < D) q[tid] = E::to_f32(a.q[t * a.q_stride + head * D + tid]);
-  const int page_size = a.page16 * 16;
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  const auto at = [&](int key, bool& there) {  // of a key's codes, in heads of codes
-    const int row = key / page_size, page = a.page_table[(long long)seq.index * a.max_pages + row];
-    there = page >= 0 && page < a.num_pages;
-    return ((long long)(there ? page : 0) * a.kv_heads + kvh) * page_size + (key - row * page_size);
+// codes of 8 values, in the order 0, 2, 1, 3, 4, 6, 5, 7
+template <typename C>
+__device__ __forceinline__ u32x4 decode8(uint32_t a, uint32_t b) {
+  const u32x2 x = C::decode4(a), y = C::decode4(b);
+  return u32x4{x.x, x.y, y.x, y.y};
+}
+
+// Fragments of a row of q (this lane's half of its values) in FP16, in decode8's order, times a power of 2; returns the
+// factor that takes it back. The sign changes where the scores' scale is negative.
+template <int KS>
+__device__ __forceinline__ float row_to_fp16(u32x4 (&qf)[KS], bool bf16, bool negate) {
+  const auto value = [&](int ks, int i) {
+    const uint16_t b = uint16_t(qf[ks][i / 2] >> (i % 2 * 16));
+    return bf16 ? Bf16::to_f32(b) : Fp16::to_f32(b);
   };
-  for (int tile = 0; tile < range.tiles; ++tile) {
-    const int key0 = tile < range.sink_tiles ? tile * TT : range.lo + (tile - range.sink_tiles) * TT;
-    const int key = key0 + tid / 4;
-    float s = -INFINITY;
-    const bool seen = sees(a, key, pos, oldest);
-    __syncthreads();
-    float sum = 0.f;
-    if (seen) {
-      bool there;
-      const long long from = at(key, there);
-      if (there) {
-        for (int d = tid % 4; d < D; d += 4) sum += q[d] * C::decode1(a.k_pages[from * D + d]);
-        sum *= clamp_scale(a.k_scales[from / kKvBlock]);
-      } else {
-        for (int d = tid % 4; d < D; d += 4) sum += q[d] * 0.f;
-      }
-    }
-    sum += __shfl_xor(sum, 1);
-    sum += __shfl_xor(sum, 2);
-    if (seen) {
-      s = sum * scale;
-      if (a.cap > 0) s = a.cap * tanhf(s / a.cap);
-    }
-    float most = s;
+  float most = 0.f;
 #pragma unroll
-    for (int d = 4; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-    if ((tid & 63) == 0) top[tid >> 6] = most;
-    if (tid % 4 == 0) weight[tid / 4] = s;
-    __syncthreads();
-    const float next = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3]));
-    const float ref = next == -INFINITY ? 0.f : next, keep = m == -INFINITY ? 1.f : expf(m - ref);
+  for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(value(ks, i)));
+  most = swap_max(most);
+  const int e = max(int(__float_as_uint(most) >> 23) - 127, -100);
+  float f = __uint_as_float(unsigned(127 + 14 - e) << 23);
+  if (negate) f = -f;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r[2 * i] = Fp16::pack2(value(ks, 4 * i) * f, value(ks, 4 * i + 2) * f);
+      r[2 * i + 1] = Fp16::pack2(value(ks, 4 * i + 1) * f, value(ks, 4 * i + 3) * f);
+    }
+    qf[ks] = r;
+  }
+  return __uint_as_float(unsigned(127 + e - 14) << 23);
+}
+
+__device__ __forceinline__ uint32_t pack_out(bool bf16, float lo, float hi) {
+  return bf16 ? Bf16::pack2(lo, hi) : Fp16::pack2(lo, hi);
+}
+
+// The weights of 32 scores (register i: key 8 (i / 4) + 4 half + i % 4, so the block i / 8), and what they do to the
+// running maximum, the sum and the rows' values. `masked`: seen(i) says whether register i's key is.
+template <bool LARGE_CAP, int DT, typename Seen>
+__device__ __forceinline__ void weigh(const AttnArgs& a, f32x16& s, const BlockScales (&sc)[2], float row_factor,
+                                      bool masked, Seen seen, float& m, float& mc, float& l, f32x16 (&o)[DT]) {
+  float f[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) f[g] = fminf(fmaxf(row_factor * sc[g].f, 0x1p-126f), 3e38f);
+  if (LARGE_CAP || a.cap > 0) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] *= f[i / 8];
+    if constexpr (LARGE_CAP)
+      cap_products(a, s);
+    else
+      cap_scores(a, s);
+    f[0] = f[1] = a.mult;
+  } else {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) f[g] = fminf(fmaxf(f[g] * a.mult, 0x1p-126f), 3e38f);
+  }
+  // (clamped above, a NaN became a number: scores of such a block are set here)
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    if (__any(!(sc[g].f == sc[g].f)))
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[8 * g + i] = __builtin_nanf("");
+  if (masked) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = seen(i) ? s[i] : -INFINITY;
+  }
+  float most[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    most[g] = s[8 * g];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) most[g] = fmaxf(most[g], s[8 * g + i]);
+    most[g] = __builtin_fmaf(most[g], f[g], sc[g].lv);
+  }
+  const float top = swap_max(fmaxf(most[0], most[1]));
+  // the maximum follows only when a weight would pass 2^8: sums and weights keep their relative precision, and most
+  // tiles leave O as it is
+  if (__any(top - m > 8.f)) {
+    const float next = fmaxf(m, top);
+    float nc = next == -INFINITY ? 0.f : next;
+    nc += __builtin_fmaf(fabsf(nc), 0x1p-22f, -kLift);  // (what rounding takes from it and from an exponent)
+    const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - nc);  // 1: nothing summed yet
     m = next;
+    mc = nc;
     l *= keep;
-    o *= keep;
-    for (int k = 0; k < TT; ++k) {
-      if (!sees(a, key0 + k, pos, oldest)) continue;
-      const float w = expf(weight[k] - ref);
-      l += w;
-      bool there;
-      const long long from = at(key0 + k, there);
-      if (there && tid < D)
-        o += w * clamp_scale(a.v_scales[from / kKvBlock]) * C::decode1(a.v_pages[from * D + tid]);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] *= keep;
+  }
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const float c = sc[g].lv - mc;
+    float sum[2] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      s[8 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * g + i], f[g], c));
+      sum[i % 2] += s[8 * g + i];
+    }
+    l = __builtin_fmaf(sum[0] + sum[1], sc[g].inv, l);
+  }
+}
+
+// ---------------------------------------------------------------- few rows: 32 for each workgroup
+// Bound by the cache's bytes. Codes go HBM -> LDS by direct loads and are decoded in the registers of the wave that
+// multiplies them: WK waves with tiles of 32 keys of their own and NST stages each, no barrier until they are joined.
+// K: 16 bytes of a row for two steps of the first product (the order of the summed values is free as long as q has the
+// same). V: ds_read_b64_tr_b8 gives a lane 8 keys of its value. 16-byte chunks of a row are permuted by the row so that
+// both reads meet no bank twice in a phase.
+template <int D>
+constexpr int kPitch8 = D == 96 ? 128 : D;  // bytes of a row of codes in LDS
+template <int D>
+__device__ __forceinline__ int k_swizzle8(int row) {
+  return D == 64 ? (row >> 2) & 3 : D == 256 ? row & 15 : (row >> 1) & 7;
+}
+template <int D>
+__device__ __forceinline__ int v_swizzle8(int row) {
+  const int far = (row >> 3) & 1;
+  return D == 64 ? far * 2 : D == 256 ? (row & 3) * 2 + far * 8 : ((row >> 1) & 1) * 2 + far * 4;
+}
+
+// a 16-lane group reads 8 rows of 16 bytes; each lane gets the 8 rows' bytes of its column
+__device__ __forceinline__ u32x2 read_transposed8(unsigned at) {
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                       reinterpret_cast<__attribute__((address_space(3))) v2i*>(size_t(at))));
+}
+
+template <typename C, int D, int WK, int NST, bool LARGE_CAP>
+__global__ __launch_bounds__(64 * WK, 1) void narrow_kernel(Kv8Args a) {
+  constexpr int TT = kNarrowKeys, GR = TT / 16, P = kPitch8<D>, KS = D / 16, KP = D / 32, DT = D / 32;
+  constexpr int kGran = 16 * P, IPG = kGran / 1024, kTileB = TT * P, kStage = 2 * kTileB, LPT = 2 * GR * IPG;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int tid = int(threadIdx.x), lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // neighbouring workgroups take different key heads, the last rows of a sequence go first
+  const int id = int(gridDim.x) - 1 - int(blockIdx.x);
+  const int kvh = id % a.kv_heads, rest = id / a.kv_heads, z = rest % a.splits;
+  const RowTile t = row_tile<kNarrowRows>(a, rest / a.splits);
+  if (t.rows <= 0) return;
+  const int last_row = t.row0 + min(t.rows, kNarrowRows) - 1;
+  const int pos_first = t.seq.base + t.row0 / a.group, pos_last = t.seq.base + last_row / a.group;
+  const KeyRange range = key_range<TT>(a, pos_first, pos_last);
+  const int tile_first = z * range.per_split;
+  if (z > 0 && z >= range.splits) return;  // the join reads as many parts as hold keys
+  const int tiles = min(range.per_split, range.tiles - tile_first);  // of the workgroup; this wave: wave, wave + WK, ...
+  const int turn = range.sink_tiles - tile_first, sink0 = tile_first * TT;
+  const int key0 = sink0 + range.lo - range.sink_tiles * TT;
+  const auto key_of = [&](int tile) { return tile * TT + (tile < turn ? sink0 : key0); };
+
+  // ---- this lane's row: row (lane & 31); rows past the last repeat it ----
+  const int row = min(t.row0 + (lane & 31), last_row);
+  const int token = row / a.group, head = kvh * a.group + (row - token * a.group);
+  int pos = t.seq.base + token;
+  if (pos >= a.capacity) pos = -1;  // no valid position: sees nothing
+  u32x4 qf[KS];
+  {
+    const uint16_t* src = a.q + (t.seq.first + token) * a.q_stride + head * D;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = load_16_bytes(src + 16 * (ks - ks % 2 + half) + 8 * (ks % 2));
+  }
+
+  // ---- loads: granule g of a tile, instruction i covers 1024 / P rows ----
+  constexpr int RI = 1024 / P;
+  int k_off[IPG], v_off[IPG];
+#pragma unroll
+  for (int i = 0; i < IPG; ++i) {
+    const int r = i * RI + lane / (P / 16), slot = lane % (P / 16);
+    const int kc = slot ^ k_swizzle8<D>(r), vc = slot ^ v_swizzle8<D>(r);
+    k_off[i] = kc < D / 16 ? r * D + kc * 16 : kOut;
+    v_off[i] = vc < D / 16 ? r * D + vc * 16 : kOut;
+  }
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds) + unsigned(wave * NST * kStage));
+  const const_int* table = (const const_int*)(uintptr_t)(a.page_table + (long long)t.seq.index * a.max_pages);
+  struct Place16 {
+    int page[GR], slot[GR];
+  };
+  const auto look_up = [&](int tile, Place16& p) {
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      const int gran = min((key_of(tile) >> 4) + g, (a.capacity >> 4) - 1);
+      const int pg = div_magic(gran, a.page_magic, a.page_shift);
+      p.page[g] = table[__builtin_amdgcn_readfirstlane(pg)];
+      p.slot[g] = gran - pg * a.page16;
+    }
+  };
+  const auto uniform = [](v4i r) {
+    return v4i{__builtin_amdgcn_readfirstlane(r.x), __builtin_amdgcn_readfirstlane(r.y),
+               __builtin_amdgcn_readfirstlane(r.z), __builtin_amdgcn_readfirstlane(r.w)};
+  };
+  const auto there = [&](const Place16& p, int g) { return p.page[g] >= 0 && p.page[g] < a.num_pages; };
+  const auto block_at = [&](const Place16& p, int g) {
+    return ((long long)(there(p, g) ? p.page[g] : 0) * a.kv_heads + kvh) * a.page16 + p.slot[g];
+  };
+  const auto issue = [&](int tile, int stage, const Place16& p) {
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      const int at = key_of(tile) + g * 16;
+      const int bytes = there(p, g) && tile < tiles ? min(max(range.hi - at, 0), 16) * D : 0;
+      const long long off = block_at(p, g) * (16ll * D);
+      v4i rk = uniform(make_vsharp(a.k_pages + off, bytes)), rv = uniform(make_vsharp(a.v_pages + off, bytes));
+      // a vector instruction may have written these scalar registers: loads may read them 5 cycles later
+      asm volatile("s_nop 4" : "+s"(rk), "+s"(rv));
+      const unsigned to = lds0 + unsigned(stage * kStage + g * kGran);
+#pragma unroll
+      for (int i = 0; i < IPG; ++i) dma16(rk, to + i * 1024, k_off[i]);
+#pragma unroll
+      for (int i = 0; i < IPG; ++i) dma16(rv, to + kTileB + i * 1024, v_off[i]);
+    }
+  };
+  // scales of a tile's blocks; of a page that is not there the smallest: its codes are zeros
+  struct Pair {
+    float k[GR], v[GR];
+  };
+  const auto scales_of = [&](const Place16& p, Pair& s) {
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      const long long at = block_at(p, g);
+      const float k = ((const const_float*)(uintptr_t)a.k_scales)[at], v = ((const const_float*)(uintptr_t)a.v_scales)[at];
+      s.k[g] = there(p, g) ? k : 0.f;
+      s.v[g] = there(p, g) ? v : 0.f;
+    }
+  };
+
+  // ---- fragment addresses ----
+  const int sl = lane & 15, chunk = (lane >> 4) & 1;
+  const unsigned k_rd = lds0 + unsigned((lane & 31) * P + ((half ^ k_swizzle8<D>(lane & 15)) << 4));
+  const int v_row = 4 * half + (sl >> 1 & 3) + 8 * (sl >> 3);
+  const unsigned v_rd = lds0 + unsigned(kTileB + v_row * P + ((chunk ^ v_swizzle8<D>(v_row)) << 4) + (sl & 1) * 8);
+
+  f32x16 o[DT] = {};
+  float m = -INFINITY, mc = 0.f, l = 0.f;  // running maximum of the exponents, what is taken from them, sum
+  float row_factor = 1.f;
+
+  const auto compute = [&](int tile, int stage, const Pair& pair) {
+    const unsigned so = unsigned(stage * kStage);
+    const int at = key_of(tile), oldest = a.window > 0 ? pos - a.window : -1;
+    u32x4 kr[KP];
+#pragma unroll
+    for (int i = 0; i < KP; ++i) kr[i] = *reinterpret_cast<const lds_v4*>(size_t((k_rd + so) ^ unsigned(i * 32)));
+    f32x16 s = {};
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      s = Fp16::mfma32(decode8<C>(kr[i].x, kr[i].y), qf[2 * i], s);
+      s = Fp16::mfma32(decode8<C>(kr[i].z, kr[i].w), qf[2 * i + 1], s);
+    }
+    u32x2 vr[2][DT];  // requested under the weights
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) vr[g][d] = read_transposed8(((v_rd + so) ^ unsigned(d * 32)) + unsigned(g * kGran));
+    BlockScales sc[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) sc[g] = block_scales<C>(pair.k[g], pair.v[g]);
+    const bool masked = at + TT - 1 > pos_first || (a.window > 0 && at <= pos_last - a.window) || pos_last >= a.capacity;
+    const auto seen = [&](int i) { return sees(a, at + 8 * (i / 4) + 4 * half + i % 4, pos, oldest); };
+    weigh<LARGE_CAP>(a, s, sc, row_factor, masked, seen, m, mc, l, o);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const u32x4 pf = {Fp16::pack2(s[8 * g], s[8 * g + 2]), Fp16::pack2(s[8 * g + 1], s[8 * g + 3]),
+                        Fp16::pack2(s[8 * g + 4], s[8 * g + 6]), Fp16::pack2(s[8 * g + 5], s[8 * g + 7])};
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] = Fp16::mfma32(decode8<C>(vr[g][d].x, vr[g][d].y), pf, o[d]);
+    }
+  };
+
+  // ---- main loop: a wave's j-th tile from stage j % NST while the next NST - 1 load; loads past the last tile read
+  // nothing and write zeros, so that every wait counts the same. Scales arrive a tile ahead, their pages two ----
+  const int mine = (tiles - wave + WK - 1) / WK;
+  const auto tile_at = [&](int j) { return wave + j * WK; };
+  Place16 next, ahead;
+  Pair now, then;
+  look_up(tile_at(0), next);
+  ahead = next;
+#pragma unroll
+  for (int j = 0; j < NST - 1; ++j) {
+    issue(tile_at(j), j, next);
+    look_up(tile_at(j + 1), next);
+  }
+  scales_of(ahead, then);
+  look_up(tile_at(1), ahead);
+  row_factor = row_to_fp16(qf, a.bf16 != 0, a.negate != 0);
+  int stage = 0;
+  for (int j = 0; j < mine; ++j) {
+    wait_vm<(NST - 2) * LPT>();
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's reads of the stage that is loaded next are done: lgkmcnt(0)
+    issue(tile_at(j + NST - 1), stage == 0 ? NST - 1 : stage - 1, next);
+    look_up(tile_at(j + NST), next);
+    now = then;
+    scales_of(ahead, then);
+    look_up(tile_at(j + 2), ahead);
+    compute(tile_at(j), stage, now);
+    stage = stage + 1 == NST ? 0 : stage + 1;
+  }
+  wait_vm<0>();
+  l = swap_add(l);
+
+  // ---- the waves' parts of the keys ----
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(lds);  // [wave][32] m, l; then [wave][32 rows][D + 4]
+  if (half == 0) {
+    sums[(wave * 32 + lane) * 2] = m == -INFINITY ? -INFINITY : mc;
+    sums[(wave * 32 + lane) * 2 + 1] = l;
+  }
+  __syncthreads();
+  float top = -INFINITY, total = 0.f;
+#pragma unroll
+  for (int w = 0; w < WK; ++w) top = fmaxf(top, sums[(w * 32 + (lane & 31)) * 2]);
+  const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int w = 0; w < WK; ++w) {
+    const float other = sums[(w * 32 + (lane & 31)) * 2];
+    // a wave without a maximum may hold a NaN all the same
+    total += sums[(w * 32 + (lane & 31)) * 2 + 1] * __builtin_amdgcn_exp2f(other == -INFINITY ? 0.f : other - ref);
+  }
+  const float keep = __builtin_amdgcn_exp2f(m == -INFINITY ? 0.f : mc - ref) * C::kUnit;
+  constexpr int kRow = D + 4;
+  float* mine_o = reinterpret_cast<float*>(lds + WK * 256) + (wave * 32 + (lane & 31)) * kRow;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4*>(mine_o + 32 * d + 8 * i + 4 * half) =
+          f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * keep;
+  // row (tid & 31) of the sums: every wave joins a part of the values
+  __syncthreads();
+  const float* all = reinterpret_cast<const float*>(lds + WK * 256);
+  const int r = lane & 31;
+  if (r >= t.rows) return;
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  for (int d = (wave * 2 + half) * 4; d < D; d += WK * 8) {
+    f32x4 v = {};
+#pragma unroll
+    for (int w = 0; w < WK; ++w) v += *reinterpret_cast<const f32x4*>(all + (w * 32 + r) * kRow + d);
+    if (range.splits > 1) {
+      float* dst = a.part + (((long long)(t.seq.first + token) * a.q_heads + head) * a.splits + z) * (D + 4);
+      *reinterpret_cast<f32x4*>(dst + d) = v;
+      if (d == 0) dst[D] = top, dst[D + 1] = total;
+    } else {
+      uint16_t* dst = a.out + (t.seq.first + token) * a.o_stride + head * D + d;
+      if (total == 0.f) v = f32x4{};
+      v *= inv;
+      store_8_bytes(dst, u32x2{pack_out(a.bf16, v[0], v[1]), pack_out(a.bf16, v[2], v[3])});
     }
   }
-  if (tid < D) a.out[t * a.o_stride + head * D + tid] = E::from_f32(l == 0.f ? 0.f : o / l);
+}
+
+// ---------------------------------------------------------------- many rows: 128 for each workgroup
+// Bound by the products and the softmax. The workgroup decodes a tile of 64 keys once, HBM -> registers -> LDS in FP16, for
+// four waves of 32 rows that share it (WD == 2: two waves for each 32 rows, half of the head's values each): a wave
+// decoding what it multiplies would decode every code four times. Codes of the next tile but one are requested before a
+// tile is worked on. Values lie in decode8's order in LDS: of K that is q's order too, of V the rows' registers are put
+// in order at the end.
+template <typename C, int D, int WD, bool LARGE_CAP>
+__global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
+  constexpr int WR = kWideRows / 32, R = kWideRows, TT = kWideKeys, NS = TT / 32, P = kPitch<D>;
+  constexpr int KS = D / 16, DT = D / 32 / WD, kTileB = TT * P, kStage = 2 * kTileB;
+  constexpr int kPieces = D, JP = (kPieces + 63) / 64;  // 16-byte pieces of a granule's codes, of a lane
+  constexpr int kConst = 2 * kStage;                    // [stage][granule] BlockScales
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int tid = int(threadIdx.x), lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave % WR, wd = wave / WR;
+
+  const int id = int(gridDim.x) - 1 - int(blockIdx.x);
+  const int kvh = id % a.kv_heads, rest = id / a.kv_heads, z = rest % a.splits;
+  const RowTile t = row_tile<R>(a, rest / a.splits);
+  if (t.rows <= 0) return;
+  const int last_row = t.row0 + min(t.rows, R) - 1;
+  const int pos_first = t.seq.base + t.row0 / a.group, pos_last = t.seq.base + last_row / a.group;
+  const KeyRange range = key_range<TT>(a, pos_first, pos_last);
+  const int tile_first = z * range.per_split;
+  if (z > 0 && z >= range.splits) return;
+  const int tiles = min(range.per_split, range.tiles - tile_first);
+  const int turn = range.sink_tiles - tile_first, sink0 = tile_first * TT;
+  const int key0 = sink0 + range.lo - range.sink_tiles * TT;
+  const auto key_of = [&](int tile) { return tile * TT + (tile < turn ? sink0 : key0); };
+
+  int pos;
+  u32x4 qf[KS];
+  {
+    const int row = min(t.row0 + wr * 32 + (lane & 31), last_row);
+    const int token = row / a.group, head = kvh * a.group + (row - token * a.group);
+    pos = t.seq.base + token;
+    if (pos >= a.capacity) pos = -1;  // no valid position: sees nothing
+    const long long src = (t.seq.first + token) * a.q_stride + head * D;
+    // whole rows, 16 bytes for each lane; they go through LDS below (WD waves: a part of the rows each)
+#pragma unroll
+    for (int j = 0; j < KS / WD; ++j) {
+      const int piece = (j + wd * (KS / WD)) * 64 + lane, row_of = piece / (D / 8);
+      const unsigned lo = unsigned(__shfl(int(src), row_of)), hi = unsigned(__shfl(int(src >> 32), row_of));
+      qf[j] = load_16_bytes(a.q + (long long)((unsigned long long)hi << 32 | lo) + piece % (D / 8) * 8);
+    }
+  }
+  const int wave_first = min(t.row0 + wr * 32, last_row), wave_last = min(t.row0 + (wr + 1) * 32 - 1, last_row);
+  const int wpos_first = t.seq.base + wave_first / a.group, wpos_last = t.seq.base + wave_last / a.group;
+
+  // ---- codes: granule wr of a tile by this wave (of K and V, or WD == 2: of one) ----
+  const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds));
+  const const_int* table = (const const_int*)(uintptr_t)(a.page_table + (long long)t.seq.index * a.max_pages);
+  constexpr int KV = 2 / WD;  // of this wave
+  u32x4 raw[KV][JP];
+  float raw_k, raw_v;
+  int page, slot;
+  const auto look_up = [&](int tile) {
+    const int gran = min((key_of(tile) >> 4) + wr, (a.capacity >> 4) - 1);
+    const int pg = div_magic(gran, a.page_magic, a.page_shift);
+    page = table[__builtin_amdgcn_readfirstlane(pg)];
+    slot = gran - pg * a.page16;
+  };
+  const auto load = [&](int tile) {
+    const bool there = page >= 0 && page < a.num_pages;
+    const int at = key_of(tile) + wr * 16;
+    const int bytes = there && tile < tiles ? min(max(range.hi - at, 0), 16) * D : 0;
+    const long long block = ((long long)(there ? page : 0) * a.kv_heads + kvh) * a.page16 + slot;
+#pragma unroll
+    for (int n = 0; n < KV; ++n) {
+      const bool is_v = WD == 1 ? n == 1 : wd == 1;
+      const uint8_t* from = (is_v ? a.v_pages : a.k_pages) + block * (16ll * D);
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from), 0, bytes, kBufferWord3);
+#pragma unroll
+      for (int j = 0; j < JP; ++j)
+        raw[n][j] = __builtin_bit_cast(
+            u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (j * 64 + lane) * 16, 0, 0));
+    }
+    const float k = ((const const_float*)(uintptr_t)a.k_scales)[block], v = ((const const_float*)(uintptr_t)a.v_scales)[block];
+    raw_k = there ? k : 0.f;
+    raw_v = there ? v : 0.f;
+  };
+  // piece j * 64 + lane: 16 values of a row, two chunks of FP16
+  unsigned k_wr[JP], v_wr[JP];
+#pragma unroll
+  for (int j = 0; j < JP; ++j) {
+    const int piece = j * 64 + lane, row = piece / (D / 16), c = piece % (D / 16) * 2;
+    k_wr[j] = unsigned((wr * 16 + row) * P + ((c ^ k_swizzle<D>(row)) << 4));
+    v_wr[j] = unsigned(kTileB + (wr * 16 + row) * P + ((c ^ v_swizzle<D>(row)) << 4));
+  }
+  const auto decode_to = [&](int stage) {
+    const unsigned so = lds0 + unsigned(stage * kStage);
+#pragma unroll
+    for (int n = 0; n < KV; ++n)
+#pragma unroll
+      for (int j = 0; j < JP; ++j) {
+        const bool is_v = WD == 1 ? n == 1 : wd == 1;
+        if (kPieces % 64 != 0 && j * 64 + lane >= kPieces) continue;
+        const unsigned to = so + (is_v ? v_wr[j] : k_wr[j]);
+        *reinterpret_cast<lds_v4*>(size_t(to)) = decode8<C>(raw[n][j].x, raw[n][j].y);
+        *reinterpret_cast<lds_v4*>(size_t(to ^ 16u)) = decode8<C>(raw[n][j].z, raw[n][j].w);
+      }
+    if (wd == 0) {
+      const BlockScales s = block_scales<C>(raw_k, raw_v);
+      if (lane == 0)
+        *reinterpret_cast<lds_f4*>(size_t(lds0 + unsigned(kConst + (stage * WR + wr) * 16))) = f32x4{s.f, s.lv, s.inv, 0.f};
+    }
+  };
+
+  // ---- fragment addresses ----
+  const int sl = lane & 15, g16 = lane >> 4;
+  const unsigned k_rd = lds0 + unsigned((lane & 31) * P + ((half ^ k_swizzle<D>(lane & 15)) << 4));
+  const unsigned v_row = unsigned(4 * half + (sl >> 2));
+  const unsigned v_chunk = unsigned((2 * (g16 & 1) + ((sl & 3) >> 1)) ^ v_swizzle<D>(sl >> 2));
+  const unsigned v_rd = (lds0 + unsigned(kTileB) + v_row * P + (v_chunk << 4) + ((sl & 1) << 3)) ^ unsigned(wd * DT * 64);
+
+  f32x16 o[DT] = {};
+  float m = -INFINITY, mc = 0.f, l = 0.f;
+  float row_factor = 1.f;
+
+  const auto compute = [&](int tile, int stage) {
+    const unsigned so = unsigned(stage * kStage);
+    const int at0 = key_of(tile), oldest = a.window > 0 ? pos - a.window : -1;
+    constexpr bool kAhead = WD == 1;  // where the registers hold it
+    u32x4 kf[KS];
+    const auto read_k = [&](int n) {
+      unsigned ko = k_rd + so;
+      asm volatile("" : "+v"(ko));  // the permuted addresses are worked out for every part: kept, they cost registers
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        kf[ks] = *reinterpret_cast<const lds_v4*>(size_t((ko ^ unsigned(ks * 32)) + unsigned(n * 32 * P)));
+    };
+    if (kAhead) read_k(0);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      const int at = at0 + n * 32;
+      f32x16 s = {};
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s = Fp16::mfma32(kf[ks], qf[ks], s);
+      } else {  // four steps ahead
+        unsigned ko = k_rd + so;
+        asm volatile("" : "+v"(ko));
+        const auto read_4 = [&](int g) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            kf[g % 2 * 4 + i] =
+                *reinterpret_cast<const lds_v4*>(size_t((ko ^ unsigned((g * 4 + i) * 32)) + unsigned(n * 32 * P)));
+        };
+        read_4(0);
+#pragma unroll
+        for (int g = 0; g < KS / 4; ++g) {
+          if (g + 1 < KS / 4) read_4(g + 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s = Fp16::mfma32(kf[g % 2 * 4 + i], qf[g * 4 + i], s);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      BlockScales sc[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const f32x4 c = *reinterpret_cast<const lds_f4*>(size_t(lds0 + unsigned(kConst + (stage * WR + 2 * n + g) * 16)));
+        sc[g] = {c[0], c[1], c[2]};
+      }
+      u32x4 vf[2][DT];
+      const auto read_v = [&](int h) {
+        unsigned vo = v_rd + so;
+        asm volatile("" : "+v"(vo));
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const unsigned p = (vo ^ unsigned(d * 64)) + unsigned((2 * n + h) * 16 * P);
+          const u32x2 x = read_transposed(p), y = read_transposed(p + unsigned(8 * P));
+          vf[h][d] = u32x4{x.x, x.y, y.x, y.y};
+        }
+      };
+      read_v(0);
+      const bool masked =
+          at + 31 > wpos_first || (a.window > 0 && at <= wpos_last - a.window) || wpos_last >= a.capacity;
+      const auto seen = [&](int i) { return sees(a, at + 8 * (i / 4) + 4 * half + i % 4, pos, oldest); };
+      weigh<LARGE_CAP>(a, s, sc, row_factor, masked, seen, m, mc, l, o);
+      u32x4 pf[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        pf[h] = u32x4{Fp16::pack2(s[8 * h], s[8 * h + 1]), Fp16::pack2(s[8 * h + 2], s[8 * h + 3]),
+                      Fp16::pack2(s[8 * h + 4], s[8 * h + 5]), Fp16::pack2(s[8 * h + 6], s[8 * h + 7])};
+      read_v(1);
+      if (kAhead && n + 1 < NS) read_k(n + 1);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] = Fp16::mfma32(vf[h][d], pf[h], o[d]);
+    }
+  };
+
+  // ---- main loop: tile j from stage j % 2; tile j + 1 is decoded into the other one, j + 2 requested, before it ----
+  look_up(0);
+  load(0);
+  look_up(1);
+  {  // rows of q to the lanes that multiply them, by way of the second stage
+    static_assert(WR * 32 * P <= kStage, "the rows fit a stage");
+    const unsigned rows = lds0 + unsigned(kStage + wr * 32 * P);
+#pragma unroll
+    for (int j = 0; j < KS / WD; ++j) {
+      const int piece = (j + wd * (KS / WD)) * 64 + lane, row = piece / (D / 8), c = piece % (D / 8);
+      *reinterpret_cast<lds_v4*>(size_t(rows + unsigned(row * P + ((c ^ k_swizzle<D>(row & 15)) << 4)))) = qf[j];
+    }
+    if (WD > 1)
+      stage_barrier();
+    else
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+    const unsigned mine = rows + unsigned((lane & 31) * P + ((half ^ k_swizzle<D>(lane & 15)) << 4));
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const lds_v4*>(size_t(mine ^ unsigned(ks * 32)));
+  }
+  row_factor = row_to_fp16(qf, a.bf16 != 0, a.negate != 0);
+  decode_to(0);
+  load(1);
+  look_up(2);
+  for (int j = 0; j < tiles; ++j) {
+    stage_barrier();
+    if (j + 1 < tiles) {
+      decode_to((j + 1) & 1);
+      load(j + 2);
+      look_up(j + 3);
+    }
+    compute(j, j & 1);
+  }
+  l = swap_add(l);
+
+  // ---- rows to out, or to the parts that are joined: through LDS, so that a store covers whole lines of a row ----
+  // where the lane's rows go, worked out again here: kept from above it would cost registers in the loop
+  int row_first = t.row0;
+  asm volatile("" : "+s"(row_first));
+  __syncthreads();  // the stages are free
+  constexpr int kRowB = DT * 64, kPad = kRowB + 16, kPadF = 128 + 16;  // a wave's part of a row; 32 FP32 values of one
+  const unsigned mine_rows = lds0 + unsigned(wave * 32 * kPad);
+  const int rl = lane & 31;
+  const bool there = wr * 32 + rl < t.rows;
+  const int row_at = min(row_first + wr * 32 + rl, last_row), token_at = row_at / a.group;
+  const int token = t.seq.first + token_at, head = kvh * a.group + (row_at - token_at * a.group);
+  const bool parts = range.splits > 1;
+  const long long to = !there  ? -1
+                       : parts ? (((long long)token * a.q_heads + head) * a.splits + z) * (D + 4) + wd * DT * 32
+                               : token * a.o_stride + head * D + wd * DT * 32;
+  const unsigned row = mine_rows + unsigned(rl * (parts ? kPadF : kPad));
+  if (half == 0) *reinterpret_cast<lds_ll*>(size_t(row + unsigned(parts ? 128 : kRowB))) = to;
+  // decode8's order undone
+  const auto four = [&](int d, int i) { return f32x4{o[d][4 * i], o[d][4 * i + 2], o[d][4 * i + 1], o[d][4 * i + 3]}; };
+  if (parts) {
+    if (there && half == 0 && wd == 0) {
+      a.part[to + D] = m == -INFINITY ? -INFINITY : mc;
+      a.part[to + D + 1] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<lds_f4*>(size_t(row + unsigned((8 * i + 4 * half) * 4))) = four(d, i) * C::kUnit;
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned from = mine_rows + unsigned((j * 8 + lane / 8) * kPadF);
+        const long long at = *reinterpret_cast<const lds_ll*>(size_t(from + 128u));
+        const f32x4 v = *reinterpret_cast<const lds_f4*>(size_t(from + unsigned(lane % 8 * 16)));
+        if (at >= 0) *reinterpret_cast<f32x4*>(a.part + at + d * 32 + lane % 8 * 4) = v;
+      }
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+    }
+  } else {
+    const float inv = l == 0.f ? 0.f : C::kUnit / l;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4 v = four(d, i);
+        if (l == 0.f) v = f32x4{};  // nothing seen
+        v *= inv;
+        *reinterpret_cast<lds_v2*>(size_t(row + unsigned((32 * d + 8 * i + 4 * half) * 2))) =
+            u32x2{pack_out(a.bf16, v[0], v[1]), pack_out(a.bf16, v[2], v[3])};
+      }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    constexpr int kOutPieces = kRowB / 16;
+#pragma unroll
+    for (int j = 0; j < kOutPieces / 2; ++j) {
+      const int piece = j * 64 + lane, from_row = piece / kOutPieces, c = piece % kOutPieces;
+      const unsigned from = mine_rows + unsigned(from_row * kPad);
+      const long long at = *reinterpret_cast<const lds_ll*>(size_t(from + unsigned(kRowB)));
+      const u32x4 v = *reinterpret_cast<const lds_v4*>(size_t(from + unsigned(c * 16)));
+      if (at >= 0) store_16_bytes(a.out + at + c * 8, v);
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+  }
+}
+
+template <typename C, int D, bool LARGE_CAP>
+int launch(const Kv8Args& a, const Shape& s, hipStream_t stream) {
+  if (!fits_launch(a, s)) return GIE_HIP_EUNSUPPORTED;
+  const int grid = int((long long)s.slots * s.splits * a.kv_heads);
+  int rc;
+  if (s.wide) {
+    constexpr int WD = D == 256 ? 2 : 1, WR = kWideRows / 32;
+    constexpr int bytes = 2 * 2 * kWideKeys * kPitch<D> + 2 * WR * 16, rows = WR * WD * 32 * (D / WD * 2 + 16);
+    static_assert(rows <= bytes && WR * WD * 32 * 144 <= bytes, "rows on their way out fit the stages");
+    rc = start(wide_kernel<C, D, WD, LARGE_CAP>, grid, 256 * WD, bytes, stream, a);
+  } else {
+    constexpr int WK = D == 256 ? 2 : 4, NST = D == 64 ? 8 : 4;
+    constexpr int bytes = WK * NST * 2 * kNarrowKeys * kPitch8<D>, join = WK * 256 + WK * 32 * (D + 4) * 4;
+    rc = start(narrow_kernel<C, D, WK, NST, LARGE_CAP>, grid, 64 * WK, bytes > join ? bytes : join, stream, a);
+  }
+  if (rc != GIE_HIP_OK || s.splits == 1) return rc;
+  return a.bf16 ? join_parts<Bf16, D>(a, s, stream) : join_parts<Fp16, D>(a, s, stream);
+}
+
+template <typename C, bool LARGE_CAP>
+int launch(const Kv8Args& a, const Shape& s, int head_dim, hipStream_t stream) {
+  switch (head_dim) {
+    case 64: return launch<C, 64, LARGE_CAP>(a, s, stream);
+    case 96: return launch<C, 96, LARGE_CAP>(a, s, stream);
+    case 128: return launch<C, 128, LARGE_CAP>(a, s, stream);
+    default: return launch<C, 256, LARGE_CAP>(a, s, stream);
+  }
 }
 
 }  // namespace
@@ -94,7 +722,10 @@ __global__ __launch_bounds__(256) void rows_kernel(Kv8Args a, int D, float scale
 
 using namespace gie_hip;
 
-extern "C" size_t gie_hip_kv8_attention_workspace(const gie_paged_geom* g) { return 0; }
+extern "C" size_t gie_hip_kv8_attention_workspace(const gie_paged_geom* g) {
+  if (!valid_paged(g) || g->total_tokens == 0) return 0;
+  return parts_bytes(*g, shape_of(*g));
+}
 
 extern "C" int gie_hip_kv8_attention(int dtype, int code, const gie_paged_geom* g, const void* q, const void* k_pages,
                                      const void* v_pages, const float* k_scales, const float* v_scales,
@@ -103,28 +734,25 @@ extern "C" int gie_hip_kv8_attention(int dtype, int code, const gie_paged_geom* 
   if (!valid_paged(g) || !valid_code(code)) return GIE_HIP_EINVAL;
   if (dtype != GIE_HIP_FP16 && dtype != GIE_HIP_BF16) return GIE_HIP_EUNSUPPORTED;
   if (g->head_dim != 64 && g->head_dim != 96 && g->head_dim != 128 && g->head_dim != 256) return GIE_HIP_EUNSUPPORTED;
+  // (a scale of 0 times a masked score is a NaN)
   if (!std::isfinite(g->scale) || g->scale == 0 || !std::isfinite(g->softcap)) return GIE_HIP_EINVAL;
   if (g->total_tokens == 0) return GIE_HIP_OK;
   if (!valid_attention(g, q, k_pages, v_pages, q_starts, seq_lens, page_table, out)) return GIE_HIP_EINVAL;
   if (!k_scales || !v_scales || k_scales == v_scales || !aligned_to(k_scales, 4) || !aligned_to(v_scales, 4))
     return GIE_HIP_EINVAL;
+  const Shape shape = shape_of(*g);
+  const size_t need = parts_bytes(*g, shape);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))) return GIE_HIP_EINVAL;
   Kv8Args a{};
   a.k_pages = static_cast<const uint8_t*>(k_pages);
   a.v_pages = static_cast<const uint8_t*>(v_pages);
   a.k_scales = k_scales;
   a.v_scales = v_scales;
-  Shape shape{};
-  shape.splits = 1;
-  shape.chunk = 1;
-  fill_args(a, g, shape, q, q_starts, seq_lens, page_table, out, workspace);
-  a.cap = g->softcap;
-  const long long grid = (long long)g->total_tokens * g->q_heads;
-  if (grid * 256 > 0xffffffffll) return GIE_HIP_EUNSUPPORTED;
+  a.bf16 = dtype == GIE_HIP_BF16;
+  const bool large_cap = fill_args(a, g, shape, q, q_starts, seq_lens, page_table, out, workspace);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const auto kernel = dtype == GIE_HIP_FP16
-                          ? (code == GIE_HIP_KV_INT8 ? rows_kernel<Fp16, Int8Code> : rows_kernel<Fp16, E4m3Code>)
-                          : (code == GIE_HIP_KV_INT8 ? rows_kernel<Bf16, Int8Code> : rows_kernel<Bf16, E4m3Code>);
-  hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(256), 0, s, a, g->head_dim, g->scale);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? GIE_HIP_OK : int(e);
+  const int D = g->head_dim;
+  if (code == GIE_HIP_KV_INT8)
+    return large_cap ? launch<Int8Code, true>(a, shape, D, s) : launch<Int8Code, false>(a, shape, D, s);
+  return large_cap ? launch<E4m3Code, true>(a, shape, D, s) : launch<E4m3Code, false>(a, shape, D, s);
 }

@@ -12,7 +12,10 @@ constexpr int kKvBlock = 16;  // positions of a head that share a scale
 constexpr float kKvLeast = 0x1p-64f;
 
 // Codes: encode4 rounds four values (already divided by the scale, so within the largest code but for FP32's rounding)
-// to nearest even, byte by byte; decode2 gives bytes 0 and 1, or 2 and 3, as FP16 times 1 / kUnit, exactly.
+// to nearest even, byte by byte; decode4 gives bytes 0 and 2, and 1 and 3, as FP16 times 1 / kUnit, exactly (five
+// instructions in both types; bytes 0 and 1 together would take one or two more).
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
 struct Int8Code {
   static constexpr float kUnit = 1.f;
   static __device__ __forceinline__ float scale(float most) { return fmaxf(most, kKvLeast) / 127.f; }
@@ -22,6 +25,14 @@ struct Int8Code {
   }
   static __device__ __forceinline__ uint32_t encode1(float a) { return encode4(a, 0.f, 0.f, 0.f); }
   static __device__ __forceinline__ float decode1(uint32_t code) { return float(int8_t(code)); }
+  static __device__ __forceinline__ u32x2 decode4(uint32_t w) {
+    // code + 128 as the low bits of 1024, less 1152
+    const uint32_t x = w ^ 0x80808080u;
+    const uint32_t even = (x & 0x00ff00ffu) | 0x64006400u, odd = __builtin_amdgcn_perm(0x64646464u, x, 0x04030401u);
+    const f16x2 less = {_Float16(-1152.f), _Float16(-1152.f)};
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, even) + less),
+                 __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, odd) + less)};
+  }
 };
 
 // e4m3 with a power of 2 as scale: a larger scale moves exponents alone, so codes that are rounded again keep their bits
@@ -40,6 +51,14 @@ struct E4m3Code {
   static __device__ __forceinline__ uint32_t encode1(float a) { return encode4(a, 0.f, 0.f, 0.f) & 255u; }
   static __device__ __forceinline__ float decode1(uint32_t code) {  // the NaN codes (0x7f, 0xff) become 480
     return float(__builtin_bit_cast(_Float16, uint16_t((code & 0x80u) << 8 | (code & 0x7fu) << 7))) * kUnit;
+  }
+  static __device__ __forceinline__ u32x2 decode4(uint32_t w) {
+    // a code in the upper byte, moved down by one with its sign kept: the sign's copy and what the lower byte left go
+    const auto down = [](uint32_t x) {
+      const s16x2 y = __builtin_bit_cast(s16x2, x) >> s16x2{1, 1};
+      return __builtin_bit_cast(uint32_t, y) & 0xbf80bf80u;
+    };
+    return u32x2{down(w << 8), down(w)};
   }
 };
 
