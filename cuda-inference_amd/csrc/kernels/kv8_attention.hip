@@ -24,7 +24,8 @@ struct Kv8Args : AttnArgs {
   const uint8_t* v_pages;
   const float* k_scales;
   const float* v_scales;
-  int bf16;  // type of q and out
+  unsigned page_blocks;  // blocks of a page of all key heads
+  int bf16;              // type of q and out
 };
 
 constexpr float kLift = 7.f;  // weights lie in 2^7 .. 2^15 at their largest: FP16 has no step under 2^-24
@@ -175,7 +176,7 @@ __device__ __forceinline__ u32x2 read_transposed8(unsigned at) {
 }
 
 template <typename C, int D, int WK, int NST, bool LARGE_CAP>
-__global__ __launch_bounds__(64 * WK, 1) void narrow_kernel(Kv8Args a) {
+__global__ __launch_bounds__(64 * WK, WK == 8 ? 2 : 1) void narrow_kernel(Kv8Args a) {
   constexpr int TT = kNarrowKeys, GR = TT / 16, P = kPitch8<D>, KS = D / 16, KP = D / 32, DT = D / 32;
   constexpr int kGran = 16 * P, IPG = kGran / 1024, kTileB = TT * P, kStage = 2 * kTileB, LPT = 2 * GR * IPG;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
@@ -221,32 +222,36 @@ __global__ __launch_bounds__(64 * WK, 1) void narrow_kernel(Kv8Args a) {
   }
   const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds) + unsigned(wave * NST * kStage));
   const const_int* table = (const const_int*)(uintptr_t)(a.page_table + (long long)t.seq.index * a.max_pages);
-  struct Place16 {
-    int page[GR], slot[GR];
-  };
-  const auto look_up = [&](int tile, Place16& p) {
+  int page[GR], slot[GR];  // of the granules that the next issue() loads
+  const auto look_up = [&](int tile) {
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
       const int gran = min((key_of(tile) >> 4) + g, (a.capacity >> 4) - 1);
       const int pg = div_magic(gran, a.page_magic, a.page_shift);
-      p.page[g] = table[__builtin_amdgcn_readfirstlane(pg)];
-      p.slot[g] = gran - pg * a.page16;
+      page[g] = table[__builtin_amdgcn_readfirstlane(pg)];
+      slot[g] = gran - pg * a.page16;
     }
   };
   const auto uniform = [](v4i r) {
     return v4i{__builtin_amdgcn_readfirstlane(r.x), __builtin_amdgcn_readfirstlane(r.y),
                __builtin_amdgcn_readfirstlane(r.z), __builtin_amdgcn_readfirstlane(r.w)};
   };
-  const auto there = [&](const Place16& p, int g) { return p.page[g] >= 0 && p.page[g] < a.num_pages; };
-  const auto block_at = [&](const Place16& p, int g) {
-    return ((long long)(there(p, g) ? p.page[g] : 0) * a.kv_heads + kvh) * a.page16 + p.slot[g];
+  struct Pair {
+    float k[GR], v[GR];
   };
-  const auto issue = [&](int tile, int stage, const Place16& p) {
+  // requests a tile's codes, and its scales (of a page that is not there the smallest: its codes are zeros)
+  const auto issue = [&](int tile, int stage, Pair& scales) {
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
       const int at = key_of(tile) + g * 16;
-      const int bytes = there(p, g) && tile < tiles ? min(max(range.hi - at, 0), 16) * D : 0;
-      const long long off = block_at(p, g) * (16ll * D);
+      const bool there = unsigned(page[g]) < unsigned(a.num_pages);
+      const int bytes = there && tile < tiles ? min(max(range.hi - at, 0), 16) * D : 0;
+      const unsigned long long block =
+          (unsigned long long)(there ? unsigned(page[g]) : 0u) * a.page_blocks + unsigned(kvh * a.page16 + slot[g]);
+      const float k = ((const const_float*)(uintptr_t)a.k_scales)[block], v = ((const const_float*)(uintptr_t)a.v_scales)[block];
+      scales.k[g] = there ? k : 0.f;
+      scales.v[g] = there ? v : 0.f;
+      const unsigned long long off = block * (16 * D);
       v4i rk = uniform(make_vsharp(a.k_pages + off, bytes)), rv = uniform(make_vsharp(a.v_pages + off, bytes));
       // a vector instruction may have written these scalar registers: loads may read them 5 cycles later
       asm volatile("s_nop 4" : "+s"(rk), "+s"(rv));
@@ -255,19 +260,6 @@ __global__ __launch_bounds__(64 * WK, 1) void narrow_kernel(Kv8Args a) {
       for (int i = 0; i < IPG; ++i) dma16(rk, to + i * 1024, k_off[i]);
 #pragma unroll
       for (int i = 0; i < IPG; ++i) dma16(rv, to + kTileB + i * 1024, v_off[i]);
-    }
-  };
-  // scales of a tile's blocks; of a page that is not there the smallest: its codes are zeros
-  struct Pair {
-    float k[GR], v[GR];
-  };
-  const auto scales_of = [&](const Place16& p, Pair& s) {
-#pragma unroll
-    for (int g = 0; g < GR; ++g) {
-      const long long at = block_at(p, g);
-      const float k = ((const const_float*)(uintptr_t)a.k_scales)[at], v = ((const const_float*)(uintptr_t)a.v_scales)[at];
-      s.k[g] = there(p, g) ? k : 0.f;
-      s.v[g] = there(p, g) ? v : 0.f;
     }
   };
 
@@ -314,30 +306,26 @@ __global__ __launch_bounds__(64 * WK, 1) void narrow_kernel(Kv8Args a) {
   };
 
   // ---- main loop: a wave's j-th tile from stage j % NST while the next NST - 1 load; loads past the last tile read
-  // nothing and write zeros, so that every wait counts the same. Scales arrive a tile ahead, their pages two ----
+  // nothing and write zeros, so that every wait counts the same ----
   const int mine = (tiles - wave + WK - 1) / WK;
   const auto tile_at = [&](int j) { return wave + j * WK; };
-  Place16 next, ahead;
-  Pair now, then;
-  look_up(tile_at(0), next);
-  ahead = next;
+  Pair scales[NST - 1];  // of the tiles that load
+  look_up(tile_at(0));
 #pragma unroll
   for (int j = 0; j < NST - 1; ++j) {
-    issue(tile_at(j), j, next);
-    look_up(tile_at(j + 1), next);
+    issue(tile_at(j), j, scales[j]);
+    look_up(tile_at(j + 1));
   }
-  scales_of(ahead, then);
-  look_up(tile_at(1), ahead);
   row_factor = row_to_fp16(qf, a.bf16 != 0, a.negate != 0);
   int stage = 0;
   for (int j = 0; j < mine; ++j) {
     wait_vm<(NST - 2) * LPT>();
     __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's reads of the stage that is loaded next are done: lgkmcnt(0)
-    issue(tile_at(j + NST - 1), stage == 0 ? NST - 1 : stage - 1, next);
-    look_up(tile_at(j + NST), next);
-    now = then;
-    scales_of(ahead, then);
-    look_up(tile_at(j + 2), ahead);
+    const Pair now = scales[0];
+#pragma unroll
+    for (int i = 0; i + 1 < NST - 1; ++i) scales[i] = scales[i + 1];
+    issue(tile_at(j + NST - 1), stage == 0 ? NST - 1 : stage - 1, scales[NST - 2]);
+    look_up(tile_at(j + NST));
     compute(tile_at(j), stage, now);
     stage = stage + 1 == NST ? 0 : stage + 1;
   }
@@ -457,14 +445,15 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
     slot = gran - pg * a.page16;
   };
   const auto load = [&](int tile) {
-    const bool there = page >= 0 && page < a.num_pages;
+    const bool there = unsigned(page) < unsigned(a.num_pages);
     const int at = key_of(tile) + wr * 16;
     const int bytes = there && tile < tiles ? min(max(range.hi - at, 0), 16) * D : 0;
-    const long long block = ((long long)(there ? page : 0) * a.kv_heads + kvh) * a.page16 + slot;
+    const unsigned long long block =
+        (unsigned long long)(there ? unsigned(page) : 0u) * a.page_blocks + unsigned(kvh * a.page16 + slot);
 #pragma unroll
     for (int n = 0; n < KV; ++n) {
       const bool is_v = WD == 1 ? n == 1 : wd == 1;
-      const uint8_t* from = (is_v ? a.v_pages : a.k_pages) + block * (16ll * D);
+      const uint8_t* from = (is_v ? a.v_pages : a.k_pages) + block * (16 * D);
       const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from), 0, bytes, kBufferWord3);
 #pragma unroll
       for (int j = 0; j < JP; ++j)
@@ -699,7 +688,7 @@ int launch(const Kv8Args& a, const Shape& s, hipStream_t stream) {
     static_assert(rows <= bytes && WR * WD * 32 * 144 <= bytes, "rows on their way out fit the stages");
     rc = start(wide_kernel<C, D, WD, LARGE_CAP>, grid, 256 * WD, bytes, stream, a);
   } else {
-    constexpr int WK = D == 256 ? 2 : 4, NST = D == 64 ? 8 : 4;
+    constexpr int WK = D == 256 ? 4 : 8, NST = D == 64 ? 4 : 2;
     constexpr int bytes = WK * NST * 2 * kNarrowKeys * kPitch8<D>, join = WK * 256 + WK * 32 * (D + 4) * 4;
     rc = start(narrow_kernel<C, D, WK, NST, LARGE_CAP>, grid, 64 * WK, bytes > join ? bytes : join, stream, a);
   }
@@ -736,6 +725,7 @@ extern "C" int gie_hip_kv8_attention(int dtype, int code, const gie_paged_geom* 
   if (g->head_dim != 64 && g->head_dim != 96 && g->head_dim != 128 && g->head_dim != 256) return GIE_HIP_EUNSUPPORTED;
   // (a scale of 0 times a masked score is a NaN)
   if (!std::isfinite(g->scale) || g->scale == 0 || !std::isfinite(g->softcap)) return GIE_HIP_EINVAL;
+  if ((long long)g->kv_heads * (g->page_size / 16) > 0x7fffffff) return GIE_HIP_EUNSUPPORTED;  // blocks of a page
   if (g->total_tokens == 0) return GIE_HIP_OK;
   if (!valid_attention(g, q, k_pages, v_pages, q_starts, seq_lens, page_table, out)) return GIE_HIP_EINVAL;
   if (!k_scales || !v_scales || k_scales == v_scales || !aligned_to(k_scales, 4) || !aligned_to(v_scales, 4))
@@ -748,6 +738,7 @@ extern "C" int gie_hip_kv8_attention(int dtype, int code, const gie_paged_geom* 
   a.v_pages = static_cast<const uint8_t*>(v_pages);
   a.k_scales = k_scales;
   a.v_scales = v_scales;
+  a.page_blocks = unsigned(g->kv_heads) * unsigned(g->page_size / 16);
   a.bf16 = dtype == GIE_HIP_BF16;
   const bool large_cap = fill_args(a, g, shape, q, q_starts, seq_lens, page_table, out, workspace);
   hipStream_t s = static_cast<hipStream_t>(stream);
