@@ -30,18 +30,19 @@ struct Kv8Args : AttnArgs {
 
 constexpr float kLift = 7.f;  // weights lie in 2^7 .. 2^15 at their largest: FP16 has no step under 2^-24
 
-// A block's scales as the scores take them: f times the product of codes is the product of keys (a NaN if either scale
-// is one: every score of the block becomes a NaN), lv = log2(vs), inv = 1 / vs.
+// A block's scales as the scores take them: f times the product of codes and the row's factor is the score's power of 2,
+// or where scores are capped the product of keys (a NaN if either scale is one: every score of the block becomes a NaN),
+// lv = log2(vs), inv = 1 / vs.
 struct BlockScales {
   float f, lv, inv;
 };
 template <typename C>
-__device__ __forceinline__ BlockScales block_scales(float ks, float vs) {
+__device__ __forceinline__ BlockScales block_scales(const AttnArgs& a, float ks, float vs) {
   const float k = fminf(fmaxf(ks, 0x1p-73f), 0x1p120f), v = fminf(fmaxf(vs, 0x1p-73f), 0x1p120f);
   const bool bad = !(ks == ks) || !(vs == vs);
   // the exponent and the quotient from the same logarithm, so that a weight and what the sum takes of it agree
   const float lv = __builtin_amdgcn_logf(v);
-  return {bad ? __builtin_nanf("") : k * C::kUnit, lv, __builtin_amdgcn_exp2f(-lv)};
+  return {bad ? __builtin_nanf("") : k * C::kUnit * (a.cap > 0 ? 1.f : a.mult), lv, __builtin_amdgcn_exp2f(-lv)};
 }
 
 // codes of 8 values, in the order 0, 2, 1, 3, 4, 6, 5, 7
@@ -53,12 +54,9 @@ __device__ __forceinline__ u32x4 decode8(uint32_t a, uint32_t b) {
 
 // Fragments of a row of q (this lane's half of its values) in FP16, in decode8's order, times a power of 2; returns the
 // factor that takes it back. The sign changes where the scores' scale is negative.
-template <int KS>
-__device__ __forceinline__ float row_to_fp16(u32x4 (&qf)[KS], bool bf16, bool negate) {
-  const auto value = [&](int ks, int i) {
-    const uint16_t b = uint16_t(qf[ks][i / 2] >> (i % 2 * 16));
-    return bf16 ? Bf16::to_f32(b) : Fp16::to_f32(b);
-  };
+template <typename E, int KS>
+__device__ __forceinline__ float row_to_fp16(u32x4 (&qf)[KS], bool negate) {
+  const auto value = [&](int ks, int i) { return E::to_f32(uint16_t(qf[ks][i / 2] >> (i % 2 * 16))); };
   float most = 0.f;
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks)
@@ -81,18 +79,22 @@ __device__ __forceinline__ float row_to_fp16(u32x4 (&qf)[KS], bool bf16, bool ne
   return __uint_as_float(unsigned(127 + e - 14) << 23);
 }
 
-__device__ __forceinline__ uint32_t pack_out(bool bf16, float lo, float hi) {
-  return bf16 ? Bf16::pack2(lo, hi) : Fp16::pack2(lo, hi);
+__device__ __forceinline__ u32x2 pack_out(bool bf16, f32x4 v) {
+  if (bf16) return u32x2{Bf16::pack2(v[0], v[1]), Bf16::pack2(v[2], v[3])};
+  return u32x2{Fp16::pack2(v[0], v[1]), Fp16::pack2(v[2], v[3])};
 }
 
 // The weights of 32 scores (register i: key 8 (i / 4) + 4 half + i % 4, so the block i / 8), and what they do to the
 // running maximum, the sum and the rows' values. `masked`: seen(i) says whether register i's key is.
+//
+// The maximum is not looked for ahead of the weights (27 of about 150 vector instructions): they are taken against what
+// is there, and as long as a lane's sum of them stays within 2^15 all of them fit FP16. Only where it does not, or a row
+// has seen nothing yet, the rows' maxima move and the weights are taken again.
 template <bool LARGE_CAP, int DT, typename Seen>
 __device__ __forceinline__ void weigh(const AttnArgs& a, f32x16& s, const BlockScales (&sc)[2], float row_factor,
                                       bool masked, Seen seen, float& m, float& mc, float& l, f32x16 (&o)[DT]) {
-  float f[2];
-#pragma unroll
-  for (int g = 0; g < 2; ++g) f[g] = fminf(fmaxf(row_factor * sc[g].f, 0x1p-126f), 3e38f);
+  const auto within = [](float f) { return __builtin_amdgcn_fmed3f(f, 0x1p-126f, 3e38f); };  // masked: no -inf times 0
+  float f[2] = {within(row_factor * sc[0].f), within(row_factor * sc[1].f)};
   if (LARGE_CAP || a.cap > 0) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] *= f[i / 8];
@@ -101,33 +103,46 @@ __device__ __forceinline__ void weigh(const AttnArgs& a, f32x16& s, const BlockS
     else
       cap_scores(a, s);
     f[0] = f[1] = a.mult;
-  } else {
-#pragma unroll
-    for (int g = 0; g < 2; ++g) f[g] = fminf(fmaxf(f[g] * a.mult, 0x1p-126f), 3e38f);
   }
-  // (clamped above, a NaN became a number: scores of such a block are set here)
+  if (__any(!(sc[0].f == sc[0].f) || !(sc[1].f == sc[1].f))) {
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
-    if (__any(!(sc[g].f == sc[g].f)))
+    for (int g = 0; g < 2; ++g)
+      if (!(sc[g].f == sc[g].f)) {
+        f[g] = 1.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[8 * g + i] = __builtin_nanf("");
+        for (int i = 0; i < 8; ++i) s[8 * g + i] = __builtin_nanf("");
+      }
+  }
   if (masked) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = seen(i) ? s[i] : -INFINITY;
   }
-  float most[2];
+  f32x16 w;
+  float sum[2];
+  const auto take = [&] {
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    most[g] = s[8 * g];
+    for (int g = 0; g < 2; ++g) {
+      const float c = sc[g].lv - mc;
+      float part[2] = {};
 #pragma unroll
-    for (int i = 1; i < 8; ++i) most[g] = fmaxf(most[g], s[8 * g + i]);
-    most[g] = __builtin_fmaf(most[g], f[g], sc[g].lv);
-  }
-  const float top = swap_max(fmaxf(most[0], most[1]));
-  // the maximum follows only when a weight would pass 2^8: sums and weights keep their relative precision, and most
-  // tiles leave O as it is
-  if (__any(top - m > 8.f)) {
-    const float next = fmaxf(m, top);
+      for (int i = 0; i < 8; ++i) {
+        w[8 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * g + i], f[g], c));
+        part[i % 2] += w[8 * g + i];
+      }
+      sum[g] = part[0] + part[1];
+    }
+  };
+  take();
+  if (__any(!(sum[0] + sum[1] <= 0x1p15f) || m == -INFINITY)) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      float most = s[8 * g];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) most = fmaxf(most, s[8 * g + i]);
+      top = fmaxf(top, __builtin_fmaf(most, f[g], sc[g].lv));
+    }
+    const float next = fmaxf(m, swap_max(top));
     float nc = next == -INFINITY ? 0.f : next;
     nc += __builtin_fmaf(fabsf(nc), 0x1p-22f, -kLift);  // (what rounding takes from it and from an exponent)
     const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - nc);  // 1: nothing summed yet
@@ -136,18 +151,11 @@ __device__ __forceinline__ void weigh(const AttnArgs& a, f32x16& s, const BlockS
     l *= keep;
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] *= keep;
+    take();
   }
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const float c = sc[g].lv - mc;
-    float sum[2] = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s[8 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * g + i], f[g], c));
-      sum[i % 2] += s[8 * g + i];
-    }
-    l = __builtin_fmaf(sum[0] + sum[1], sc[g].inv, l);
-  }
+  l = __builtin_fmaf(sum[0], sc[0].inv, l);
+  l = __builtin_fmaf(sum[1], sc[1].inv, l);
+  s = w;
 }
 
 // ---------------------------------------------------------------- few rows: 32 for each workgroup
@@ -292,7 +300,7 @@ __global__ __launch_bounds__(64 * WK, WK == 8 ? 2 : 1) void narrow_kernel(Kv8Arg
       for (int d = 0; d < DT; ++d) vr[g][d] = read_transposed8(((v_rd + so) ^ unsigned(d * 32)) + unsigned(g * kGran));
     BlockScales sc[2];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) sc[g] = block_scales<C>(pair.k[g], pair.v[g]);
+    for (int g = 0; g < 2; ++g) sc[g] = block_scales<C>(a, pair.k[g], pair.v[g]);
     const bool masked = at + TT - 1 > pos_first || (a.window > 0 && at <= pos_last - a.window) || pos_last >= a.capacity;
     const auto seen = [&](int i) { return sees(a, at + 8 * (i / 4) + 4 * half + i % 4, pos, oldest); };
     weigh<LARGE_CAP>(a, s, sc, row_factor, masked, seen, m, mc, l, o);
@@ -316,7 +324,7 @@ __global__ __launch_bounds__(64 * WK, WK == 8 ? 2 : 1) void narrow_kernel(Kv8Arg
     issue(tile_at(j), j, scales[j]);
     look_up(tile_at(j + 1));
   }
-  row_factor = row_to_fp16(qf, a.bf16 != 0, a.negate != 0);
+  row_factor = a.bf16 ? row_to_fp16<Bf16>(qf, a.negate != 0) : row_to_fp16<Fp16>(qf, a.negate != 0);
   int stage = 0;
   for (int j = 0; j < mine; ++j) {
     wait_vm<(NST - 2) * LPT>();
@@ -377,7 +385,7 @@ __global__ __launch_bounds__(64 * WK, WK == 8 ? 2 : 1) void narrow_kernel(Kv8Arg
       uint16_t* dst = a.out + (t.seq.first + token) * a.o_stride + head * D + d;
       if (total == 0.f) v = f32x4{};
       v *= inv;
-      store_8_bytes(dst, u32x2{pack_out(a.bf16, v[0], v[1]), pack_out(a.bf16, v[2], v[3])});
+      store_8_bytes(dst, pack_out(a.bf16, v));
     }
   }
 }
@@ -435,7 +443,11 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
   const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds));
   const const_int* table = (const const_int*)(uintptr_t)(a.page_table + (long long)t.seq.index * a.max_pages);
   constexpr int KV = 2 / WD;  // of this wave
-  u32x4 raw[KV][JP];
+  static_assert(NS == 2, "a half of the pieces for each part");
+  // Half of a tile's pieces at a time: K's, then V's (WD == 2: two halves of the one). Pieces go under the first products
+  // of one part of the tile before: decoded there they cost no time of their own.
+  constexpr int kHalf = KV * JP / 2;
+  u32x4 raw[2][kHalf];
   float raw_k, raw_v;
   int page, slot;
   const auto look_up = [&](int tile) {
@@ -444,22 +456,23 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
     page = table[__builtin_amdgcn_readfirstlane(pg)];
     slot = gran - pg * a.page16;
   };
-  const auto load = [&](int tile) {
+  const auto load = [&](int tile, int n) {
     const bool there = unsigned(page) < unsigned(a.num_pages);
     const int at = key_of(tile) + wr * 16;
     const int bytes = there && tile < tiles ? min(max(range.hi - at, 0), 16) * D : 0;
     const unsigned long long block =
         (unsigned long long)(there ? unsigned(page) : 0u) * a.page_blocks + unsigned(kvh * a.page16 + slot);
+    const uint8_t* from = ((WD == 1 ? n == 1 : wd == 1) ? a.v_pages : a.k_pages) + block * (16 * D);
+    // uniform by construction; readfirstlane states it for the compiler
+    const unsigned long long address = reinterpret_cast<unsigned long long>(from);
+    const unsigned lo = __builtin_amdgcn_readfirstlane(unsigned(address)), hi = __builtin_amdgcn_readfirstlane(unsigned(address >> 32));
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((unsigned long long)hi << 32 | lo), 0,
+                                                        __builtin_amdgcn_readfirstlane(bytes), kBufferWord3);
 #pragma unroll
-    for (int n = 0; n < KV; ++n) {
-      const bool is_v = WD == 1 ? n == 1 : wd == 1;
-      const uint8_t* from = (is_v ? a.v_pages : a.k_pages) + block * (16 * D);
-      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from), 0, bytes, kBufferWord3);
-#pragma unroll
-      for (int j = 0; j < JP; ++j)
-        raw[n][j] = __builtin_bit_cast(
-            u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (j * 64 + lane) * 16, 0, 0));
-    }
+    for (int j = 0; j < kHalf; ++j)
+      raw[n][j] = __builtin_bit_cast(
+          u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (((WD == 1 ? 0 : n * kHalf) + j) * 64 + lane) * 16, 0, 0));
+    if (n == 1) return;
     const float k = ((const const_float*)(uintptr_t)a.k_scales)[block], v = ((const const_float*)(uintptr_t)a.v_scales)[block];
     raw_k = there ? k : 0.f;
     raw_v = there ? v : 0.f;
@@ -472,23 +485,20 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
     k_wr[j] = unsigned((wr * 16 + row) * P + ((c ^ k_swizzle<D>(row)) << 4));
     v_wr[j] = unsigned(kTileB + (wr * 16 + row) * P + ((c ^ v_swizzle<D>(row)) << 4));
   }
-  const auto decode_to = [&](int stage) {
-    const unsigned so = lds0 + unsigned(stage * kStage);
-#pragma unroll
-    for (int n = 0; n < KV; ++n)
-#pragma unroll
-      for (int j = 0; j < JP; ++j) {
-        const bool is_v = WD == 1 ? n == 1 : wd == 1;
-        if (kPieces % 64 != 0 && j * 64 + lane >= kPieces) continue;
-        const unsigned to = so + (is_v ? v_wr[j] : k_wr[j]);
-        *reinterpret_cast<lds_v4*>(size_t(to)) = decode8<C>(raw[n][j].x, raw[n][j].y);
-        *reinterpret_cast<lds_v4*>(size_t(to ^ 16u)) = decode8<C>(raw[n][j].z, raw[n][j].w);
-      }
-    if (wd == 0) {
-      const BlockScales s = block_scales<C>(raw_k, raw_v);
-      if (lane == 0)
-        *reinterpret_cast<lds_f4*>(size_t(lds0 + unsigned(kConst + (stage * WR + wr) * 16))) = f32x4{s.f, s.lv, s.inv, 0.f};
-    }
+  // unit u of 2 kHalf: 8 values of a piece for each lane
+  const auto decode_unit = [&](int n, int u, int stage) {
+    const bool is_v = WD == 1 ? n == 1 : wd == 1;
+    const int j = u / 2, at = (WD == 1 ? 0 : n * kHalf) + j;
+    if (kPieces % 64 != 0 && at * 64 + lane >= kPieces) return;
+    const unsigned to = lds0 + unsigned(stage * kStage) + (is_v ? v_wr[at] : k_wr[at]);
+    const u32x4 r = raw[n][j];
+    *reinterpret_cast<lds_v4*>(size_t(u % 2 ? to ^ 16u : to)) = u % 2 ? decode8<C>(r.z, r.w) : decode8<C>(r.x, r.y);
+  };
+  const auto store_scales = [&](int stage) {
+    if (wd != 0) return;
+    const BlockScales s = block_scales<C>(a, raw_k, raw_v);
+    if (lane == 0)
+      *reinterpret_cast<lds_f4*>(size_t(lds0 + unsigned(kConst + (stage * WR + wr) * 16))) = f32x4{s.f, s.lv, s.inv, 0.f};
   };
 
   // ---- fragment addresses ----
@@ -505,6 +515,7 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
   const auto compute = [&](int tile, int stage) {
     const unsigned so = unsigned(stage * kStage);
     const int at0 = key_of(tile), oldest = a.window > 0 ? pos - a.window : -1;
+    store_scales(stage ^ 1);
     constexpr bool kAhead = WD == 1;  // where the registers hold it
     u32x4 kf[KS];
     const auto read_k = [&](int n) {
@@ -521,7 +532,12 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
       f32x16 s = {};
       if constexpr (kAhead) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = Fp16::mfma32(kf[ks], qf[ks], s);
+        for (int ks = 0; ks < KS; ++ks) {
+          s = Fp16::mfma32(kf[ks], qf[ks], s);
+#pragma unroll
+          for (int u = ks * 2 * kHalf / KS; u < (ks + 1) * 2 * kHalf / KS; ++u) decode_unit(n, u, stage ^ 1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       } else {  // four steps ahead
         unsigned ko = k_rd + so;
         asm volatile("" : "+v"(ko));
@@ -538,9 +554,12 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int i = 0; i < 4; ++i) s = Fp16::mfma32(kf[g % 2 * 4 + i], qf[g * 4 + i], s);
+#pragma unroll
+          for (int u = g * 2 * kHalf * 4 / KS; u < (g + 1) * 2 * kHalf * 4 / KS; ++u) decode_unit(n, u, stage ^ 1);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      load(tile + 2, n);
       BlockScales sc[2];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
@@ -577,9 +596,10 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
     }
   };
 
-  // ---- main loop: tile j from stage j % 2; tile j + 1 is decoded into the other one, j + 2 requested, before it ----
+  // ---- main loop: tile j from stage j % 2; tile j + 1 is decoded into the other one and j + 2 requested under it ----
   look_up(0);
-  load(0);
+  load(0, 0);
+  load(0, 1);
   look_up(1);
   {  // rows of q to the lanes that multiply them, by way of the second stage
     static_assert(WR * 32 * P <= kStage, "the rows fit a stage");
@@ -597,18 +617,19 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const lds_v4*>(size_t(mine ^ unsigned(ks * 32)));
   }
-  row_factor = row_to_fp16(qf, a.bf16 != 0, a.negate != 0);
-  decode_to(0);
-  load(1);
+  row_factor = a.bf16 ? row_to_fp16<Bf16>(qf, a.negate != 0) : row_to_fp16<Fp16>(qf, a.negate != 0);
+  store_scales(0);
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+#pragma unroll
+    for (int u = 0; u < 2 * kHalf; ++u) decode_unit(n, u, 0);
+    load(1, n);
+  }
   look_up(2);
   for (int j = 0; j < tiles; ++j) {
     stage_barrier();
-    if (j + 1 < tiles) {
-      decode_to((j + 1) & 1);
-      load(j + 2);
-      look_up(j + 3);
-    }
     compute(j, j & 1);
+    look_up(j + 3);
   }
   l = swap_add(l);
 
@@ -653,16 +674,23 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
     }
   } else {
     const float inv = l == 0.f ? 0.f : C::kUnit / l;
+    const auto rows_as = [&](auto type) {
+      using E = decltype(type);
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f32x4 v = four(d, i);
-        if (l == 0.f) v = f32x4{};  // nothing seen
-        v *= inv;
-        *reinterpret_cast<lds_v2*>(size_t(row + unsigned((32 * d + 8 * i + 4 * half) * 2))) =
-            u32x2{pack_out(a.bf16, v[0], v[1]), pack_out(a.bf16, v[2], v[3])};
-      }
+        for (int i = 0; i < 4; ++i) {
+          f32x4 v = four(d, i);
+          if (l == 0.f) v = f32x4{};  // nothing seen
+          v *= inv;
+          *reinterpret_cast<lds_v2*>(size_t(row + unsigned((32 * d + 8 * i + 4 * half) * 2))) =
+              u32x2{E::pack2(v[0], v[1]), E::pack2(v[2], v[3])};
+        }
+    };
+    if (a.bf16)
+      rows_as(Bf16{});
+    else
+      rows_as(Fp16{});
     __builtin_amdgcn_s_waitcnt(0xc07f);
     constexpr int kOutPieces = kRowB / 16;
 #pragma unroll

@@ -28,7 +28,8 @@ struct Int8Code {
   static __device__ __forceinline__ u32x2 decode4(uint32_t w) {
     // code + 128 as the low bits of 1024, less 1152
     const uint32_t x = w ^ 0x80808080u;
-    const uint32_t even = (x & 0x00ff00ffu) | 0x64006400u, odd = __builtin_amdgcn_perm(0x64646464u, x, 0x04030401u);
+    const uint32_t even = __builtin_amdgcn_perm(0x64646464u, x, 0x04020400u);
+    const uint32_t odd = __builtin_amdgcn_perm(0x64646464u, x, 0x04030401u);
     const f16x2 less = {_Float16(-1152.f), _Float16(-1152.f)};
     return u32x2{__builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, even) + less),
                  __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, odd) + less)};
