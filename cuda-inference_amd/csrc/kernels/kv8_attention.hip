@@ -17,8 +17,6 @@
 namespace gie_hip {
 namespace {
 
-typedef __attribute__((address_space(4))) const float const_float;
-
 struct Kv8Args : AttnArgs {
   const uint8_t* k_pages;
   const uint8_t* v_pages;
@@ -43,6 +41,33 @@ __device__ __forceinline__ BlockScales block_scales(const AttnArgs& a, float ks,
   // the exponent and the quotient from the same logarithm, so that a weight and what the sum takes of it agree
   const float lv = __builtin_amdgcn_logf(v);
   return {bad ? __builtin_nanf("") : k * C::kUnit * (a.cap > 0 ? 1.f : a.mult), lv, __builtin_amdgcn_exp2f(-lv)};
+}
+
+// A block of a sequence as a lane finds it: where it lies among all blocks (kNoBlock: its page is not there, its codes
+// count as zeros), and its scales.
+constexpr unsigned kNoBlock = 0xffffffffu;
+struct BlockAt {
+  unsigned at;
+  BlockScales s;
+};
+// The lanes look up 64 blocks at once, and the loop takes them by readlane: loads through the scalar cache would share
+// their counter with LDS, so that every wait for a fragment waited for them.
+template <typename C>
+__device__ __forceinline__ BlockAt find_block(const Kv8Args& a, const int* table, int kvh, int position) {
+  const int gran = min(position >> 4, (a.capacity >> 4) - 1), pg = div_magic(gran, a.page_magic, a.page_shift);
+  const int page = table[pg];
+  const bool there = unsigned(page) < unsigned(a.num_pages);
+  BlockAt b;
+  b.at = there ? unsigned(page) * a.page_blocks + unsigned(kvh * a.page16 + gran - pg * a.page16) : kNoBlock;
+  b.s = block_scales<C>(a, there ? a.k_scales[b.at] : 0.f, there ? a.v_scales[b.at] : 0.f);
+  return b;
+}
+__device__ __forceinline__ float read_lane(float v, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
+}
+__device__ __forceinline__ BlockAt block_of_lane(const BlockAt& b, int lane) {
+  return {unsigned(__builtin_amdgcn_readlane(int(b.at), lane)),
+          {read_lane(b.s.f, lane), read_lane(b.s.lv, lane), read_lane(b.s.inv, lane)}};
 }
 
 // codes of 8 values, in the order 0, 2, 1, 3, 4, 6, 5, 7
@@ -229,37 +254,27 @@ __global__ __launch_bounds__(64 * WK, WK == 8 ? 2 : 1) void narrow_kernel(Kv8Arg
     v_off[i] = vc < D / 16 ? r * D + vc * 16 : kOut;
   }
   const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds) + unsigned(wave * NST * kStage));
-  const const_int* table = (const const_int*)(uintptr_t)(a.page_table + (long long)t.seq.index * a.max_pages);
-  int page[GR], slot[GR];  // of the granules that the next issue() loads
-  const auto look_up = [&](int tile) {
-#pragma unroll
-    for (int g = 0; g < GR; ++g) {
-      const int gran = min((key_of(tile) >> 4) + g, (a.capacity >> 4) - 1);
-      const int pg = div_magic(gran, a.page_magic, a.page_shift);
-      page[g] = table[__builtin_amdgcn_readfirstlane(pg)];
-      slot[g] = gran - pg * a.page16;
-    }
-  };
+  const int* table = a.page_table + (long long)t.seq.index * a.max_pages;
+  const auto tile_at = [&](int j) { return wave + j * WK; };  // the wave's j-th tile
+  BlockAt blocks;  // lane 2 i + g: granule g of the wave's tile j with j % 32 == i
   const auto uniform = [](v4i r) {
     return v4i{__builtin_amdgcn_readfirstlane(r.x), __builtin_amdgcn_readfirstlane(r.y),
                __builtin_amdgcn_readfirstlane(r.z), __builtin_amdgcn_readfirstlane(r.w)};
   };
   struct Pair {
-    float k[GR], v[GR];
+    BlockScales g[GR];
   };
-  // requests a tile's codes, and its scales (of a page that is not there the smallest: its codes are zeros)
-  const auto issue = [&](int tile, int stage, Pair& scales) {
+  // requests the wave's j-th tile
+  const auto issue = [&](int j, int stage, Pair& scales) {
+    if (j % 32 == 0) blocks = find_block<C>(a, table, kvh, key_of(tile_at(j + lane / GR)) + lane % GR * 16);
+    const int tile = tile_at(j);
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
+      const BlockAt b = block_of_lane(blocks, j % 32 * GR + g);
+      scales.g[g] = b.s;
       const int at = key_of(tile) + g * 16;
-      const bool there = unsigned(page[g]) < unsigned(a.num_pages);
-      const int bytes = there && tile < tiles ? min(max(range.hi - at, 0), 16) * D : 0;
-      const unsigned long long block =
-          (unsigned long long)(there ? unsigned(page[g]) : 0u) * a.page_blocks + unsigned(kvh * a.page16 + slot[g]);
-      const float k = ((const const_float*)(uintptr_t)a.k_scales)[block], v = ((const const_float*)(uintptr_t)a.v_scales)[block];
-      scales.k[g] = there ? k : 0.f;
-      scales.v[g] = there ? v : 0.f;
-      const unsigned long long off = block * (16 * D);
+      const int bytes = b.at != kNoBlock && tile < tiles ? min(max(range.hi - at, 0), 16) * D : 0;
+      const unsigned long long off = (b.at != kNoBlock ? b.at : 0u) * (unsigned long long)(16 * D);
       v4i rk = uniform(make_vsharp(a.k_pages + off, bytes)), rv = uniform(make_vsharp(a.v_pages + off, bytes));
       // a vector instruction may have written these scalar registers: loads may read them 5 cycles later
       asm volatile("s_nop 4" : "+s"(rk), "+s"(rv));
@@ -298,12 +313,9 @@ __global__ __launch_bounds__(64 * WK, WK == 8 ? 2 : 1) void narrow_kernel(Kv8Arg
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int d = 0; d < DT; ++d) vr[g][d] = read_transposed8(((v_rd + so) ^ unsigned(d * 32)) + unsigned(g * kGran));
-    BlockScales sc[2];
-#pragma unroll
-    for (int g = 0; g < 2; ++g) sc[g] = block_scales<C>(a, pair.k[g], pair.v[g]);
     const bool masked = at + TT - 1 > pos_first || (a.window > 0 && at <= pos_last - a.window) || pos_last >= a.capacity;
     const auto seen = [&](int i) { return sees(a, at + 8 * (i / 4) + 4 * half + i % 4, pos, oldest); };
-    weigh<LARGE_CAP>(a, s, sc, row_factor, masked, seen, m, mc, l, o);
+    weigh<LARGE_CAP>(a, s, pair.g, row_factor, masked, seen, m, mc, l, o);
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const u32x4 pf = {Fp16::pack2(s[8 * g], s[8 * g + 2]), Fp16::pack2(s[8 * g + 1], s[8 * g + 3]),
@@ -316,14 +328,9 @@ __global__ __launch_bounds__(64 * WK, WK == 8 ? 2 : 1) void narrow_kernel(Kv8Arg
   // ---- main loop: a wave's j-th tile from stage j % NST while the next NST - 1 load; loads past the last tile read
   // nothing and write zeros, so that every wait counts the same ----
   const int mine = (tiles - wave + WK - 1) / WK;
-  const auto tile_at = [&](int j) { return wave + j * WK; };
   Pair scales[NST - 1];  // of the tiles that load
-  look_up(tile_at(0));
 #pragma unroll
-  for (int j = 0; j < NST - 1; ++j) {
-    issue(tile_at(j), j, scales[j]);
-    look_up(tile_at(j + 1));
-  }
+  for (int j = 0; j < NST - 1; ++j) issue(j, j, scales[j]);
   row_factor = a.bf16 ? row_to_fp16<Bf16>(qf, a.negate != 0) : row_to_fp16<Fp16>(qf, a.negate != 0);
   int stage = 0;
   for (int j = 0; j < mine; ++j) {
@@ -332,8 +339,7 @@ __global__ __launch_bounds__(64 * WK, WK == 8 ? 2 : 1) void narrow_kernel(Kv8Arg
     const Pair now = scales[0];
 #pragma unroll
     for (int i = 0; i + 1 < NST - 1; ++i) scales[i] = scales[i + 1];
-    issue(tile_at(j + NST - 1), stage == 0 ? NST - 1 : stage - 1, scales[NST - 2]);
-    look_up(tile_at(j + NST));
+    issue(j + NST - 1, stage == 0 ? NST - 1 : stage - 1, scales[NST - 2]);
     compute(tile_at(j), stage, now);
     stage = stage + 1 == NST ? 0 : stage + 1;
   }
@@ -441,28 +447,24 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
 
   // ---- codes: granule wr of a tile by this wave (of K and V, or WD == 2: of one) ----
   const unsigned lds0 = __builtin_amdgcn_readfirstlane(lds_addr(lds));
-  const const_int* table = (const const_int*)(uintptr_t)(a.page_table + (long long)t.seq.index * a.max_pages);
+  const int* table = a.page_table + (long long)t.seq.index * a.max_pages;
+  BlockAt blocks;  // lane i: granule wr of the tile j with j % 64 == i
   constexpr int KV = 2 / WD;  // of this wave
   static_assert(NS == 2, "a half of the pieces for each part");
   // Half of a tile's pieces at a time: K's, then V's (WD == 2: two halves of the one). Pieces go under the first products
   // of one part of the tile before: decoded there they cost no time of their own.
   constexpr int kHalf = KV * JP / 2;
   u32x4 raw[2][kHalf];
-  float raw_k, raw_v;
-  int page, slot;
-  const auto look_up = [&](int tile) {
-    const int gran = min((key_of(tile) >> 4) + wr, (a.capacity >> 4) - 1);
-    const int pg = div_magic(gran, a.page_magic, a.page_shift);
-    page = table[__builtin_amdgcn_readfirstlane(pg)];
-    slot = gran - pg * a.page16;
-  };
+  BlockAt now;
   const auto load = [&](int tile, int n) {
-    const bool there = unsigned(page) < unsigned(a.num_pages);
+    if (n == 0) {
+      if (tile % 64 == 0) blocks = find_block<C>(a, table, kvh, key_of(tile + lane) + wr * 16);
+      now = block_of_lane(blocks, tile % 64);
+    }
     const int at = key_of(tile) + wr * 16;
-    const int bytes = there && tile < tiles ? min(max(range.hi - at, 0), 16) * D : 0;
-    const unsigned long long block =
-        (unsigned long long)(there ? unsigned(page) : 0u) * a.page_blocks + unsigned(kvh * a.page16 + slot);
-    const uint8_t* from = ((WD == 1 ? n == 1 : wd == 1) ? a.v_pages : a.k_pages) + block * (16 * D);
+    const int bytes = now.at != kNoBlock && tile < tiles ? min(max(range.hi - at, 0), 16) * D : 0;
+    const unsigned long long off = (now.at != kNoBlock ? now.at : 0u) * (unsigned long long)(16 * D);
+    const uint8_t* from = ((WD == 1 ? n == 1 : wd == 1) ? a.v_pages : a.k_pages) + off;
     // uniform by construction; readfirstlane states it for the compiler
     const unsigned long long address = reinterpret_cast<unsigned long long>(from);
     const unsigned lo = __builtin_amdgcn_readfirstlane(unsigned(address)), hi = __builtin_amdgcn_readfirstlane(unsigned(address >> 32));
@@ -472,10 +474,6 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
     for (int j = 0; j < kHalf; ++j)
       raw[n][j] = __builtin_bit_cast(
           u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (((WD == 1 ? 0 : n * kHalf) + j) * 64 + lane) * 16, 0, 0));
-    if (n == 1) return;
-    const float k = ((const const_float*)(uintptr_t)a.k_scales)[block], v = ((const const_float*)(uintptr_t)a.v_scales)[block];
-    raw_k = there ? k : 0.f;
-    raw_v = there ? v : 0.f;
   };
   // piece j * 64 + lane: 16 values of a row, two chunks of FP16
   unsigned k_wr[JP], v_wr[JP];
@@ -496,9 +494,9 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
   };
   const auto store_scales = [&](int stage) {
     if (wd != 0) return;
-    const BlockScales s = block_scales<C>(a, raw_k, raw_v);
     if (lane == 0)
-      *reinterpret_cast<lds_f4*>(size_t(lds0 + unsigned(kConst + (stage * WR + wr) * 16))) = f32x4{s.f, s.lv, s.inv, 0.f};
+      *reinterpret_cast<lds_f4*>(size_t(lds0 + unsigned(kConst + (stage * WR + wr) * 16))) =
+          f32x4{now.s.f, now.s.lv, now.s.inv, 0.f};
   };
 
   // ---- fragment addresses ----
@@ -597,10 +595,8 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
   };
 
   // ---- main loop: tile j from stage j % 2; tile j + 1 is decoded into the other one and j + 2 requested under it ----
-  look_up(0);
   load(0, 0);
   load(0, 1);
-  look_up(1);
   {  // rows of q to the lanes that multiply them, by way of the second stage
     static_assert(WR * 32 * P <= kStage, "the rows fit a stage");
     const unsigned rows = lds0 + unsigned(kStage + wr * 32 * P);
@@ -625,11 +621,9 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
     for (int u = 0; u < 2 * kHalf; ++u) decode_unit(n, u, 0);
     load(1, n);
   }
-  look_up(2);
   for (int j = 0; j < tiles; ++j) {
     stage_barrier();
     compute(j, j & 1);
-    look_up(j + 3);
   }
   l = swap_add(l);
 
@@ -753,7 +747,7 @@ extern "C" int gie_hip_kv8_attention(int dtype, int code, const gie_paged_geom* 
   if (g->head_dim != 64 && g->head_dim != 96 && g->head_dim != 128 && g->head_dim != 256) return GIE_HIP_EUNSUPPORTED;
   // (a scale of 0 times a masked score is a NaN)
   if (!std::isfinite(g->scale) || g->scale == 0 || !std::isfinite(g->softcap)) return GIE_HIP_EINVAL;
-  if ((long long)g->kv_heads * (g->page_size / 16) > 0x7fffffff) return GIE_HIP_EUNSUPPORTED;  // blocks of a page
+  if ((long long)g->kv_heads * (g->page_size / 16) > 0x7fffffff / g->num_pages) return GIE_HIP_EUNSUPPORTED;  // blocks
   if (g->total_tokens == 0) return GIE_HIP_OK;
   if (!valid_attention(g, q, k_pages, v_pages, q_starts, seq_lens, page_table, out)) return GIE_HIP_EINVAL;
   if (!k_scales || !v_scales || k_scales == v_scales || !aligned_to(k_scales, 4) || !aligned_to(v_scales, 4))
