@@ -148,11 +148,11 @@ __device__ __forceinline__ void weigh(const AttnArgs& a, f32x16& s, const BlockS
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const float c = sc[g].lv - mc;
-      float part[2] = {};
+      float part[2];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         w[8 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * g + i], f[g], c));
-        part[i % 2] += w[8 * g + i];
+        part[i % 2] = i < 2 ? w[8 * g + i] : part[i % 2] + w[8 * g + i];
       }
       sum[g] = part[0] + part[1];
     }

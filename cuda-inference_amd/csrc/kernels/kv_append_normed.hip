@@ -1,7 +1,16 @@
 // Appends the keys and values of new tokens to a paged cache as kv_append does, with a norm of each head of q and k ahead
 // of the rotation, into pages of the tokens' own type or into 8-bit pages with a scale for each block of 16 positions:
 //   x'_d = x_d / sqrt(mean_d x_d^2 + eps) * w_d;  pairs (u, v) -> (u cos - v sin, u sin + v cos);  FP32 up to one rounding.
+//
+// Bytes-bound. A lane takes 16 values of a head, 8 pairs where they rotate, in 16-byte pieces; 4, 8 or 16 lanes make a
+// head and sum its squares among them; the weights of a lane's values stay in its registers for all of its heads.
+// Rows (q, and k and v of a cache in the tokens' type) go by token: a workgroup finds the places of one or more tokens and
+// spreads all their heads over its lanes. Blocks of 8-bit pages go by position: a wave has one head's whole block, up to
+// 16 tokens, in registers, so that the scale is the largest of them and every code is written once. Both parts are
+// workgroups of one launch.
+// Heads whose rotating part is no multiple of 16 take a form that goes value by value.
 #include <cmath>
+#include <type_traits>
 
 #include "kv8_common.h"
 
@@ -155,6 +164,249 @@ __global__ __launch_bounds__(64) void block_values_kernel(NormedArgs a) {
   if (lane == 0) *scale_at = scale;
 }
 
+// ---- 16 values a lane
+template <int D>
+constexpr int kHeadLanes = D == 64 ? 4 : D == 256 ? 16 : 8;  // of a head (6 of 8 at 96)
+
+// where a lane's 16 values lie in its head: 8 from `at`, 8 from `next`; pairs: they rotate (values i and 8 + i, or
+// interleaved 2 i and 2 i + 1, by the angles from `angle` on)
+struct Unit {
+  int at, next, angle;
+  bool there, pairs;
+};
+template <bool INTERLEAVED, int D>
+__device__ __forceinline__ Unit unit_of(int unit, int rotary) {
+  Unit u;
+  u.there = unit < D / 16;
+  u.pairs = u.there && unit < rotary / 16;
+  u.angle = unit * 8;
+  u.at = u.pairs && !INTERLEAVED ? unit * 8 : unit * 16;
+  u.next = u.pairs && !INTERLEAVED ? u.at + rotary / 2 : u.at + 8;
+  return u;
+}
+
+template <typename E>
+__device__ __forceinline__ void load_unit(const uint16_t* head, const Unit& u, float (&x)[16]) {
+  const u32x4 a = u.there ? load_16_bytes(head + u.at) : u32x4{}, b = u.there ? load_16_bytes(head + u.next) : u32x4{};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = E::to_f32(uint16_t(a[i])), x[2 * i + 1] = E::to_f32(uint16_t(a[i] >> 16));
+    x[8 + 2 * i] = E::to_f32(uint16_t(b[i])), x[9 + 2 * i] = E::to_f32(uint16_t(b[i] >> 16));
+  }
+}
+__device__ __forceinline__ void load_weights(const float* w, const Unit& u, float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = 1.f;
+  if (w == nullptr || !u.there) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = w[u.at + i], x[8 + i] = w[u.next + i];
+}
+template <int D>
+__device__ __forceinline__ void norm_unit(float (&x)[16], const float (&w)[16], float eps) {
+  float sum[2] = {};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum[i % 2] = __builtin_fmaf(x[i], x[i], sum[i % 2]);
+  float all = sum[0] + sum[1];
+#pragma unroll
+  for (int d = 1; d < kHeadLanes<D>; d <<= 1) all += __shfl_xor(all, d);
+  const float inv = 1.f / sqrtf(all * (1.f / D) + eps);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = x[i] * inv * w[i];
+}
+template <bool INTERLEAVED>
+__device__ __forceinline__ void turn_unit(float (&x)[16], const float* cos, const float* sin) {
+  const f32x4 c[2] = {__builtin_bit_cast(f32x4, load_16_bytes(cos)), __builtin_bit_cast(f32x4, load_16_bytes(cos + 4))};
+  const f32x4 s[2] = {__builtin_bit_cast(f32x4, load_16_bytes(sin)), __builtin_bit_cast(f32x4, load_16_bytes(sin + 4))};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float& u = x[INTERLEAVED ? 2 * i : i];
+    float& v = x[INTERLEAVED ? 2 * i + 1 : 8 + i];
+    const float a = u, b = v;
+    u = a * c[i / 4][i % 4] - b * s[i / 4][i % 4];
+    v = a * s[i / 4][i % 4] + b * c[i / 4][i % 4];
+  }
+}
+
+constexpr int kMostTokens = 8;  // of a workgroup
+
+// rows: tokens t0 .. t0 + count - 1, heads of q (if it is there), and of k and v with ALL
+template <typename E, bool INTERLEAVED, int D, bool ALL>
+__device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int count) {
+  __shared__ Place places[kMostTokens];
+  const gie_paged_geom& g = a.g;
+  constexpr int L = kHeadLanes<D>;
+  const int tid = int(threadIdx.x), threads = int(blockDim.x);
+  for (int i = tid >> 6; i < count; i += threads >> 6) {
+    const Place p = place_of(g, a.q_starts, a.seq_lens, a.page_table, t0 + i);
+    if ((tid & 63) == 0) places[i] = p;
+  }
+  const Unit u = unit_of<INTERLEAVED, D>(tid % L, g.rotary_dim);
+  float wq[16], wk[16];
+  load_weights(a.q_norm, u, wq);
+  if (ALL) load_weights(a.k_norm, u, wk);
+  __syncthreads();
+  const int q_heads = a.q ? g.q_heads : 0, heads = q_heads + (ALL ? 2 * g.kv_heads : 0), half = g.rotary_dim / 2;
+#pragma unroll 2
+  for (int i = tid / L; i < count * heads; i += threads / L) {
+    const int j = i / heads, t = t0 + j;
+    int head = i - j * heads;
+    const Place p = places[j];
+    const bool is_q = head < q_heads;
+    if (!is_q) head -= q_heads;
+    const bool is_v = !is_q && head >= g.kv_heads;
+    if (is_v) head -= g.kv_heads;
+    if (!p.present || (!is_q && p.page < 0)) continue;
+    const uint16_t* src = (is_q ? a.q + t * g.q_stride : is_v ? a.v + t * g.v_stride : a.k + t * g.k_stride) + head * D;
+    uint16_t* dst = is_q ? a.q_out + t * g.o_stride + head * D
+                         : static_cast<uint16_t*>(is_v ? a.v_pages : a.k_pages) +
+                               (((long long)p.page * g.kv_heads + head) * g.page_size + p.slot) * D;
+    float x[16];
+    load_unit<E>(src, u, x);
+    if (is_q && a.q_norm) norm_unit<D>(x, wq, g.norm_eps);
+    if (ALL && !is_q && !is_v && a.k_norm) norm_unit<D>(x, wk, g.norm_eps);
+    if (u.pairs && !is_v && p.position >= 0)
+      turn_unit<INTERLEAVED>(x, a.cos + (long long)p.position * half + u.angle, a.sin + (long long)p.position * half + u.angle);
+    if (!u.there) continue;
+    u32x4 y = {E::pack2(x[0], x[1]), E::pack2(x[2], x[3]), E::pack2(x[4], x[5]), E::pack2(x[6], x[7])};
+    u32x4 z = {E::pack2(x[8], x[9]), E::pack2(x[10], x[11]), E::pack2(x[12], x[13]), E::pack2(x[14], x[15])};
+    if (p.position < 0) y = z = u32x4{};
+    store_16_bytes(dst + u.at, y);
+    store_16_bytes(dst + u.next, z);
+  }
+}
+
+// block `slot` of the batch's: a wave for each head of k and v
+template <typename E, typename C, bool INTERLEAVED, int D>
+__device__ __forceinline__ void append_block(const NormedArgs& a, int slot) {
+  const gie_paged_geom& g = a.g;
+  constexpr int L = kHeadLanes<D>, T = 64 / L, kPasses = kKvBlock / T;  // T tokens at once
+  const int tid = int(threadIdx.x), lane = tid & 63, half = g.rotary_dim / 2;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = int(blockDim.x) >> 6;
+  const Block b = block_of(g, a.q_starts, a.seq_lens, a.page_table, slot);
+  if (b.first >= b.end || b.page < 0) return;
+  const Unit u = unit_of<INTERLEAVED, D>(lane % L, g.rotary_dim), straight = {lane % L * 16, lane % L * 16 + 8, 0, u.there, false};
+  for (int item = wave; item < 2 * g.kv_heads; item += waves) {
+    const bool is_v = item >= g.kv_heads;
+    const int head = is_v ? item - g.kv_heads : item;
+    const long long stride = is_v ? g.v_stride : g.k_stride;
+    const uint16_t* src = (is_v ? a.v : a.k) + b.row0 * stride + head * D;
+    const long long at = ((long long)b.page * g.kv_heads + head) * g.page_size + b.slot;
+    uint8_t* codes = static_cast<uint8_t*>(is_v ? a.v_pages : a.k_pages) + at * D;
+    float* scale_at = (is_v ? a.v_scales : a.k_scales) + at / kKvBlock;
+    const bool starts = b.first == b.start;
+    const float before = starts ? 0.f : *scale_at;
+    const Unit w = is_v ? straight : u;
+    float x[kPasses][16];
+    float most = 0.f;
+    bool finite = true;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int position = b.start + p * T + lane / L;
+      if (position < b.first || position >= b.end) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[p][i] = 0.f;
+        continue;
+      }
+      load_unit<E>(src + (position - b.first) * stride, w, x[p]);
+    }
+    if (!is_v && (a.k_norm || half > 0)) {
+      float wk[16];
+      load_weights(a.k_norm, u, wk);
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        const int position = b.start + p * T + lane / L;
+        if (position < b.first || position >= b.end) continue;
+        if (a.k_norm) norm_unit<D>(x[p], wk, g.norm_eps);
+        if (u.pairs)
+          turn_unit<INTERLEAVED>(x[p], a.cos + (long long)position * half + u.angle, a.sin + (long long)position * half + u.angle);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        most = fmaxf(most, fabsf(x[p][i]));
+        finite = finite && fabsf(x[p][i]) <= 3.402823466e38f;
+      }
+    most = wave_max(most);
+    if (__any(!finite) || !(before == before)) {
+      if (lane == 0) *scale_at = __builtin_nanf("");
+      continue;
+    }
+    const float scale = fmaxf(before, C::scale(most)), inv = 1.f / scale;
+    const bool grows = !starts && scale > before;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int position = b.start + p * T + lane / L;
+      uint8_t* dst = codes + (position - b.start) * D;
+      if (!w.there || position >= b.end) continue;
+      if (position < b.first) {
+        if (!grows) continue;
+        const float factor = before * inv;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const u32x2 c = __builtin_bit_cast(u32x2, *reinterpret_cast<const unsigned long long*>(dst + (i ? w.next : w.at)));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[p][8 * i + e] = C::decode1(c[e / 4] >> (e % 4 * 8) & 255u) * factor;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[p][i] *= inv;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const u32x2 c = {C::encode4(x[p][8 * i], x[p][8 * i + 1], x[p][8 * i + 2], x[p][8 * i + 3]),
+                         C::encode4(x[p][8 * i + 4], x[p][8 * i + 5], x[p][8 * i + 6], x[p][8 * i + 7])};
+        *reinterpret_cast<unsigned long long*>(dst + (i ? w.next : w.at)) = __builtin_bit_cast(unsigned long long, c);
+      }
+    }
+    if (lane == 0) *scale_at = scale;
+  }
+}
+
+// C void: pages in the tokens' type
+template <typename E, typename C, bool INTERLEAVED, int D>
+__global__ __launch_bounds__(512) void append_kernel(NormedArgs a, int slots, int tokens) {
+  int id = int(blockIdx.x);
+  if constexpr (!std::is_void<C>::value) {
+    if (id < slots) {
+      append_block<E, C, INTERLEAVED, D>(a, id);
+      return;
+    }
+    id -= slots;
+  }
+  append_rows<E, INTERLEAVED, D, std::is_void<C>::value>(a, id * tokens, min(tokens, a.g.total_tokens - id * tokens));
+}
+
+template <typename E, typename C>
+int launch_units(const NormedArgs& a, hipStream_t s) {
+  constexpr bool k8 = !std::is_void<C>::value;
+  const gie_paged_geom& g = a.g;
+  const int D = g.head_dim, lanes = D == 64 ? 4 : D == 256 ? 16 : 8;
+  const long long heads = (a.q ? g.q_heads : 0) + (k8 ? 0 : 2 * g.kv_heads), work = heads * lanes;  // of a token's lanes
+  // one token for each workgroup spreads a step of few tokens; of many, as many as give every lane two heads
+  long long tokens = g.total_tokens < 1024 || work == 0 ? 1 : 1024 / work;
+  tokens = tokens < 1 ? 1 : tokens > kMostTokens ? kMostTokens : tokens;
+  const long long slots = k8 ? block_slots(g) : 0, rows = heads == 0 ? 0 : (g.total_tokens + tokens - 1) / tokens;
+  long long threads = (work * tokens + (tokens > 1 ? 127 : 63)) / (tokens > 1 ? 128 : 64) * 64;
+  if (k8 && threads < 2ll * g.kv_heads * 64) threads = 2ll * g.kv_heads * 64;  // a wave for each head's block
+  if (threads > 512) threads = 512;
+  if ((slots + rows) * threads > 0xffffffffll || slots > 0x3fffffff) return GIE_HIP_EUNSUPPORTED;  // a launch's threads
+  const auto kernel = [&](auto interleaved) {
+    constexpr bool I = decltype(interleaved)::value;
+    switch (D) {
+      case 64: return append_kernel<E, C, I, 64>;
+      case 96: return append_kernel<E, C, I, 96>;
+      case 128: return append_kernel<E, C, I, 128>;
+      default: return append_kernel<E, C, I, 256>;
+    }
+  };
+  hipLaunchKernelGGL(g.interleaved ? kernel(std::true_type{}) : kernel(std::false_type{}), dim3(unsigned(slots + rows)),
+                     dim3(unsigned(threads)), 0, s, a, int(slots), int(tokens));
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? GIE_HIP_OK : int(e);
+}
+
 bool valid_rows(const gie_paged_geom* g, const void* q, const void* k, const void* v, const float* q_norm,
                 const float* k_norm, const float* cos, const float* sin, const int* q_starts, const int* seq_lens,
                 const int* page_table, const void* q_out, const void* k_pages, const void* v_pages) {
@@ -176,6 +428,7 @@ bool supported(int dtype, const gie_paged_geom* g) {
 
 template <typename E, typename C>
 int launch_blocks(const NormedArgs& a, hipStream_t s) {
+  if (a.g.rotary_dim % 16 == 0) return launch_units<E, C>(a, s);
   const long long grid = block_slots(a.g) * 2 * a.g.kv_heads;
   const long long rows = a.q ? (long long)a.g.total_tokens * a.g.q_heads : 0;
   if (grid * 64 > 0xffffffffll || rows * 64 > 0xffffffffll) return GIE_HIP_EUNSUPPORTED;  // a launch's threads
@@ -204,9 +457,10 @@ extern "C" int gie_hip_kv_append_normed(int dtype, const gie_paged_geom* g, cons
   const NormedArgs a{*g, static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
                      static_cast<const uint16_t*>(v), q_norm, k_norm, cos, sin, q_starts, seq_lens, page_table,
                      static_cast<uint16_t*>(q_out), k_pages, v_pages, nullptr, nullptr};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (g->rotary_dim % 16 == 0) return dtype == GIE_HIP_FP16 ? launch_units<Fp16, void>(a, s) : launch_units<Bf16, void>(a, s);
   const long long heads = (q ? g->q_heads : 0) + 2 * g->kv_heads, grid = heads * g->total_tokens;
   if (grid * 64 > 0xffffffffll) return GIE_HIP_EUNSUPPORTED;  // a launch's threads
-  hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == GIE_HIP_FP16)
     hipLaunchKernelGGL(normed_rows_kernel<Fp16>, dim3(unsigned(grid)), dim3(64), 0, s, a, int(heads));
   else
