@@ -11,17 +11,20 @@ constexpr int kKvBlock = 16;  // positions of a head that share a scale
 // block's scale, which stays far inside FP32's range so.
 constexpr float kKvLeast = 0x1p-64f;
 
-// Codes: encode4 rounds four values (already divided by the scale, so within the largest code but for FP32's rounding)
-// to nearest even, byte by byte; decode4 gives bytes 0 and 2, and 1 and 3, as FP16 times 1 / kUnit, exactly (five
-// instructions in both types; bytes 0 and 1 together would take one or two more).
+// Codes: encode4 rounds four values to nearest even, byte by byte; they are already divided by the scale, so within the
+// largest code but for FP32's rounding, which does not reach the next step. decode4 gives bytes 0 and 2, and 1 and 3, as
+// FP16 times 1 / kUnit, exactly (five instructions in both types; bytes 0 and 1 together would take one or two more).
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 struct Int8Code {
   static constexpr float kUnit = 1.f;
   static __device__ __forceinline__ float scale(float most) { return fmaxf(most, kKvLeast) / 127.f; }
   static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
-    const auto one = [](float x) { return uint32_t(int(rintf(fminf(fmaxf(x, -127.f), 127.f)))) & 255u; };
-    return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+    // added to 1.5 2^23 a value is rounded to a whole number in the lowest bits
+    const auto whole = [](float x) { return __float_as_uint(x + 12582912.f); };
+    const uint32_t lo = __builtin_amdgcn_perm(whole(b), whole(a), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(whole(d), whole(c), 0x04000c0cu);
+    return lo | hi;
   }
   static __device__ __forceinline__ uint32_t encode1(float a) { return encode4(a, 0.f, 0.f, 0.f); }
   static __device__ __forceinline__ float decode1(uint32_t code) { return float(int8_t(code)); }
@@ -45,9 +48,8 @@ struct E4m3Code {
     return __uint_as_float(((bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u)) << 23);
   }
   static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
-    const auto in = [](float x) { return fminf(fmaxf(x, -448.f), 448.f); };
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(in(a), in(b), 0, false);
-    return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(in(c), in(d), r, true));
+    const int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true));
   }
   static __device__ __forceinline__ uint32_t encode1(float a) { return encode4(a, 0.f, 0.f, 0.f) & 255u; }
   static __device__ __forceinline__ float decode1(uint32_t code) {  // the NaN codes (0x7f, 0xff) become 480

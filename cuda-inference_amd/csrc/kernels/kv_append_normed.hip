@@ -194,24 +194,30 @@ __device__ __forceinline__ void load_unit(const uint16_t* head, const Unit& u, f
     x[8 + 2 * i] = E::to_f32(uint16_t(b[i])), x[9 + 2 * i] = E::to_f32(uint16_t(b[i] >> 16));
   }
 }
-__device__ __forceinline__ void load_weights(const float* w, const Unit& u, float (&x)[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = 1.f;
-  if (w == nullptr || !u.there) return;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = w[u.at + i], x[8 + i] = w[u.next + i];
-}
+// w: the weights in LDS (kept in registers they cost a third of the waves)
 template <int D>
-__device__ __forceinline__ void norm_unit(float (&x)[16], const float (&w)[16], float eps) {
+__device__ __forceinline__ void norm_unit(float (&x)[16], const float* w, const Unit& u, float eps) {
   float sum[2] = {};
 #pragma unroll
   for (int i = 0; i < 16; ++i) sum[i % 2] = __builtin_fmaf(x[i], x[i], sum[i % 2]);
   float all = sum[0] + sum[1];
 #pragma unroll
   for (int d = 1; d < kHeadLanes<D>; d <<= 1) all += __shfl_xor(all, d);
-  const float inv = 1.f / sqrtf(all * (1.f / D) + eps);
+  const float inv = __builtin_amdgcn_rsqf(all * (1.f / D) + eps);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = x[i] * inv * w[i];
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(w + (u.there ? (i < 2 ? u.at : u.next - 8) + 4 * i : 0));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * i + e] = x[4 * i + e] * inv * v[e];
+  }
+}
+// the weights of q's and k's norms, ones without one
+template <int D>
+__device__ __forceinline__ void stage_weights(const NormedArgs& a, float (*w)[D]) {
+  for (int i = int(threadIdx.x); i < 2 * D; i += int(blockDim.x)) {
+    const float* from = i < D ? a.q_norm : a.k_norm;
+    w[i / D][i % D] = from ? from[i % D] : 1.f;
+  }
 }
 template <bool INTERLEAVED>
 __device__ __forceinline__ void turn_unit(float (&x)[16], const float* cos, const float* sin) {
@@ -233,6 +239,7 @@ constexpr int kMostTokens = 8;  // of a workgroup
 template <typename E, bool INTERLEAVED, int D, bool ALL>
 __device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int count) {
   __shared__ Place places[kMostTokens];
+  __shared__ __attribute__((aligned(16))) float weights[2][D];
   const gie_paged_geom& g = a.g;
   constexpr int L = kHeadLanes<D>;
   const int tid = int(threadIdx.x), threads = int(blockDim.x);
@@ -241,9 +248,7 @@ __device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int cou
     if ((tid & 63) == 0) places[i] = p;
   }
   const Unit u = unit_of<INTERLEAVED, D>(tid % L, g.rotary_dim);
-  float wq[16], wk[16];
-  load_weights(a.q_norm, u, wq);
-  if (ALL) load_weights(a.k_norm, u, wk);
+  stage_weights<D>(a, weights);
   __syncthreads();
   const int q_heads = a.q ? g.q_heads : 0, heads = q_heads + (ALL ? 2 * g.kv_heads : 0), half = g.rotary_dim / 2;
 #pragma unroll 2
@@ -262,8 +267,8 @@ __device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int cou
                                (((long long)p.page * g.kv_heads + head) * g.page_size + p.slot) * D;
     float x[16];
     load_unit<E>(src, u, x);
-    if (is_q && a.q_norm) norm_unit<D>(x, wq, g.norm_eps);
-    if (ALL && !is_q && !is_v && a.k_norm) norm_unit<D>(x, wk, g.norm_eps);
+    if (is_q && a.q_norm) norm_unit<D>(x, weights[0], u, g.norm_eps);
+    if (ALL && !is_q && !is_v && a.k_norm) norm_unit<D>(x, weights[1], u, g.norm_eps);
     if (u.pairs && !is_v && p.position >= 0)
       turn_unit<INTERLEAVED>(x, a.cos + (long long)p.position * half + u.angle, a.sin + (long long)p.position * half + u.angle);
     if (!u.there) continue;
@@ -282,8 +287,13 @@ __device__ __forceinline__ void append_block(const NormedArgs& a, int slot) {
   constexpr int L = kHeadLanes<D>, T = 64 / L, kPasses = kKvBlock / T;  // T tokens at once
   const int tid = int(threadIdx.x), lane = tid & 63, half = g.rotary_dim / 2;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = int(blockDim.x) >> 6;
+  __shared__ __attribute__((aligned(16))) float weights[2][D];
   const Block b = block_of(g, a.q_starts, a.seq_lens, a.page_table, slot);
   if (b.first >= b.end || b.page < 0) return;
+  if (a.k_norm) {
+    stage_weights<D>(a, weights);
+    __syncthreads();
+  }
   const Unit u = unit_of<INTERLEAVED, D>(lane % L, g.rotary_dim), straight = {lane % L * 16, lane % L * 16 + 8, 0, u.there, false};
   for (int item = wave; item < 2 * g.kv_heads; item += waves) {
     const bool is_v = item >= g.kv_heads;
@@ -297,8 +307,6 @@ __device__ __forceinline__ void append_block(const NormedArgs& a, int slot) {
     const float before = starts ? 0.f : *scale_at;
     const Unit w = is_v ? straight : u;
     float x[kPasses][16];
-    float most = 0.f;
-    bool finite = true;
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int position = b.start + p * T + lane / L;
@@ -310,26 +318,24 @@ __device__ __forceinline__ void append_block(const NormedArgs& a, int slot) {
       load_unit<E>(src + (position - b.first) * stride, w, x[p]);
     }
     if (!is_v && (a.k_norm || half > 0)) {
-      float wk[16];
-      load_weights(a.k_norm, u, wk);
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
         const int position = b.start + p * T + lane / L;
         if (position < b.first || position >= b.end) continue;
-        if (a.k_norm) norm_unit<D>(x[p], wk, g.norm_eps);
+        if (a.k_norm) norm_unit<D>(x[p], weights[1], u, g.norm_eps);
         if (u.pairs)
           turn_unit<INTERLEAVED>(x[p], a.cos + (long long)position * half + u.angle, a.sin + (long long)position * half + u.angle);
       }
     }
+    unsigned bits = 0;  // of the largest |x|: infinities and NaNs are larger than all numbers
 #pragma unroll
     for (int p = 0; p < kPasses; ++p)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        most = fmaxf(most, fabsf(x[p][i]));
-        finite = finite && fabsf(x[p][i]) <= 3.402823466e38f;
-      }
-    most = wave_max(most);
-    if (__any(!finite) || !(before == before)) {
+      for (int i = 0; i < 16; ++i) bits = max(bits, __float_as_uint(x[p][i]) & 0x7fffffffu);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) bits = max(bits, unsigned(__shfl_xor(int(bits), d)));
+    const float most = __uint_as_float(bits);
+    if (bits >= 0x7f800000u || !(before == before)) {
       if (lane == 0) *scale_at = __builtin_nanf("");
       continue;
     }
