@@ -280,13 +280,13 @@ __device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int cou
   }
 }
 
-// block `slot` of the batch's: a wave for each head of k and v
+// block `slot` of the batch's: a wave for each head of k and v, from `first_item` on
 template <typename E, typename C, bool INTERLEAVED, int D>
-__device__ __forceinline__ void append_block(const NormedArgs& a, int slot) {
+__device__ __forceinline__ void append_block(const NormedArgs& a, int slot, int first_item) {
   const gie_paged_geom& g = a.g;
   constexpr int L = kHeadLanes<D>, T = 64 / L, kPasses = kKvBlock / T;  // T tokens at once
   const int tid = int(threadIdx.x), lane = tid & 63, half = g.rotary_dim / 2;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = int(blockDim.x) >> 6;
+  const int item = first_item + __builtin_amdgcn_readfirstlane(tid >> 6);
   __shared__ __attribute__((aligned(16))) float weights[2][D];
   const Block b = block_of(g, a.q_starts, a.seq_lens, a.page_table, slot);
   if (b.first >= b.end || b.page < 0) return;
@@ -295,7 +295,7 @@ __device__ __forceinline__ void append_block(const NormedArgs& a, int slot) {
     __syncthreads();
   }
   const Unit u = unit_of<INTERLEAVED, D>(lane % L, g.rotary_dim), straight = {lane % L * 16, lane % L * 16 + 8, 0, u.there, false};
-  for (int item = wave; item < 2 * g.kv_heads; item += waves) {
+  if (item < 2 * g.kv_heads) {
     const bool is_v = item >= g.kv_heads;
     const int head = is_v ? item - g.kv_heads : item;
     const long long stride = is_v ? g.v_stride : g.k_stride;
@@ -337,7 +337,7 @@ __device__ __forceinline__ void append_block(const NormedArgs& a, int slot) {
     const float most = __uint_as_float(bits);
     if (bits >= 0x7f800000u || !(before == before)) {
       if (lane == 0) *scale_at = __builtin_nanf("");
-      continue;
+      return;
     }
     const float scale = fmaxf(before, C::scale(most)), inv = 1.f / scale;
     const bool grows = !starts && scale > before;
@@ -370,16 +370,16 @@ __device__ __forceinline__ void append_block(const NormedArgs& a, int slot) {
   }
 }
 
-// C void: pages in the tokens' type
+// C void: pages in the tokens' type. Otherwise the first `blocks` workgroups take blocks, `parts` of them one block's heads.
 template <typename E, typename C, bool INTERLEAVED, int D>
-__global__ __launch_bounds__(512) void append_kernel(NormedArgs a, int slots, int tokens) {
+__global__ __launch_bounds__(512) void append_kernel(NormedArgs a, int blocks, int parts, int tokens) {
   int id = int(blockIdx.x);
   if constexpr (!std::is_void<C>::value) {
-    if (id < slots) {
-      append_block<E, C, INTERLEAVED, D>(a, id);
+    if (id < blocks) {
+      append_block<E, C, INTERLEAVED, D>(a, id / parts, id % parts * (int(blockDim.x) >> 6));
       return;
     }
-    id -= slots;
+    id -= blocks;
   }
   append_rows<E, INTERLEAVED, D, std::is_void<C>::value>(a, id * tokens, min(tokens, a.g.total_tokens - id * tokens));
 }
@@ -393,11 +393,13 @@ int launch_units(const NormedArgs& a, hipStream_t s) {
   // one token for each workgroup spreads a step of few tokens; of many, as many as give every lane two heads
   long long tokens = g.total_tokens < 1024 || work == 0 ? 1 : 1024 / work;
   tokens = tokens < 1 ? 1 : tokens > kMostTokens ? kMostTokens : tokens;
-  const long long slots = k8 ? block_slots(g) : 0, rows = heads == 0 ? 0 : (g.total_tokens + tokens - 1) / tokens;
+  const long long rows = heads == 0 ? 0 : (g.total_tokens + tokens - 1) / tokens;
   long long threads = (work * tokens + (tokens > 1 ? 127 : 63)) / (tokens > 1 ? 128 : 64) * 64;
-  if (k8 && threads < 2ll * g.kv_heads * 64) threads = 2ll * g.kv_heads * 64;  // a wave for each head's block
   if (threads > 512) threads = 512;
-  if ((slots + rows) * threads > 0xffffffffll || slots > 0x3fffffff) return GIE_HIP_EUNSUPPORTED;  // a launch's threads
+  // blocks are a wave's work each: four waves to a workgroup spread them
+  if (k8) threads = 256;
+  const long long parts = (2ll * g.kv_heads + threads / 64 - 1) / (threads / 64), blocks = k8 ? block_slots(g) * parts : 0;
+  if ((blocks + rows) * threads > 0xffffffffll) return GIE_HIP_EUNSUPPORTED;  // a launch's threads
   const auto kernel = [&](auto interleaved) {
     constexpr bool I = decltype(interleaved)::value;
     switch (D) {
@@ -407,8 +409,8 @@ int launch_units(const NormedArgs& a, hipStream_t s) {
       default: return append_kernel<E, C, I, 256>;
     }
   };
-  hipLaunchKernelGGL(g.interleaved ? kernel(std::true_type{}) : kernel(std::false_type{}), dim3(unsigned(slots + rows)),
-                     dim3(unsigned(threads)), 0, s, a, int(slots), int(tokens));
+  hipLaunchKernelGGL(g.interleaved ? kernel(std::true_type{}) : kernel(std::false_type{}), dim3(unsigned(blocks + rows)),
+                     dim3(unsigned(threads)), 0, s, a, int(blocks), int(parts), int(tokens));
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? GIE_HIP_OK : int(e);
 }
