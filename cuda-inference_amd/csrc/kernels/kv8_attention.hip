@@ -11,6 +11,8 @@
 // registers: ks is a factor of the exponent, vs a term of it, x_j = s_j log2(e) + log2(vs_j). The weight 2^(x_j - m) that
 // the second product takes has vs in it, and m is the maximum of x: weights keep their bits however much the blocks'
 // sizes differ. The sum of p_j takes 1 / vs once for each block.
+#include <type_traits>
+
 #include "attention_common.h"
 #include "kv8_common.h"
 
@@ -115,18 +117,25 @@ __device__ __forceinline__ u32x2 pack_out(bool bf16, f32x4 v) {
 // The maximum is not looked for ahead of the weights (27 of about 150 vector instructions): they are taken against what
 // is there, and as long as a lane's sum of them stays within 2^15 all of them fit FP16. Only where it does not, or a row
 // has seen nothing yet, the rows' maxima move and the weights are taken again.
-template <bool LARGE_CAP, int DT, typename Seen>
-__device__ __forceinline__ void weigh(const AttnArgs& a, f32x16& s, const BlockScales (&sc)[2], float row_factor,
-                                      bool masked, Seen seen, float& m, float& mc, float& l, f32x16 (&o)[DT]) {
-  const auto within = [](float f) { return __builtin_amdgcn_fmed3f(f, 0x1p-126f, 3e38f); };  // masked: no -inf times 0
-  float f[2] = {within(row_factor * sc[0].f), within(row_factor * sc[1].f)};
+template <bool LARGE_CAP, typename Seen>
+__device__ __forceinline__ void cap_and_mask(const AttnArgs& a, f32x16& s, const BlockScales (&sc)[2], float row_factor,
+                                             bool masked, Seen seen, float (&f)[2]) {
+  const auto within = [](float x) { return __builtin_amdgcn_fmed3f(x, 0x1p-126f, 3e38f); };  // masked: no -inf times 0
+  f[0] = within(row_factor * sc[0].f);
+  f[1] = within(row_factor * sc[1].f);
   if (LARGE_CAP || a.cap > 0) {
+    if constexpr (LARGE_CAP) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] *= f[i / 8];
-    if constexpr (LARGE_CAP)
+      for (int i = 0; i < 16; ++i) s[i] *= f[i / 8];
       cap_products(a, s);
-    else
-      cap_scores(a, s);
+    } else {  // cap_scores with the block's factor in the exponent's
+      const float in[2] = {fminf(f[0] * a.cap_in, 3e38f), fminf(f[1] * a.cap_in, 3e38f)};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(s[i] * in[i / 8]);
+        s[i] = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(e + 1.f);
+      }
+    }
     f[0] = f[1] = a.mult;
   }
   if (__any(!(sc[0].f == sc[0].f) || !(sc[1].f == sc[1].f))) {
@@ -142,22 +151,25 @@ __device__ __forceinline__ void weigh(const AttnArgs& a, f32x16& s, const BlockS
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = seen(i) ? s[i] : -INFINITY;
   }
+}
+struct Weights {
   f32x16 w;
-  float sum[2];
-  const auto take = [&] {
+  float c[2], sum[2][2];
+  __device__ __forceinline__ void begin(const BlockScales (&sc)[2], float mc) { c[0] = sc[0].lv - mc, c[1] = sc[1].lv - mc; }
+  __device__ __forceinline__ void take(const f32x16& s, const float (&f)[2], int i) {
+    const int g = i / 8;
+    w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], f[g], c[g]));
+    sum[g][i % 2] = i % 8 < 2 ? w[i] : sum[g][i % 2] + w[i];
+  }
+  __device__ __forceinline__ void take_all(const f32x16& s, const float (&f)[2]) {
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const float c = sc[g].lv - mc;
-      float part[2];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[8 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * g + i], f[g], c));
-        part[i % 2] = i < 2 ? w[8 * g + i] : part[i % 2] + w[8 * g + i];
-      }
-      sum[g] = part[0] + part[1];
-    }
-  };
-  take();
+    for (int i = 0; i < 16; ++i) take(s, f, i);
+  }
+};
+template <int DT>
+__device__ __forceinline__ void settle(Weights& w, const f32x16& s, const float (&f)[2], const BlockScales (&sc)[2],
+                                       float& m, float& mc, float& l, f32x16 (&o)[DT]) {
+  float sum[2] = {w.sum[0][0] + w.sum[0][1], w.sum[1][0] + w.sum[1][1]};
   if (__any(!(sum[0] + sum[1] <= 0x1p15f) || m == -INFINITY)) {
     float top = -INFINITY;
 #pragma unroll
@@ -176,11 +188,24 @@ __device__ __forceinline__ void weigh(const AttnArgs& a, f32x16& s, const BlockS
     l *= keep;
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] *= keep;
-    take();
+    w.begin(sc, mc);
+    w.take_all(s, f);
+    sum[0] = w.sum[0][0] + w.sum[0][1];
+    sum[1] = w.sum[1][0] + w.sum[1][1];
   }
   l = __builtin_fmaf(sum[0], sc[0].inv, l);
   l = __builtin_fmaf(sum[1], sc[1].inv, l);
-  s = w;
+}
+template <bool LARGE_CAP, int DT, typename Seen>
+__device__ __forceinline__ void weigh(const AttnArgs& a, f32x16& s, const BlockScales (&sc)[2], float row_factor,
+                                      bool masked, Seen seen, float& m, float& mc, float& l, f32x16 (&o)[DT]) {
+  float f[2];
+  cap_and_mask<LARGE_CAP>(a, s, sc, row_factor, masked, seen, f);
+  Weights w;
+  w.begin(sc, mc);
+  w.take_all(s, f);
+  settle(w, s, f, sc, m, mc, l, o);
+  s = w.w;
 }
 
 // ---------------------------------------------------------------- few rows: 32 for each workgroup
@@ -594,6 +619,72 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
     }
   };
 
+  // One part of a tile, half of a tile's work: the weights of scores that are there (s), under them the scores of the part
+  // after it, then the values, under them codes of the next tile.
+  const auto step = [&](int tile, auto part, f32x16& s) {
+    constexpr int n = decltype(part)::value;
+    const int stage = tile & 1, k_stage = n == 0 ? stage : stage ^ 1;
+    const int at = key_of(tile) + n * 32, oldest = a.window > 0 ? pos - a.window : -1;
+    if (n == 0) store_scales(stage ^ 1);
+    u32x4 kf[KS], vf[2][DT];
+    {
+      unsigned ko = k_rd + unsigned(k_stage * kStage + (n ^ 1) * 32 * P);
+      asm volatile("" : "+v"(ko));
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const lds_v4*>(size_t(ko ^ unsigned(ks * 32)));
+    }
+    BlockScales sc[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const f32x4 c = *reinterpret_cast<const lds_f4*>(size_t(lds0 + unsigned(kConst + (stage * WR + 2 * n + g) * 16)));
+      sc[g] = {c[0], c[1], c[2]};
+    }
+    const auto read_v = [&](int h) {
+      unsigned vo = v_rd + unsigned(stage * kStage);
+      asm volatile("" : "+v"(vo));
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const unsigned p = (vo ^ unsigned(d * 64)) + unsigned((2 * n + h) * 16 * P);
+        const u32x2 x = read_transposed(p), y = read_transposed(p + unsigned(8 * P));
+        vf[h][d] = u32x4{x.x, x.y, y.x, y.y};
+      }
+    };
+    const bool masked =
+        at + 31 > wpos_first || (a.window > 0 && at <= wpos_last - a.window) || wpos_last >= a.capacity;
+    const auto seen = [&](int i) { return sees(a, at + 8 * (i / 4) + 4 * half + i % 4, pos, oldest); };
+    float f[2];
+    cap_and_mask<LARGE_CAP>(a, s, sc, row_factor, masked, seen, f);
+    Weights w;
+    w.begin(sc, mc);
+    f32x16 after = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      after = Fp16::mfma32(kf[ks], qf[ks], after);
+#pragma unroll
+      for (int i = ks * 16 / KS; i < (ks + 1) * 16 / KS; ++i) w.take(s, f, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    read_v(0);
+    settle(w, s, f, sc, m, mc, l, o);
+    u32x4 pf[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      pf[h] = u32x4{Fp16::pack2(w.w[8 * h], w.w[8 * h + 1]), Fp16::pack2(w.w[8 * h + 2], w.w[8 * h + 3]),
+                    Fp16::pack2(w.w[8 * h + 4], w.w[8 * h + 5]), Fp16::pack2(w.w[8 * h + 6], w.w[8 * h + 7])};
+    read_v(1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        o[d] = Fp16::mfma32(vf[h][d], pf[h], o[d]);
+#pragma unroll
+        for (int u = (h * DT + d) * kHalf / DT; u < (h * DT + d + 1) * kHalf / DT; ++u) decode_unit(n, u, stage ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    load(tile + 2, n);
+    s = after;
+  };
+
   // ---- main loop: tile j from stage j % 2; tile j + 1 is decoded into the other one and j + 2 requested under it ----
   load(0, 0);
   load(0, 1);
@@ -621,9 +712,23 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
     for (int u = 0; u < 2 * kHalf; ++u) decode_unit(n, u, 0);
     load(1, n);
   }
-  for (int j = 0; j < tiles; ++j) {
+  if constexpr (WD == 1) {
     stage_barrier();
-    compute(j, j & 1);
+    f32x16 s = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      s = Fp16::mfma32(*reinterpret_cast<const lds_v4*>(size_t(k_rd ^ unsigned(ks * 32))), qf[ks], s);
+    for (int j = 0; j < tiles; ++j) {
+      step(j, std::integral_constant<int, 0>{}, s);
+      stage_barrier();
+      step(j, std::integral_constant<int, 1>{}, s);
+      stage_barrier();
+    }
+  } else {
+    for (int j = 0; j < tiles; ++j) {
+      stage_barrier();
+      compute(j, j & 1);
+    }
   }
   l = swap_add(l);
 
