@@ -19,6 +19,8 @@
 namespace gie_hip {
 namespace {
 
+typedef __attribute__((address_space(3))) float lds_float;
+
 struct Kv8Args : AttnArgs {
   const uint8_t* k_pages;
   const uint8_t* v_pages;
@@ -165,21 +167,25 @@ struct Weights {
 #pragma unroll
     for (int i = 0; i < 16; ++i) take(s, f, i);
   }
-};
-template <int DT>
-__device__ __forceinline__ void settle(Weights& w, const f32x16& s, const float (&f)[2], const BlockScales (&sc)[2],
-                                       float& m, float& mc, float& l, f32x16 (&o)[DT]) {
-  float sum[2] = {w.sum[0][0] + w.sum[0][1], w.sum[1][0] + w.sum[1][1]};
-  if (__any(!(sum[0] + sum[1] <= 0x1p15f) || m == -INFINITY)) {
-    float top = -INFINITY;
+  __device__ __forceinline__ bool overflows() const {
+    return !((sum[0][0] + sum[0][1]) + (sum[1][0] + sum[1][1]) <= 0x1p15f);  // (or a NaN)
+  }
+  // the scores' largest exponent, the same in both halves of the wave
+  __device__ __forceinline__ float top(const f32x16& s, const float (&f)[2], const BlockScales (&sc)[2]) const {
+    float t = -INFINITY;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       float most = s[8 * g];
 #pragma unroll
       for (int i = 1; i < 8; ++i) most = fmaxf(most, s[8 * g + i]);
-      top = fmaxf(top, __builtin_fmaf(most, f[g], sc[g].lv));
+      t = fmaxf(t, __builtin_fmaf(most, f[g], sc[g].lv));
     }
-    const float next = fmaxf(m, swap_max(top));
+    return swap_max(t);
+  }
+  // a row's maximum to what it is with `top`
+  template <int DT>
+  static __device__ __forceinline__ void move(float top, float& m, float& mc, float& l, f32x16 (&o)[DT]) {
+    const float next = fmaxf(m, top);
     float nc = next == -INFINITY ? 0.f : next;
     nc += __builtin_fmaf(fabsf(nc), 0x1p-22f, -kLift);  // (what rounding takes from it and from an exponent)
     const float keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - nc);  // 1: nothing summed yet
@@ -188,24 +194,26 @@ __device__ __forceinline__ void settle(Weights& w, const f32x16& s, const float 
     l *= keep;
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] *= keep;
+  }
+  __device__ __forceinline__ void add_to(float& l, const BlockScales (&sc)[2]) const {
+    l = __builtin_fmaf(sum[0][0] + sum[0][1], sc[0].inv, l);
+    l = __builtin_fmaf(sum[1][0] + sum[1][1], sc[1].inv, l);
+  }
+  // of one block, in the order of its keys
+  __device__ __forceinline__ u32x4 packed(int h) const {
+    return u32x4{Fp16::pack2(w[8 * h], w[8 * h + 1]), Fp16::pack2(w[8 * h + 2], w[8 * h + 3]),
+                 Fp16::pack2(w[8 * h + 4], w[8 * h + 5]), Fp16::pack2(w[8 * h + 6], w[8 * h + 7])};
+  }
+};
+template <int DT>
+__device__ __forceinline__ void settle(Weights& w, const f32x16& s, const float (&f)[2], const BlockScales (&sc)[2],
+                                       float& m, float& mc, float& l, f32x16 (&o)[DT]) {
+  if (__any(w.overflows() || m == -INFINITY)) {
+    w.move(w.top(s, f, sc), m, mc, l, o);
     w.begin(sc, mc);
     w.take_all(s, f);
-    sum[0] = w.sum[0][0] + w.sum[0][1];
-    sum[1] = w.sum[1][0] + w.sum[1][1];
   }
-  l = __builtin_fmaf(sum[0], sc[0].inv, l);
-  l = __builtin_fmaf(sum[1], sc[1].inv, l);
-}
-template <bool LARGE_CAP, int DT, typename Seen>
-__device__ __forceinline__ void weigh(const AttnArgs& a, f32x16& s, const BlockScales (&sc)[2], float row_factor,
-                                      bool masked, Seen seen, float& m, float& mc, float& l, f32x16 (&o)[DT]) {
-  float f[2];
-  cap_and_mask<LARGE_CAP>(a, s, sc, row_factor, masked, seen, f);
-  Weights w;
-  w.begin(sc, mc);
-  w.take_all(s, f);
-  settle(w, s, f, sc, m, mc, l, o);
-  s = w.w;
+  w.add_to(l, sc);
 }
 
 // ---------------------------------------------------------------- few rows: 32 for each workgroup
@@ -340,11 +348,17 @@ __global__ __launch_bounds__(64 * WK, WK == 8 ? 2 : 1) void narrow_kernel(Kv8Arg
       for (int d = 0; d < DT; ++d) vr[g][d] = read_transposed8(((v_rd + so) ^ unsigned(d * 32)) + unsigned(g * kGran));
     const bool masked = at + TT - 1 > pos_first || (a.window > 0 && at <= pos_last - a.window) || pos_last >= a.capacity;
     const auto seen = [&](int i) { return sees(a, at + 8 * (i / 4) + 4 * half + i % 4, pos, oldest); };
-    weigh<LARGE_CAP>(a, s, pair.g, row_factor, masked, seen, m, mc, l, o);
+    float f[2];
+    cap_and_mask<LARGE_CAP>(a, s, pair.g, row_factor, masked, seen, f);
+    Weights w;
+    w.begin(pair.g, mc);
+    w.take_all(s, f);
+    settle(w, s, f, pair.g, m, mc, l, o);
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const u32x4 pf = {Fp16::pack2(s[8 * g], s[8 * g + 2]), Fp16::pack2(s[8 * g + 1], s[8 * g + 3]),
-                        Fp16::pack2(s[8 * g + 4], s[8 * g + 6]), Fp16::pack2(s[8 * g + 5], s[8 * g + 7])};
+    for (int g = 0; g < 2; ++g) {  // in decode8's order of the keys
+      const f32x16& p = w.w;
+      const u32x4 pf = {Fp16::pack2(p[8 * g], p[8 * g + 2]), Fp16::pack2(p[8 * g + 1], p[8 * g + 3]),
+                        Fp16::pack2(p[8 * g + 4], p[8 * g + 6]), Fp16::pack2(p[8 * g + 5], p[8 * g + 7])};
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] = Fp16::mfma32(decode8<C>(vr[g][d].x, vr[g][d].y), pf, o[d]);
     }
@@ -433,6 +447,8 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
   constexpr int KS = D / 16, DT = D / 32 / WD, kTileB = TT * P, kStage = 2 * kTileB;
   constexpr int kPieces = D, JP = (kPieces + 63) / 64;  // 16-byte pieces of a granule's codes, of a lane
   constexpr int kConst = 2 * kStage;                    // [stage][granule] BlockScales
+  // WD == 2: weights [wave][block of 16][lane], whether a wave's maxima move [wave], maxima [wave][row]
+  constexpr int kExchange = kConst + 2 * WR * 16, kFlags = kExchange + 2 * WR * 2048, kTops = kFlags + 2 * WR * 4;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = int(threadIdx.x), lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave % WR, wd = wave / WR;
@@ -535,87 +551,107 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
   float m = -INFINITY, mc = 0.f, l = 0.f;
   float row_factor = 1.f;
 
-  const auto compute = [&](int tile, int stage) {
+  // WD == 2: a tile by the two waves of the same rows. Each works out the scores of one part's keys and their weights; they
+  // exchange the weights through LDS (and, when one of the workgroup's maxima has to move, the maxima first) and sum their
+  // halves of the values over both parts. l is a wave's own part of the sum until the end.
+  const auto pair_tile = [&](int tile, auto stage_of) {
+    const int stage = stage_of;
     const unsigned so = unsigned(stage * kStage);
-    const int at0 = key_of(tile), oldest = a.window > 0 ? pos - a.window : -1;
+    const int at = key_of(tile) + wd * 32, oldest = a.window > 0 ? pos - a.window : -1;
     store_scales(stage ^ 1);
-    constexpr bool kAhead = WD == 1;  // where the registers hold it
-    u32x4 kf[KS];
-    const auto read_k = [&](int n) {
-      unsigned ko = k_rd + so;
-      asm volatile("" : "+v"(ko));  // the permuted addresses are worked out for every part: kept, they cost registers
+    f32x16 s = {};
+    {
+      u32x4 kf[8];
+      unsigned ko = k_rd + so + unsigned(wd * 32 * P);
+      asm volatile("" : "+v"(ko));  // the permuted addresses are worked out for every tile: kept, they cost registers
+      const auto read_4 = [&](int g) {  // four steps ahead
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        kf[ks] = *reinterpret_cast<const lds_v4*>(size_t((ko ^ unsigned(ks * 32)) + unsigned(n * 32 * P)));
-    };
-    if (kAhead) read_k(0);
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      const int at = at0 + n * 32;
-      f32x16 s = {};
-      if constexpr (kAhead) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          s = Fp16::mfma32(kf[ks], qf[ks], s);
-#pragma unroll
-          for (int u = ks * 2 * kHalf / KS; u < (ks + 1) * 2 * kHalf / KS; ++u) decode_unit(n, u, stage ^ 1);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      } else {  // four steps ahead
-        unsigned ko = k_rd + so;
-        asm volatile("" : "+v"(ko));
-        const auto read_4 = [&](int g) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            kf[g % 2 * 4 + i] =
-                *reinterpret_cast<const lds_v4*>(size_t((ko ^ unsigned((g * 4 + i) * 32)) + unsigned(n * 32 * P)));
-        };
-        read_4(0);
-#pragma unroll
-        for (int g = 0; g < KS / 4; ++g) {
-          if (g + 1 < KS / 4) read_4(g + 1);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s = Fp16::mfma32(kf[g % 2 * 4 + i], qf[g * 4 + i], s);
-#pragma unroll
-          for (int u = g * 2 * kHalf * 4 / KS; u < (g + 1) * 2 * kHalf * 4 / KS; ++u) decode_unit(n, u, stage ^ 1);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-      load(tile + 2, n);
-      BlockScales sc[2];
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const f32x4 c = *reinterpret_cast<const lds_f4*>(size_t(lds0 + unsigned(kConst + (stage * WR + 2 * n + g) * 16)));
-        sc[g] = {c[0], c[1], c[2]};
-      }
-      u32x4 vf[2][DT];
-      const auto read_v = [&](int h) {
-        unsigned vo = v_rd + so;
-        asm volatile("" : "+v"(vo));
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const unsigned p = (vo ^ unsigned(d * 64)) + unsigned((2 * n + h) * 16 * P);
-          const u32x2 x = read_transposed(p), y = read_transposed(p + unsigned(8 * P));
-          vf[h][d] = u32x4{x.x, x.y, y.x, y.y};
-        }
+        for (int i = 0; i < 4; ++i)
+          kf[g % 2 * 4 + i] = *reinterpret_cast<const lds_v4*>(size_t(ko ^ unsigned((g * 4 + i) * 32)));
       };
-      read_v(0);
-      const bool masked =
-          at + 31 > wpos_first || (a.window > 0 && at <= wpos_last - a.window) || wpos_last >= a.capacity;
-      const auto seen = [&](int i) { return sees(a, at + 8 * (i / 4) + 4 * half + i % 4, pos, oldest); };
-      weigh<LARGE_CAP>(a, s, sc, row_factor, masked, seen, m, mc, l, o);
-      u32x4 pf[2];
+      read_4(0);
+      constexpr int kUnits = 4 * kHalf, G = KS / 4;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        pf[h] = u32x4{Fp16::pack2(s[8 * h], s[8 * h + 1]), Fp16::pack2(s[8 * h + 2], s[8 * h + 3]),
-                      Fp16::pack2(s[8 * h + 4], s[8 * h + 5]), Fp16::pack2(s[8 * h + 6], s[8 * h + 7])};
-      read_v(1);
-      if (kAhead && n + 1 < NS) read_k(n + 1);
+      for (int g = 0; g < G; ++g) {
+        if (g + 1 < G) read_4(g + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < 4; ++i) s = Fp16::mfma32(kf[g % 2 * 4 + i], qf[g * 4 + i], s);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = Fp16::mfma32(vf[h][d], pf[h], o[d]);
+        for (int u = g * kUnits / G; u < (g + 1) * kUnits / G; ++u) decode_unit(u / (2 * kHalf), u % (2 * kHalf), stage ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    load(tile + 2, 0);
+    load(tile + 2, 1);
+    BlockScales sc[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const f32x4 c = *reinterpret_cast<const lds_f4*>(size_t(lds0 + unsigned(kConst + (stage * WR + 2 * wd + g) * 16)));
+      sc[g] = {c[0], c[1], c[2]};
+    }
+    // V: granules of this wave's own part first
+    u32x4 vf[2][DT];
+    const auto read_v = [&](int k) {
+      unsigned vo = v_rd + so + unsigned((k / 2 == 0 ? wd : wd ^ 1) * 32 * P);
+      asm volatile("" : "+v"(vo));
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const unsigned p = (vo ^ unsigned(d * 64)) + unsigned(k % 2 * 16 * P);
+        const u32x2 x = read_transposed(p), y = read_transposed(p + unsigned(8 * P));
+        vf[k % 2][d] = u32x4{x.x, x.y, y.x, y.y};
+      }
+    };
+    read_v(0);
+    const bool masked = at + 31 > wpos_first || (a.window > 0 && at <= wpos_last - a.window) || wpos_last >= a.capacity;
+    const auto seen = [&](int i) { return sees(a, at + 8 * (i / 4) + 4 * half + i % 4, pos, oldest); };
+    float f[2];
+    cap_and_mask<LARGE_CAP>(a, s, sc, row_factor, masked, seen, f);
+    Weights w;
+    w.begin(sc, mc);
+    w.take_all(s, f);
+    u32x4 pf[2];
+    const unsigned exchange = lds0 + unsigned(kExchange + lane * 16), flags = lds0 + unsigned(kFlags);
+    const auto give = [&] {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        pf[h] = w.packed(h);
+        *reinterpret_cast<lds_v4*>(size_t(exchange + unsigned(wave * 2048 + h * 1024))) = pf[h];
+      }
+    };
+    give();
+    const bool moves = w.overflows() || m == -INFINITY;
+    const int any_moves = __any(moves);
+    if (lane == 0) *reinterpret_cast<lds_i*>(size_t(flags + unsigned(wave * 4))) = any_moves;
+    stage_barrier();
+    int all_moves = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const u32x4 x = *reinterpret_cast<const lds_v4*>(size_t(flags + unsigned(i * 16)));
+      all_moves |= int(x.x | x.y | x.z | x.w);
+    }
+    if (__builtin_amdgcn_readfirstlane(all_moves) != 0) {  // the same in all waves
+      const float top = w.top(s, f, sc);
+      const unsigned tops = lds0 + unsigned(kTops + (lane & 31) * 4);
+      *reinterpret_cast<lds_float*>(size_t(tops + unsigned(wave * 128))) = top;
+      stage_barrier();
+      const float other = *reinterpret_cast<const lds_float*>(size_t(tops + unsigned((wave ^ WR) * 128)));
+      w.move(fmaxf(top, other), m, mc, l, o);
+      w.begin(sc, mc);
+      w.take_all(s, f);
+      give();
+      stage_barrier();
+    }
+    w.add_to(l, sc);
+    u32x4 of[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      of[h] = *reinterpret_cast<const lds_v4*>(size_t(exchange + unsigned((wave ^ WR) * 2048 + h * 1024)));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (k < 3) read_v(k + 1);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] = Fp16::mfma32(vf[k % 2][d], k < 2 ? pf[k] : of[k - 2], o[d]);
     }
   };
 
@@ -666,11 +702,7 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
     }
     read_v(0);
     settle(w, s, f, sc, m, mc, l, o);
-    u32x4 pf[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      pf[h] = u32x4{Fp16::pack2(w.w[8 * h], w.w[8 * h + 1]), Fp16::pack2(w.w[8 * h + 2], w.w[8 * h + 3]),
-                    Fp16::pack2(w.w[8 * h + 4], w.w[8 * h + 5]), Fp16::pack2(w.w[8 * h + 6], w.w[8 * h + 7])};
+    const u32x4 pf[2] = {w.packed(0), w.packed(1)};
     read_v(1);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -727,10 +759,17 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
   } else {
     for (int j = 0; j < tiles; ++j) {
       stage_barrier();
-      compute(j, j & 1);
+      pair_tile(j, j & 1);
     }
   }
   l = swap_add(l);
+  if constexpr (WD == 2) {  // the waves' parts of the sum
+    const unsigned sums = lds0 + unsigned(kTops + (lane & 31) * 4);
+    stage_barrier();
+    *reinterpret_cast<lds_float*>(size_t(sums + unsigned(wave * 128))) = l;
+    stage_barrier();
+    l += *reinterpret_cast<const lds_float*>(size_t(sums + unsigned((wave ^ WR) * 128)));
+  }
 
   // ---- rows to out, or to the parts that are joined: through LDS, so that a store covers whole lines of a row ----
   // where the lane's rows go, worked out again here: kept from above it would cost registers in the loop
@@ -811,7 +850,8 @@ int launch(const Kv8Args& a, const Shape& s, hipStream_t stream) {
   int rc;
   if (s.wide) {
     constexpr int WD = D == 256 ? 2 : 1, WR = kWideRows / 32;
-    constexpr int bytes = 2 * 2 * kWideKeys * kPitch<D> + 2 * WR * 16, rows = WR * WD * 32 * (D / WD * 2 + 16);
+    constexpr int exchange = WD == 1 ? 0 : WR * WD * (2048 + 4 + 128);
+    constexpr int bytes = 2 * 2 * kWideKeys * kPitch<D> + 2 * WR * 16 + exchange, rows = WR * WD * 32 * (D / WD * 2 + 16);
     static_assert(rows <= bytes && WR * WD * 32 * 144 <= bytes, "rows on their way out fit the stages");
     rc = start(wide_kernel<C, D, WD, LARGE_CAP>, grid, 256 * WD, bytes, stream, a);
   } else {
