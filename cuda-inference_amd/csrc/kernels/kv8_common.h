@@ -26,7 +26,6 @@ struct Int8Code {
     const uint32_t hi = __builtin_amdgcn_perm(whole(d), whole(c), 0x04000c0cu);
     return lo | hi;
   }
-  static __device__ __forceinline__ uint32_t encode1(float a) { return encode4(a, 0.f, 0.f, 0.f); }
   static __device__ __forceinline__ float decode1(uint32_t code) { return float(int8_t(code)); }
   static __device__ __forceinline__ u32x2 decode4(uint32_t w) {
     // code + 128 as the low bits of 1024, less 1152
@@ -51,7 +50,6 @@ struct E4m3Code {
     const int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true));
   }
-  static __device__ __forceinline__ uint32_t encode1(float a) { return encode4(a, 0.f, 0.f, 0.f) & 255u; }
   static __device__ __forceinline__ float decode1(uint32_t code) {  // the NaN codes (0x7f, 0xff) become 480
     return float(__builtin_bit_cast(_Float16, uint16_t((code & 0x80u) << 8 | (code & 0x7fu) << 7))) * kUnit;
   }

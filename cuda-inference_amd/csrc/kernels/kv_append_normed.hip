@@ -8,7 +8,8 @@
 // spreads all their heads over its lanes. Blocks of 8-bit pages go by position: a wave has one head's whole block, up to
 // 16 tokens, in registers, so that the scale is the largest of them and every code is written once. Both parts are
 // workgroups of one launch.
-// Heads whose rotating part is no multiple of 16 take a form that goes value by value.
+// A rotating part that is no multiple of 16 does not fall into such pieces: there a lane has 16 values side by side and
+// finds the other one of a pair through LDS.
 #include <cmath>
 #include <type_traits>
 
@@ -36,152 +37,27 @@ struct NormedArgs {
   float* v_scales;
 };
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-  return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
-}
-
-// One head by one wave: values lane, lane + 64, ... normed (w not null) and turned (position >= 0) in x; `row` is LDS of
-// the wave's own for the pairs. The wave is its whole workgroup.
-template <typename E>
-__device__ __forceinline__ void head_values(const NormedArgs& a, const uint16_t* src, const float* w, bool turns,
-                                            int position, float* row, float (&x)[4]) {
-  const int D = a.g.head_dim, lane = int(threadIdx.x), rotary = a.g.rotary_dim, half = rotary / 2;
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    x[i] = d < D ? E::to_f32(src[d]) : 0.f;
-    sum += x[i] * x[i];
-  }
-  if (w != nullptr) {
-    const float inv = 1.f / sqrtf(wave_sum(sum) / float(D) + a.g.norm_eps);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d < D) x[i] = x[i] * inv * w[d];
-    }
-  }
-  if (!turns || rotary == 0) return;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < D) row[lane + 64 * i] = x[i];
-  __syncthreads();
-  const float* cos = a.cos + (long long)position * half;
-  const float* sin = a.sin + (long long)position * half;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    if (d >= rotary) continue;
-    const bool second = a.g.interleaved ? d & 1 : d >= half;
-    const int other = a.g.interleaved ? d ^ 1 : second ? d - half : d + half;
-    const int j = a.g.interleaved ? d >> 1 : second ? d - half : d;
-    x[i] = second ? row[other] * sin[j] + x[i] * cos[j] : x[i] * cos[j] - row[other] * sin[j];
-  }
-}
-
-// one head of one token's q, and of its k and v where the pages hold the tokens' own type
-template <typename E>
-__global__ __launch_bounds__(64) void normed_rows_kernel(NormedArgs a, int heads) {
-  __shared__ float row[256];
-  const gie_paged_geom& g = a.g;
-  const int t = int(blockIdx.x) / heads, lane = int(threadIdx.x), D = g.head_dim;
-  int head = int(blockIdx.x) % heads;
-  const Place p = place_of(g, a.q_starts, a.seq_lens, a.page_table, t);
-  if (!p.present) return;
-  const int q_heads = a.q ? g.q_heads : 0;
-  const bool is_q = head < q_heads;
-  if (!is_q && p.page < 0) return;
-  if (!is_q) head -= q_heads;
-  const bool is_v = !is_q && head >= g.kv_heads;
-  if (is_v) head -= g.kv_heads;
-  const uint16_t* src = is_q ? a.q + t * g.q_stride : is_v ? a.v + t * g.v_stride : a.k + t * g.k_stride;
-  uint16_t* dst = is_q ? a.q_out + t * g.o_stride + head * D
-                       : static_cast<uint16_t*>(is_v ? a.v_pages : a.k_pages) +
-                             (((long long)p.page * g.kv_heads + head) * g.page_size + p.slot) * D;
-  float x[4];
-  head_values<E>(a, src + head * D, is_q ? a.q_norm : is_v ? nullptr : a.k_norm, !is_v && p.position >= 0, p.position, row, x);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    if (d < D) dst[d] = p.position < 0 ? uint16_t(0) : E::from_f32(x[i]);
-  }
-}
-
-// one block of 16 positions of one key head's k or v
-template <typename E, typename C>
-__global__ __launch_bounds__(64) void block_values_kernel(NormedArgs a) {
-  __shared__ float row[256];
-  __shared__ float all[kKvBlock][256];
-  const gie_paged_geom& g = a.g;
-  const int items = 2 * g.kv_heads, D = g.head_dim, lane = int(threadIdx.x);
-  const Block b = block_of(g, a.q_starts, a.seq_lens, a.page_table, int(blockIdx.x) / items);
-  if (b.first >= b.end || b.page < 0) return;
-  const int item = int(blockIdx.x) % items, head = item % g.kv_heads;
-  const bool is_v = item >= g.kv_heads;
-  const uint16_t* src = (is_v ? a.v + b.row0 * g.v_stride : a.k + b.row0 * g.k_stride) + head * D;
-  const long long stride = is_v ? g.v_stride : g.k_stride;
-  const long long at = ((long long)b.page * g.kv_heads + head) * g.page_size + b.slot;
-  uint8_t* codes = static_cast<uint8_t*>(is_v ? a.v_pages : a.k_pages) + at * D;
-  float* scale_at = (is_v ? a.v_scales : a.k_scales) + at / kKvBlock;
-  float most = 0.f;
-  bool finite = true;
-  for (int p = b.first; p < b.end; ++p) {
-    float x[4];
-    head_values<E>(a, src + (p - b.first) * stride, is_v ? nullptr : a.k_norm, !is_v, p, row, x);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d >= D) continue;
-      all[p - b.start][d] = x[i];
-      most = fmaxf(most, fabsf(x[i]));
-      finite = finite && fabsf(x[i]) <= 3.402823466e38f;
-    }
-  }
-  most = wave_max(most);
-  const bool starts = b.first == b.start;
-  const float before = starts ? 0.f : *scale_at;
-  if (__any(!finite) || !(before == before)) {
-    if (lane == 0) *scale_at = __builtin_nanf("");
-    return;
-  }
-  const float needed = C::scale(most), scale = fmaxf(before, needed), inv = 1.f / scale;
-  if (!starts && scale > before)
-    for (int p = b.start; p < b.first; ++p)
-      for (int d = lane; d < D; d += 64) {
-        uint8_t* c = codes + (p - b.start) * D + d;
-        *c = uint8_t(C::encode1(C::decode1(*c) * (before * inv)));
-      }
-  for (int p = b.first; p < b.end; ++p)
-    for (int d = lane; d < D; d += 64) codes[(p - b.start) * D + d] = uint8_t(C::encode1(all[p - b.start][d] * inv));
-  if (lane == 0) *scale_at = scale;
-}
-
 // ---- 16 values a lane
 template <int D>
 constexpr int kHeadLanes = D == 64 ? 4 : D == 256 ? 16 : 8;  // of a head (6 of 8 at 96)
 
+// how a head rotates: pairs of its halves or neighbours, in pieces of 16 values; kAny: either, any even number of values
+enum Form { kHalves, kNeighbours, kAny };
+
 // where a lane's 16 values lie in its head: 8 from `at`, 8 from `next`; pairs: they rotate (values i and 8 + i, or
-// interleaved 2 i and 2 i + 1, by the angles from `angle` on)
+// neighbours 2 i and 2 i + 1, by the angles from `angle` on; kAny: some of them do)
 struct Unit {
   int at, next, angle;
   bool there, pairs;
 };
-template <bool INTERLEAVED, int D>
+template <Form F, int D>
 __device__ __forceinline__ Unit unit_of(int unit, int rotary) {
   Unit u;
   u.there = unit < D / 16;
-  u.pairs = u.there && unit < rotary / 16;
+  u.pairs = u.there && unit * 16 < rotary;
   u.angle = unit * 8;
-  u.at = u.pairs && !INTERLEAVED ? unit * 8 : unit * 16;
-  u.next = u.pairs && !INTERLEAVED ? u.at + rotary / 2 : u.at + 8;
+  u.at = u.pairs && F == kHalves ? unit * 8 : unit * 16;
+  u.next = u.pairs && F == kHalves ? u.at + rotary / 2 : u.at + 8;
   return u;
 }
 
@@ -219,8 +95,42 @@ __device__ __forceinline__ void stage_weights(const NormedArgs& a, float (*w)[D]
     w[i / D][i % D] = from ? from[i % D] : 1.f;
   }
 }
-template <bool INTERLEAVED>
-__device__ __forceinline__ void turn_unit(float (&x)[16], const float* cos, const float* sin) {
+// cos, sin: the position's rows of the tables; row: LDS for the head's values (kAny)
+template <Form F>
+__device__ __forceinline__ void turn_unit(float (&x)[16], const Unit& u, const gie_paged_geom& g, const float* cos,
+                                          const float* sin, float* row) {
+  const int half = g.rotary_dim / 2;
+  if constexpr (F == kAny) {
+    if (g.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = u.angle + i;
+        if (j >= half) break;
+        const float a = x[2 * i], b = x[2 * i + 1], c = cos[j], s = sin[j];
+        x[2 * i] = a * c - b * s;
+        x[2 * i + 1] = a * s + b * c;
+      }
+      return;
+    }
+    // (both values of a pair lie with lanes of one wave that come here, and a wave's LDS accesses keep their order)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) row[u.at + i] = x[i];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int d = u.at + i;
+      if (d >= 2 * half) break;
+      const bool second = d >= half;
+      const int j = second ? d - half : d;
+      const float other = row[second ? j : d + half];
+      x[i] = second ? other * sin[j] + x[i] * cos[j] : x[i] * cos[j] - other * sin[j];
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    return;
+  }
+  cos += u.angle;
+  sin += u.angle;
+  constexpr bool INTERLEAVED = F == kNeighbours;
   const f32x4 c[2] = {__builtin_bit_cast(f32x4, load_16_bytes(cos)), __builtin_bit_cast(f32x4, load_16_bytes(cos + 4))};
   const f32x4 s[2] = {__builtin_bit_cast(f32x4, load_16_bytes(sin)), __builtin_bit_cast(f32x4, load_16_bytes(sin + 4))};
 #pragma unroll
@@ -233,13 +143,12 @@ __device__ __forceinline__ void turn_unit(float (&x)[16], const float* cos, cons
   }
 }
 
-constexpr int kMostTokens = 8;  // of a workgroup
+constexpr int kMostTokens = 8, kMostThreads = 512;  // of a workgroup
 
 // rows: tokens t0 .. t0 + count - 1, heads of q (if it is there), and of k and v with ALL
-template <typename E, bool INTERLEAVED, int D, bool ALL>
-__device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int count) {
+template <typename E, Form F, int D, bool ALL>
+__device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int count, float (*weights)[D], float* values) {
   __shared__ Place places[kMostTokens];
-  __shared__ __attribute__((aligned(16))) float weights[2][D];
   const gie_paged_geom& g = a.g;
   constexpr int L = kHeadLanes<D>;
   const int tid = int(threadIdx.x), threads = int(blockDim.x);
@@ -247,7 +156,7 @@ __device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int cou
     const Place p = place_of(g, a.q_starts, a.seq_lens, a.page_table, t0 + i);
     if ((tid & 63) == 0) places[i] = p;
   }
-  const Unit u = unit_of<INTERLEAVED, D>(tid % L, g.rotary_dim);
+  const Unit u = unit_of<F, D>(tid % L, g.rotary_dim);
   stage_weights<D>(a, weights);
   __syncthreads();
   const int q_heads = a.q ? g.q_heads : 0, heads = q_heads + (ALL ? 2 * g.kv_heads : 0), half = g.rotary_dim / 2;
@@ -270,7 +179,8 @@ __device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int cou
     if (is_q && a.q_norm) norm_unit<D>(x, weights[0], u, g.norm_eps);
     if (ALL && !is_q && !is_v && a.k_norm) norm_unit<D>(x, weights[1], u, g.norm_eps);
     if (u.pairs && !is_v && p.position >= 0)
-      turn_unit<INTERLEAVED>(x, a.cos + (long long)p.position * half + u.angle, a.sin + (long long)p.position * half + u.angle);
+      turn_unit<F>(x, u, g, a.cos + (long long)p.position * half, a.sin + (long long)p.position * half,
+                   values + (F == kAny ? tid / L * L * 16 : 0));
     if (!u.there) continue;
     u32x4 y = {E::pack2(x[0], x[1]), E::pack2(x[2], x[3]), E::pack2(x[4], x[5]), E::pack2(x[6], x[7])};
     u32x4 z = {E::pack2(x[8], x[9]), E::pack2(x[10], x[11]), E::pack2(x[12], x[13]), E::pack2(x[14], x[15])};
@@ -281,20 +191,20 @@ __device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int cou
 }
 
 // block `slot` of the batch's: a wave for each head of k and v, from `first_item` on
-template <typename E, typename C, bool INTERLEAVED, int D>
-__device__ __forceinline__ void append_block(const NormedArgs& a, int slot, int first_item) {
+template <typename E, typename C, Form F, int D>
+__device__ __forceinline__ void append_block(const NormedArgs& a, int slot, int first_item, float (*weights)[D],
+                                             float* values) {
   const gie_paged_geom& g = a.g;
   constexpr int L = kHeadLanes<D>, T = 64 / L, kPasses = kKvBlock / T;  // T tokens at once
   const int tid = int(threadIdx.x), lane = tid & 63, half = g.rotary_dim / 2;
   const int item = first_item + __builtin_amdgcn_readfirstlane(tid >> 6);
-  __shared__ __attribute__((aligned(16))) float weights[2][D];
   const Block b = block_of(g, a.q_starts, a.seq_lens, a.page_table, slot);
   if (b.first >= b.end || b.page < 0) return;
   if (a.k_norm) {
     stage_weights<D>(a, weights);
     __syncthreads();
   }
-  const Unit u = unit_of<INTERLEAVED, D>(lane % L, g.rotary_dim), straight = {lane % L * 16, lane % L * 16 + 8, 0, u.there, false};
+  const Unit u = unit_of<F, D>(lane % L, g.rotary_dim), straight = {lane % L * 16, lane % L * 16 + 8, 0, u.there, false};
   if (item < 2 * g.kv_heads) {
     const bool is_v = item >= g.kv_heads;
     const int head = is_v ? item - g.kv_heads : item;
@@ -324,7 +234,8 @@ __device__ __forceinline__ void append_block(const NormedArgs& a, int slot, int 
         if (position < b.first || position >= b.end) continue;
         if (a.k_norm) norm_unit<D>(x[p], weights[1], u, g.norm_eps);
         if (u.pairs)
-          turn_unit<INTERLEAVED>(x[p], a.cos + (long long)position * half + u.angle, a.sin + (long long)position * half + u.angle);
+          turn_unit<F>(x[p], u, g, a.cos + (long long)position * half, a.sin + (long long)position * half,
+                       values + (F == kAny ? tid / L * L * 16 : 0));
       }
     }
     unsigned bits = 0;  // of the largest |x|: infinities and NaNs are larger than all numbers
@@ -371,21 +282,24 @@ __device__ __forceinline__ void append_block(const NormedArgs& a, int slot, int 
 }
 
 // C void: pages in the tokens' type. Otherwise the first `blocks` workgroups take blocks, `parts` of them one block's heads.
-template <typename E, typename C, bool INTERLEAVED, int D>
-__global__ __launch_bounds__(512) void append_kernel(NormedArgs a, int blocks, int parts, int tokens) {
+template <typename E, typename C, Form F, int D>
+__global__ __launch_bounds__(kMostThreads) void append_kernel(NormedArgs a, int blocks, int parts, int tokens) {
+  __shared__ __attribute__((aligned(16))) float weights[2][D];
+  __shared__ __attribute__((aligned(16))) float values[F == kAny ? kMostThreads * 16 : 4];  // 16 of each lane
   int id = int(blockIdx.x);
   if constexpr (!std::is_void<C>::value) {
     if (id < blocks) {
-      append_block<E, C, INTERLEAVED, D>(a, id / parts, id % parts * (int(blockDim.x) >> 6));
+      append_block<E, C, F, D>(a, id / parts, id % parts * (int(blockDim.x) >> 6), weights, values);
       return;
     }
     id -= blocks;
   }
-  append_rows<E, INTERLEAVED, D, std::is_void<C>::value>(a, id * tokens, min(tokens, a.g.total_tokens - id * tokens));
+  append_rows<E, F, D, std::is_void<C>::value>(a, id * tokens, min(tokens, a.g.total_tokens - id * tokens),
+                                                         weights, values);
 }
 
 template <typename E, typename C>
-int launch_units(const NormedArgs& a, hipStream_t s) {
+int launch(const NormedArgs& a, hipStream_t s) {
   constexpr bool k8 = !std::is_void<C>::value;
   const gie_paged_geom& g = a.g;
   const int D = g.head_dim, lanes = D == 64 ? 4 : D == 256 ? 16 : 8;
@@ -395,21 +309,24 @@ int launch_units(const NormedArgs& a, hipStream_t s) {
   tokens = tokens < 1 ? 1 : tokens > kMostTokens ? kMostTokens : tokens;
   const long long rows = heads == 0 ? 0 : (g.total_tokens + tokens - 1) / tokens;
   long long threads = (work * tokens + (tokens > 1 ? 127 : 63)) / (tokens > 1 ? 128 : 64) * 64;
-  if (threads > 512) threads = 512;
+  if (threads > kMostThreads) threads = kMostThreads;
   // blocks are a wave's work each: four waves to a workgroup spread them
   if (k8) threads = 256;
   const long long parts = (2ll * g.kv_heads + threads / 64 - 1) / (threads / 64), blocks = k8 ? block_slots(g) * parts : 0;
   if ((blocks + rows) * threads > 0xffffffffll) return GIE_HIP_EUNSUPPORTED;  // a launch's threads
-  const auto kernel = [&](auto interleaved) {
-    constexpr bool I = decltype(interleaved)::value;
+  const auto kernel_of = [&](auto form) {
+    constexpr Form F = decltype(form)::value;
     switch (D) {
-      case 64: return append_kernel<E, C, I, 64>;
-      case 96: return append_kernel<E, C, I, 96>;
-      case 128: return append_kernel<E, C, I, 128>;
-      default: return append_kernel<E, C, I, 256>;
+      case 64: return append_kernel<E, C, F, 64>;
+      case 96: return append_kernel<E, C, F, 96>;
+      case 128: return append_kernel<E, C, F, 128>;
+      default: return append_kernel<E, C, F, 256>;
     }
   };
-  hipLaunchKernelGGL(g.interleaved ? kernel(std::true_type{}) : kernel(std::false_type{}), dim3(unsigned(blocks + rows)),
+  const auto kernel = g.rotary_dim % 16 != 0 ? kernel_of(std::integral_constant<Form, kAny>{})
+                      : g.interleaved        ? kernel_of(std::integral_constant<Form, kNeighbours>{})
+                                             : kernel_of(std::integral_constant<Form, kHalves>{});
+  hipLaunchKernelGGL(kernel, dim3(unsigned(blocks + rows)),
                      dim3(unsigned(threads)), 0, s, a, int(blocks), int(parts), int(tokens));
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? GIE_HIP_OK : int(e);
@@ -434,18 +351,6 @@ bool supported(int dtype, const gie_paged_geom* g) {
          (g->head_dim == 64 || g->head_dim == 96 || g->head_dim == 128 || g->head_dim == 256);
 }
 
-template <typename E, typename C>
-int launch_blocks(const NormedArgs& a, hipStream_t s) {
-  if (a.g.rotary_dim % 16 == 0) return launch_units<E, C>(a, s);
-  const long long grid = block_slots(a.g) * 2 * a.g.kv_heads;
-  const long long rows = a.q ? (long long)a.g.total_tokens * a.g.q_heads : 0;
-  if (grid * 64 > 0xffffffffll || rows * 64 > 0xffffffffll) return GIE_HIP_EUNSUPPORTED;  // a launch's threads
-  hipLaunchKernelGGL((block_values_kernel<E, C>), dim3(unsigned(grid)), dim3(64), 0, s, a);
-  if (rows > 0) hipLaunchKernelGGL(normed_rows_kernel<E>, dim3(unsigned(rows)), dim3(64), 0, s, a, a.g.q_heads);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? GIE_HIP_OK : int(e);
-}
-
 }  // namespace
 }  // namespace gie_hip
 
@@ -466,15 +371,7 @@ extern "C" int gie_hip_kv_append_normed(int dtype, const gie_paged_geom* g, cons
                      static_cast<const uint16_t*>(v), q_norm, k_norm, cos, sin, q_starts, seq_lens, page_table,
                      static_cast<uint16_t*>(q_out), k_pages, v_pages, nullptr, nullptr};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (g->rotary_dim % 16 == 0) return dtype == GIE_HIP_FP16 ? launch_units<Fp16, void>(a, s) : launch_units<Bf16, void>(a, s);
-  const long long heads = (q ? g->q_heads : 0) + 2 * g->kv_heads, grid = heads * g->total_tokens;
-  if (grid * 64 > 0xffffffffll) return GIE_HIP_EUNSUPPORTED;  // a launch's threads
-  if (dtype == GIE_HIP_FP16)
-    hipLaunchKernelGGL(normed_rows_kernel<Fp16>, dim3(unsigned(grid)), dim3(64), 0, s, a, int(heads));
-  else
-    hipLaunchKernelGGL(normed_rows_kernel<Bf16>, dim3(unsigned(grid)), dim3(64), 0, s, a, int(heads));
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? GIE_HIP_OK : int(e);
+  return dtype == GIE_HIP_FP16 ? launch<Fp16, void>(a, s) : launch<Bf16, void>(a, s);
 }
 
 extern "C" int gie_hip_kv8_append(int dtype, int code, const gie_paged_geom* g, const void* q, const void* k,
@@ -493,6 +390,6 @@ extern "C" int gie_hip_kv8_append(int dtype, int code, const gie_paged_geom* g, 
                      static_cast<uint16_t*>(q_out), k_pages, v_pages, k_scales, v_scales};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool fp16 = dtype == GIE_HIP_FP16;
-  if (code == GIE_HIP_KV_INT8) return fp16 ? launch_blocks<Fp16, Int8Code>(a, s) : launch_blocks<Bf16, Int8Code>(a, s);
-  return fp16 ? launch_blocks<Fp16, E4m3Code>(a, s) : launch_blocks<Bf16, E4m3Code>(a, s);
+  if (code == GIE_HIP_KV_INT8) return fp16 ? launch<Fp16, Int8Code>(a, s) : launch<Bf16, Int8Code>(a, s);
+  return fp16 ? launch<Fp16, E4m3Code>(a, s) : launch<Bf16, E4m3Code>(a, s);
 }
