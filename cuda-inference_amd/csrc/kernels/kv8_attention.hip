@@ -11,6 +11,16 @@
 // registers: ks is a factor of the exponent, vs a term of it, x_j = s_j log2(e) + log2(vs_j). The weight 2^(x_j - m) that
 // the second product takes has vs in it, and m is the maximum of x: weights keep their bits however much the blocks'
 // sizes differ. The sum of p_j takes 1 / vs once for each block.
+//
+// Few rows: one token over 65536 positions of 8 key heads of 128 in 32 parts 27 us (134 MB, 5.0 TB/s) + 4 for the join; a
+// step of 64 sequences of 1 to 8001 120 us, 4.3 TB/s (a large copy 4.7). Many rows: two prompts of 4096 tokens, 32 heads of
+// 128, 326 to 343 us by the card, 0.80 to 0.84 PFLOP/s (a large library product 1.2), where paged_attention over 16 bits
+// takes 300 to 311. The vector unit is busy 0.61 of the time and the matrix cores 0.39, one after the other whatever was
+// tried: codes decoded under matrix instructions, scores of the next part under the weights (2 %, kept), wave priorities;
+// so what helps is fewer vector instructions. Of the 240 that a wave has for a tile of 64 keys, and 32 exponentials at a
+// quarter of their rate, 80 decode and 80 are the weights, their sum and their rounding. 256 rows that share a tile (half
+// the decoding for each) took from 8 % less (one prompt) to 30 % more (ragged ones, narrow heads).
+// Outputs are off by 1.7e-3 of their size in BF16 and 2.2e-4 in FP16, as FP32 weights with one rounding would be.
 #include <type_traits>
 
 #include "attention_common.h"
@@ -116,8 +126,8 @@ __device__ __forceinline__ u32x2 pack_out(bool bf16, f32x4 v) {
 // The weights of 32 scores (register i: key 8 (i / 4) + 4 half + i % 4, so the block i / 8), and what they do to the
 // running maximum, the sum and the rows' values. `masked`: seen(i) says whether register i's key is.
 //
-// The maximum is not looked for ahead of the weights (27 of about 150 vector instructions): they are taken against what
-// is there, and as long as a lane's sum of them stays within 2^15 all of them fit FP16. Only where it does not, or a row
+// The maximum is not looked for ahead of the weights (which took 27 of about 150 vector instructions, and 8 % of the time
+// of two prompts of 4096): they are taken against what is there, and as long as a lane's sum of them stays within 2^15 all of them fit FP16. Only where it does not, or a row
 // has seen nothing yet, the rows' maxima move and the weights are taken again.
 template <bool LARGE_CAP, typename Seen>
 __device__ __forceinline__ void cap_and_mask(const AttnArgs& a, f32x16& s, const BlockScales (&sc)[2], float row_factor,
@@ -437,10 +447,12 @@ __global__ __launch_bounds__(64 * WK, WK == 8 ? 2 : 1) void narrow_kernel(Kv8Arg
 
 // ---------------------------------------------------------------- many rows: 128 for each workgroup
 // Bound by the products and the softmax. The workgroup decodes a tile of 64 keys once, HBM -> registers -> LDS in FP16, for
-// four waves of 32 rows that share it (WD == 2: two waves for each 32 rows, half of the head's values each): a wave
-// decoding what it multiplies would decode every code four times. Codes of the next tile but one are requested before a
-// tile is worked on. Values lie in decode8's order in LDS: of K that is q's order too, of V the rows' registers are put
-// in order at the end.
+// the waves that share it: a wave decoding what it multiplies would decode every code four times. Codes of the next tile
+// but one are requested before a tile is worked on. Values lie in decode8's order in LDS: of K that is q's order too, of
+// V the rows' registers are put in order at the end.
+// Up to head_dim 128 four waves take 32 rows each, in steps of half a tile. At 256 (WD == 2) two waves share 32 rows, for
+// each has registers for half of the values; each works out half of a tile's scores, and they exchange the weights through
+// LDS (512 tokens over 8192, 32 heads: 174 us; with all scores worked out by both 219).
 template <typename C, int D, int WD, bool LARGE_CAP>
 __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
   constexpr int WR = kWideRows / 32, R = kWideRows, TT = kWideKeys, NS = TT / 32, P = kPitch<D>;
