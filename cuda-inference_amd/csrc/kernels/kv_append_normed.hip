@@ -264,17 +264,15 @@ __device__ __forceinline__ void append_block(const NormedArgs& a, int slot, int 
       if (!w.there || position >= b.end) continue;
       if (position < b.first) {
         if (!grows) continue;
-        const float factor = before * inv;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const u32x2 c = __builtin_bit_cast(u32x2, *reinterpret_cast<const unsigned long long*>(dst + (i ? w.next : w.at)));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[p][8 * i + e] = C::decode1(c[e / 4] >> (e % 4 * 8) & 255u) * factor;
+          for (int e = 0; e < 8; ++e) x[p][8 * i + e] = C::decode1(c[e / 4] >> (e % 4 * 8) & 255u) * before;
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[p][i] *= inv;
       }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[p][i] = C::divide(x[p][i], scale, inv);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const u32x2 c = {C::encode4(x[p][8 * i], x[p][8 * i + 1], x[p][8 * i + 2], x[p][8 * i + 3]),

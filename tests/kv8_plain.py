@@ -46,8 +46,8 @@ def scale_for(most, cache):
 
 
 def encode(x, scale, cache):
-    """Codes of FP32 values under FP32 scales, with the library's FP32 steps: one reciprocal, one product, one rounding."""
-    y = x.astype(np.float32) * (np.float32(1) / scale.astype(np.float32))
+    """Codes of FP32 values under FP32 scales, with the library's steps: one quotient in FP32, one rounding."""
+    y = x.astype(np.float32) / scale.astype(np.float32)
     if cache == "int8":
         return np.rint(np.clip(y, -127, 127)).astype(np.int8).view(np.uint8)
     return encode_e4m3(np.clip(y.astype(np.float64), -448, 448))

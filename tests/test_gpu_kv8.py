@@ -177,8 +177,8 @@ def test_append_codes_bit_for_bit(cache, precision):
                 at = slice(block * BLOCK, block * BLOCK + first)
                 if first and s > old:
                     was = codes[n][pg, h, at]
-                    # code times the quotient of scales, each one FP32 operation
-                    moved = decode(was, cache).astype(np.float32) * (old * (np.float32(1) / s))
+                    # what the code stood for, divided by the new scale, each one FP32 operation
+                    moved = decode(was, cache).astype(np.float32) * old / s
                     codes[n][pg, h, at] = np.rint(moved).astype(np.int8).view(np.uint8) if cache == "int8" else \
                         encode_e4m3(moved.astype(np.float64))
                 codes[n][pg, h, slot] = encode(rows[n][0, h], np.float32(s), cache)
