@@ -8,10 +8,12 @@
 #include <algorithm>
 #include <chrono>
 #include <cmath>
+#include <cstddef>
 #include <functional>
 #include <cstring>
 #include <memory>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #include "gpu_inference/autotuner.h"
@@ -122,7 +124,13 @@ LinearI8Problem to_linear(const gie_linear_i8_problem* p) {
   return r;
 }
 
-PagedKvProblem to_paged(const gie_paged_kv_problem* p) {
+// the fields that both structures begin with
+static_assert(offsetof(gie_kv_problem, sinks) == sizeof(gie_paged_kv_problem) &&
+                  offsetof(gie_kv_problem, q_stride) == offsetof(gie_paged_kv_problem, q_stride) &&
+                  offsetof(gie_kv_problem, max_len) == offsetof(gie_paged_kv_problem, max_len),
+              "gie_kv_problem begins with gie_paged_kv_problem");
+template <typename P>
+PagedKvProblem to_paged(const P* p) {
   GIE_REQUIRE(p != nullptr, StatusCode::kInvalidArgument, "null problem");
   GIE_REQUIRE(p->precision >= 0 && p->precision <= 3, StatusCode::kInvalidArgument, "bad precision");
   PagedKvProblem r;
@@ -147,10 +155,12 @@ PagedKvProblem to_paged(const gie_paged_kv_problem* p) {
   r.window = p->window;
   r.max_new = p->max_new;
   r.max_len = p->max_len;
-  r.sinks = p->sinks;
-  r.norm_eps = p->norm_eps;
-  GIE_REQUIRE(p->code >= 0 && p->code <= 2, StatusCode::kInvalidArgument, "bad code");
-  r.code = static_cast<KvCode>(p->code);
+  if constexpr (std::is_same_v<P, gie_kv_problem>) {
+    r.sinks = p->sinks;
+    r.norm_eps = p->norm_eps;
+    GIE_REQUIRE(p->code >= 0 && p->code <= 2, StatusCode::kInvalidArgument, "bad code");
+    r.code = static_cast<KvCode>(p->code);
+  }
   return r;
 }
 
@@ -997,7 +1007,7 @@ extern "C" int gie_paged_attention(const gie_paged_kv_problem* p, const void* q,
   });
 }
 
-extern "C" int gie_kv_append_normed(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v,
+extern "C" int gie_kv_append_normed(const gie_kv_problem* p, const void* q, const void* k, const void* v,
                                     const float* q_norm, const float* k_norm, const float* cos, const float* sin,
                                     const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
                                     void* k_pages, void* v_pages, void* stream) {
@@ -1007,13 +1017,29 @@ extern "C" int gie_kv_append_normed(const gie_paged_kv_problem* p, const void* q
   });
 }
 
+extern "C" int gie_kv_attention_workspace_size(const gie_kv_problem* p, size_t* bytes) {
+  return guarded([&] {
+    GIE_REQUIRE(bytes != nullptr, StatusCode::kInvalidArgument, "null out");
+    *bytes = PagedKv::workspace_size(to_paged(p));
+  });
+}
+
+extern "C" int gie_kv_attention(const gie_kv_problem* p, const void* q, const void* k_pages, const void* v_pages,
+                                const int* q_starts, const int* seq_lens, const int* page_table, void* out,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    PagedKv::attention(q, k_pages, v_pages, q_starts, seq_lens, page_table, to_paged(p), out, workspace,
+                       workspace_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
 namespace {
 Kv8Pages kv8_pages(const void* k, const void* v, const float* k_scales, const float* v_scales) {
   return {const_cast<void*>(k), const_cast<void*>(v), const_cast<float*>(k_scales), const_cast<float*>(v_scales)};
 }
 }  // namespace
 
-extern "C" int gie_kv8_append(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v,
+extern "C" int gie_kv8_append(const gie_kv_problem* p, const void* q, const void* k, const void* v,
                               const float* q_norm, const float* k_norm, const float* cos, const float* sin,
                               const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
                               void* k_pages, void* v_pages, float* k_scales, float* v_scales, void* stream) {
@@ -1023,7 +1049,7 @@ extern "C" int gie_kv8_append(const gie_paged_kv_problem* p, const void* q, cons
   });
 }
 
-extern "C" int gie_kv8_read(const gie_paged_kv_problem* p, const void* k_pages, const void* v_pages,
+extern "C" int gie_kv8_read(const gie_kv_problem* p, const void* k_pages, const void* v_pages,
                             const float* k_scales, const float* v_scales, const int* q_starts, const int* seq_lens,
                             const int* page_table, void* k, void* v, void* stream) {
   return guarded([&] {
@@ -1032,14 +1058,14 @@ extern "C" int gie_kv8_read(const gie_paged_kv_problem* p, const void* k_pages, 
   });
 }
 
-extern "C" int gie_kv8_attention_workspace_size(const gie_paged_kv_problem* p, size_t* bytes) {
+extern "C" int gie_kv8_attention_workspace_size(const gie_kv_problem* p, size_t* bytes) {
   return guarded([&] {
     GIE_REQUIRE(bytes != nullptr, StatusCode::kInvalidArgument, "null out");
     *bytes = PagedKv8::workspace_size(to_paged(p));
   });
 }
 
-extern "C" int gie_kv8_attention(const gie_paged_kv_problem* p, const void* q, const void* k_pages,
+extern "C" int gie_kv8_attention(const gie_kv_problem* p, const void* q, const void* k_pages,
                                  const void* v_pages, const float* k_scales, const float* v_scales,
                                  const int* q_starts, const int* seq_lens, const int* page_table, void* out,
                                  void* workspace, size_t workspace_bytes, void* stream) {

@@ -232,7 +232,7 @@ struct Shape {
 
 constexpr int kNarrowRows = 32, kWideRows = 128, kNarrowKeys = 32, kWideKeys = 64;  // a tile's
 
-inline Shape shape_of(const gie_paged_geom& g) {
+inline Shape shape_of(const gie_kv_geom& g) {
   Shape s;
   const int group = g.q_heads / g.kv_heads;
   const long long rows = (long long)g.total_tokens * group;
@@ -310,18 +310,18 @@ inline bool fits_launch(const AttnArgs& a, const Shape& s) {
   return grid * 512 <= 0xffffffffll && joining <= 0xffffff00ll;
 }
 
-inline size_t parts_bytes(const gie_paged_geom& g, const Shape& s) {
+inline size_t parts_bytes(const gie_kv_geom& g, const Shape& s) {
   return s.splits == 1 ? 0 : size_t(g.total_tokens) * g.q_heads * s.splits * (g.head_dim + 4) * sizeof(float);
 }
 
-inline bool valid_attention(const gie_paged_geom* g, const void* q, const void* k_pages, const void* v_pages,
+inline bool valid_attention(const gie_kv_geom* g, const void* q, const void* k_pages, const void* v_pages,
                             const int* q_starts, const int* seq_lens, const int* page_table, const void* out) {
   if (!q || !k_pages || !v_pages || !q_starts || !seq_lens || !page_table || !out || q == out) return false;
   return aligned_to(q, 2) && aligned_to(out, 2) && aligned_to(k_pages, 16) && aligned_to(v_pages, 16);
 }
 
 // the arguments but for the cache's pages; returns whether the cap is past kExpCap
-inline bool fill_args(AttnArgs& a, const gie_paged_geom* g, const Shape& shape, const void* q, const int* q_starts,
+inline bool fill_args(AttnArgs& a, const gie_kv_geom* g, const Shape& shape, const void* q, const int* q_starts,
                       const int* seq_lens, const int* page_table, void* out, void* workspace) {
   a.q = static_cast<const uint16_t*>(q);
   a.q_starts = q_starts;

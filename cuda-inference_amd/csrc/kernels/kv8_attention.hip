@@ -893,12 +893,12 @@ int launch(const Kv8Args& a, const Shape& s, int head_dim, hipStream_t stream) {
 
 using namespace gie_hip;
 
-extern "C" size_t gie_hip_kv8_attention_workspace(const gie_paged_geom* g) {
+extern "C" size_t gie_hip_kv8_attention_workspace(const gie_kv_geom* g) {
   if (!valid_paged(g) || g->total_tokens == 0) return 0;
   return parts_bytes(*g, shape_of(*g));
 }
 
-extern "C" int gie_hip_kv8_attention(int dtype, int code, const gie_paged_geom* g, const void* q, const void* k_pages,
+extern "C" int gie_hip_kv8_attention(int dtype, int code, const gie_kv_geom* g, const void* q, const void* k_pages,
                                      const void* v_pages, const float* k_scales, const float* v_scales,
                                      const int* q_starts, const int* seq_lens, const int* page_table, void* out,
                                      void* workspace, size_t workspace_bytes, void* stream) {

@@ -77,7 +77,7 @@ struct Block {
   int start, first, end, page, slot;
   int row0;  // row of q, k, v of position `first`
 };
-__device__ __forceinline__ Block block_of(const gie_paged_geom& g, const int* __restrict__ q_starts,
+__device__ __forceinline__ Block block_of(const gie_kv_geom& g, const int* __restrict__ q_starts,
                                           const int* __restrict__ seq_lens, const int* __restrict__ page_table, int slot) {
   // n tokens from any position on touch at most n / 16 + 2 blocks, so sequence b's slots start at floor(first / 16) + 2 b
   const auto from = [&](int first, int b) { return min(max(first, 0), g.total_tokens) / kKvBlock + 2 * b; };
@@ -98,7 +98,7 @@ __device__ __forceinline__ Block block_of(const gie_paged_geom& g, const int* __
   }
   return r;
 }
-inline long long block_slots(const gie_paged_geom& g) { return (long long)g.total_tokens / kKvBlock + 2ll * g.batch; }
+inline long long block_slots(const gie_kv_geom& g) { return (long long)g.total_tokens / kKvBlock + 2ll * g.batch; }
 
 inline bool valid_code(int code) { return code == GIE_HIP_KV_INT8 || code == GIE_HIP_KV_E4M3; }
 

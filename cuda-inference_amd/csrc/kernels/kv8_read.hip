@@ -10,7 +10,7 @@ namespace gie_hip {
 namespace {
 
 struct ReadArgs {
-  gie_paged_geom g;
+  gie_kv_geom g;
   const uint8_t* k_pages;
   const uint8_t* v_pages;
   const float* k_scales;
@@ -27,7 +27,7 @@ constexpr int kMostTokens = 8;  // of a workgroup
 template <typename E, typename C, int D>
 __global__ __launch_bounds__(512) void read_kernel(ReadArgs a, int tokens) {
   __shared__ Place places[kMostTokens];
-  const gie_paged_geom& g = a.g;
+  const gie_kv_geom& g = a.g;
   const int tid = int(threadIdx.x), threads = int(blockDim.x);
   const int t0 = int(blockIdx.x) * tokens, count = min(tokens, g.total_tokens - t0);
   for (int i = tid >> 6; i < count; i += threads >> 6) {
@@ -94,7 +94,7 @@ int launch(int code, const ReadArgs& a, hipStream_t s) {
 
 using namespace gie_hip;
 
-extern "C" int gie_hip_kv8_read(int dtype, int code, const gie_paged_geom* g, const void* k_pages, const void* v_pages,
+extern "C" int gie_hip_kv8_read(int dtype, int code, const gie_kv_geom* g, const void* k_pages, const void* v_pages,
                                 const float* k_scales, const float* v_scales, const int* q_starts, const int* seq_lens,
                                 const int* page_table, void* k, void* v, void* stream) {
   if (!valid_paged(g) || !valid_code(code)) return GIE_HIP_EINVAL;

@@ -19,7 +19,7 @@ namespace {
 constexpr int kMostTokens = 8;  // of a workgroup
 
 struct AppendArgs {
-  gie_paged_geom g;
+  gie_kv_geom g;
   const uint16_t* q;  // null: only keys and values
   const uint16_t* k;
   const uint16_t* v;
@@ -41,7 +41,7 @@ struct Head {
   bool turns, stored;
 };
 __device__ __forceinline__ Head head_of(const AppendArgs& a, int t, int head, const Place& p) {
-  const gie_paged_geom& g = a.g;
+  const gie_kv_geom& g = a.g;
   const int D = g.head_dim, q_heads = a.q ? g.q_heads : 0;
   if (head < q_heads) return {a.q + t * g.q_stride + head * D, a.q_out + t * g.o_stride + head * D, true, true};
   head -= q_heads;
@@ -178,9 +178,11 @@ void launch(AppendArgs a, bool vec, hipStream_t s) {
 
 using namespace gie_hip;
 
-extern "C" int gie_hip_kv_append(int dtype, const gie_paged_geom* g, const void* q, const void* k, const void* v,
+extern "C" int gie_hip_kv_append(int dtype, const gie_paged_geom* given, const void* q, const void* k, const void* v,
                                  const float* cos, const float* sin, const int* q_starts, const int* seq_lens,
                                  const int* page_table, void* q_out, void* k_pages, void* v_pages, void* stream) {
+  if (!given) return GIE_HIP_EINVAL;
+  const gie_kv_geom geom = widened(*given), *g = &geom;
   if (!valid_paged(g)) return GIE_HIP_EINVAL;
   if (dtype != GIE_HIP_FP16 && dtype != GIE_HIP_BF16) return GIE_HIP_EUNSUPPORTED;
   if (g->head_dim != 64 && g->head_dim != 96 && g->head_dim != 128 && g->head_dim != 256) return GIE_HIP_EUNSUPPORTED;

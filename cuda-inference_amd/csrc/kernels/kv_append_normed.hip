@@ -24,7 +24,7 @@ namespace gie_hip {
 namespace {
 
 struct NormedArgs {
-  gie_paged_geom g;
+  gie_kv_geom g;
   const uint16_t* q;  // null: only keys and values
   const uint16_t* k;
   const uint16_t* v;
@@ -102,7 +102,7 @@ __device__ __forceinline__ void stage_weights(const NormedArgs& a, float (*w)[D]
 }
 // cos, sin: the position's rows of the tables; row: LDS for the head's values (kAny)
 template <Form F>
-__device__ __forceinline__ void turn_unit(float (&x)[16], const Unit& u, const gie_paged_geom& g, const float* cos,
+__device__ __forceinline__ void turn_unit(float (&x)[16], const Unit& u, const gie_kv_geom& g, const float* cos,
                                           const float* sin, float* row) {
   const int half = g.rotary_dim / 2;
   if constexpr (F == kAny) {
@@ -154,7 +154,7 @@ constexpr int kMostTokens = 8, kMostThreads = 512;  // of a workgroup
 template <typename E, Form F, int D, bool ALL>
 __device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int count, float (*weights)[D], float* values) {
   __shared__ Place places[kMostTokens];
-  const gie_paged_geom& g = a.g;
+  const gie_kv_geom& g = a.g;
   constexpr int L = kHeadLanes<D>;
   const int tid = int(threadIdx.x), threads = int(blockDim.x);
   for (int i = tid >> 6; i < count; i += threads >> 6) {
@@ -199,7 +199,7 @@ __device__ __forceinline__ void append_rows(const NormedArgs& a, int t0, int cou
 template <typename E, typename C, Form F, int D>
 __device__ __forceinline__ void append_block(const NormedArgs& a, int slot, int first_item, float (*weights)[D],
                                              float* values) {
-  const gie_paged_geom& g = a.g;
+  const gie_kv_geom& g = a.g;
   constexpr int L = kHeadLanes<D>, T = 64 / L, kPasses = kKvBlock / T;  // T tokens at once
   const int tid = int(threadIdx.x), lane = tid & 63, half = g.rotary_dim / 2;
   const int item = first_item + __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(kMostThreads) void append_kernel(NormedArgs a, int 
 template <typename E, typename C>
 int launch(const NormedArgs& a, hipStream_t s) {
   constexpr bool k8 = !std::is_void<C>::value;
-  const gie_paged_geom& g = a.g;
+  const gie_kv_geom& g = a.g;
   const int D = g.head_dim, lanes = D == 64 ? 4 : D == 256 ? 16 : 8;
   const long long heads = (a.q ? g.q_heads : 0) + (k8 ? 0 : 2 * g.kv_heads), work = heads * lanes;  // of a token's lanes
   // one token for each workgroup spreads a step of few tokens; of many, as many as give every lane two heads
@@ -337,7 +337,7 @@ int launch(const NormedArgs& a, hipStream_t s) {
   return e == hipSuccess ? GIE_HIP_OK : int(e);
 }
 
-bool valid_rows(const gie_paged_geom* g, const void* q, const void* k, const void* v, const float* q_norm,
+bool valid_rows(const gie_kv_geom* g, const void* q, const void* k, const void* v, const float* q_norm,
                 const float* k_norm, const float* cos, const float* sin, const int* q_starts, const int* seq_lens,
                 const int* page_table, const void* q_out, const void* k_pages, const void* v_pages) {
   if (!k || !v || !q_starts || !seq_lens || !page_table || !k_pages || !v_pages || k_pages == v_pages ||
@@ -351,7 +351,7 @@ bool valid_rows(const gie_paged_geom* g, const void* q, const void* k, const voi
          aligned_to(k_norm, 4);
 }
 
-bool supported(int dtype, const gie_paged_geom* g) {
+bool supported(int dtype, const gie_kv_geom* g) {
   return (dtype == GIE_HIP_FP16 || dtype == GIE_HIP_BF16) &&
          (g->head_dim == 64 || g->head_dim == 96 || g->head_dim == 128 || g->head_dim == 256);
 }
@@ -361,13 +361,15 @@ bool supported(int dtype, const gie_paged_geom* g) {
 
 using namespace gie_hip;
 
-extern "C" int gie_hip_kv_append_normed(int dtype, const gie_paged_geom* g, const void* q, const void* k, const void* v,
+extern "C" int gie_hip_kv_append_normed(int dtype, const gie_kv_geom* g, const void* q, const void* k, const void* v,
                                         const float* q_norm, const float* k_norm, const float* cos, const float* sin,
                                         const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
                                         void* k_pages, void* v_pages, void* stream) {
-  if (!q_norm && !k_norm)
-    return gie_hip_kv_append(dtype, g, q, k, v, cos, sin, q_starts, seq_lens, page_table, q_out, k_pages, v_pages, stream);
   if (!valid_paged(g)) return GIE_HIP_EINVAL;
+  if (!q_norm && !k_norm) {
+    const gie_paged_geom geom = narrowed(*g);
+    return gie_hip_kv_append(dtype, &geom, q, k, v, cos, sin, q_starts, seq_lens, page_table, q_out, k_pages, v_pages, stream);
+  }
   if (!supported(dtype, g)) return GIE_HIP_EUNSUPPORTED;
   if (g->total_tokens == 0) return GIE_HIP_OK;
   if (!valid_rows(g, q, k, v, q_norm, k_norm, cos, sin, q_starts, seq_lens, page_table, q_out, k_pages, v_pages))
@@ -379,7 +381,7 @@ extern "C" int gie_hip_kv_append_normed(int dtype, const gie_paged_geom* g, cons
   return dtype == GIE_HIP_FP16 ? launch<Fp16, void>(a, s) : launch<Bf16, void>(a, s);
 }
 
-extern "C" int gie_hip_kv8_append(int dtype, int code, const gie_paged_geom* g, const void* q, const void* k,
+extern "C" int gie_hip_kv8_append(int dtype, int code, const gie_kv_geom* g, const void* q, const void* k,
                                   const void* v, const float* q_norm, const float* k_norm, const float* cos,
                                   const float* sin, const int* q_starts, const int* seq_lens, const int* page_table,
                                   void* q_out, void* k_pages, void* v_pages, float* k_scales, float* v_scales,

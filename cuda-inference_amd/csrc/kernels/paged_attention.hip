@@ -554,15 +554,15 @@ int launch(const PagedArgs& a, const Shape& s, int head_dim, hipStream_t stream)
 
 using namespace gie_hip;
 
-extern "C" size_t gie_hip_paged_attention_workspace(const gie_paged_geom* g) {
+extern "C" size_t gie_hip_kv_attention_workspace(const gie_kv_geom* g) {
   if (!valid_paged(g) || g->total_tokens == 0) return 0;
   return parts_bytes(*g, shape_of(*g));
 }
 
-extern "C" int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const void* q, const void* k_pages,
-                                       const void* v_pages, const int* q_starts, const int* seq_lens,
-                                       const int* page_table, void* out, void* workspace, size_t workspace_bytes,
-                                       void* stream) {
+extern "C" int gie_hip_kv_attention(int dtype, const gie_kv_geom* g, const void* q, const void* k_pages,
+                                    const void* v_pages, const int* q_starts, const int* seq_lens,
+                                    const int* page_table, void* out, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
   if (!valid_paged(g)) return GIE_HIP_EINVAL;
   if (dtype != GIE_HIP_FP16 && dtype != GIE_HIP_BF16) return GIE_HIP_EUNSUPPORTED;
   if (g->head_dim != 64 && g->head_dim != 96 && g->head_dim != 128 && g->head_dim != 256) return GIE_HIP_EUNSUPPORTED;
@@ -570,7 +570,7 @@ extern "C" int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const
   if (!std::isfinite(g->scale) || g->scale == 0 || !std::isfinite(g->softcap)) return GIE_HIP_EINVAL;
   if (g->total_tokens == 0) return GIE_HIP_OK;
   if (!valid_attention(g, q, k_pages, v_pages, q_starts, seq_lens, page_table, out)) return GIE_HIP_EINVAL;
-  const size_t need = gie_hip_paged_attention_workspace(g);
+  const size_t need = gie_hip_kv_attention_workspace(g);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))) return GIE_HIP_EINVAL;
   const Shape shape = shape_of(*g);
   PagedArgs a{};
@@ -581,4 +581,20 @@ extern "C" int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const
   const int D = g->head_dim;
   if (dtype == GIE_HIP_FP16) return large_cap ? launch<Fp16, true>(a, shape, D, s) : launch<Fp16, false>(a, shape, D, s);
   return large_cap ? launch<Bf16, true>(a, shape, D, s) : launch<Bf16, false>(a, shape, D, s);
+}
+
+extern "C" size_t gie_hip_paged_attention_workspace(const gie_paged_geom* g) {
+  if (!g) return 0;
+  const gie_kv_geom geom = widened(*g);
+  return gie_hip_kv_attention_workspace(&geom);
+}
+
+extern "C" int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const void* q, const void* k_pages,
+                                       const void* v_pages, const int* q_starts, const int* seq_lens,
+                                       const int* page_table, void* out, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  if (!g) return GIE_HIP_EINVAL;
+  const gie_kv_geom geom = widened(*g);
+  return gie_hip_kv_attention(dtype, &geom, q, k_pages, v_pages, q_starts, seq_lens, page_table, out, workspace,
+                              workspace_bytes, stream);
 }

@@ -2,6 +2,9 @@
 // to, and the bounds that what the device arrays hold is put under. Private to csrc/kernels.
 #pragma once
 
+#include <cstddef>
+#include <cstring>
+
 #include "device_common.h"
 
 namespace gie_hip {
@@ -68,7 +71,7 @@ struct Place {
   int position, page, slot, present;
 };
 
-__device__ __forceinline__ Place place_of(const gie_paged_geom& g, const int* __restrict__ q_starts,
+__device__ __forceinline__ Place place_of(const gie_kv_geom& g, const int* __restrict__ q_starts,
                                           const int* __restrict__ seq_lens, const int* __restrict__ page_table, int t) {
   const Sequence s = locate(q_starts, seq_lens, g.batch, g.total_tokens, t, [](int first, int) { return first; });
   Place p;
@@ -86,8 +89,23 @@ __device__ __forceinline__ Place place_of(const gie_paged_geom& g, const int* __
   return p;
 }
 
+// gie_kv_geom is gie_paged_geom with more fields behind it, and the entries that take the one may read no further
+static_assert(offsetof(gie_kv_geom, sinks) == sizeof(gie_paged_geom) && offsetof(gie_kv_geom, q_stride) == offsetof(gie_paged_geom, q_stride) &&
+                  offsetof(gie_kv_geom, max_len) == offsetof(gie_paged_geom, max_len),
+              "the same fields up to sinks");
+inline gie_kv_geom widened(const gie_paged_geom& g) {
+  gie_kv_geom r{};
+  std::memcpy(&r, &g, sizeof g);
+  return r;
+}
+inline gie_paged_geom narrowed(const gie_kv_geom& g) {
+  gie_paged_geom r;
+  std::memcpy(&r, &g, sizeof r);
+  return r;
+}
+
 // what the kernels' grids and offsets assume
-inline bool valid_paged(const gie_paged_geom* g) {
+inline bool valid_paged(const gie_kv_geom* g) {
   if (!g || g->batch < 0 || g->total_tokens < 0 || (g->batch == 0 && g->total_tokens > 0)) return false;
   if (g->q_heads <= 0 || g->kv_heads <= 0 || g->q_heads % g->kv_heads != 0) return false;
   if (g->head_dim <= 0 || g->page_size <= 0 || g->page_size % 16 != 0 || g->num_pages <= 0 || g->max_pages <= 0)

@@ -1,5 +1,5 @@
 // PagedKv: argument checks, the calls into the cache and attention kernels (gie_hip_kv_append,
-// gie_hip_paged_attention), and the host tables of the rotation.
+// gie_hip_kv_attention), and the host tables of the rotation.
 #include "gpu_inference/paged_kv.h"
 
 #include <cmath>
@@ -17,8 +17,8 @@ void require(bool ok, const char* what) { GIE_REQUIRE(ok, StatusCode::kInvalidAr
 void support(bool ok, const char* what) { GIE_REQUIRE(ok, StatusCode::kUnsupported, std::string("PagedKv: ") + what); }
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
-gie_paged_geom geom_of(const PagedKvProblem& p) {
-  gie_paged_geom g{};
+gie_kv_geom geom_of(const PagedKvProblem& p) {
+  gie_kv_geom g{};
   g.batch = p.batch;
   g.total_tokens = p.total_tokens;
   g.q_heads = p.q_heads;
@@ -73,7 +73,7 @@ void require_pages(const Kv8Pages& c, const int* q_starts, const int* seq_lens, 
 }
 
 void require_rows(const void* q, const void* k, const void* v, const float* q_norm, const float* k_norm,
-                  const float* cos, const float* sin, const PagedKvProblem& p, const gie_paged_geom& g,
+                  const float* cos, const float* sin, const PagedKvProblem& p, const gie_kv_geom& g,
                   const void* q_out) {
   require(k && v, "k and v must not be null");
   require((q == nullptr) == (q_out == nullptr), "q and q_out go together");
@@ -140,11 +140,11 @@ void PagedKv::append(const void* q, const void* k, const void* v, const float* c
   if (p.total_tokens == 0) return;
   require_held(p, false);
   require_cache(k_pages, v_pages, q_starts, seq_lens, page_table);
-  const gie_paged_geom g = geom_of(p);
+  const gie_kv_geom g = geom_of(p);
   require_rows(q, k, v, nullptr, nullptr, cos, sin, p, g, q_out);
   RoctxRange range("gie::PagedKv::append");
-  check_kernel_status(gie_hip_kv_append(dtype_of(p.precision), &g, q, k, v, cos, sin, q_starts, seq_lens, page_table,
-                                        q_out, k_pages, v_pages, stream),
+  check_kernel_status(gie_hip_kv_append_normed(dtype_of(p.precision), &g, q, k, v, nullptr, nullptr, cos, sin, q_starts,
+                                               seq_lens, page_table, q_out, k_pages, v_pages, stream),
                       "PagedKv::append");
 }
 
@@ -156,7 +156,7 @@ void PagedKv::append_normed(const void* q, const void* k, const void* v, const f
   if (p.total_tokens == 0) return;
   require_held(p, false);
   require_cache(k_pages, v_pages, q_starts, seq_lens, page_table);
-  const gie_paged_geom g = geom_of(p);
+  const gie_kv_geom g = geom_of(p);
   require_rows(q, k, v, q_norm, k_norm, cos, sin, p, g, q_out);
   RoctxRange range("gie::PagedKv::append_normed");
   check_kernel_status(gie_hip_kv_append_normed(dtype_of(p.precision), &g, q, k, v, q_norm, k_norm, cos, sin, q_starts,
@@ -172,7 +172,7 @@ void PagedKv8::append(const void* q, const void* k, const void* v, const float* 
   require_held(p, true);
   if (p.total_tokens == 0) return;
   require_pages(pages, q_starts, seq_lens, page_table);
-  const gie_paged_geom g = geom_of(p);
+  const gie_kv_geom g = geom_of(p);
   require_rows(q, k, v, q_norm, k_norm, cos, sin, p, g, q_out);
   RoctxRange range("gie::PagedKv8::append");
   check_kernel_status(gie_hip_kv8_append(dtype_of(p.precision), code_of(p.code), &g, q, k, v, q_norm, k_norm, cos, sin,
@@ -189,7 +189,7 @@ void PagedKv8::read(const Kv8Pages& pages, const int* q_starts, const int* seq_l
   require_pages(pages, q_starts, seq_lens, page_table);
   require(aligned(k, 2) && aligned(v, 2), "k and v must be aligned to their elements");
   require(k != v, "k and v need rows of their own");
-  const gie_paged_geom g = geom_of(p);
+  const gie_kv_geom g = geom_of(p);
   RoctxRange range("gie::PagedKv8::read");
   check_kernel_status(gie_hip_kv8_read(dtype_of(p.precision), code_of(p.code), &g, pages.k, pages.v, pages.k_scales,
                                        pages.v_scales, q_starts, seq_lens, page_table, k, v, stream),
@@ -199,7 +199,7 @@ void PagedKv8::read(const Kv8Pages& pages, const int* q_starts, const int* seq_l
 size_t PagedKv8::workspace_size(const PagedKvProblem& p) {
   validate_problem(p);
   require_held(p, true);
-  const gie_paged_geom g = geom_of(p);
+  const gie_kv_geom g = geom_of(p);
   return gie_hip_kv8_attention_workspace(&g);
 }
 
@@ -210,7 +210,7 @@ void PagedKv8::attention(const void* q, const Kv8Pages& pages, const int* q_star
   require_held(p, true);
   if (p.total_tokens == 0) return;
   require_pages(pages, q_starts, seq_lens, page_table);
-  const gie_paged_geom g = geom_of(p);
+  const gie_kv_geom g = geom_of(p);
   require_attention(q, out, workspace, workspace_bytes, gie_hip_kv8_attention_workspace(&g));
   RoctxRange range("gie::PagedKv8::attention");
   check_kernel_status(gie_hip_kv8_attention(dtype_of(p.precision), code_of(p.code), &g, q, pages.k, pages.v,
@@ -222,8 +222,8 @@ void PagedKv8::attention(const void* q, const Kv8Pages& pages, const int* q_star
 size_t PagedKv::workspace_size(const PagedKvProblem& p) {
   validate_problem(p);
   require_held(p, false);
-  const gie_paged_geom g = geom_of(p);
-  return gie_hip_paged_attention_workspace(&g);
+  const gie_kv_geom g = geom_of(p);
+  return gie_hip_kv_attention_workspace(&g);
 }
 
 void PagedKv::attention(const void* q, const void* k_pages, const void* v_pages, const int* q_starts,
@@ -233,10 +233,10 @@ void PagedKv::attention(const void* q, const void* k_pages, const void* v_pages,
   if (p.total_tokens == 0) return;
   require_held(p, false);
   require_cache(k_pages, v_pages, q_starts, seq_lens, page_table);
-  const gie_paged_geom g = geom_of(p);
-  require_attention(q, out, workspace, workspace_bytes, gie_hip_paged_attention_workspace(&g));
+  const gie_kv_geom g = geom_of(p);
+  require_attention(q, out, workspace, workspace_bytes, gie_hip_kv_attention_workspace(&g));
   RoctxRange range("gie::PagedKv::attention");
-  check_kernel_status(gie_hip_paged_attention(dtype_of(p.precision), &g, q, k_pages, v_pages, q_starts, seq_lens,
+  check_kernel_status(gie_hip_kv_attention(dtype_of(p.precision), &g, q, k_pages, v_pages, q_starts, seq_lens,
                                               page_table, out, workspace, workspace_bytes, stream),
                       "PagedKv::attention");
 }

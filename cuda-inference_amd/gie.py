@@ -94,6 +94,7 @@ class GieLinearI8Problem(ctypes.Structure):
 
 
 class GiePagedKvProblem(ctypes.Structure):
+    """gie_kv_problem, which begins with the fields of gie_paged_kv_problem: for the calls that take either."""
     _fields_ = [(n, ctypes.c_int) for n in ("batch", "total_tokens", "q_heads", "kv_heads", "head_dim", "page_size",
                                             "num_pages", "max_pages", "precision")] + \
                [(n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + \
@@ -109,6 +110,7 @@ class GieLinearGeom(ctypes.Structure):
 
 
 class GiePagedGeom(ctypes.Structure):
+    """gie_kv_geom, which begins with the fields of gie_paged_geom: for the calls that take either."""
     _fields_ = [(n, ctypes.c_int) for n in ("batch", "total_tokens", "q_heads", "kv_heads", "head_dim", "page_size",
                                             "num_pages", "max_pages")] + \
                [(n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + \
@@ -197,6 +199,8 @@ _CAPI = {
     "gie_kv_append": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 12, _i),
     "gie_paged_attention_workspace_size": ([ctypes.POINTER(GiePagedKvProblem), ctypes.POINTER(_sz)], _i),
     "gie_kv_append_normed": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 14, _i),
+    "gie_kv_attention_workspace_size": ([ctypes.POINTER(GiePagedKvProblem), ctypes.POINTER(_sz)], _i),
+    "gie_kv_attention": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 8 + [_sz, _vp], _i),
     "gie_kv8_append": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 16, _i),
     "gie_kv8_read": ([ctypes.POINTER(GiePagedKvProblem)] + [_vp] * 10, _i),
     "gie_kv8_attention_workspace_size": ([ctypes.POINTER(GiePagedKvProblem), ctypes.POINTER(_sz)], _i),
@@ -287,6 +291,8 @@ _HIP = {
     "gie_hip_linear_i8": ([_i, ctypes.POINTER(GieLinearGeom)] + [_vp] * 7 + [_sz, _vp], _i),
     "gie_hip_kv_append": ([_i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 12, _i),
     "gie_hip_kv_append_normed": ([_i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 14, _i),
+    "gie_hip_kv_attention_workspace": ([ctypes.POINTER(GiePagedGeom)], _sz),
+    "gie_hip_kv_attention": ([_i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 8 + [_sz, _vp], _i),
     "gie_hip_kv8_append": ([_i, _i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 16, _i),
     "gie_hip_kv8_read": ([_i, _i, ctypes.POINTER(GiePagedGeom)] + [_vp] * 10, _i),
     "gie_hip_kv8_attention_workspace": ([ctypes.POINTER(GiePagedGeom)], _sz),
@@ -1101,22 +1107,22 @@ class PagedKv:
 def kv_append(p: PagedKv, k: int, v: int, q_starts: int, seq_lens: int, page_table: int, k_pages: int, v_pages: int,
               cos: int | None = None, sin: int | None = None, q: int | None = None, q_out: int | None = None,
               stream=None):
-    """PagedKv::append on raw device addresses."""
-    check(capi().gie_kv_append(p._ref, q, k, v, cos, sin, q_starts, seq_lens, page_table, q_out, k_pages, v_pages,
-                               _stream(stream)), "PagedKv::append")
+    """PagedKv::append on raw device addresses (by the entry that reads p.cache, so that a cache in 8 bits is refused)."""
+    check(capi().gie_kv_append_normed(p._ref, q, k, v, None, None, cos, sin, q_starts, seq_lens, page_table, q_out,
+                                      k_pages, v_pages, _stream(stream)), "PagedKv::append")
 
 
 def paged_attention_workspace_size(p: PagedKv) -> int:
     n = ctypes.c_size_t()
-    check(capi().gie_paged_attention_workspace_size(p._ref, ctypes.byref(n)), "PagedKv::workspace_size")
+    check(capi().gie_kv_attention_workspace_size(p._ref, ctypes.byref(n)), "PagedKv::workspace_size")
     return n.value
 
 
 def paged_attention(p: PagedKv, q: int, k_pages: int, v_pages: int, q_starts: int, seq_lens: int, page_table: int,
                     out: int, workspace: int | None = None, ws_bytes: int = 0, stream=None):
     """PagedKv::attention on raw device addresses."""
-    check(capi().gie_paged_attention(p._ref, q, k_pages, v_pages, q_starts, seq_lens, page_table, out, workspace,
-                                     ws_bytes, _stream(stream)), "PagedKv::attention")
+    check(capi().gie_kv_attention(p._ref, q, k_pages, v_pages, q_starts, seq_lens, page_table, out, workspace,
+                                  ws_bytes, _stream(stream)), "PagedKv::attention")
 
 
 def kv_append_normed(p: PagedKv, k: int, v: int, q_starts: int, seq_lens: int, page_table: int, k_pages: int,

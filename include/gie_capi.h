@@ -214,32 +214,48 @@ typedef struct gie_paged_kv_problem {
   int rotary_dim, interleaved, max_positions;
   float scale, softcap;                            /* scale 0: 1 / sqrt(head_dim) */
   int window, max_new, max_len;
-  int sinks;                                       /* with a window: first positions that stay visible beside it */
-  float norm_eps;
-  int code;                                        /* of gie_kv8_*: 1 int8, 2 e4m3; 0 for the others */
 } gie_paged_kv_problem;
 int gie_kv_append(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v, const float* cos,
                   const float* sin, const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
                   void* k_pages, void* v_pages, void* stream);
-/* each head of q and k normed on the way (q_norm, k_norm: FP32 [head_dim] or null) */
-int gie_kv_append_normed(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v,
-                         const float* q_norm, const float* k_norm, const float* cos, const float* sin,
-                         const int* q_starts, const int* seq_lens, const int* page_table, void* q_out, void* k_pages,
-                         void* v_pages, void* stream);
 int gie_paged_attention_workspace_size(const gie_paged_kv_problem* p, size_t* bytes);
 int gie_paged_attention(const gie_paged_kv_problem* p, const void* q, const void* k_pages, const void* v_pages,
                         const int* q_starts, const int* seq_lens, const int* page_table, void* out, void* workspace,
                         size_t workspace_bytes, void* stream);
+/* What the calls below take: gie_paged_kv_problem, whose fields it begins with, and more behind them. (A structure of its
+   own: a caller that fills the other one leaves what is behind it as it is.) */
+typedef struct gie_kv_problem {
+  int batch, total_tokens, q_heads, kv_heads, head_dim;
+  int page_size, num_pages, max_pages;
+  int precision;                                   /* 1 fp16, 2 bf16 */
+  int64_t q_stride, k_stride, v_stride, o_stride;  /* elements between tokens; 0: packed */
+  int rotary_dim, interleaved, max_positions;
+  float scale, softcap;                            /* scale 0: 1 / sqrt(head_dim) */
+  int window, max_new, max_len;
+  int sinks;                                       /* with a window: first positions that stay visible beside it */
+  float norm_eps;
+  int code;                                        /* of gie_kv8_*: 1 int8, 2 e4m3; 0 for the others */
+} gie_kv_problem;
+/* gie_kv_append with each head of q and k normed on the way (q_norm, k_norm: FP32 [head_dim] or null) */
+int gie_kv_append_normed(const gie_kv_problem* p, const void* q, const void* k, const void* v, const float* q_norm,
+                         const float* k_norm, const float* cos, const float* sin, const int* q_starts,
+                         const int* seq_lens, const int* page_table, void* q_out, void* k_pages, void* v_pages,
+                         void* stream);
+/* gie_paged_attention with sinks */
+int gie_kv_attention_workspace_size(const gie_kv_problem* p, size_t* bytes);
+int gie_kv_attention(const gie_kv_problem* p, const void* q, const void* k_pages, const void* v_pages,
+                     const int* q_starts, const int* seq_lens, const int* page_table, void* out, void* workspace,
+                     size_t workspace_bytes, void* stream);
 /* PagedKv8: the cache in 8 bits, FP32 scales [num_pages][kv_heads][page_size / 16] */
-int gie_kv8_append(const gie_paged_kv_problem* p, const void* q, const void* k, const void* v, const float* q_norm,
+int gie_kv8_append(const gie_kv_problem* p, const void* q, const void* k, const void* v, const float* q_norm,
                    const float* k_norm, const float* cos, const float* sin, const int* q_starts, const int* seq_lens,
                    const int* page_table, void* q_out, void* k_pages, void* v_pages, float* k_scales, float* v_scales,
                    void* stream);
-int gie_kv8_read(const gie_paged_kv_problem* p, const void* k_pages, const void* v_pages, const float* k_scales,
+int gie_kv8_read(const gie_kv_problem* p, const void* k_pages, const void* v_pages, const float* k_scales,
                  const float* v_scales, const int* q_starts, const int* seq_lens, const int* page_table, void* k,
                  void* v, void* stream);
-int gie_kv8_attention_workspace_size(const gie_paged_kv_problem* p, size_t* bytes);
-int gie_kv8_attention(const gie_paged_kv_problem* p, const void* q, const void* k_pages, const void* v_pages,
+int gie_kv8_attention_workspace_size(const gie_kv_problem* p, size_t* bytes);
+int gie_kv8_attention(const gie_kv_problem* p, const void* q, const void* k_pages, const void* v_pages,
                       const float* k_scales, const float* v_scales, const int* q_starts, const int* seq_lens,
                       const int* page_table, void* out, void* workspace, size_t workspace_bytes, void* stream);
 /* host tables of the rotation, [max_positions][rotary_dim / 2] FP32 each, computed in 64 bits:

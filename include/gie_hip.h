@@ -414,8 +414,6 @@ typedef struct gie_paged_geom {
   int window;        /* > 0: a token sees its own position and the window - 1 before it */
   int max_new;       /* most new tokens and longest length of a sequence, as the host knows them (0: not known): */
   int max_len;       /* they choose the launch shape, no result depends on them */
-  int sinks;         /* with a window: positions from 0 on that stay visible beside it */
-  float norm_eps;    /* of the appends that norm heads: finite, not negative */
 } gie_paged_geom;
 
 /* Rotates q and k by their positions (cos, sin: FP32 [max_positions][rotary_dim / 2]), writes q to q_out (o_stride;
@@ -424,13 +422,6 @@ int gie_hip_kv_append(int dtype, const gie_paged_geom* g, const void* q, const v
                       const float* sin, const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
                       void* k_pages, void* v_pages, void* stream);
 
-/* The same with each head of q and k normed first, x_d / sqrt(mean_d x_d^2 + norm_eps) * weight_d in FP32, where
-   q_norm or k_norm (FP32 [head_dim]) is not NULL; q_norm needs q. */
-int gie_hip_kv_append_normed(int dtype, const gie_paged_geom* g, const void* q, const void* k, const void* v,
-                             const float* q_norm, const float* k_norm, const float* cos, const float* sin,
-                             const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
-                             void* k_pages, void* v_pages, void* stream);
-
 /* out[t][h] = sum_j softmax_j(s_j) v_j over the positions j that token t sees, s_j = scale * q[t][h] . k_j (capped);
    a token that sees nothing gets zeros. FP32 statistics and sums. dtype FP16 or BF16; head_dim 64, 96, 128 or 256;
    page_size a multiple of 16. The workspace (16-byte aligned) is scratch of this call alone. */
@@ -438,6 +429,38 @@ size_t gie_hip_paged_attention_workspace(const gie_paged_geom* g);
 int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const void* q, const void* k_pages, const void* v_pages,
                             const int* q_starts, const int* seq_lens, const int* page_table, void* out,
                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* What the calls below take: gie_paged_geom, whose fields it begins with, and more behind them. (A structure of its own:
+   a caller that fills the other one leaves what is behind it as it is.) */
+typedef struct gie_kv_geom {
+  int batch, total_tokens;
+  int q_heads, kv_heads, head_dim;
+  int page_size, num_pages, max_pages;
+  int64_t q_stride, k_stride, v_stride, o_stride;
+  int rotary_dim;
+  int interleaved;
+  int max_positions;
+  float scale;
+  float softcap;
+  int window;
+  int max_new;
+  int max_len;
+  int sinks;      /* with a window: positions from 0 on that stay visible beside it */
+  float norm_eps; /* of the appends that norm heads: finite, not negative */
+} gie_kv_geom;
+
+/* gie_hip_kv_append with each head of q and k normed first, x_d / sqrt(mean_d x_d^2 + norm_eps) * weight_d in FP32, where
+   q_norm or k_norm (FP32 [head_dim]) is not NULL; q_norm needs q. */
+int gie_hip_kv_append_normed(int dtype, const gie_kv_geom* g, const void* q, const void* k, const void* v,
+                             const float* q_norm, const float* k_norm, const float* cos, const float* sin,
+                             const int* q_starts, const int* seq_lens, const int* page_table, void* q_out,
+                             void* k_pages, void* v_pages, void* stream);
+
+/* gie_hip_paged_attention with sinks */
+size_t gie_hip_kv_attention_workspace(const gie_kv_geom* g);
+int gie_hip_kv_attention(int dtype, const gie_kv_geom* g, const void* q, const void* k_pages, const void* v_pages,
+                         const int* q_starts, const int* seq_lens, const int* page_table, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 /* ---- the paged cache in 8 bits ----
    Pages hold codes, int8 or e4m3, [num_pages][kv_heads][page_size][head_dim], 16-byte aligned, and FP32 scales
@@ -449,18 +472,18 @@ int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const void* q, c
 #define GIE_HIP_KV_INT8 1
 #define GIE_HIP_KV_E4M3 2
 /* gie_hip_kv_append_normed into such pages (q_norm, k_norm may be NULL) */
-int gie_hip_kv8_append(int dtype, int code, const gie_paged_geom* g, const void* q, const void* k, const void* v,
+int gie_hip_kv8_append(int dtype, int code, const gie_kv_geom* g, const void* q, const void* k, const void* v,
                        const float* q_norm, const float* k_norm, const float* cos, const float* sin,
                        const int* q_starts, const int* seq_lens, const int* page_table, void* q_out, void* k_pages,
                        void* v_pages, float* k_scales, float* v_scales, void* stream);
 /* the rows' keys and values (k_stride, v_stride; either may be NULL) in `dtype`, one rounding */
-int gie_hip_kv8_read(int dtype, int code, const gie_paged_geom* g, const void* k_pages, const void* v_pages,
+int gie_hip_kv8_read(int dtype, int code, const gie_kv_geom* g, const void* k_pages, const void* v_pages,
                      const float* k_scales, const float* v_scales, const int* q_starts, const int* seq_lens,
                      const int* page_table, void* k, void* v, void* stream);
-/* gie_hip_paged_attention over such pages; an e4m3 code for a NaN counts as 480 with its sign, scales are clamped to
+/* gie_hip_kv_attention over such pages; an e4m3 code for a NaN counts as 480 with its sign, scales are clamped to
    2^-73 .. 2^120 (a NaN stays one: rows that see its block are NaN) */
-size_t gie_hip_kv8_attention_workspace(const gie_paged_geom* g);
-int gie_hip_kv8_attention(int dtype, int code, const gie_paged_geom* g, const void* q, const void* k_pages,
+size_t gie_hip_kv8_attention_workspace(const gie_kv_geom* g);
+int gie_hip_kv8_attention(int dtype, int code, const gie_kv_geom* g, const void* q, const void* k_pages,
                           const void* v_pages, const float* k_scales, const float* v_scales, const int* q_starts,
                           const int* seq_lens, const int* page_table, void* out, void* workspace,
                           size_t workspace_bytes, void* stream);
