@@ -101,3 +101,35 @@ def test_append_and_attention(what):
         results.append([c.read_rows(o, 8) for o in out])
     assert all(np.array_equal(a, b) for a, b in zip(*results))
     assert np.array_equal(results[0][1], results[0][2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotary", [0, 64, 6])
+def test_the_older_entries_do_what_the_newer_ones_do(rotary):
+    """gie_kv_append beside gie_kv_append_normed without norms, gie_paged_attention beside gie_kv_attention without sinks."""
+    from paged_plain import Cache
+    vp, results = ctypes.c_void_p, []
+    for older in (True, False):
+        c = Cache([3, 40], [90, 300], heads=8, kv_heads=2, dim=64, page=16, seed=6)
+        d = c.device()
+        tables = [gie.to_device(t) for t in gie.rotary_tables(c.max_pages * 16, rotary)] if rotary else []
+        turn = [t.addr for t in tables] or [None, None]
+        more = dict(rotary_dim=rotary, max_positions=c.max_pages * 16, window=50, max_new=40, max_len=300)
+        p = c.p(**more)
+        ws, out = gie.DeviceBuffer(max(16, gie.paged_attention_workspace_size(p))), [c.blank_rows(8) for _ in range(2)]
+        rows, where = [d[n].addr for n in "qkv"], [d[n].addr for n in ("starts", "lens", "table")]
+        pages = [d[n].addr for n in ("k_pages", "v_pages")]
+        gie.synchronize()
+        at = ctypes.addressof(p._c)
+        if older:
+            assert symbol(gie.capi(), "gie_kv_append", *[vp] * 13)(at, *rows, *turn, *where, out[0].addr, *pages, None) == 0
+            assert symbol(gie.capi(), "gie_paged_attention", *[vp] * 9, ctypes.c_size_t, vp)(
+                at, out[0].addr, *pages, *where, out[1].addr, ws.addr, ws.nbytes, None) == 0
+        else:
+            assert symbol(gie.capi(), "gie_kv_append_normed", *[vp] * 15)(
+                at, *rows, None, None, *turn, *where, out[0].addr, *pages, None) == 0
+            assert symbol(gie.capi(), "gie_kv_attention", *[vp] * 9, ctypes.c_size_t, vp)(
+                at, out[0].addr, *pages, *where, out[1].addr, ws.addr, ws.nbytes, None) == 0
+        gie.synchronize()
+        results.append([c.read_rows(o, 8) for o in out] + [d[n].download(np.uint16, c.k_pages.size) for n in ("k_pages", "v_pages")])
+    assert all(np.array_equal(a, b) for a, b in zip(*results))
