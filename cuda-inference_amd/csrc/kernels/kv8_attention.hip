@@ -50,7 +50,8 @@ struct BlockScales {
 };
 template <typename C>
 __device__ __forceinline__ BlockScales block_scales(const AttnArgs& a, float ks, float vs) {
-  const float k = fminf(fmaxf(ks, 0x1p-73f), 0x1p120f), v = fminf(fmaxf(vs, 0x1p-73f), 0x1p120f);
+  // (int8's scale of the largest FP32 value lies just above 2^121)
+  const float k = fminf(fmaxf(ks, 0x1p-73f), 0x1p122f), v = fminf(fmaxf(vs, 0x1p-73f), 0x1p122f);
   const bool bad = !(ks == ks) || !(vs == vs);
   // the exponent and the quotient from the same logarithm, so that a weight and what the sum takes of it agree
   const float lv = __builtin_amdgcn_logf(v);

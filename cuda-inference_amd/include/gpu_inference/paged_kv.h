@@ -27,7 +27,7 @@
 // read: the rows' keys and values back in the problem's precision, one rounding: the tokens that append would write,
 //   so n_b = seq_lens[b] reads a whole sequence. A row without a valid position, or of a page outside the cache, is zero.
 // attention: as above over code * scale. A code of e4m3 that stands for a NaN (append writes none) counts as 480 with its
-//   sign. Scales are taken to lie within 2^-73 and 2^120; one that is not counts as the nearer of these.
+//   sign. Scales are taken to lie within 2^-73 and 2^122; one that is not counts as the nearer of these.
 // Calls only enqueue work on `stream`; no allocation, no synchronization, so both can be captured into a graph.
 #pragma once
 

@@ -481,7 +481,7 @@ int gie_hip_kv8_read(int dtype, int code, const gie_kv_geom* g, const void* k_pa
                      const float* k_scales, const float* v_scales, const int* q_starts, const int* seq_lens,
                      const int* page_table, void* k, void* v, void* stream);
 /* gie_hip_kv_attention over such pages; an e4m3 code for a NaN counts as 480 with its sign, scales are clamped to
-   2^-73 .. 2^120 (a NaN stays one: rows that see its block are NaN) */
+   2^-73 .. 2^122 (a NaN stays one: rows that see its block are NaN) */
 size_t gie_hip_kv8_attention_workspace(const gie_kv_geom* g);
 int gie_hip_kv8_attention(int dtype, int code, const gie_kv_geom* g, const void* q, const void* k_pages,
                           const void* v_pages, const float* k_scales, const float* v_scales, const int* q_starts,
