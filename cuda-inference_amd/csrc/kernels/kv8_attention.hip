@@ -44,18 +44,17 @@ constexpr float kLift = 7.f;  // weights lie in 2^7 .. 2^15 at their largest: FP
 
 // A block's scales as the scores take them: f times the product of codes and the row's factor is the score's power of 2,
 // or where scores are capped the product of keys (a NaN if either scale is one: every score of the block becomes a NaN),
-// lv = log2(vs), inv = 1 / vs.
+// lv = log2(vs), inv = 1 / vs. The codes' unit is in the row's factor: the largest scale times it passes FP32's range.
 struct BlockScales {
   float f, lv, inv;
 };
-template <typename C>
 __device__ __forceinline__ BlockScales block_scales(const AttnArgs& a, float ks, float vs) {
   // (int8's scale of the largest FP32 value lies just above 2^121)
   const float k = fminf(fmaxf(ks, 0x1p-73f), 0x1p122f), v = fminf(fmaxf(vs, 0x1p-73f), 0x1p122f);
   const bool bad = !(ks == ks) || !(vs == vs);
   // the exponent and the quotient from the same logarithm, so that a weight and what the sum takes of it agree
   const float lv = __builtin_amdgcn_logf(v);
-  return {bad ? __builtin_nanf("") : k * C::kUnit * (a.cap > 0 ? 1.f : a.mult), lv, __builtin_amdgcn_exp2f(-lv)};
+  return {bad ? __builtin_nanf("") : k * (a.cap > 0 ? 1.f : a.mult), lv, __builtin_amdgcn_exp2f(-lv)};
 }
 
 // A block of a sequence as a lane finds it: where it lies among all blocks (kNoBlock: its page is not there, its codes
@@ -67,14 +66,13 @@ struct BlockAt {
 };
 // The lanes look up 64 blocks at once, and the loop takes them by readlane: loads through the scalar cache would share
 // their counter with LDS, so that every wait for a fragment waited for them.
-template <typename C>
 __device__ __forceinline__ BlockAt find_block(const Kv8Args& a, const int* table, int kvh, int position) {
   const int gran = min(position >> 4, (a.capacity >> 4) - 1), pg = div_magic(gran, a.page_magic, a.page_shift);
   const int page = table[pg];
   const bool there = unsigned(page) < unsigned(a.num_pages);
   BlockAt b;
   b.at = there ? unsigned(page) * a.page_blocks + unsigned(kvh * a.page16 + gran - pg * a.page16) : kNoBlock;
-  b.s = block_scales<C>(a, there ? a.k_scales[b.at] : 0.f, there ? a.v_scales[b.at] : 0.f);
+  b.s = block_scales(a, there ? a.k_scales[b.at] : 0.f, there ? a.v_scales[b.at] : 0.f);
   return b;
 }
 __device__ __forceinline__ float read_lane(float v, int lane) {
@@ -313,7 +311,7 @@ __global__ __launch_bounds__(64 * WK, D == 64 ? 4 : WK == 8 ? 2 : 1) void narrow
   };
   // requests the wave's j-th tile
   const auto issue = [&](int j, int stage, Pair& scales) {
-    if (j % 32 == 0) blocks = find_block<C>(a, table, kvh, key_of(tile_at(j + lane / GR)) + lane % GR * 16);
+    if (j % 32 == 0) blocks = find_block(a, table, kvh, key_of(tile_at(j + lane / GR)) + lane % GR * 16);
     const int tile = tile_at(j);
 #pragma unroll
     for (int g = 0; g < GR; ++g) {
@@ -384,7 +382,7 @@ __global__ __launch_bounds__(64 * WK, D == 64 ? 4 : WK == 8 ? 2 : 1) void narrow
   Pair scales[NST - 1];  // of the tiles that load
 #pragma unroll
   for (int j = 0; j < NST - 1; ++j) issue(j, j, scales[j]);
-  row_factor = a.bf16 ? row_to_fp16<Bf16>(qf, a.negate != 0) : row_to_fp16<Fp16>(qf, a.negate != 0);
+  row_factor = (a.bf16 ? row_to_fp16<Bf16>(qf, a.negate != 0) : row_to_fp16<Fp16>(qf, a.negate != 0)) * C::kUnit;
   int stage = 0;
   for (int j = 0; j < mine; ++j) {
     wait_vm<(NST - 2) * LPT>();
@@ -515,7 +513,7 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
   BlockAt now;
   const auto load = [&](int tile, int n) {
     if (n == 0) {
-      if (tile % 64 == 0) blocks = find_block<C>(a, table, kvh, key_of(tile + lane) + wr * 16);
+      if (tile % 64 == 0) blocks = find_block(a, table, kvh, key_of(tile + lane) + wr * 16);
       now = block_of_lane(blocks, tile % 64);
     }
     const int at = key_of(tile) + wr * 16;
@@ -752,7 +750,7 @@ __global__ __launch_bounds__(256 * WD, 2) void wide_kernel(Kv8Args a) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const lds_v4*>(size_t(mine ^ unsigned(ks * 32)));
   }
-  row_factor = a.bf16 ? row_to_fp16<Bf16>(qf, a.negate != 0) : row_to_fp16<Fp16>(qf, a.negate != 0);
+  row_factor = (a.bf16 ? row_to_fp16<Bf16>(qf, a.negate != 0) : row_to_fp16<Fp16>(qf, a.negate != 0)) * C::kUnit;
   store_scales(0);
 #pragma unroll
   for (int n = 0; n < 2; ++n) {

@@ -34,6 +34,20 @@ def test_blocks_of_the_largest_values(dim, cache):
 
 
 @pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("softcap", [0.0, 5.0])
+@pytest.mark.parametrize("dim", DIMS)
+def test_keys_of_the_largest_values(dim, softcap, cache):
+    """Scales of K likewise, with queries and a scale of the scores that make ordinary ones of them."""
+    for new, lens in BATCHES:
+        c = Cache8(new, lens, dim=dim, precision="bf16", cache=cache, seed=2)
+        c.k_scales[:] = scale_for(LARGEST, cache)
+        if cache == "fp8":
+            c.k_pages = np.where((c.k_pages & 0x7f) > 0x76, 0x76, c.k_pages).astype(np.uint8)
+        c.q = c.q * np.float32(2.0 ** -95)  # exact in BF16
+        check(c, scale=2.0 ** -33, softcap=softcap)
+
+
+@pytest.mark.parametrize("cache", CACHES)
 def test_append_and_attention_agree_on_the_largest(cache):
     """A sequence of one value: attention gives it back, whatever the weights."""
     c = Cache8([20], [20], dim=64, precision="bf16", cache=cache, seed=3)
