@@ -61,3 +61,17 @@ def test_append_and_attention_agree_on_the_largest(cache):
     got = c.attend(d=d)
     # one code, half a step of it (int8 127 is exact up to the scale's rounding), and BF16's rounding
     assert (np.abs(got - x) <= (2.0 ** -8 + 2.0 ** -12) * x).all()
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("dim", DIMS)
+def test_blocks_of_values_2_to_the_100_apart(dim, cache):
+    """Weights of the smaller blocks count in the sum in full, whichever block comes first, in one part and in joined ones."""
+    for new, lens, hints in (([1, 1], [90, 300], {}), ([70], [200], {}), ([1], [3000], dict(max_new=1, max_len=3000))):
+        for first in (0, 1):
+            c = Cache8(new, lens, dim=dim, heads=2, kv_heads=1, page=16, precision="bf16", cache=cache, seed=4)
+            for j in range(c.max_pages):
+                c.v_scales[c.table[0, j]] *= np.float32(2.0 ** (50 if j % 2 == first else -50))
+            got = c.attend(**hints).astype(np.float64)
+            want, bound = attention(c)
+            assert (np.abs(got - want) <= bound).all()
