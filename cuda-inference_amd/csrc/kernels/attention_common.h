@@ -24,7 +24,7 @@ struct AttnArgs {
   const int* seq_lens;
   const int* page_table;
   uint16_t* out;
-  float* part;  // splits > 1: [row = token * q_heads + head][split][head_dim + 2]: O, m (in powers of 2), l
+  float* part;  // splits > 1: [row = token * q_heads + head][split][head_dim + 4]: O, m (in powers of 2), l, two unused
   long long q_stride, o_stride;
   int batch, total_tokens, q_heads, kv_heads, group;
   int page16, num_pages, max_pages;  // page16: a page's size in units of 16 positions
@@ -251,7 +251,9 @@ inline Shape shape_of(const gie_kv_geom& g) {
   const long long most = tiles / fewest > 1 ? tiles / fewest : 1;
   long long splits = 1;
   if (!s.wide) {
-    // bytes bound: one workgroup for each compute unit, whose LDS holds 64 KiB and more on their way
+    // Bytes bound: one workgroup for each compute unit, whose LDS holds 64 KiB and more on their way; over 8 bits at
+    // head_dim 64 it is half of that and a second workgroup would fit, which this rule does not use (one token over 65536,
+    // 8 key heads: 20.6 us with the join's launch, 14.2 of bytes).
     splits = 256 / blocks;
   } else {
     // Products: what a tile of 64 keys takes on a compute unit by itself, and the share of one that two workgroups have,

@@ -14,13 +14,15 @@
 //
 // Few rows: one token over 65536 positions of 8 key heads of 128 in 32 parts 27 us (134 MB, 5.0 TB/s) + 4 for the join; a
 // step of 64 sequences of 1 to 8001 120 us, 4.3 TB/s (a large copy 4.7). Many rows: two prompts of 4096 tokens, 32 heads of
-// 128, 326 to 343 us by the card, 0.80 to 0.84 PFLOP/s (a large library product 1.2), where paged_attention over 16 bits
-// takes 300 to 311. The vector unit is busy 0.61 of the time and the matrix cores 0.39, one after the other whatever was
+// 128, 322 to 343 us by the card, 0.80 to 0.84 PFLOP/s (a large library product 1.2), where paged_attention over 16 bits
+// takes 293 to 311. The vector unit is busy 0.61 of the time and the matrix cores 0.39, one after the other whatever was
 // tried: codes decoded under matrix instructions, scores of the next part under the weights (2 %, kept), wave priorities;
 // so what helps is fewer vector instructions. Of the 240 that a wave has for a tile of 64 keys, and 32 exponentials at a
 // quarter of their rate, 80 decode and 80 are the weights, their sum and their rounding. 256 rows that share a tile (half
 // the decoding for each) took from 8 % less (one prompt) to 30 % more (ragged ones, narrow heads).
-// Outputs are off by 1.7e-3 of their size in BF16 and 2.2e-4 in FP16, as FP32 weights with one rounding would be.
+// Outputs are off by 1.7e-3 of their size in BF16, as FP32 weights with one rounding would be: FP16's rounding of the
+// weights is small beside it. In FP16 it is not: 2.2e-4 over long contexts, up to 3.1e-4 over short ones (1.4 times the
+// FP32 form).
 #include <type_traits>
 
 #include "attention_common.h"

@@ -11,9 +11,11 @@ constexpr int kKvBlock = 16;  // positions of a head that share a scale
 // block's scale, which stays far inside FP32's range so.
 constexpr float kKvLeast = 0x1p-64f;
 
-// Codes: divide gives x / scale, correctly rounded to FP32 (a product with the reciprocal is off by a step now and then,
+// Codes: divide gives x / scale, correctly rounded to FP32: the product with the correctly rounded reciprocal and one
+// correction by its residual (Markstein's division; without the correction a quotient is off by a step now and then,
 // and values that lie halfway between two codes are common: half of a block's largest is 63.5). It costs two instructions
-// a value and hardly any time (int8, 4 prompts of 8192 tokens with 32 + 2 * 8 heads of 128: 200.4 us, 199.7 without).
+// a value and hardly any time (int8, 4 prompts of 8192 tokens with 32 + 2 * 8 heads of 128, appended and read back: 200.4 us,
+// 199.7 without).
 // encode4 rounds four quotients to nearest even, byte by byte; they are within the largest code but for FP32's rounding,
 // which does not reach the next step. decode4 gives bytes 0 and 2, and 1 and 3, as FP16 times 1 / kUnit, exactly (five
 // instructions in both types; bytes 0 and 1 together would take one or two more).
@@ -82,7 +84,8 @@ __device__ __forceinline__ Block block_of(const gie_kv_geom& g, const int* __res
   // n tokens from any position on touch at most n / 16 + 2 blocks, so sequence b's slots start at floor(first / 16) + 2 b
   const auto from = [&](int first, int b) { return min(max(first, 0), g.total_tokens) / kKvBlock + 2 * b; };
   const Sequence s = locate(q_starts, seq_lens, g.batch, g.total_tokens, slot, from);
-  const int p0 = max(s.base, 0), p1 = int(min((long long)s.base + s.count, (long long)g.max_pages * g.page_size)), at = slot - from(s.first, s.index);
+  const int p0 = max(s.base, 0), at = slot - from(s.first, s.index);
+  const int p1 = int(min((long long)s.base + s.count, (long long)g.max_pages * g.page_size));
   Block r;
   r.start = (p0 / kKvBlock + at) * kKvBlock;
   r.first = max(r.start, p0);

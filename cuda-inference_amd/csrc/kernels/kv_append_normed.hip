@@ -3,18 +3,21 @@
 //   x'_d = x_d / sqrt(mean_d x_d^2 + eps) * w_d;  pairs (u, v) -> (u cos - v sin, u sin + v cos);  FP32 up to one rounding.
 //
 // Bytes-bound. A lane takes 16 values of a head, 8 pairs where they rotate, in 16-byte pieces; 4, 8 or 16 lanes make a
-// head and sum its squares among them; the weights of a lane's values stay in its registers for all of its heads.
+// head and sum its squares among them; the norms' weights lie in LDS (in registers they cost a third of the waves).
 // Rows (q, and k and v of a cache in the tokens' type) go by token: a workgroup finds the places of one or more tokens and
 // spreads all their heads over its lanes. Blocks of 8-bit pages go by position: a wave has one head's whole block, up to
 // 16 tokens, in registers, so that the scale is the largest of them and every code is written once. Both parts are
 // workgroups of one launch.
 // A rotating part that is no multiple of 16 does not fall into such pieces: there a lane has 16 values side by side and
-// finds the other one of a pair through LDS.
+// finds the other one of a pair through LDS. That form takes 109 to 117 registers where the others take 56 to 73 up to
+// head_dim 128 (half the waves), and its few rotating lanes go value by value while the others wait.
 //
 // 8192 tokens of 32 + 2 x 8 heads of 128, both norms: 33 us alone, 43 among calls on other data (206 MB, 4.8 TB/s; a large
-// copy 4.7), with the weights in registers 54; 6 of 128 values rotating 87. 64 tokens of one sequence each 4.1 us, into
-// 8-bit pages 5.6 (the older codes of the blocks and their scales come on top of the chain lengths -> page -> store).
-// 6089 tokens of 12 + 2 x 12 heads of 96 into 8-bit pages 20 us, 3.5 TB/s.
+// copy 4.7), with the weights in registers 54; into 8-bit pages 44 among calls on other data. With 6 of 128 values rotating
+// 87 and 66. 64 tokens of one sequence each 4.1 us, into 8-bit pages 5.8 (the older codes of the blocks and their scales come
+// on top of the chain lengths -> page -> store).
+// 6089 tokens of 12 + 2 x 12 heads of 96 into 8-bit pages 20 us, 3.5 TB/s: two of eight lanes are idle, and every workgroup
+// looks its block up, stages the weights and passes a barrier for four heads' 16 rows.
 #include <cmath>
 #include <type_traits>
 
@@ -84,6 +87,7 @@ __device__ __forceinline__ void norm_unit(float (&x)[16], const float* w, const 
   float all = sum[0] + sum[1];
 #pragma unroll
   for (int d = 1; d < kHeadLanes<D>; d <<= 1) all += __shfl_xor(all, d);
+  // (off by an ulp: less than the sum)
   const float inv = __builtin_amdgcn_rsqf(all * (1.f / D) + eps);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {

@@ -1,7 +1,7 @@
 // Attention of new tokens over a paged key/value cache:
 //   out[t][h] = sum_j softmax_j(s_j) v_j,  s_j = scale * q[t][h] . k_j  (or softcap * tanh(that / softcap)),
-// over the positions j <= p (and j > p - window or j < sinks) of the token's sequence, in one pass over the keys with the running
-// maximum m and sum l of the softmax.
+// over the positions j <= p (and j > p - window or j < sinks) of the token's sequence, in one pass over the keys with the
+// running maximum m and sum l of the softmax.
 //
 // Rows. All (token, head) pairs of a sequence that read one key head are rows of one matrix, r = token * group + head in
 // group, so a tile of rows shares every key it reads and one token of a grouped head fills part of a tile instead of a

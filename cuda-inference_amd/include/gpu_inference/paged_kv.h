@@ -12,10 +12,12 @@
 //   with the tables' row of the token's position, in FP32 with one rounding. Tables from rotary_tables() or the
 //   caller's own (any scaling for long contexts is in them).
 // append_normed: each head of q and k is normed first, x_d / sqrt(mean_d x_d^2 + norm_eps) * weight_d, with weights
-//   [head_dim] in FP32 shared by the heads (either may be null: not normed), and rotated without a rounding between.
+//   [head_dim] in FP32 shared by the heads (either may be null: not normed), and rotated without a rounding between. The
+//   squares are summed in FP32: heads of values past 10^19 leave its range, and with norm_eps 0 those of values under 10^-19.
 // attention: out = sum_j softmax_j(s_j) v_j over the positions j <= p (and j > p - window or j < sinks), with
 //   s_j = scale * q . k_j, or softcap * tanh(that / softcap). Query head h reads key head h / (q_heads / kv_heads).
-//   Scores, statistics and sums are FP32. A token that sees nothing gets zeros.
+//   Scores, statistics and sums are FP32; the softmax's weights are rounded once to the problem's precision ahead of the
+//   second product. A token that sees nothing gets zeros.
 //
 // PagedKv8 is the same cache held in 8 bits: pages of codes, int8 or e4m3, and FP32 scales [num_pages][kv_heads]
 // [page_size / 16], one for each head's block of 16 positions; a code c stands for c * scale.
@@ -26,8 +28,11 @@
 //   first position is written again. No two sequences of a call may append to the same block.
 // read: the rows' keys and values back in the problem's precision, one rounding: the tokens that append would write,
 //   so n_b = seq_lens[b] reads a whole sequence. A row without a valid position, or of a page outside the cache, is zero.
+//   (An e4m3 code may stand for up to 2^-4 more than what was appended: FP16 values from 63488 on read as infinities.)
 // attention: as above over code * scale. A code of e4m3 that stands for a NaN (append writes none) counts as 480 with its
-//   sign. Scales are taken to lie within 2^-73 and 2^122; one that is not counts as the nearer of these.
+//   sign. Scales are taken to lie within 2^-73 and 2^122; one that is not counts as the nearer of these. Scales of V that
+//   a row sees may lie 2^100 apart before the weights of the smaller one's block are lost from the sum. The softmax's weights
+//   are rounded once to FP16, times their block's scale.
 // Calls only enqueue work on `stream`; no allocation, no synchronization, so both can be captured into a graph.
 #pragma once
 
@@ -55,7 +60,7 @@ struct PagedKvProblem {
   float softcap = 0;         // 0: not capped
   int window = 0;            // 0: unlimited
   int max_new = 0, max_len = 0;  // most new tokens and longest sequence if the host knows them (0: not known): they
-                                 // choose the launch shape, no result depends on them
+                                 // choose the launch shape; results depend on them by the sums' rounding alone
   int sinks = 0;         // attention: positions from 0 on that stay visible to rows whose window has passed them
   float norm_eps = 0;    // of append_normed and PagedKv8::append
   KvCode code = KvCode::kNone;  // PagedKv8: what its pages hold; PagedKv: kNone

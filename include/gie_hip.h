@@ -413,7 +413,7 @@ typedef struct gie_paged_geom {
   float softcap;     /* > 0: scores become softcap * tanh(score / softcap) */
   int window;        /* > 0: a token sees its own position and the window - 1 before it */
   int max_new;       /* most new tokens and longest length of a sequence, as the host knows them (0: not known): */
-  int max_len;       /* they choose the launch shape, no result depends on them */
+  int max_len;       /* they choose the launch shape; results depend on them by the sums' rounding alone */
 } gie_paged_geom;
 
 /* Rotates q and k by their positions (cos, sin: FP32 [max_positions][rotary_dim / 2]), writes q to q_out (o_stride;
@@ -423,7 +423,8 @@ int gie_hip_kv_append(int dtype, const gie_paged_geom* g, const void* q, const v
                       void* k_pages, void* v_pages, void* stream);
 
 /* out[t][h] = sum_j softmax_j(s_j) v_j over the positions j that token t sees, s_j = scale * q[t][h] . k_j (capped);
-   a token that sees nothing gets zeros. FP32 statistics and sums. dtype FP16 or BF16; head_dim 64, 96, 128 or 256;
+   a token that sees nothing gets zeros. FP32 statistics and sums, weights rounded once to dtype (over 8-bit pages to
+   FP16, times their block's scale). dtype FP16 or BF16; head_dim 64, 96, 128 or 256;
    page_size a multiple of 16. The workspace (16-byte aligned) is scratch of this call alone. */
 size_t gie_hip_paged_attention_workspace(const gie_paged_geom* g);
 int gie_hip_paged_attention(int dtype, const gie_paged_geom* g, const void* q, const void* k_pages, const void* v_pages,
@@ -476,12 +477,13 @@ int gie_hip_kv8_append(int dtype, int code, const gie_kv_geom* g, const void* q,
                        const float* q_norm, const float* k_norm, const float* cos, const float* sin,
                        const int* q_starts, const int* seq_lens, const int* page_table, void* q_out, void* k_pages,
                        void* v_pages, float* k_scales, float* v_scales, void* stream);
-/* the rows' keys and values (k_stride, v_stride; either may be NULL) in `dtype`, one rounding */
+/* the rows' keys and values (k_stride, v_stride; either may be NULL) in `dtype`, one rounding; up to 2^23 - 1 tokens,
+   GIE_HIP_EUNSUPPORTED otherwise */
 int gie_hip_kv8_read(int dtype, int code, const gie_kv_geom* g, const void* k_pages, const void* v_pages,
                      const float* k_scales, const float* v_scales, const int* q_starts, const int* seq_lens,
                      const int* page_table, void* k, void* v, void* stream);
 /* gie_hip_kv_attention over such pages; an e4m3 code for a NaN counts as 480 with its sign, scales are clamped to
-   2^-73 .. 2^122 (a NaN stays one: rows that see its block are NaN) */
+   2^-73 .. 2^122 (a NaN stays one: rows that see its block are NaN), those of V that a row sees may lie 2^100 apart */
 size_t gie_hip_kv8_attention_workspace(const gie_kv_geom* g);
 int gie_hip_kv8_attention(int dtype, int code, const gie_kv_geom* g, const void* q, const void* k_pages,
                           const void* v_pages, const float* k_scales, const float* v_scales, const int* q_starts,
