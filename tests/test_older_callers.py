@@ -133,3 +133,17 @@ def test_the_older_entries_do_what_the_newer_ones_do(rotary):
         gie.synchronize()
         results.append([c.read_rows(o, 8) for o in out] + [d[n].download(np.uint16, c.k_pages.size) for n in ("k_pages", "v_pages")])
     assert all(np.array_equal(a, b) for a, b in zip(*results))
+
+
+def test_no_structure_is_refused():
+    """A null structure, by the older entries and by the newer ones."""
+    vp, size, n = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_size_t()
+    for name, pointers in (("gie_kv_append", 13), ("gie_kv_append_normed", 15), ("gie_kv8_append", 17), ("gie_kv8_read", 11)):
+        assert symbol(gie.capi(), name, *[vp] * pointers)(*[None] * pointers) == 1
+    for name in ("gie_paged_attention", "gie_kv_attention"):
+        assert symbol(gie.capi(), name, *[vp] * 9, size, vp)(*[None] * 9, 0, None) == 1
+        assert symbol(gie.capi(), name + "_workspace_size", vp, vp)(None, ctypes.addressof(n)) == 1
+        assert symbol(gie.hip(), name.replace("gie_", "gie_hip_"), INTS, *[vp] * 9, size, vp)(gie.FP16, *[None] * 9, 0, None) == -1
+        assert symbol(gie.hip(), name.replace("gie_", "gie_hip_") + "_workspace", vp, result=size)(None) == 0
+    assert symbol(gie.hip(), "gie_hip_kv_append", INTS, *[vp] * 13)(gie.FP16, *[None] * 13) == -1
+    assert symbol(gie.hip(), "gie_hip_kv_append_normed", INTS, *[vp] * 15)(gie.FP16, *[None] * 15) == -1
